@@ -22,7 +22,7 @@ import time
 from ..errors import KernelError
 
 CSRC_DIR = os.path.dirname(os.path.abspath(__file__))
-HEADERS = ["common.cuh", "attention_common.cuh", "argmax_static.h", "gemm_f32_tc.cuh", "activations.cuh"]
+HEADERS = ["common.cuh", "attention_common.cuh", "argmax_static.h", "gemm_f32_tc.cuh", "activations.cuh", "row_select.cuh"]
 MODULES = {
     "rowwise": ["rowwise.cu"],
     "rope_kv": ["rope_kv.cu"],
@@ -39,6 +39,9 @@ MODULES = {
     "attention_window": ["attention_window.cu"],
     "attention_latent": ["attention_latent.cu"],
     "experts": ["experts.cu"],
+    "attention_weights": ["attention_weights.cu"],
+    "eviction": ["eviction.cu"],
+    "verify": ["verify.cu"],
 }
 NVCC_FLAGS = ["-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
               "--shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=default"]

@@ -199,6 +199,14 @@ _SIGNATURES = {
                                    c_void_p, c_int, c_int, c_float, c_void_p, c_int, c_void_p, c_long, c_void_p, c_int, c_long, c_void_p, c_void_p],
     ("gemm_few", "cml_gemm_few_experts"): [c_void_p, c_long, c_int, c_int, c_void_p, c_long, c_int, c_int, c_int, c_void_p, c_long, c_int,
                                            c_void_p, c_void_p, c_void_p],
+    ("attention_weights", "cml_attn_paged_weights"): [c_void_p, c_int, c_long, c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_void_p,
+                                                      c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                                                      c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p],
+    ("eviction", "cml_evict_positions"): [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                          c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p],
+    ("verify", "cml_verify_drafts"): [c_void_p, c_long, c_int, c_int, c_void_p, c_void_p, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p,
+                                      c_long, c_void_p, c_int, c_int, c_float, c_int, c_float, c_float, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_void_p],
     ("random_fill", "cml_random_fill"): [c_void_p, c_int, ctypes.c_longlong, ctypes.c_ulonglong, ctypes.c_ulonglong,
                                          ctypes.c_double, ctypes.c_double, c_void_p],
 }
@@ -244,6 +252,20 @@ def _dev(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise KernelError("camelid_b200 kernels run on CUDA tensors only; there is no CPU path")
+
+
+def _here(*tensors):
+    """All given tensors stand on the current device, whose current stream the kernels run on."""
+    now = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise KernelError("camelid_b200 kernels run on CUDA tensors only; there is no CPU path")
+        if now is None:
+            now = torch.cuda.current_device()
+        if t.device.index != now:
+            raise KernelError(f"a tensor stands on {t.device}, the current device is cuda:{now}")
 
 
 def _p(t):
@@ -2003,6 +2025,152 @@ def draws_at(positions: torch.Tensor, seed: torch.Tensor, draws: torch.Tensor):
     assert positions.dtype == torch.int32 and positions.numel() >= rows and seed.dtype == torch.int64
     assert draws.dtype == torch.float32
     _check(_fn("sampling", "cml_draws_at")(_p(positions), _p(seed), _p(draws), rows, _stream()), "draws_at")
+
+# ---------------------------------------------------------------------------------------
+# between two steps: which positions the cache keeps, which drafted tokens stay
+
+@functools.lru_cache(maxsize=512)
+def attn_weights_plan(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int, value_dim: int, dtype: torch.dtype, max_new: int,
+                      max_len: int, with_output: bool) -> tuple:
+    """(keys of a stretch, float32 numbers of scratch) of ``attn_paged_weights``: a sequence's keys are cut into stretches so that
+    the blocks fill the device, none shorter than four pages. Made from sizes alone, without a device."""
+    pairs, rows = n_seqs * n_kv_heads, max_new * (n_heads // n_kv_heads)
+    blocks = pairs * ((rows + 7) // 8)
+    splits = max(1, min((4 * SMS + blocks - 1) // blocks, (max_len + 4 * PAGE - 1) // (4 * PAGE)))
+    split_keys = (((max_len + splits - 1) // splits + PAGE - 1) // PAGE) * PAGE
+    splits = (max_len + split_keys - 1) // split_keys
+    return split_keys, pairs * rows * 2 * (1 + splits) + (pairs * rows * splits * value_dim if with_output else 0)
+
+
+def attn_weights_floats(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype, max_new: int, max_len: int,
+                        with_output: bool, value_dim: int | None = None) -> int:
+    """float32 numbers of scratch that ``attn_paged_weights`` needs for these sizes."""
+    return attn_weights_plan(n_seqs, n_heads, n_kv_heads, head_dim, head_dim if value_dim is None else value_dim, dtype, max_new, max_len,
+                             bool(with_output))[1]
+
+
+def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, seq_start, seq_new, n_heads: int, max_new: int,
+                       max_len: int, scale: float, scratch, scores_out=None):
+    """Attention of a step's rows over the paged cache that keeps what it weighed. Sequence i owns the rows
+    seq_row0[i] .. + seq_new[i] of ``q`` [rows, heads * head_dim]; its row j stands at place seq_start[i] + j and sees the
+    places up to its own (keys and values of the new places are in the cache already). ``out`` [rows, heads * value_dim] gets the
+    attention output (None, with ``v_pages`` None: scores only, for the last rows of a prompt). ``scores`` (float32 [pages, kv
+    heads, 64]) gain every place's weight, summed over the rows and the query heads of its kv head; new places start from
+    zero, whatever their page held. The new scores go to ``scores_out`` (None: in place), where nothing but the sequences'
+    places is written. ``max_new`` and ``max_len`` bound the sequences' new tokens and lengths (rows and places beyond them are
+    left out); ``scratch``: float32, ``attn_weights_floats`` numbers, free again when the call's work is done. No page
+    stands in two rows of the table."""
+    scores_out = scores if scores_out is None else scores_out
+    _here(q, out, k_pages, v_pages, scores, scores_out, block_table, seq_row0, seq_start, seq_new, scratch)
+    n_pages, kv_heads, page, head_dim = k_pages.shape
+    n_seqs, width = block_table.shape
+    rows = q.shape[0]
+    assert page == PAGE and k_pages.dtype == q.dtype and k_pages.is_contiguous() and q.dim() == 2 and q.stride(1) == 1
+    assert n_heads % kv_heads == 0 and q.shape[1] == n_heads * head_dim
+    assert scores.dtype == torch.float32 and scores.shape == (n_pages, kv_heads, PAGE) and scores.is_contiguous()
+    assert scores_out.dtype == torch.float32 and scores_out.shape == scores.shape and scores_out.is_contiguous()
+    assert block_table.dtype == torch.int32 and block_table.is_contiguous()
+    for t in (seq_row0, seq_start, seq_new):
+        assert t.dtype == torch.int32 and t.numel() == n_seqs and t.is_contiguous()
+    assert (out is None) == (v_pages is None), "an output needs values, and values an output"
+    value_dim = head_dim
+    if out is not None:
+        value_dim = v_pages.shape[3]
+        assert v_pages.shape == (n_pages, kv_heads, PAGE, value_dim) and v_pages.dtype == q.dtype and v_pages.is_contiguous()
+        assert out.dtype == q.dtype and out.shape == (rows, n_heads * value_dim) and out.stride(1) == 1
+    if max_new < 1 or max_len < 1:
+        raise KernelError(f"attn_paged_weights: max_new {max_new} and max_len {max_len} must be at least one")
+    split_keys, floats = attn_weights_plan(n_seqs, n_heads, kv_heads, head_dim, value_dim, q.dtype, max_new, max_len, out is not None)
+    if scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < floats:
+        raise KernelError(f"attn_paged_weights: the scratch must be {floats} contiguous float32 numbers (attn_weights_floats)")
+    _check(_fn("attention_weights", "cml_attn_paged_weights")(
+        _p(q), dtype_code(q.dtype), q.stride(0), _p(out), 0 if out is None else out.stride(0), _p(k_pages), _p(v_pages), _p(scores),
+        _p(scores_out), _p(block_table), width, n_pages, _p(seq_row0), _p(seq_start), _p(seq_new), n_seqs, rows, n_heads, kv_heads,
+        head_dim, value_dim, int(max_new), int(max_len), float(scale), split_keys, _p(scratch), _stream()), "attn_paged_weights", 3)
+
+
+def evict_positions(k_pages, v_pages, scores, block_table, out_table, lengths, keeps, kept, first: int, recent: int, inv_freq=None,
+                    interleaved: bool = False):
+    """Keep min(keeps[i], lengths[i]) places of every sequence i, chosen for each cache entry and kv head: its ``first`` places, its
+    ``recent`` last ones (cut to what is kept in all) and those of the largest ``scores``, the lower place among equals (a
+    score that is not a number counts as the lowest). They move, in order, to the places 0.. of the pages in
+    ``out_table``, which is ``block_table`` itself (the cache closes its gaps in place) or names pages that ``block_table``
+    does not. Keys, values and scores: [pages, kv heads, 64(, size)] or, for several entries with one table, [entries, pages, ...];
+    ``v_pages`` None: values live in the key rows. ``kept`` int32 [(entries,) sequences, kv heads, room] gets the old places in order
+    (what lies behind them stays as it was); no more than ``room`` places are kept. ``inv_freq`` (float32 [rotary size / 2]): the
+    keys' rotary pairs (split halves, or neighbours where ``interleaved``) are turned to their new places, so that a place is
+    a position again."""
+    _here(k_pages, v_pages, scores, block_table, out_table, lengths, keeps, kept, inv_freq)
+    if k_pages.dim() == 4:
+        k_pages, scores, kept = k_pages.unsqueeze(0), scores.unsqueeze(0), kept.unsqueeze(0)
+        v_pages = v_pages.unsqueeze(0) if v_pages is not None else None
+    entries, n_pages, heads, page, k_dim = k_pages.shape
+    n_seqs, width = block_table.shape
+    assert page == PAGE and k_pages.is_contiguous()
+    assert scores.dtype == torch.float32 and scores.shape == (entries, n_pages, heads, PAGE) and scores.is_contiguous()
+    v_dim = 0
+    if v_pages is not None:
+        v_dim = v_pages.shape[-1]
+        assert v_pages.dtype == k_pages.dtype and v_pages.shape == (entries, n_pages, heads, PAGE, v_dim) and v_pages.is_contiguous()
+    assert block_table.dtype == torch.int32 and block_table.is_contiguous()
+    assert out_table.dtype == torch.int32 and out_table.is_contiguous() and out_table.dim() == 2 and out_table.shape[0] == n_seqs
+    assert lengths.dtype == torch.int32 and lengths.numel() == n_seqs and keeps.dtype == torch.int32 and keeps.numel() == n_seqs
+    assert kept.dtype == torch.int32 and kept.is_contiguous() and kept.dim() == 4 and kept.shape[:3] == (entries, n_seqs, heads)
+    if first < 0 or recent < 0:
+        raise KernelError(f"evict_positions: first {first} and recent {recent} must not be negative")
+    rotary_dim = 0
+    if inv_freq is not None:
+        rotary_dim = 2 * inv_freq.numel()
+        assert inv_freq.dtype == torch.float32 and inv_freq.is_contiguous() and 0 < rotary_dim <= k_dim
+    _check(_fn("eviction", "cml_evict_positions")(
+        _p(k_pages), _p(v_pages), _p(scores), dtype_code(k_pages.dtype), _p(block_table), width, _p(out_table), out_table.shape[1],
+        _p(lengths), _p(keeps), _p(kept), kept.shape[3], entries, n_pages, n_seqs, heads, k_dim, v_dim, int(first), int(recent),
+        _p(inv_freq), rotary_dim, 1 if interleaved else 0, _stream()), "evict_positions", 2)
+
+
+VERIFY_PART = 8192              # columns of a row of logits that a block adds up; VF_PART in verify.cu
+
+
+def verify_bytes(rows: int, n_seqs: int, vocab: int) -> int:
+    """Bytes of scratch that ``verify_drafts`` needs for ``rows`` rows of ``vocab`` logits of ``n_seqs`` sequences."""
+    return max(16, rows * (16 * ((vocab + VERIFY_PART - 1) // VERIFY_PART) + 8))
+
+
+def verify_drafts(logits, row0, lens, drafts, draft_probs, accept_draws, next_draws, temperature: float, top_k: int, top_p: float,
+                  min_p: float, counts, tokens, err, scratch):
+    """Which drafted tokens stay, and the token behind them, so that every token is distributed as the target's own.
+    Sequence i drafted lens[i] tokens (``drafts`` int32 [sequences, room]) and owns the rows row0[i] .. row0[i] + lens[i] of
+    ``logits`` (float32 [rows, vocabulary]): row j holds the logits of draft j's place, the last one those behind the drafts.
+    The target's probabilities p are those ``sample_rows`` draws from (``temperature`` 0: one at the largest logit), the drafter's q stand
+    in ``draft_probs`` (float32 [sequences, room, vocabulary]; None: each draft was certain). Draft j is accepted while
+    accept_draws[i, j] * q(draft) < p(draft); the token behind the accepted ones is drawn by next_draws[i] from
+    max(p - q, 0) after a rejection (from p where nothing is left of it) and from p otherwise: the first token, by ascending id,
+    at which the cumulative weight exceeds the draw's share of the total. ``counts`` int32 [sequences] gets the accepted drafts,
+    ``tokens`` int32 [sequences, room + 1] them, the token behind them, and -1. ``err`` (int32 [1]) gains 1 for a logit
+    that is not finite in a row of the sequence (its count is 0, its token 0), 4 for a draft outside the vocabulary (it is rejected)
+    or a negative or not finite probability, 8 for rows that do not exist (no token at all). ``scratch``: uint8, ``verify_bytes``."""
+    _here(logits, row0, lens, drafts, draft_probs, accept_draws, next_draws, counts, tokens, err, scratch)
+    rows, vocab = logits.shape
+    n, room = drafts.shape
+    assert logits.dtype == torch.float32 and logits.stride(1) == 1
+    assert drafts.dtype == torch.int32 and (room < 2 or drafts.stride(1) == 1)
+    assert accept_draws.dtype == torch.float32 and accept_draws.shape == (n, room) and (room < 2 or accept_draws.stride(1) == 1)
+    assert next_draws.dtype == torch.float32 and next_draws.numel() == n and next_draws.is_contiguous()
+    for t in (row0, lens, counts):
+        assert t.dtype == torch.int32 and t.numel() == n and t.is_contiguous()
+    assert tokens.dtype == torch.int32 and tokens.shape == (n, room + 1) and tokens.is_contiguous() and err.dtype == torch.int32
+    if draft_probs is not None:
+        assert draft_probs.dtype == torch.float32 and draft_probs.shape == (n, room, vocab) and draft_probs.stride(2) == 1
+    if not (0.0 <= temperature < float("inf")) or top_k < 0 or not top_p > 0.0 or not 0.0 <= min_p <= 1.0:
+        raise KernelError(f"verify_drafts: temperature {temperature}, top_k {top_k}, top_p {top_p} or min_p {min_p} is outside its range")
+    need = verify_bytes(rows, n, vocab)
+    if scratch.dtype != torch.uint8 or not scratch.is_contiguous() or scratch.numel() < need:
+        raise KernelError(f"verify_drafts: the scratch must be {need} contiguous bytes (verify_bytes)")
+    _check(_fn("verify", "cml_verify_drafts")(
+        _p(logits), logits.stride(0), rows, vocab, _p(row0), _p(lens), _p(drafts), drafts.stride(0), _p(draft_probs),
+        0 if draft_probs is None else draft_probs.stride(0), 0 if draft_probs is None else draft_probs.stride(1), _p(accept_draws),
+        accept_draws.stride(0), _p(next_draws), n, room, float(temperature), int(top_k), float(top_p), float(min_p), _p(counts),
+        _p(tokens), _p(err), _p(scratch), _stream()), "verify_drafts", 2)
 
 
 class NativeDecodeLoop:

@@ -1,0 +1,507 @@
+// Verification of drafted tokens against the target's probabilities, from given random numbers.
+//
+// Sequence i drafted len[i] tokens x_0 .. and owns the rows row0[i] .. row0[i] + len[i] of the target's logits: row j
+// holds the logits of the place where x_j would stand, the last one those of the place behind all of them. With the
+// target's distribution p_j = softmax(logits / T) (after the sampler's top_k, min_p and top_p) and the drafter's q_j:
+//
+//   x_j is accepted while  u_j q_j(x_j) < p_j(x_j)
+//   at the first rejection the next token is drawn from max(p_j - q_j, 0) normalised, with all accepted from p_len
+//
+// which makes every token distributed as the target's own. A drafter without probabilities is certain of its tokens
+// (q = 1 there, 0 elsewhere). The draw walks the tokens in ascending order of their ids: the next token is the first at
+// which the cumulative weight exceeds draw * total. Temperature 0 is the greedy target: p = 1 at the largest logit,
+// the lowest id among equals.
+//
+// Everything that a decision rests on is computed in double, because a rounding of 2^-24 in a sum over 128,256 tokens
+// would move one draw in a hundred to a neighbouring token: exp((l - max) / T), its sums, the thresholds.
+//
+// Two launches, three with filters: (1) the maximum and the sum of every row, in parts of 8,192 columns, or, with
+// filters, the same of the candidates, by a cluster per row (row_select.cuh); (2) a cluster per sequence decides how
+// many tokens stay, adds up the one row that the next token is drawn from, warp by warp, and walks the warp's stretch
+// in which the crossing lies.
+#include "row_select.cuh"
+
+#define VF_PART 8192            // columns of a row that one block adds up
+#define VF_PART_THREADS 256
+#define VF_THREADS 512          // threads of a block that decides
+#define VF_WARPS (VF_THREADS / 32)
+
+#define VF_ERR_NONFINITE 1
+#define VF_ERR_EMPTY 2
+#define VF_ERR_DRAFT 4          // a drafted token outside the vocabulary, or a probability that is none
+#define VF_ERR_ROW 8            // a sequence names rows that the logits do not have
+
+// What is known of a part of a row: its maximum (NaN where a logit is not finite) with the lowest place of it, and the
+// sum of exp((l - max) / T) over its candidates.
+struct PartStat {
+    double sum;
+    float max;
+    int arg;
+};
+
+struct VerifyArgs {
+    const float* logits;
+    long long ld;
+    int n_rows, vocab;
+    const int* row0;
+    const int* lens;
+    const int* drafts;
+    long long drafts_ld;
+    const float* probs;
+    long long probs_seq, probs_step;
+    const float* accept;
+    long long accept_ld;
+    const float* draws;
+    int n_seqs, width;           // width: drafted tokens a sequence has room for
+    float temperature;           // 0: greedy
+    int top_k;
+    float top_p, min_p;
+    int* counts;
+    int* tokens;
+    int* err;
+    PartStat* stats;             // [rows][parts]
+    unsigned long long* floors;  // [rows]: the last candidate's key, 0 without filters
+    int parts;
+};
+
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < CUDART_INF_F; }
+
+// (1a) without filters. A thread keeps its 32 columns in registers, so the row is read once; the block's maximum is the
+// reference of its exponentials, and the parts are joined where they are read.
+__global__ void __launch_bounds__(VF_PART_THREADS) verify_stats_kernel(VerifyArgs a) {
+    __shared__ float fred[33];
+    __shared__ double dred[33];
+    __shared__ int ired[33];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+    const float* r = a.logits + (long long)row * a.ld;
+    const int begin = part * VF_PART, end = min(a.vocab, begin + VF_PART);
+    constexpr int U = VF_PART / (4 * VF_PART_THREADS);
+    float4 v[U];
+    const bool vec = (((uintptr_t)r) & 15) == 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int i = begin + 4 * (u * VF_PART_THREADS + (int)threadIdx.x);
+        if (vec && i + 4 <= end) v[u] = *reinterpret_cast<const float4*>(r + i);
+        else {
+            v[u].x = i < end ? r[i] : -CUDART_INF_F;
+            v[u].y = i + 1 < end ? r[i + 1] : -CUDART_INF_F;
+            v[u].z = i + 2 < end ? r[i + 2] : -CUDART_INF_F;
+            v[u].w = i + 3 < end ? r[i + 3] : -CUDART_INF_F;
+        }
+    }
+    float mx = -CUDART_INF_F;
+    int arg = 0x7fffffff;
+    bool bad = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int i = begin + 4 * (u * VF_PART_THREADS + (int)threadIdx.x);
+        const float e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (i + k < end) {
+                bad = bad || !finite(e[k]);
+                if (e[k] > mx || (arg == 0x7fffffff)) mx = e[k], arg = i + k;
+            }
+        }
+    }
+    const float bmax = block_max(mx, fred);
+    // the lowest place of the maximum (a thread's places ascend, and it keeps the first)
+    int at = mx == bmax ? arg : 0x7fffffff;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
+    if ((threadIdx.x & 31) == 0) ired[threadIdx.x >> 5] = at;
+    double s = 0.0;
+    if (a.temperature > 0.f) {
+        const double inv_t = 1.0 / (double)a.temperature, m = (double)bmax;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = begin + 4 * (u * VF_PART_THREADS + (int)threadIdx.x);
+            const float e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (i + k < end) s += exp(((double)e[k] - m) * inv_t);
+        }
+    }
+    s = block_sum_double(s, dred);
+    const int any_bad = __syncthreads_or(bad ? 1 : 0);
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < VF_PART_THREADS / 32; ++w) at = min(at, ired[w]);
+        PartStat st;
+        st.sum = s;
+        st.max = any_bad ? CUDART_NAN_F : bmax;
+        st.arg = at;
+        a.stats[(size_t)row * a.parts + part] = st;
+    }
+}
+
+// (1b) with filters: a cluster per row finds the last candidate's key, and the sum over the candidates. The order and
+// the stages are the sampler's: the k first, then p >= min_p * p_max, then the shortest prefix whose cumulative
+// probability reaches top_p.
+__global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyArgs a) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    FastSharedOf<double>& fs = *reinterpret_cast<FastSharedOf<double>*>(raw);
+    __shared__ SelectShared sh;
+    __shared__ TeamSlots ts;
+    __shared__ float fred[33];
+    pdl_wait();
+    pdl_launch_dependents();
+    Team tm;
+    tm.n = (int)cg::this_cluster().num_blocks();
+    tm.rank = (int)cg::this_cluster().block_rank();
+    const int row_index = blockIdx.x / tm.n;
+    const int vocab = a.vocab;
+    {
+        const int per = (((vocab + tm.n - 1) / tm.n) + 3) & ~3;
+        tm.begin = min(vocab, tm.rank * per);
+        tm.end = min(vocab, tm.begin + per);
+    }
+    TeamSlots* ts0 = tm.at0(&ts);
+    FastSharedOf<double>* fs0 = tm.at0(&fs);
+    const float* row = a.logits + (long long)row_index * a.ld;
+    float mx = -CUDART_INF_F, mn = CUDART_INF_F;
+    bool bad = false;
+    for_each_in_slice(row, tm, [&](float v, int) {
+        if (!finite(v)) bad = true;
+        mx = fmaxf(mx, v);
+        mn = fminf(mn, v);
+    });
+    {
+        const float bmx = block_max(mx, fred), bmn = -block_max(-mn, fred);
+        const int any_bad = __syncthreads_or(bad ? 1 : 0);
+        if (threadIdx.x == 0) ts0->f[0][tm.rank] = bmx, ts0->f[1][tm.rank] = bmn, ts0->u[1][tm.rank] = any_bad ? 1u : 0u;
+    }
+    tm.sync();
+    mx = -CUDART_INF_F, mn = CUDART_INF_F;
+    unsigned int team_bad = 0u;
+    for (int r = 0; r < tm.n; ++r) {
+        mx = fmaxf(mx, ts0->f[0][r]);
+        mn = fminf(mn, ts0->f[1][r]);
+        team_bad |= ts0->u[1][r];
+    }
+    const bool writer = tm.rank == 0 && threadIdx.x == 0;
+    PartStat st;
+    st.sum = 0.0;
+    st.max = CUDART_NAN_F;
+    st.arg = 0;
+    if (team_bad != 0u) {
+        if (writer) a.stats[row_index] = st, a.floors[row_index] = 0ull;
+        tm.sync();
+        return;
+    }
+    const double inv_t = 1.0 / (double)a.temperature, m = (double)mx;
+    // the place of a value in the order: never negative, monotone, and finite (masks of the type's lowest value are
+    // all put at one far place, where their weight is zero)
+    const float inv_tf = (float)fmin(inv_t, 1e30), far = 1e30f;
+    auto xof = [=](float v) { return fminf(fmaxf((float)((m - (double)v) * (double)inv_tf), 0.f), far); };
+    const float x_max = xof(mn);
+    auto raw_weight = [=](float v, int) { return exp(((double)v - m) * inv_t); };
+    unsigned long long floor_key = 0ull, key;
+    double cum;
+    auto select_slow = [&](unsigned long long floor, double target, int strict, auto weight) {
+        if (tm.rank == 0) {
+            unsigned long long k;
+            double c;
+            select_by_mass(row, vocab, floor, target, strict, weight, &sh, &k, &c);
+            if (threadIdx.x == 0) fs.key = k, fs.cum = c;
+        }
+        tm.sync();
+        key = fs0->key;
+        cum = fs0->cum;
+        tm.sync();
+    };
+    if (a.top_k > 0 && a.top_k < vocab) {
+        auto one = [](float, int) { return 1.0; };
+        auto one_at = [](float) { return 1.0f; };
+        if (!select_fast(row, tm, 0ull, (double)a.top_k, 0, xof, x_max, one, one_at, &fs, &ts, &key, &cum))
+            select_slow(0ull, (double)a.top_k, 0, one);
+        floor_key = key;
+    }
+    // min_p: the weight of the maximum is one, so a candidate's own weight is compared
+    const double least = (double)a.min_p;
+    double part = 0.0;
+    unsigned long long kmin = ~0ull;
+    for_each_in_slice(row, tm, [&](float v, int i) {
+        const unsigned long long ck = composite_key(v, i);
+        if (ck < floor_key) return;
+        const double w = raw_weight(v, i);
+        if (w >= least) { part += w; kmin = ck < kmin ? ck : kmin; }
+    });
+    part = block_sum_double(part, fs.dred);
+    {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const unsigned long long ok = __shfl_xor_sync(0xffffffffu, kmin, o);
+            kmin = ok < kmin ? ok : kmin;
+        }
+        __syncthreads();
+        if (lane == 0) fs.list[warp] = kmin;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < nw; ++w) kmin = fs.list[w] < kmin ? fs.list[w] : kmin;
+            ts0->d[3][tm.rank] = part;
+            ts0->k[0][tm.rank] = kmin;
+        }
+    }
+    tm.sync();
+    double total = 0.0;
+    unsigned long long k_all = ~0ull;
+    for (int r = 0; r < tm.n; ++r) {
+        total += ts0->d[3][r];
+        k_all = ts0->k[0][r] < k_all ? ts0->k[0][r] : k_all;
+    }
+    if (a.min_p > 0.f && k_all != ~0ull) floor_key = k_all;
+    if (a.top_p < 1.f) {
+        auto a1 = [=](float x) { return __expf(-x); };
+        const double target = (double)a.top_p * total;
+        if (!select_fast(row, tm, floor_key, target, 0, xof, x_max, raw_weight, a1, &fs, &ts, &key, &cum))
+            select_slow(floor_key, target, 0, raw_weight);
+        floor_key = key;
+        total = cum;
+    }
+    if (writer) {
+        st.sum = total;
+        st.max = mx;
+        a.stats[row_index] = st;
+        a.floors[row_index] = floor_key;
+    }
+    tm.sync();                       // block 0's shared memory stays until every block has read it
+}
+
+struct RowStat {
+    double max, total;               // the maximum as a double, and the sum against it
+    int arg;
+    bool bad;
+};
+
+// The parts of a row joined, in their order.
+__device__ RowStat join_parts(const VerifyArgs& a, int row) {
+    RowStat r;
+    float mx = -CUDART_INF_F;
+    r.bad = false;
+    r.arg = 0;
+    const PartStat* s = a.stats + (size_t)row * a.parts;
+    for (int p = 0; p < a.parts; ++p) {
+        const float m = s[p].max;
+        if (!finite(m)) r.bad = true;
+        if (m > mx) mx = m, r.arg = s[p].arg;
+    }
+    r.max = (double)mx;
+    r.total = 0.0;
+    if (a.temperature > 0.f && !r.bad) {
+        const double inv_t = 1.0 / (double)a.temperature;
+        for (int p = 0; p < a.parts; ++p) r.total += s[p].sum * exp(((double)s[p].max - r.max) * inv_t);
+    }
+    return r;
+}
+
+// (2) a cluster per sequence.
+__global__ void __launch_bounds__(VF_THREADS) verify_decide_kernel(VerifyArgs a) {
+    __shared__ double warp_sums[SAMPLE_MAX_TEAM * VF_WARPS];      // block 0's: every block's warps, in order
+    __shared__ int first_bad, row_bad, err_bits;
+    __shared__ RowStat chosen;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int team = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank();
+    const int seq = blockIdx.x / team;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int len = max(0, min(a.lens[seq], a.width)), row0 = a.row0[seq];
+    const int vocab = a.vocab;
+    const bool greedy = !(a.temperature > 0.f), filtered = a.floors != nullptr;
+    const double inv_t = greedy ? 0.0 : 1.0 / (double)a.temperature;
+    double* sums0 = cg::this_cluster().map_shared_rank(&warp_sums[0], 0);
+    int* out = a.tokens + (size_t)seq * (a.width + 1);
+    if (row0 < 0 || row0 > a.n_rows - 1 - len) {                  // the same in every block of the cluster
+        if (rank == 0) {
+            if (threadIdx.x == 0) atomicOr(a.err, VF_ERR_ROW), a.counts[seq] = 0;
+            for (int j = threadIdx.x; j <= a.width; j += blockDim.x) out[j] = -1;
+        }
+        return;
+    }
+    if (threadIdx.x == 0) first_bad = len, row_bad = 0, err_bits = 0;
+    __syncthreads();
+    // every draft by a thread of its own: is it accepted?
+    for (int j = threadIdx.x; j <= len; j += blockDim.x) {
+        const RowStat r = join_parts(a, row0 + j);
+        int bits = r.bad ? VF_ERR_NONFINITE : (!greedy && !(r.total > 0.0) ? VF_ERR_EMPTY : 0);
+        if (bits) atomicOr(&row_bad, 1);
+        if (j < len) {
+            const int x = a.drafts[(long long)seq * a.drafts_ld + j];
+            bool ok = false;
+            if (x < 0 || x >= vocab) bits |= VF_ERR_DRAFT;
+            else if (!r.bad) {
+                const float q = a.probs ? a.probs[(long long)seq * a.probs_seq + (long long)j * a.probs_step + x] : 1.f;
+                if (!(q >= 0.f) || !finite(q)) bits |= VF_ERR_DRAFT;
+                const double u = (double)a.accept[(long long)seq * a.accept_ld + j];
+                double p;
+                if (greedy) p = x == r.arg ? 1.0 : 0.0;
+                else {
+                    const float l = a.logits[(long long)(row0 + j) * a.ld + x];
+                    const bool in = !filtered || composite_key(l, x) >= a.floors[row0 + j];
+                    p = in ? exp(((double)l - r.max) * inv_t) / r.total : 0.0;
+                }
+                ok = u * (double)q < p;
+            }
+            if (!ok) atomicMin(&first_bad, j);
+        }
+        if (bits) atomicOr(&err_bits, bits);
+    }
+    __syncthreads();
+    const int count = row_bad ? 0 : first_bad;
+    const int row = row0 + count;
+    if (threadIdx.x == 0) chosen = join_parts(a, row);
+    __syncthreads();
+    const RowStat st = chosen;
+    if (rank == 0) {
+        if (threadIdx.x == 0) {
+            a.counts[seq] = count;
+            if (err_bits) atomicOr(a.err, err_bits);
+        }
+        for (int j = threadIdx.x; j <= a.width; j += blockDim.x)
+            if (j != count) out[j] = j < count ? a.drafts[(long long)seq * a.drafts_ld + j] : -1;
+    }
+    if (row_bad || greedy) {                                      // the same in every block
+        if (rank == 0 && threadIdx.x == 0) out[count] = row_bad ? 0 : st.arg;
+        return;
+    }
+    // the weight of the next token: the target's probability, less the drafter's where a draft was rejected
+    const float* r = a.logits + (long long)row * a.ld;
+    const bool rejected = count < len;
+    const float* q = (rejected && a.probs) ? a.probs + (long long)seq * a.probs_seq + (long long)count * a.probs_step : nullptr;
+    const int without = (rejected && !a.probs) ? a.drafts[(long long)seq * a.drafts_ld + count] : -1;
+    const unsigned long long floor_key = filtered ? a.floors[row] : 0ull;
+    const double inv_total = 1.0 / st.total;
+    bool bad_q = false;
+    bool plain = false;                                           // nothing is left of p - q: draw from p
+    auto weight = [&](int i) {
+        const float l = r[i];
+        if (filtered && composite_key(l, i) < floor_key) return 0.0;
+        const double p = exp(((double)l - st.max) * inv_t) * inv_total;
+        if (plain) return p;
+        if (q) {
+            const float qi = q[i];
+            if (!(qi >= 0.f)) bad_q = true;
+            const double d = p - (double)qi;
+            return d > 0.0 ? d : 0.0;
+        }
+        return i == without ? 0.0 : p;
+    };
+    // stretches of whole tiles of 32 columns, one a warp, in ascending order over the blocks of the cluster
+    const int warps = team * VF_WARPS;
+    const int per = (((vocab + warps - 1) / warps) + 31) & ~31;
+    const int mine = rank * VF_WARPS + warp;
+    const int begin = min(vocab, mine * per), end = min(vocab, begin + per);
+    int owner = -1;
+    double before = 0.0, total = 0.0, target = 0.0;
+    for (int round = 0; round < 2; ++round) {
+        double s = 0.0;
+        for (int i = begin + lane; i < end; i += 32) s += weight(i);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (lane == 0) sums0[mine] = s;
+        cg::this_cluster().sync();
+        total = 0.0;
+        for (int w = 0; w < warps; ++w) total += sums0[w];
+        if (total > 0.0 || round == 1) break;
+        plain = true;
+        cg::this_cluster().sync();                                // before the sums are written again
+    }
+    target = (double)a.draws[seq] * total;
+    {
+        double run = 0.0;
+        for (int w = 0; w < warps; ++w) {
+            const double s = sums0[w];
+            if (s > 0.0) owner = w, before = run;                 // never reached: the last stretch with any weight
+            run += s;
+            if (run > target) break;
+        }
+    }
+    if (mine == owner) {
+        double run = before;
+        int found = -1, last = -1;
+        for (int i0 = begin; i0 < end; i0 += 32) {
+            const int i = i0 + lane;
+            const double w = i < end ? weight(i) : 0.0;
+            double incl = w;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double t = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += t;
+            }
+            const unsigned int some = __ballot_sync(0xffffffffu, w > 0.0);
+            const unsigned int hit = __ballot_sync(0xffffffffu, w > 0.0 && run + incl > target);
+            if (hit) { found = i0 + __ffs(hit) - 1; break; }
+            if (some) last = i0 + 31 - __clz(some);
+            run += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) out[count] = found >= 0 ? found : last;
+    } else if (owner < 0 && rank == 0 && threadIdx.x == 0) {      // not a number in the sums
+        out[count] = st.arg;
+        atomicOr(a.err, VF_ERR_EMPTY);
+    }
+    if (__syncthreads_or(bad_q ? 1 : 0) && threadIdx.x == 0) atomicOr(a.err, VF_ERR_DRAFT);
+    cg::this_cluster().sync();                                    // block 0's sums stay until every block has read them
+}
+
+static int verify_parts(int vocab) { return (vocab + VF_PART - 1) / VF_PART; }
+
+template <typename K>
+static cudaError_t launch_cluster(K kernel, int blocks, int threads, size_t smem, int team, cudaStream_t stream, VerifyArgs a) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)team;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cml_pdl_enabled() ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+// `scratch`: 16 bytes a row and part of 8,192 columns, then 8 bytes a row (16-byte aligned).
+extern "C" int cml_verify_drafts(const float* logits, long long ld, int n_rows, int vocab, const int* row0, const int* lens,
+                                 const int* drafts, long long drafts_ld, const float* probs, long long probs_seq,
+                                 long long probs_step, const float* accept, long long accept_ld, const float* draws, int n_seqs,
+                                 int width, float temperature, int top_k, float top_p, float min_p, int* counts, int* tokens,
+                                 int* err, void* scratch, void* stream) {
+    if (n_seqs <= 0) return 0;
+    if (vocab <= 0 || vocab > 0x7fffff00 || n_rows < 0 || width < 0 || width > 65535 || !(temperature >= 0.f) ||
+        !(temperature < __builtin_inff()))
+        return CML_ERR_BAD_SIZE;
+    if (((uintptr_t)scratch) & 15) return CML_ERR_BAD_ALIGN;
+    const bool filters = temperature > 0.f && ((top_k > 0 && top_k < vocab) || top_p < 1.f || min_p > 0.f);
+    VerifyArgs a = {};
+    a.logits = logits; a.ld = ld; a.n_rows = n_rows; a.vocab = vocab; a.row0 = row0; a.lens = lens;
+    a.drafts = drafts; a.drafts_ld = drafts_ld; a.probs = probs; a.probs_seq = probs_seq; a.probs_step = probs_step;
+    a.accept = accept; a.accept_ld = accept_ld; a.draws = draws; a.n_seqs = n_seqs; a.width = width;
+    a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p;
+    a.counts = counts; a.tokens = tokens; a.err = err;
+    a.stats = (PartStat*)scratch;
+    a.parts = filters ? 1 : verify_parts(vocab);
+    if ((long long)n_rows * max(a.parts, 8) > 0x7fffffffLL || (long long)n_seqs * 8 > 0x7fffffffLL) return CML_ERR_BAD_SIZE;
+    cudaStream_t s = (cudaStream_t)stream;
+    int team = vocab >= 32768 ? 8 : (vocab >= 8192 ? 4 : 1);
+    if (n_rows > 0) {
+        cudaError_t e;
+        if (filters) {
+            a.floors = (unsigned long long*)((char*)scratch + 16ll * n_rows * verify_parts(vocab));
+            e = cml_allow_smem<verify_floor_kernel>(sizeof(FastSharedOf<double>));
+            if (e != cudaSuccess) return (int)e;
+            e = launch_cluster(verify_floor_kernel, n_rows * team, SAMPLE_THREADS, sizeof(FastSharedOf<double>), team, s, a);
+        } else {
+            e = launch_pdl(verify_stats_kernel, dim3((unsigned)(n_rows * a.parts)), dim3(VF_PART_THREADS), 0, s, a);
+        }
+        if (e != cudaSuccess) return (int)e;
+    }
+    const cudaError_t e = launch_cluster(verify_decide_kernel, n_seqs * team, VF_THREADS, 0, team, s, a);
+    if (e != cudaSuccess) return (int)e;
+    return cml_launch_status();
+}

@@ -1,0 +1,428 @@
+"""The operators between two steps on the device, against their plain 64-bit forms: attention that keeps its weights,
+eviction of cached positions, verification of drafted tokens."""
+import math
+import random
+
+import pytest
+import torch
+
+import plain_between as pb
+
+pytestmark = pytest.mark.gpu
+PAGE = 64
+
+
+def _rounding(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _tables(rng, lengths, extra_pages, spare=0):
+    """(table rows with -1 behind a sequence's pages, number of pages, ids not used)"""
+    used = [(n + PAGE - 1) // PAGE for n in lengths]
+    n_pages = max(1, sum(used) + extra_pages)
+    ids = list(range(n_pages))
+    rng.shuffle(ids)
+    width, rows, at = max(used + [1]) + spare, [], 0
+    for u in used:
+        rows.append(ids[at:at + u] + [-1] * (width - u))
+        at += u
+    return rows, n_pages, ids[at:]
+
+
+# ---- attention that keeps its weights --------------------------------------------------------------------------------
+def _attention(cuda, starts, news, heads, kv_heads, dim, dtype, with_out=True, v_dim=None, seed=0, in_place=True, spoil=None, q_pad=0,
+               loose=False, scale=None):
+    from camelid_b200.csrc import ops
+    rng, gen = random.Random(seed), torch.Generator().manual_seed(seed)
+    lengths = [s + n for s, n in zip(starts, news)]
+    table, n_pages, _ = _tables(rng, lengths, 2, spare=1)
+    v_dim = v_dim or dim
+    k = torch.randn(n_pages, kv_heads, PAGE, dim, generator=gen).to(dtype)
+    v = torch.randn(n_pages, kv_heads, PAGE, v_dim, generator=gen).to(dtype)
+    scores = torch.rand(n_pages, kv_heads, PAGE, generator=gen) * 3
+    rows = sum(news)
+    q = (1.5 * torch.randn(rows + 2, heads * dim + q_pad, generator=gen)).to(dtype)
+    row0 = [sum(news[:i]) for i in range(len(news))]
+    k_dev, v_dev, s_dev = k.clone(), v.clone(), scores.clone()
+    if spoil is not None:                     # what lies behind a sequence's last place must not matter
+        for i, n in enumerate(lengths):
+            for p in range(n, (n + PAGE - 1) // PAGE * PAGE):
+                k_dev[table[i][p // PAGE], :, p % PAGE] = spoil
+                v_dev[table[i][p // PAGE], :, p % PAGE] = spoil
+            for p in range(starts[i], n):     # nor what a new place's score was
+                s_dev[table[i][p // PAGE], :, p % PAGE] = spoil
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)        # noqa: E731
+    out = torch.full((rows + 2, heads * v_dim), 7.0, dtype=dtype, device=cuda)
+    q_dev = q.to(cuda)[:, :heads * dim]
+    k_dev, v_dev, s_dev = k_dev.to(cuda), v_dev.to(cuda), s_dev.to(cuda)
+    s_out = s_dev if in_place else s_dev.clone()
+    max_new, max_len = max(news + [1]), max(lengths + [1])
+    if loose:
+        max_new, max_len = max_new + 3, max_len + 200
+    scratch = torch.empty(ops.attn_weights_floats(len(news), heads, kv_heads, dim, dtype, max_new, max_len, with_out, v_dim), device=cuda)
+    scratch.fill_(float("nan"))
+    scale = 1 / math.sqrt(dim) if scale is None else scale
+    ops.attn_paged_weights(q_dev, out if with_out else None, k_dev, v_dev if with_out else None, s_dev, ints(table), ints(row0), ints(starts),
+                           ints(news), heads, max_new, max_len, scale, scratch, None if in_place else s_out)
+    torch.cuda.synchronize()
+    ref, ref_scores, tol, tol_scores = pb.weights(q[:, :heads * dim], k, v if with_out else None, scores, table, row0, starts, news, heads, scale)
+    if with_out:
+        got = out.cpu().double()
+        assert bool((got[rows:] == 7.0).all()), "rows behind the last sequence were written"
+        mma = dtype == torch.bfloat16
+        # bfloat16 probabilities times values: half a step of each, of the sum of the products' sizes
+        absolute = torch.zeros_like(ref)
+        if mma:
+            absolute = pb.weights(q[:, :heads * dim], k, v.abs(), scores, table, row0, starts, news, heads, scale)[0] * _rounding(dtype)
+        bound = tol + absolute + _rounding(dtype) * (ref.abs() + tol + absolute) + 1e-30
+        assert bool(((got - ref)[:rows].abs() <= bound[:rows]).all()), float(((got - ref)[:rows].abs() / bound[:rows]).max())
+    new_scores = s_out.cpu().double()
+    live = torch.zeros(ref_scores.shape, dtype=torch.bool)
+    for i, n in enumerate(lengths):
+        for p in range(n if news[i] else 0):
+            live[table[i][p // PAGE], :, p % PAGE] = True
+    assert bool(((new_scores - ref_scores).abs() <= tol_scores + 1e-30)[live].all()), float(
+        ((new_scores - ref_scores).abs() / (tol_scores + 1e-30))[live].max())
+    untouched = s_dev if not in_place else None
+    if untouched is not None:
+        assert torch.equal(torch.nan_to_num(s_out.cpu()[~live]), torch.nan_to_num(s_dev.cpu()[~live]))
+    elif spoil is None:
+        assert torch.equal(s_out.cpu()[~live], scores[~live])
+    return out, s_out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (4, 4, 128), (6, 1, 96), (8, 1, 16), (3, 1, 256), (16, 1, 64)])
+def test_weights_of_single_tokens(cuda, dtype, heads, kv_heads, dim):
+    _attention(cuda, [0, 1, 62, 63, 64, 200, 517], [1] * 7, heads, kv_heads, dim, dtype, seed=heads + dim)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim", [64, 128, 48])
+def test_weights_of_drafted_steps(cuda, dtype, dim):
+    """Unequal numbers of new tokens, a sequence without any, places that later rows alone see."""
+    _attention(cuda, [0, 130, 61, 7, 300], [5, 1, 8, 0, 3], 8, 2, dim, dtype, seed=dim)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.bfloat16, 80), (torch.float32, 64)])
+def test_weights_of_a_prompts_last_rows(cuda, dtype, dim):
+    _attention(cuda, [0, 500, 129], [33, 64, 2], 8, 2, dim, dtype, with_out=False, seed=3)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.bfloat16, 112), (torch.float32, 32)])
+def test_weights_do_not_read_behind_the_end(cuda, dtype, dim):
+    for spoil in (float("nan"), float("inf"), -float("inf")):
+        _attention(cuda, [10, 64, 190], [3, 1, 2], 4, 2, dim, dtype, spoil=spoil, in_place=False)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.float32, 64), (torch.bfloat16, 128)])
+def test_weights_with_strided_rows_and_loose_bounds(cuda, dtype, dim):
+    _attention(cuda, [10, 333], [2, 1], 8, 4, dim, dtype, q_pad=40, loose=True, in_place=False)
+    _attention(cuda, [10, 333], [2, 1], 8, 4, dim, dtype, q_pad=3, loose=True)
+
+
+def test_weights_with_values_of_another_size(cuda):
+    _attention(cuda, [100, 3], [1, 2], 4, 2, 64, torch.bfloat16, v_dim=32)
+    _attention(cuda, [100, 3], [1, 2], 4, 2, 32, torch.float32, v_dim=128)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.float32, 64), (torch.bfloat16, 128)])
+def test_a_later_rows_value_does_not_reach_an_earlier_row(cuda, dtype, dim):
+    """Infinite keys and values at a place that only the last row sees."""
+    from camelid_b200.csrc import ops
+    gen = torch.Generator().manual_seed(5)
+    k, v = (torch.randn(4, 1, PAGE, dim, generator=gen).to(dtype) for _ in range(2))
+    q = torch.randn(3, 2 * dim, generator=gen).to(dtype)
+    k[1, 0, 10], v[1, 0, 10] = float("inf"), float("nan")         # place 74: the third row's own
+    scores = torch.zeros(4, 1, PAGE)
+    out = torch.zeros(3, 2 * dim, dtype=dtype, device=cuda)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)        # noqa: E731
+    scratch = torch.empty(ops.attn_weights_floats(1, 2, 1, dim, dtype, 3, 75, True), device=cuda)
+    s_dev = scores.to(cuda)
+    ops.attn_paged_weights(q.to(cuda), out, k.to(cuda), v.to(cuda), s_dev, ints([[0, 1]]), ints([0]), ints([72]), ints([3]), 2, 3, 75,
+                           dim ** -0.5, scratch)
+    ref = pb.weights(q[:2], k, v, scores, [[0, 1]], [0], [72], [2], 2, dim ** -0.5)[0]
+    got = out.cpu().double()[:2]
+    assert bool(torch.isfinite(got).all())
+    assert float((got - ref).abs().max()) <= 4 * _rounding(dtype) * float(ref.abs().max()) + 1e-5
+
+
+def test_weights_with_missing_pages(cuda):
+    """A page that the table does not name holds nothing to see; a row without any place gives zeros."""
+    from camelid_b200.csrc import ops
+    for dtype, dim in ((torch.bfloat16, 64), (torch.float32, 32), (torch.bfloat16, 128)):
+        gen = torch.Generator().manual_seed(6)
+        k, v = (torch.randn(3, 1, PAGE, dim, generator=gen).to(dtype) for _ in range(2))
+        q = torch.randn(2, 2 * dim, generator=gen).to(dtype)
+        table, start = [[-1, 1, 3], [-1, 99, -1]], [130, 70]
+        scores = torch.rand(3, 1, PAGE, generator=gen)
+        out = torch.ones(2, 2 * dim, dtype=dtype, device=cuda)
+        ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)    # noqa: E731
+        scratch = torch.empty(ops.attn_weights_floats(2, 2, 1, dim, dtype, 1, 131, True), device=cuda)
+        s_dev = scores.to(cuda)
+        ops.attn_paged_weights(q.to(cuda), out, k.to(cuda), v.to(cuda), s_dev, ints(table), ints([0, 1]), ints(start), ints([1, 1]), 2, 1,
+                               131, dim ** -0.5, scratch)
+        ref, ref_scores, tol, tol_scores = pb.weights(q, k, v, scores, table, [0, 1], start, [1, 1], 2, dim ** -0.5)
+        got = out.cpu().double()
+        assert bool((got[1] == 0).all())
+        assert float((got - ref).abs().max()) <= 4 * _rounding(dtype) * float(ref.abs().max()) + 1e-5
+        assert bool(((s_dev.cpu().double() - ref_scores).abs() <= tol_scores + 1e-30).all())
+
+
+def test_weights_of_large_scores(cuda):
+    """Scores of hundreds: nothing overflows, one place takes everything."""
+    for dtype, dim in ((torch.bfloat16, 64), (torch.float32, 64), (torch.bfloat16, 128)):
+        _attention(cuda, [150, 40], [1, 2], 4, 2, dim, dtype, scale=20.0)
+
+
+# ---- eviction ---------------------------------------------------------------------------------------------------------
+def _evict(cuda, lengths, keeps, first, recent, dtype=torch.bfloat16, entries=2, heads=2, dim=64, v_dim=64, in_place=False, rotary=0,
+           interleaved=False, seed=0, scores=None, room=None):
+    from camelid_b200.csrc import ops
+    rng, gen = random.Random(seed), torch.Generator().manual_seed(seed)
+    kept_n = [min(n, m) for n, m in zip(lengths, keeps)]
+    out_used = [(m + PAGE - 1) // PAGE for m in kept_n]
+    table, n_pages, ids = _tables(rng, lengths, 1 if in_place else sum(out_used) + 1, spare=1)
+    if in_place:
+        out_table = table
+    else:
+        width, out_table, at = max(out_used + [1]), [], 0
+        for u in out_used:
+            out_table.append(ids[at:at + u] + [-1] * (width - u))
+            at += u
+    k = torch.randn(entries, n_pages, heads, PAGE, dim, generator=gen).to(dtype)
+    v = torch.randn(entries, n_pages, heads, PAGE, v_dim, generator=gen).to(dtype) if v_dim else None
+    s = torch.randint(0, 40, (entries, n_pages, heads, PAGE), generator=gen).float() / 8 if scores is None else scores(entries, n_pages, heads)
+    inv_freq = (10000.0 ** (-torch.arange(rotary // 2).double() / max(rotary // 2, 1))).float() if rotary else None
+    room = max(kept_n + [1]) if room is None else room
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)        # noqa: E731
+    k_dev, s_dev = k.to(cuda), s.to(cuda)
+    v_dev = v.to(cuda) if v_dim else None
+    kept = torch.full((entries, len(lengths), heads, room), -7, dtype=torch.int32, device=cuda)
+    t_dev = ints(table)
+    ops.evict_positions(k_dev, v_dev, s_dev, t_dev, t_dev if in_place else ints(out_table), ints(lengths), ints(keeps), kept, first, recent,
+                        inv_freq=inv_freq.to(cuda) if rotary else None, interleaved=interleaved)
+    torch.cuda.synchronize()
+    want_k, want_v, want_s = k.double(), v.double() if v_dim else None, s.clone()
+    turned = torch.zeros(k.shape[:-1], dtype=torch.bool)
+    for e in range(entries):
+        for i, n in enumerate(lengths):
+            for h in range(heads):
+                line = [float(s[e, table[i][p // PAGE], h, p % PAGE]) for p in range(n)]
+                places = pb.choose(line, n, min(keeps[i], room), first, recent)
+                assert kept[e, i, h].tolist() == places + [-7] * (room - len(places)), (e, i, h)
+                rows = []
+                for j, p in enumerate(places):
+                    src = (e, table[i][p // PAGE], h, p % PAGE)
+                    key = k[src].double()
+                    rows.append((pb.turn(key, j - p, inv_freq, interleaved) if rotary and j != p else key, v[src].double() if v_dim else None, s[src]))
+                for j, (key, val, score) in enumerate(rows):
+                    dst = (e, out_table[i][j // PAGE], h, j % PAGE)
+                    want_k[dst], want_s[dst] = key, score
+                    turned[dst] = bool(rotary) and j != places[j]
+                    if v_dim:
+                        want_v[dst] = val
+    got_k = k_dev.cpu().double()
+    assert torch.equal(got_k[~turned], want_k[~turned])
+    if bool(turned.any()):
+        # float turn: the angle is off by 2^-23 of a turn's half at most, sine, cosine, two products and a sum by a rounding each
+        size = want_k[turned].abs().amax(-1, keepdim=True) * 1.5
+        assert bool(((got_k - want_k)[turned].abs() <= size * 16 * 2.0 ** -24 + _rounding(dtype) * want_k[turned].abs() * 1.01 + 1e-30).all())
+    if v_dim:
+        assert torch.equal(v_dev.cpu().double(), want_v)
+    assert torch.equal(torch.nan_to_num(s_dev.cpu(), nan=-1.0), torch.nan_to_num(want_s, nan=-1.0))
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("first,recent", [(0, 0), (4, 16), (3, 500), (200, 9)])
+def test_evict_ragged_sequences(cuda, in_place, first, recent):
+    _evict(cuda, [1, 63, 64, 65, 200, 450, 7], [1, 10, 64, 64, 77, 130, 0], first, recent, in_place=in_place, seed=first + recent)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("dtype,dim,v_dim,rotary,interleaved", [
+    (torch.bfloat16, 64, 64, 64, False), (torch.float32, 128, 128, 128, False), (torch.bfloat16, 96, 32, 32, True),
+    (torch.float32, 256, 256, 64, True), (torch.bfloat16, 80, 0, 80, False), (torch.bfloat16, 256, 256, 0, False)])
+def test_evict_turns_keys(cuda, in_place, dtype, dim, v_dim, rotary, interleaved):
+    _evict(cuda, [300, 129, 640], [200, 128, 65], 2, 20, dtype=dtype, entries=1, heads=1, dim=dim, v_dim=v_dim, rotary=rotary,
+           interleaved=interleaved, in_place=in_place, seed=dim)
+
+
+def test_evict_scores_that_are_equal_infinite_or_no_numbers(cuda):
+    def odd(entries, n_pages, heads):
+        gen = torch.Generator().manual_seed(1)
+        s = torch.randint(0, 3, (entries, n_pages, heads, PAGE), generator=gen).float()
+        pick = torch.randint(0, 8, s.shape, generator=gen)
+        for value, at in ((float("nan"), 0), (float("inf"), 1), (-float("inf"), 2), (-0.0, 3), (-3.4e38, 4)):
+            s[pick == at] = value
+        return s
+    for keeps in ([70, 100], [190, 5], [130, 250]):
+        _evict(cuda, [200, 300], keeps, 1, 3, scores=odd)
+    _evict(cuda, [200, 300], [64, 100], 0, 0, scores=lambda e, p, h: torch.full((e, p, h, PAGE), 2.5))
+
+
+def test_evict_keeps_no_more_than_there_is_room_for(cuda):
+    _evict(cuda, [300, 100], [200, 100], 2, 5, room=90)
+
+
+def test_evict_many_pages_in_place_by_few_units(cuda):
+    """Clusters of blocks that share a unit, over many rounds."""
+    for seed in range(3):
+        _evict(cuda, [6000], [5000 - 700 * seed], 4, 64, entries=1, heads=1, dim=16, v_dim=16, in_place=True, rotary=16, seed=seed)
+
+
+def test_evict_twice_and_one_entry(cuda):
+    """A cache without the axis of entries; a second eviction of what the first left."""
+    from camelid_b200.csrc import ops
+    gen = torch.Generator().manual_seed(0)
+    k, v = (torch.randn(6, 2, PAGE, 32, generator=gen).to(cuda) for _ in range(2))
+    s = torch.rand(6, 2, PAGE, generator=gen).to(cuda)
+    before = k.clone()
+    table = torch.tensor([[5, 0, 3, 1]], dtype=torch.int32, device=cuda)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)        # noqa: E731
+    first = torch.zeros(1, 2, 150, dtype=torch.int32, device=cuda)
+    second = torch.zeros(1, 2, 80, dtype=torch.int32, device=cuda)
+    ops.evict_positions(k, v, s, table, table, ints([250]), ints([150]), first, 2, 10)
+    ops.evict_positions(k, v, s, table, table, ints([150]), ints([80]), second, 2, 10)
+    for h in range(2):
+        for j in (0, 1, 2, 40, 79):
+            p = int(first[0, h, int(second[0, h, j])])
+            assert torch.equal(k[int(table[0, j // PAGE]), h, j % PAGE], before[int(table[0, p // PAGE]), h, p % PAGE])
+
+
+# ---- verification of drafts ---------------------------------------------------------------------------------------------
+def _verify(cuda, vocab, lens, temperature, with_probs, seed=0, room=None, pad=0, spread=3.0, logits=None, drafts=None, probs=None, **filters):
+    from camelid_b200.csrc import ops
+    gen = torch.Generator().manual_seed(seed)
+    n, room = len(lens), max(lens + [0]) if room is None else room
+    row0 = [sum(lens[:i]) + i for i in range(n)]
+    rows = sum(lens) + n
+    if logits is None:
+        logits = spread * torch.randn(rows, vocab, generator=gen)
+    if probs is None and with_probs:
+        probs = torch.zeros(n, room, vocab)
+    given = drafts is not None
+    if not given:
+        drafts = torch.zeros(n, room, dtype=torch.int32)
+    for i in range(n):
+        for j in range(0 if given else lens[i]):
+            row = logits[row0[i] + j]
+            q = torch.softmax((row + 0.7 * torch.randn(vocab, generator=gen)) / (temperature or 1.0), 0)
+            drafts[i, j] = int(torch.multinomial(q, 1, generator=gen)) if with_probs else int(row.argmax())
+            if with_probs:
+                probs[i, j] = q
+    accept, draw = torch.rand(n, room, generator=gen), torch.rand(n, generator=gen)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)        # noqa: E731
+    padded = torch.full((rows, vocab + pad), float("nan"))
+    padded[:, :vocab] = logits
+    counts = torch.full((n,), -9, dtype=torch.int32, device=cuda)
+    tokens = torch.full((n, room + 1), -9, dtype=torch.int32, device=cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    scratch = torch.full((ops.verify_bytes(rows, n, vocab),), 255, dtype=torch.uint8, device=cuda)
+    ops.verify_drafts(padded.to(cuda)[:, :vocab], ints(row0), ints(lens), drafts.to(cuda), probs.to(cuda) if with_probs else None,
+                      accept.to(cuda), draw.to(cuda), temperature, filters.get("top_k", 0), filters.get("top_p", 1.0),
+                      filters.get("min_p", 0.0), counts, tokens, err, scratch)
+    for i in range(n):
+        count, token = pb.verify(logits, row0[i], lens[i], drafts[i], probs[i] if with_probs else None, accept[i], draw[i], temperature,
+                                 **filters)
+        want = drafts[i, :count].tolist() + [token] + [-1] * (room - count)
+        assert int(counts[i]) == count and tokens[i].tolist() == want, (i, int(counts[i]), tokens[i].tolist(), count, token)
+    return counts, tokens, int(err)
+
+
+@pytest.mark.parametrize("with_probs", [True, False])
+@pytest.mark.parametrize("temperature", [0.0, 0.3, 1.0, 2.0])
+@pytest.mark.parametrize("vocab", [1, 5, 97, 1531, 8192, 8193, 50257])
+def test_verify_matches_plain(cuda, vocab, temperature, with_probs):
+    for seed in range(3):
+        assert _verify(cuda, vocab, [4, 0, 2, 7, 1], temperature, with_probs, seed=seed)[2] == 0
+
+
+@pytest.mark.parametrize("filters", [{"top_k": 1}, {"top_k": 40}, {"top_k": 1000}, {"top_p": 0.5}, {"top_p": 0.95, "min_p": 0.02},
+                                     {"min_p": 0.2}, {"top_k": 50, "top_p": 0.9, "min_p": 0.01}])
+@pytest.mark.parametrize("vocab", [97, 1531, 40000])
+def test_verify_with_the_samplers_filters(cuda, vocab, filters):
+    for with_probs in (True, False):
+        assert _verify(cuda, vocab, [3, 0, 5], 0.8, with_probs, seed=vocab, **filters)[2] == 0
+
+
+def test_verify_strided_rows(cuda):
+    for pad in (1, 3, 4):
+        _verify(cuda, 1000, [3, 2], 0.9, True, pad=pad, room=6)
+        _verify(cuda, 1001, [3, 2], 0.9, False, pad=pad, top_p=0.9)
+        _verify(cuda, 9001, [3, 2], 0.0, False, pad=pad)
+
+
+def test_verify_logits_at_the_types_lowest(cuda):
+    """Tokens that a mask of the lowest value excludes are never drawn, at any temperature."""
+    gen = torch.Generator().manual_seed(2)
+    for temperature in (0.1, 1.0, 0.0):
+        for filters in ({}, {"top_p": 0.9}, {"top_k": 20}):
+            logits = torch.randn(8, 3000, generator=gen)
+            logits[:, ::2] = torch.finfo(torch.float32).min
+            _, tokens, err = _verify(cuda, 3000, [3, 3], temperature, False, logits=logits, **filters)
+            assert err == 0 and all(t == -1 or t % 2 == 1 for t in tokens.flatten().tolist())
+
+
+def test_verify_equal_logits(cuda):
+    """Ties: the lowest id at temperature 0, the draw's share of the ids otherwise."""
+    logits = torch.zeros(2, 40000)
+    _, tokens, _ = _verify(cuda, 40000, [0, 0], 0.0, False, logits=logits, room=1)
+    assert tokens.tolist() == [[0, -1], [0, -1]]
+    _verify(cuda, 40000, [0, 0], 1.0, False, logits=logits, room=1, top_p=0.7001)
+    _verify(cuda, 40000, [0, 0], 1.0, False, logits=logits, room=1, top_k=12345)
+
+
+def test_verify_drafters_own_distribution_is_the_targets(cuda):
+    """q = p: every draft stays, and where the draw of a rejection would be from nothing, p is drawn from."""
+    gen = torch.Generator().manual_seed(4)
+    logits = torch.randn(5, 700, generator=gen)
+    probs = torch.softmax(logits[:4].double(), -1).float()[None] * 0.999
+    drafts = torch.multinomial(probs[0], 1, generator=gen).T.int()
+    counts, _, err = _verify(cuda, 700, [4], 1.0, True, logits=logits, drafts=drafts, probs=probs)
+    assert int(counts) == 4 and err == 0
+    over = probs * 3.0                          # no probabilities: more than p everywhere, a draft of which is rejected
+    _verify(cuda, 700, [4], 1.0, True, logits=logits, drafts=drafts, probs=over)
+
+
+def test_verify_reports_what_it_cannot_use(cuda):
+    gen = torch.Generator().manual_seed(8)
+    for value in (float("nan"), float("inf"), -float("inf")):
+        from camelid_b200.csrc import ops
+        for top_p in (1.0, 0.9):
+            logits = torch.randn(4, 9000, generator=gen)
+            logits[2, 8500] = value             # the second sequence's first row
+            ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)        # noqa: E731
+            counts, tokens, err = ints([-9, -9, -9]), ints([[-9, -9]] * 3), ints([0])
+            scratch = torch.empty(ops.verify_bytes(4, 3, 9000), dtype=torch.uint8, device=cuda)
+            ops.verify_drafts(logits.to(cuda), ints([0, 2, 3]), ints([1, 1, 1]), ints([[int(logits[0].argmax())], [9000], [4]]), None,
+                              torch.zeros(3, 1, device=cuda), torch.full((3,), 0.5, device=cuda), 1.0, 0, top_p, 0.0, counts, tokens, err,
+                              scratch)
+            assert counts.tolist() == [1, 0, 0] and tokens[1].tolist() == [0, -1]
+            assert tokens[2].tolist() == [-1, -1]          # rows 3 and 4: there is no row 4
+            assert int(err) == 1 | 4 | 8
+    drafts = torch.tensor([[-1, 3]], dtype=torch.int32)
+    counts, tokens, err = _verify(cuda, 500, [2], 1.0, False, drafts=drafts)
+    assert int(counts) == 0 and err == 4
+    probs = torch.full((1, 2, 500), -1.0)
+    counts, tokens, err = _verify(cuda, 500, [2], 1.0, True, drafts=torch.tensor([[1, 3]], dtype=torch.int32), probs=probs)
+    assert err == 4
+
+
+def test_verify_keeps_the_targets_distribution(cuda):
+    """Over many sequences with one draft each, the first token is distributed as the target's own."""
+    from camelid_b200.csrc import ops
+    n, vocab = 20000, 16
+    gen = torch.Generator().manual_seed(3)
+    p_logits, q = torch.randn(vocab, generator=gen), torch.softmax(torch.randn(vocab, generator=gen), 0)
+    drafts = torch.multinomial(q, n, replacement=True, generator=gen).int()[:, None]
+    ints = lambda x: x.to(torch.int32).to(cuda)        # noqa: E731
+    counts, tokens = torch.zeros(n, dtype=torch.int32, device=cuda), torch.zeros(n, 2, dtype=torch.int32, device=cuda)
+    err = torch.zeros(1, dtype=torch.int32, device=cuda)
+    scratch = torch.empty(ops.verify_bytes(2 * n, n, vocab), dtype=torch.uint8, device=cuda)
+    ops.verify_drafts(p_logits.expand(2 * n, vocab).contiguous().to(cuda), ints(torch.arange(n) * 2), ints(torch.ones(n)), drafts.to(cuda),
+                      q.expand(n, 1, vocab).contiguous().to(cuda), torch.rand(n, 1, generator=gen).to(cuda), torch.rand(n, generator=gen).to(cuda),
+                      1.0, 0, 1.0, 0.0, counts, tokens, err, scratch)
+    share = torch.bincount(tokens[:, 0].cpu().long(), minlength=vocab).double() / n
+    p = torch.softmax(p_logits.double(), 0)
+    assert bool(((share - p).abs() <= 5 * torch.sqrt(p * (1 - p) / n)).all())       # five standard deviations
