@@ -33,12 +33,13 @@ struct WeightArgs {
     const int* fresh;            // new tokens of each sequence
     int n_seqs, n_rows, heads, kv_heads, k_dim, v_dim;
     int max_new, max_len;
-    float scale;
+    float scale;                 // of the scores, times log2(e): the softmax is taken in powers of two
     int stages;                  // pages of keys and values a block of (1) keeps in shared memory: 2, or 1 where two do not fit
     int split_keys, n_splits;    // keys of a stretch (a multiple of the page), stretches of the longest sequence
     float* stats;                // [seqs * kv heads][splits][rows][2]: maximum and sum of a stretch
     float* joined;               // [seqs * kv heads][rows][2]: maximum and 1 / sum of all
     float* acc;                  // [seqs * kv heads][splits][rows][v_dim]
+    float* kept;                 // [seqs * kv heads][rows][splits * split_keys]: q . k, scaled, of steps of few rows
 };
 
 struct Seq {
@@ -177,8 +178,8 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
             const int m = warp * 2 + mm;
             const float a0 = p_s[m * CML_PAGE + lane], a1 = p_s[m * CML_PAGE + lane + 32];
             const float old = m_s[m], now = fmaxf(old, warp_max(fmaxf(a0, a1)));
-            const float e0 = a0 == -CUDART_INF_F ? 0.f : expf(a0 - now), e1 = a1 == -CUDART_INF_F ? 0.f : expf(a1 - now);
-            const float corr = old == -CUDART_INF_F ? 0.f : expf(old - now);
+            const float e0 = a0 == -CUDART_INF_F ? 0.f : exp2f(a0 - now), e1 = a1 == -CUDART_INF_F ? 0.f : exp2f(a1 - now);
+            const float corr = old == -CUDART_INF_F ? 0.f : exp2f(old - now);
             const float sum = warp_sum(e0 + e1);
             p_s[m * CML_PAGE + lane] = e0;
             p_s[m * CML_PAGE + lane + 32] = e1;
@@ -244,12 +245,12 @@ __global__ void __launch_bounds__(AW_THREADS) weights_join_kernel(WeightArgs a) 
     for (int i = 0; i < splits; ++i) top = fmaxf(top, a.stats[(base + (size_t)i * group_rows) * 2]);
     for (int i = 0; i < splits; ++i) {
         const float t = a.stats[(base + (size_t)i * group_rows) * 2];
-        if (t != -CUDART_INF_F) sum += expf(t - top) * a.stats[(base + (size_t)i * group_rows) * 2 + 1];
+        if (t != -CUDART_INF_F) sum += exp2f(t - top) * a.stats[(base + (size_t)i * group_rows) * 2 + 1];
     }
     const float inv = top == -CUDART_INF_F ? 0.f : 1.f / sum;
     if (threadIdx.x == 0) {
         float* j = a.joined + ((size_t)blockIdx.y * group_rows + m) * 2;
-        j[0] = top;
+        j[0] = top == -CUDART_INF_F ? 0.f : top;
         j[1] = inv;
     }
     if (a.out == nullptr) return;
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(AW_THREADS) weights_join_kernel(WeightArgs a) 
         float x = 0.f;
         for (int i = 0; i < splits; ++i) {
             const float t = a.stats[(base + (size_t)i * group_rows) * 2];
-            if (t != -CUDART_INF_F) x += expf(t - top) * a.acc[(base + (size_t)i * group_rows) * a.v_dim + d];
+            if (t != -CUDART_INF_F) x += exp2f(t - top) * a.acc[(base + (size_t)i * group_rows) * a.v_dim + d];
         }
         out[d] = from_f32<T>(x * inv);
     }
@@ -297,7 +298,7 @@ __global__ void __launch_bounds__(AW_THREADS) weights_sum_kernel(WeightArgs a) {
             const int r = m0 + half * 4 + m;
             if (r >= s.rows || sc[m] == -CUDART_INF_F) continue;
             const float* j = a.joined + ((size_t)blockIdx.y * group_rows + r) * 2;
-            gained += expf(sc[m] - j[0]) * j[1];
+            gained += exp2f(sc[m] - j[0]) * j[1];
         }
     }
     if (half == 1) other[key] = gained;
@@ -305,6 +306,361 @@ __global__ void __launch_bounds__(AW_THREADS) weights_sum_kernel(WeightArgs a) {
     if (half == 0 && key < valid) {
         const int place = p * CML_PAGE + key;
         a.scores_out[at + key] = (place < s.start ? a.scores[at + key] : 0.f) + (gained + other[key]);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// bfloat16 with head sizes 64 and 128 on the tensor cores (mma.sync m16n8k16: what bounds these kernels is memory, or the
+// exponentials of many rows, not the products). Shared-memory rows are padded by 16 bytes, so ldmatrix meets no bank twice.
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ float fast_exp2(float x) {            // 2^x to 2^-22 of itself; 0 for -inf
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool there) {
+    const int n = there ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
+#define AM_WARPS 4
+#define AM_STAGES 3
+
+// (1) a stretch of keys for up to 16 * MT rows of a (sequence, kv head); grid (stretches, pairs, row chunks). A warp takes every
+// fourth tile of TILE keys with a ring of its own in shared memory, and the warps' ranges are joined at the end in
+// their order. OUT: with values and output. KEEP: the scaled products are kept for (3).
+template <int HD, int MT, bool OUT, bool KEEP>
+__global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightArgs a) {
+    constexpr int TILE = HD == 128 ? 16 : 32;
+    constexpr int LDS = HD + 8, KS = HD / 16, DT = HD / 8, NT = TILE / 8, KK = TILE / 16, CH = HD / 8;
+    constexpr int HALF = TILE * LDS * 2, STAGE = HALF * (OUT ? 2 : 1);        // bytes
+    extern __shared__ __align__(16) unsigned char raw[];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int split = blockIdx.x, seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads, m0 = blockIdx.z * 16 * MT;
+    const Seq s = seq_of(a, seq);
+    const int first = split * a.split_keys, last = min(s.length, first + a.split_keys);
+    if (first >= last || m0 >= s.rows) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group = a.heads / a.kv_heads;
+    const int* pages = a.table + (size_t)seq * a.width;
+    const bf16* kp = (const bf16*)a.k;
+    const bf16* vp = (const bf16*)a.v;
+    unsigned char* mine = raw + (size_t)warp * AM_STAGES * STAGE;
+    const uint32_t mine32 = (uint32_t)__cvta_generic_to_shared(mine);
+    const int t_first = first / TILE, t_last = (last + TILE - 1) / TILE;
+    const int n_mine = (t_last - t_first - warp + AM_WARPS - 1) / AM_WARPS;
+    auto page_of = [&](int t) { return pages[t * TILE / CML_PAGE]; };
+    auto there = [&](int page) { return page >= 0 && page < a.n_pages; };
+    int page_next = 0 < n_mine ? page_of(t_first + warp) : -1;               // a tile's page is looked up a tile ahead
+    auto issue = [&](int it) {
+        if (it < n_mine) {
+            const int t = t_first + warp + it * AM_WARPS;
+            const int page = page_next;
+            if (it + 1 < n_mine) page_next = page_of(t + AM_WARPS);
+            const bool ok = there(page);
+            const size_t base = (((size_t)(ok ? page : 0) * a.kv_heads + kvh) * CML_PAGE + (t * TILE) % CML_PAGE) * HD;
+            const uint32_t dst = mine32 + (uint32_t)(it % AM_STAGES) * STAGE;
+            const int valid = ok ? last - t * TILE : 0;
+#pragma unroll
+            for (int c0 = 0; c0 < TILE * CH; c0 += 32) {
+                const int c = c0 + lane, r = c / CH, cc = c % CH;
+                cp_async16_or_zero(dst + (uint32_t)(r * LDS + cc * 8) * 2, kp + base + (size_t)r * HD + cc * 8, r < valid);
+                if (OUT) cp_async16_or_zero(dst + HALF + (uint32_t)(r * LDS + cc * 8) * 2, vp + base + (size_t)r * HD + cc * 8, r < valid);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < AM_STAGES - 1; ++i) issue(i);
+    // the rows of q as A fragments (zero where there is no row); a thread holds rows lane / 4 and + 8 of each 16
+    uint32_t qa[MT][KS][4];
+    int pos[MT][2];                                                           // the last place a row sees, -1: no row
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int m = m0 + mt * 16 + (lane >> 2) + 8 * h;
+            const bool in = m < s.rows;
+            const int j = in ? m / group : 0;
+            pos[mt][h] = in ? s.start + j : -1;
+            const bf16* qr = (const bf16*)a.q + (long long)(s.row0 + j) * a.q_stride + (long long)(kvh * group + (in ? m % group : 0)) * HD + 2 * (lane & 3);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                qa[mt][ks][h] = in ? *reinterpret_cast<const uint32_t*>(qr + ks * 16) : 0u;
+                qa[mt][ks][h + 2] = in ? *reinterpret_cast<const uint32_t*>(qr + ks * 16 + 8) : 0u;
+            }
+        }
+    float top[MT][2], sum[MT][2];
+    float o[MT][OUT ? DT : 1][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        top[mt][0] = top[mt][1] = -CUDART_INF_F;
+        sum[mt][0] = sum[mt][1] = 0.f;
+#pragma unroll
+        for (int d = 0; d < (OUT ? DT : 1); ++d) o[mt][d][0] = o[mt][d][1] = o[mt][d][2] = o[mt][d][3] = 0.f;
+    }
+    const int mat = lane >> 3, rr = lane & 7;
+    const int group_rows = a.max_new * group;
+    float* const kept = KEEP ? a.kept + (size_t)blockIdx.y * group_rows * a.n_splits * a.split_keys : nullptr;
+    for (int it = 0; it < n_mine; ++it) {
+        const int t = t_first + warp + it * AM_WARPS;
+        cp_async_wait<AM_STAGES - 2>();
+        __syncwarp();
+        const bool ok = there(page_of(t));
+        issue(it + AM_STAGES - 1);
+        const uint32_t k32 = mine32 + (uint32_t)(it % AM_STAGES) * STAGE, v32 = k32 + HALF;
+        const int place0 = t * TILE;
+        float x[MT][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) x[mt][n][0] = x[mt][n][1] = x[mt][n][2] = x[mt][n][3] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int np = 0; np < NT / 2; ++np) {
+                uint32_t b0, b1, b2, b3;
+                ldsm_x4(k32 + (uint32_t)((np * 16 + (mat >> 1) * 8 + rr) * LDS + ks * 16 + (mat & 1) * 8) * 2, b0, b1, b2, b3);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    mma_bf16(x[mt][np * 2], qa[mt][ks], b0, b1);
+                    mma_bf16(x[mt][np * 2 + 1], qa[mt][ks], b2, b3);
+                }
+            }
+        // scale, mask, running maximum
+        const int key0 = place0 + 2 * (lane & 3);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            float now[2] = {top[mt][0], top[mt][1]};
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = key0 + n * 8 + (i & 1);
+                    x[mt][n][i] = ok && key < last && key <= pos[mt][i >> 1] ? x[mt][n][i] * a.scale : -CUDART_INF_F;
+                    now[i >> 1] = fmaxf(now[i >> 1], x[mt][n][i]);
+                }
+            if (KEEP) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (pos[mt][h] >= 0) {
+                        float* row = kept + (size_t)(m0 + mt * 16 + (lane >> 2) + 8 * h) * a.n_splits * a.split_keys + key0;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(row + n * 8) = make_float2(x[mt][n][2 * h], x[mt][n][2 * h + 1]);
+                    }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                now[h] = fmaxf(now[h], __shfl_xor_sync(0xffffffffu, now[h], 1));
+                now[h] = fmaxf(now[h], __shfl_xor_sync(0xffffffffu, now[h], 2));
+            }
+            if (__any_sync(0xffffffffu, now[0] != top[mt][0] || now[1] != top[mt][1])) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float corr = top[mt][h] == -CUDART_INF_F ? 0.f : fast_exp2(top[mt][h] - now[h]);
+                    top[mt][h] = now[h];
+                    sum[mt][h] *= corr;
+#pragma unroll
+                    for (int d = 0; d < (OUT ? DT : 1); ++d) o[mt][d][2 * h] *= corr, o[mt][d][2 * h + 1] *= corr;
+                }
+            }
+            const float ref[2] = {top[mt][0] == -CUDART_INF_F ? 0.f : top[mt][0], top[mt][1] == -CUDART_INF_F ? 0.f : top[mt][1]};
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[mt][n][i] = fast_exp2(x[mt][n][i] - ref[i >> 1]);
+                    sum[mt][i >> 1] += x[mt][n][i];
+                }
+        }
+        if (OUT) {
+            bf16* vs = reinterpret_cast<bf16*>(mine + (size_t)(it % AM_STAGES) * STAGE + HALF);
+            if (s.fresh > 1 && place0 + TILE > s.start + 1) {
+                // New places that not every row sees: a probability of zero times what such a place holds must stay zero even
+                // where that is infinite, so their products are made apart, and the tensor cores get zeros.
+#pragma unroll
+                for (int kk = 0; kk < TILE; ++kk) {
+                    const int place = place0 + kk;
+                    if (place <= s.start || place >= last) continue;          // the same in the whole warp
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float p = __shfl_sync(0xffffffffu, x[mt][kk / 8][2 * h + (kk & 1)], (lane & ~3) | ((kk & 7) >> 1));
+                            if (p != 0.f) {
+#pragma unroll
+                                for (int d = 0; d < DT; ++d) {
+                                    o[mt][d][2 * h] += p * to_f32(vs[kk * LDS + d * 8 + 2 * (lane & 3)]);
+                                    o[mt][d][2 * h + 1] += p * to_f32(vs[kk * LDS + d * 8 + 2 * (lane & 3) + 1]);
+                                }
+                            }
+                        }
+                }
+                __syncwarp();
+                const int from = max(0, s.start + 1 - place0);
+                for (int c = lane; c < (TILE - from) * CH; c += 32)
+                    *reinterpret_cast<uint4*>(vs + (from + c / CH) * LDS + (c % CH) * 8) = make_uint4(0, 0, 0, 0);
+                __syncwarp();
+            }
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+                uint32_t pa[MT][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    pa[mt][0] = pack_bf16(x[mt][2 * kk][0], x[mt][2 * kk][1]);
+                    pa[mt][1] = pack_bf16(x[mt][2 * kk][2], x[mt][2 * kk][3]);
+                    pa[mt][2] = pack_bf16(x[mt][2 * kk + 1][0], x[mt][2 * kk + 1][1]);
+                    pa[mt][3] = pack_bf16(x[mt][2 * kk + 1][2], x[mt][2 * kk + 1][3]);
+                }
+#pragma unroll
+                for (int dp = 0; dp < DT / 2; ++dp) {
+                    uint32_t b0, b1, b2, b3;
+                    ldsm_x4_t(v32 + (uint32_t)((kk * 16 + (mat & 1) * 8 + rr) * LDS + dp * 16 + (mat >> 1) * 8) * 2, b0, b1, b2, b3);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        mma_bf16(o[mt][dp * 2], pa[mt], b0, b1);
+                        mma_bf16(o[mt][dp * 2 + 1], pa[mt], b2, b3);
+                    }
+                }
+            }
+        }
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            sum[mt][h] += __shfl_xor_sync(0xffffffffu, sum[mt][h], 1);
+            sum[mt][h] += __shfl_xor_sync(0xffffffffu, sum[mt][h], 2);
+        }
+    __syncthreads();                                                          // every warp is done with its ring
+    // the warps' ranges: [warp][16 * MT rows][maximum, sum, output]
+    constexpr int RW = OUT ? HD + 4 : 4;
+    float* red = reinterpret_cast<float*>(raw);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float* dst = red + ((size_t)warp * 16 * MT + mt * 16 + (lane >> 2) + 8 * h) * RW;
+            if ((lane & 3) == 0) dst[0] = top[mt][h], dst[1] = sum[mt][h];
+            if (OUT) {
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    dst[4 + d * 8 + 2 * (lane & 3)] = o[mt][d][2 * h];
+                    dst[4 + d * 8 + 2 * (lane & 3) + 1] = o[mt][d][2 * h + 1];
+                }
+            }
+        }
+    __syncthreads();
+    const size_t base = ((size_t)blockIdx.y * a.n_splits + split) * group_rows + m0;
+    const int rows = min(16 * MT, s.rows - m0);
+    constexpr int PER = OUT ? HD / 4 : 1;
+    for (int i = threadIdx.x; i < rows * PER; i += AM_WARPS * 32) {
+        const int m = i / PER, d = i % PER * 4;
+        float most = -CUDART_INF_F, f[AM_WARPS], l = 0.f;
+#pragma unroll
+        for (int w = 0; w < AM_WARPS; ++w) most = fmaxf(most, red[((size_t)w * 16 * MT + m) * RW]);
+#pragma unroll
+        for (int w = 0; w < AM_WARPS; ++w) {
+            const float* src = red + ((size_t)w * 16 * MT + m) * RW;
+            f[w] = src[0] == -CUDART_INF_F ? 0.f : fast_exp2(src[0] - most);
+            l += f[w] * src[1];
+        }
+        if (OUT) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < AM_WARPS; ++w) {
+                const float4 t = *reinterpret_cast<const float4*>(red + ((size_t)w * 16 * MT + m) * RW + 4 + d);
+                v.x += f[w] * t.x; v.y += f[w] * t.y; v.z += f[w] * t.z; v.w += f[w] * t.w;
+            }
+            *reinterpret_cast<float4*>(a.acc + (base + m) * HD + d) = v;
+        }
+        if (d == 0) {
+            a.stats[(base + m) * 2] = most;
+            a.stats[(base + m) * 2 + 1] = l;
+        }
+    }
+}
+
+// (2 and 3) of steps whose products are kept: the first blocks of a pair sum the weights of 256 keys each, the others join
+// the output of a row each. Grid (key blocks + rows, pairs).
+#define AK_THREADS 256
+#define AK_ROWS 16
+template <typename T, int HD>
+__global__ void __launch_bounds__(AK_THREADS) weights_finish_kernel(WeightArgs a, int key_blocks) {
+    __shared__ float top_s[AK_ROWS], inv_s[AK_ROWS];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
+    const Seq s = seq_of(a, seq);
+    const int group = a.heads / a.kv_heads, group_rows = a.max_new * group;
+    const int splits = (s.length + a.split_keys - 1) / a.split_keys;
+    const size_t base = (size_t)blockIdx.y * a.n_splits * group_rows;
+    const bool keys = (int)blockIdx.x < key_blocks;
+    const int key0 = blockIdx.x * AK_THREADS, row = (int)blockIdx.x - key_blocks;
+    if (keys ? key0 >= s.length : row >= s.rows) return;
+    // a warp joins a row's stretches: lanes take every 32nd, then a tree over the lanes
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int m = keys ? warp : row; m < (keys ? s.rows : row + 1); m += AK_THREADS / 32) {
+        float top = -CUDART_INF_F, sum = 0.f;
+        for (int i = lane; i < splits; i += 32) {
+            const float2 t = *reinterpret_cast<const float2*>(a.stats + (base + (size_t)i * group_rows + m) * 2);
+            const float now = fmaxf(top, t.x);
+            if (now != -CUDART_INF_F) sum = sum * exp2f(top - now) + exp2f(t.x - now) * t.y;
+            top = now;
+        }
+        const float most = warp_max(top);
+        sum = most == -CUDART_INF_F ? 0.f : warp_sum(sum * exp2f(top - most));
+        if (lane == 0) {
+            top_s[m & (AK_ROWS - 1)] = most == -CUDART_INF_F ? 0.f : most;
+            inv_s[m & (AK_ROWS - 1)] = most == -CUDART_INF_F ? 0.f : 1.f / sum;
+        }
+        if (!keys) break;
+    }
+    __syncthreads();
+    if (keys) {
+        const int place = key0 + threadIdx.x;
+        if (place >= s.length) return;
+        const int page = a.table[(size_t)seq * a.width + place / CML_PAGE];
+        if (page < 0 || page >= a.n_pages) return;
+        const size_t at = ((size_t)page * a.kv_heads + kvh) * CML_PAGE + place % CML_PAGE;
+        const float old = place < s.start ? a.scores[at] : 0.f;
+        const size_t stride = (size_t)a.n_splits * a.split_keys;
+        const float* x = a.kept + (size_t)blockIdx.y * group_rows * stride + place;
+        float gained = 0.f;
+#pragma unroll 4
+        for (int m = 0; m < s.rows; ++m) gained += fast_exp2(x[m * stride] - top_s[m]) * inv_s[m];
+        a.scores_out[at] = old + gained;
+    } else {
+        const float top = top_s[row & (AK_ROWS - 1)], inv = inv_s[row & (AK_ROWS - 1)];
+        T* out = (T*)a.out + (long long)(s.row0 + row / group) * a.out_stride + (long long)(kvh * group + row % group) * HD;
+        for (int d = threadIdx.x; d < HD; d += AK_THREADS) {
+            float x = 0.f;
+            for (int i = 0; i < splits; ++i) {
+                const float t = a.stats[(base + (size_t)i * group_rows + row) * 2];
+                x += fast_exp2(t - top) * a.acc[(base + (size_t)i * group_rows + row) * HD + d];
+            }
+            out[d] = from_f32<T>(x * inv);
+        }
     }
 }
 
@@ -328,6 +684,344 @@ static cudaError_t launch_plain(WeightArgs& a, cudaStream_t s) {
     return launch_pdl(weights_sum_kernel<T>, dim3((unsigned)((a.max_len + CML_PAGE - 1) / CML_PAGE), pairs), dim3(AW_THREADS), smem3, s, a);
 }
 
+// (1) without output, for many rows (a prompt's last ones): a warp keeps 64 rows of q in registers and lets the keys pass;
+// grid (stretches, pairs, row chunks). The block's warps share the rows (`row_warps` of them) and the 16-key pieces of
+// a page. A thread keeps a maximum and a sum of its own for each of its eight rows, the maximum moves only when it is passed
+// by a factor of 2^6, and lanes and warps meet at the end. The exponentials (one a row and key) bound this kernel.
+#define AR_STAGES 4
+template <int HD>
+__global__ void __launch_bounds__(AM_WARPS * 32, 2) weights_rows_mma_kernel(WeightArgs a, int row_warps) {
+    constexpr int LDS = HD + 8, KS = HD / 16, CH = HD / 8, STAGE = CML_PAGE * LDS * 2;
+    extern __shared__ __align__(16) unsigned char raw[];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = blockIdx.x, seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
+    const int m0 = ((int)blockIdx.z * row_warps + warp % row_warps) * 64, key_group = warp / row_warps, key_groups = AM_WARPS / row_warps;
+    const Seq s = seq_of(a, seq);
+    const int first = split * a.split_keys, last = min(s.length, first + a.split_keys);
+    if (first >= last || (int)blockIdx.z * row_warps * 64 >= s.rows) return;
+    const int group = a.heads / a.kv_heads, group_rows = a.max_new * group;
+    const int* pages = a.table + (size_t)seq * a.width;
+    const uint32_t raw32 = (uint32_t)__cvta_generic_to_shared(raw);
+    const int p_first = first / CML_PAGE, p_last = (last + CML_PAGE - 1) / CML_PAGE;
+    auto valid_of = [&](int p) {
+        const int page = pages[p];
+        return page < 0 || page >= a.n_pages ? 0 : min(CML_PAGE, last - p * CML_PAGE);
+    };
+    auto issue = [&](int p) {
+        if (p < p_last) {
+            const int valid = valid_of(p);
+            const bf16* src = (const bf16*)a.k + ((size_t)(valid ? pages[p] : 0) * a.kv_heads + kvh) * CML_PAGE * HD;
+            const uint32_t dst = raw32 + (uint32_t)((p - p_first) % AR_STAGES) * STAGE;
+#pragma unroll
+            for (int c0 = 0; c0 < CML_PAGE * CH; c0 += AM_WARPS * 32) {
+                const int c = c0 + threadIdx.x, r = c / CH, cc = c % CH;
+                cp_async16_or_zero(dst + (uint32_t)(r * LDS + cc * 8) * 2, src + (size_t)r * HD + cc * 8, r < valid);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < AR_STAGES - 1; ++i) issue(p_first + i);
+    uint32_t qa[4][KS][4];
+    int pos[4][2];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int m = m0 + mt * 16 + (lane >> 2) + 8 * h;
+            const bool in = m < s.rows;
+            const int j = in ? m / group : 0;
+            pos[mt][h] = in ? s.start + j : -1;
+            const bf16* qr = (const bf16*)a.q + (long long)(s.row0 + j) * a.q_stride + (long long)(kvh * group + (in ? m % group : 0)) * HD + 2 * (lane & 3);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                qa[mt][ks][h] = in ? *reinterpret_cast<const uint32_t*>(qr + ks * 16) : 0u;
+                qa[mt][ks][h + 2] = in ? *reinterpret_cast<const uint32_t*>(qr + ks * 16 + 8) : 0u;
+            }
+        }
+    float top[4][2], sum[4][2];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) top[mt][0] = top[mt][1] = -CUDART_INF_F, sum[mt][0] = sum[mt][1] = 0.f;
+    const int mat = lane >> 3, rr = lane & 7;
+    const bool any_rows = m0 < s.rows;
+    for (int p = p_first; p < p_last; ++p) {
+        cp_async_wait<AR_STAGES - 2>();
+        __syncthreads();
+        issue(p + AR_STAGES - 1);
+        if (!any_rows) continue;
+        const int valid = valid_of(p);
+        const uint32_t k32 = raw32 + (uint32_t)((p - p_first) % AR_STAGES) * STAGE;
+        const bool whole = valid == CML_PAGE && p * CML_PAGE + CML_PAGE - 1 <= s.start;      // every row sees every key
+        for (int c = key_group; c < CML_PAGE / 16; c += key_groups) {
+            float x[4][2][4];
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) x[mt][n][0] = x[mt][n][1] = x[mt][n][2] = x[mt][n][3] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                uint32_t b0, b1, b2, b3;
+                ldsm_x4(k32 + (uint32_t)((c * 16 + (mat >> 1) * 8 + rr) * LDS + ks * 16 + (mat & 1) * 8) * 2, b0, b1, b2, b3);
+#pragma unroll
+                for (int mt = 0; mt < 4; ++mt) {
+                    mma_bf16(x[mt][0], qa[mt][ks], b0, b1);
+                    mma_bf16(x[mt][1], qa[mt][ks], b2, b3);
+                }
+            }
+            if (!whole) {
+                const int at = c * 16 + 2 * (lane & 3);
+#pragma unroll
+                for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int key = at + n * 8 + (i & 1);
+                            if (!(key < valid && p * CML_PAGE + key <= pos[mt][i >> 1])) x[mt][n][i] = -CUDART_INF_F;
+                        }
+            }
+            bool passed = false;
+            float now[4][2];
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float hi = fmaxf(fmaxf(x[mt][0][2 * h], x[mt][0][2 * h + 1]), fmaxf(x[mt][1][2 * h], x[mt][1][2 * h + 1]));
+                    now[mt][h] = hi * a.scale;
+                    passed = passed || now[mt][h] > top[mt][h] + 6.f;
+                }
+            if (__any_sync(0xffffffffu, passed)) {
+#pragma unroll
+                for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float next = fmaxf(top[mt][h], now[mt][h]);
+                        if (next != -CUDART_INF_F) sum[mt][h] *= fast_exp2(top[mt][h] - next);
+                        top[mt][h] = next;
+                    }
+            }
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float ref = top[mt][h] == -CUDART_INF_F ? 0.f : top[mt][h];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) sum[mt][h] += fast_exp2(fmaf(x[mt][n][2 * h + i], a.scale, -ref));
+                }
+        }
+    }
+    cp_async_wait<0>();
+    __syncthreads();                                                          // the ring is free: the warps' results take its place
+    float2* red = reinterpret_cast<float2*>(raw);                             // [warps][64 rows]
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float t = top[mt][h], l = sum[mt][h];
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                const float t2 = __shfl_xor_sync(0xffffffffu, t, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+                const float most = fmaxf(t, t2);
+                if (most != -CUDART_INF_F) l = l * fast_exp2(t - most) + l2 * fast_exp2(t2 - most);
+                t = most;
+            }
+            if ((lane & 3) == 0) red[warp * 64 + mt * 16 + (lane >> 2) + 8 * h] = make_float2(t, l);
+        }
+    __syncthreads();
+    const size_t base = ((size_t)blockIdx.y * a.n_splits + split) * group_rows;
+    for (int i = threadIdx.x; i < row_warps * 64; i += AM_WARPS * 32) {
+        const int m = (int)blockIdx.z * row_warps * 64 + i;
+        if (m >= s.rows) break;
+        float t = -CUDART_INF_F, l = 0.f;
+        for (int w = 0; w < key_groups; ++w) t = fmaxf(t, red[(w * row_warps + i / 64) * 64 + i % 64].x);
+        for (int w = 0; w < key_groups; ++w) {
+            const float2 one = red[(w * row_warps + i / 64) * 64 + i % 64];
+            if (one.x != -CUDART_INF_F) l += fast_exp2(one.x - t) * one.y;
+        }
+        *reinterpret_cast<float2*>(a.stats + (base + m) * 2) = make_float2(t, l);
+    }
+}
+
+// (3) for more than 16 rows: a warp keeps 64 keys in registers as the operand of 16 rows and lets the rows of q pass, so that a
+// key's sum over the rows stays in one quad of lanes, in the order of the rows. Grid (256 keys, pairs).
+#define AC_ROWS 32              // rows of q in a stage
+#define AC_STAGES 4
+template <int HD>
+__global__ void __launch_bounds__(AM_WARPS * 32, 2) weights_keys_mma_kernel(WeightArgs a) {
+    constexpr int LDS = HD + 8, KS = HD / 16, CH = HD / 8, KEYS = AM_WARPS * 64;
+    constexpr int QSTAGE = AC_ROWS * LDS * 2 + AC_ROWS * 16;                  // rows, then (maximum, 1 / sum, last place) of each
+    extern __shared__ __align__(16) unsigned char raw[];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads, key0 = blockIdx.x * KEYS;
+    const Seq s = seq_of(a, seq);
+    if (key0 >= s.length) return;
+    const int group = a.heads / a.kv_heads, group_rows = a.max_new * group;
+    const int* pages = a.table + (size_t)seq * a.width;
+    const uint32_t raw32 = (uint32_t)__cvta_generic_to_shared(raw);
+    // this warp's page of keys
+    const int place0 = key0 + warp * 64;
+    int page = place0 < s.length ? pages[place0 / CML_PAGE] : -1;
+    if (page >= a.n_pages) page = -1;
+    const int valid = page < 0 ? 0 : min(64, s.length - place0);
+    {
+        const bf16* src = (const bf16*)a.k + ((size_t)max(page, 0) * a.kv_heads + kvh) * CML_PAGE * HD;
+        const uint32_t dst = raw32 + (uint32_t)(warp * 64 * LDS) * 2;
+#pragma unroll
+        for (int c0 = 0; c0 < 64 * CH; c0 += 32) {
+            const int c = c0 + lane, r = c / CH, cc = c % CH;
+            cp_async16_or_zero(dst + (uint32_t)(r * LDS + cc * 8) * 2, src + (size_t)r * HD + cc * 8, r < valid);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        __syncwarp();
+    }
+    const int mat = lane >> 3, rr = lane & 7;
+    uint32_t ka[4][KS][4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+            ldsm_x4(raw32 + (uint32_t)((warp * 64 + mt * 16 + (mat & 1) * 8 + rr) * LDS + ks * 16 + (mat >> 1) * 8) * 2, ka[mt][ks][0], ka[mt][ks][1],
+                    ka[mt][ks][2], ka[mt][ks][3]);
+    __syncthreads();                                                          // the keys are in registers: their room holds the rows of q now
+    const int chunks = (s.rows + AC_ROWS - 1) / AC_ROWS;
+    auto issue = [&](int c) {
+        if (c < chunks) {
+            unsigned char* st = raw + (size_t)(c % AC_STAGES) * QSTAGE;
+            const uint32_t dst = raw32 + (uint32_t)(c % AC_STAGES) * QSTAGE;
+#pragma unroll
+            for (int c0 = 0; c0 < AC_ROWS * CH; c0 += AM_WARPS * 32) {
+                const int i = c0 + threadIdx.x, r = i / CH, cc = i % CH, m = c * AC_ROWS + r;
+                const bool in = m < s.rows;
+                const bf16* src = (const bf16*)a.q + (long long)(s.row0 + (in ? m / group : 0)) * a.q_stride + (long long)(kvh * group + (in ? m % group : 0)) * HD + cc * 8;
+                cp_async16_or_zero(dst + (uint32_t)(r * LDS + cc * 8) * 2, src, in);
+            }
+            if (threadIdx.x < AC_ROWS) {
+                const int m = c * AC_ROWS + threadIdx.x;
+                float2 j = make_float2(0.f, 0.f);
+                if (m < s.rows) j = *reinterpret_cast<const float2*>(a.joined + ((size_t)blockIdx.y * group_rows + m) * 2);
+                float4* tail = reinterpret_cast<float4*>(st + AC_ROWS * LDS * 2);
+                tail[threadIdx.x] = make_float4(j.x, j.y, __int_as_float(m < s.rows ? s.start + m / group : -1), 0.f);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < AC_STAGES - 1; ++i) issue(i);
+    float gained[4][2];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) gained[mt][0] = gained[mt][1] = 0.f;
+    const bool whole = place0 + 63 <= s.start;                                // every row sees every key of this warp
+    for (int c = 0; c < chunks; ++c) {
+        cp_async_wait<AC_STAGES - 2>();
+        __syncthreads();
+        issue(c + AC_STAGES - 1);
+        if (valid == 0) continue;
+        const uint32_t q32 = raw32 + (uint32_t)(c % AC_STAGES) * QSTAGE;
+        const float4* tail = reinterpret_cast<const float4*>(raw + (size_t)(c % AC_STAGES) * QSTAGE + AC_ROWS * LDS * 2);
+#pragma unroll 1
+        for (int half = 0; half < AC_ROWS / 16; ++half) {
+            float x[4][2][4];
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) x[mt][n][0] = x[mt][n][1] = x[mt][n][2] = x[mt][n][3] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                uint32_t b0, b1, b2, b3;
+                ldsm_x4(q32 + (uint32_t)((half * 16 + (mat >> 1) * 8 + rr) * LDS + ks * 16 + (mat & 1) * 8) * 2, b0, b1, b2, b3);
+#pragma unroll
+                for (int mt = 0; mt < 4; ++mt) {
+                    mma_bf16(x[mt][0], ka[mt][ks], b0, b1);
+                    mma_bf16(x[mt][1], ka[mt][ks], b2, b3);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float4 row = tail[half * 16 + n * 8 + 2 * (lane & 3) + i];
+                    if (whole) {
+#pragma unroll
+                        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) gained[mt][h] = fmaf(fast_exp2(fmaf(x[mt][n][2 * h + i], a.scale, -row.x)), row.y, gained[mt][h]);
+                    } else {
+                        const int sees = __float_as_int(row.z) - place0;
+#pragma unroll
+                        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                if (mt * 16 + (lane >> 2) + 8 * h <= sees)
+                                    gained[mt][h] = fmaf(fast_exp2(fmaf(x[mt][n][2 * h + i], a.scale, -row.x)), row.y, gained[mt][h]);
+                    }
+                }
+        }
+    }
+    cp_async_wait<0>();
+    const size_t at = ((size_t)max(page, 0) * a.kv_heads + kvh) * CML_PAGE;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float g = gained[mt][h];
+            g += __shfl_xor_sync(0xffffffffu, g, 1);
+            g += __shfl_xor_sync(0xffffffffu, g, 2);
+            const int key = mt * 16 + (lane >> 2) + 8 * h;
+            if ((lane & 3) == 0 && key < valid) a.scores_out[at + key] = (place0 + key < s.start ? a.scores[at + key] : 0.f) + g;
+        }
+}
+
+template <int HD>
+static cudaError_t launch_mma(const WeightArgs& a, cudaStream_t s) {
+    constexpr int TILE = HD == 128 ? 16 : 32;
+    const unsigned pairs = (unsigned)a.n_seqs * (unsigned)a.kv_heads;
+    const int rows = a.max_new * (a.heads / a.kv_heads);
+    constexpr size_t ring = (size_t)AM_WARPS * AM_STAGES * TILE * (HD + 8) * 2;
+    cudaError_t e;
+#define AW_PART(MT, OUT, KEEP)                                                                                                   \
+    do {                                                                                                                         \
+        const size_t smem = ring * (OUT ? 2 : 1);                                                                                \
+        e = cml_allow_smem<weights_part_mma_kernel<HD, MT, OUT, KEEP>>(smem);                                                    \
+        if (e == cudaSuccess)                                                                                                    \
+            e = launch_pdl(weights_part_mma_kernel<HD, MT, OUT, KEEP>,                                                           \
+                           dim3((unsigned)a.n_splits, pairs, (unsigned)((rows + 16 * MT - 1) / (16 * MT))), dim3(AM_WARPS * 32), \
+                           smem, s, a);                                                                                          \
+    } while (0)
+    if (rows <= AK_ROWS) {
+        if (a.out) AW_PART(1, true, true);
+        else AW_PART(1, false, true);
+        if (e != cudaSuccess) return e;
+        const int key_blocks = (a.max_len + AK_THREADS - 1) / AK_THREADS;
+        return launch_pdl(weights_finish_kernel<bf16, HD>, dim3((unsigned)(key_blocks + (a.out ? rows : 0)), pairs), dim3(AK_THREADS), 0, s, a, key_blocks);
+    }
+    if (a.out) {
+        AW_PART(2, true, false);
+    } else {
+        const int row_warps = rows <= 64 ? 1 : (rows <= 128 ? 2 : 4);
+        constexpr size_t smem = (size_t)AR_STAGES * CML_PAGE * (HD + 8) * 2;
+        e = cml_allow_smem<weights_rows_mma_kernel<HD>>(smem);
+        if (e == cudaSuccess)
+            e = launch_pdl(weights_rows_mma_kernel<HD>, dim3((unsigned)a.n_splits, pairs, (unsigned)((rows + 64 * row_warps - 1) / (64 * row_warps))),
+                           dim3(AM_WARPS * 32), smem, s, a, row_warps);
+    }
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(weights_join_kernel<bf16>, dim3((unsigned)rows, pairs), dim3(AW_THREADS), 0, s, a);
+    if (e != cudaSuccess) return e;
+    constexpr size_t keys = (size_t)AM_WARPS * 64 * (HD + 8) * 2, stages = (size_t)AC_STAGES * AC_ROWS * ((HD + 8) * 2 + 16);
+    constexpr size_t smem = keys > stages ? keys : stages;
+    e = cml_allow_smem<weights_keys_mma_kernel<HD>>(smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(weights_keys_mma_kernel<HD>, dim3((unsigned)((a.max_len + AM_WARPS * 64 - 1) / (AM_WARPS * 64)), pairs), dim3(AM_WARPS * 32), smem, s, a);
+#undef AW_PART
+}
+
 extern "C" int cml_attn_paged_weights(const void* q, int dtype, long long q_stride, void* out, long long out_stride, const void* k,
                                       const void* v, const float* scores, float* scores_out, const int* table, int width, int n_pages,
                                       const int* row0, const int* start, const int* fresh, int n_seqs, int n_rows, int heads,
@@ -337,6 +1031,7 @@ extern "C" int cml_attn_paged_weights(const void* q, int dtype, long long q_stri
     if (n_seqs <= 0 || n_rows <= 0) return 0;
     if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || k_dim < 16 || k_dim > 256 || k_dim % 16 || v_dim < 16 || v_dim > 256 || v_dim % 16)
         return CML_ERR_BAD_SIZE;
+    if (!(scale > 0.f) || !(scale < __builtin_inff())) return CML_ERR_BAD_SIZE;
     if (width <= 0 || n_pages <= 0 || max_new <= 0 || max_len <= 0 || split_keys <= 0 || split_keys % CML_PAGE) return CML_ERR_BAD_SIZE;
     const long long pairs = (long long)n_seqs * kv_heads, rows = (long long)max_new * (heads / kv_heads);
     if (pairs > 65535 || rows > 65535ll * AW_ROWS || max_len > (1 << 28) || width > (1 << 24)) return CML_ERR_BAD_SIZE;
@@ -345,12 +1040,20 @@ extern "C" int cml_attn_paged_weights(const void* q, int dtype, long long q_stri
     a.q = q; a.q_stride = q_stride; a.out = out; a.out_stride = out_stride; a.k = k; a.v = v; a.scores = scores; a.scores_out = scores_out;
     a.table = table; a.width = width; a.n_pages = n_pages; a.row0 = row0; a.start = start; a.fresh = fresh; a.n_seqs = n_seqs;
     a.n_rows = n_rows; a.heads = heads; a.kv_heads = kv_heads; a.k_dim = k_dim; a.v_dim = v_dim; a.max_new = max_new; a.max_len = max_len;
-    a.scale = scale; a.split_keys = split_keys;
+    a.scale = scale * 1.4426950408889634f; a.split_keys = split_keys;
     a.n_splits = (max_len + split_keys - 1) / split_keys;
+    auto room = [](long long n) { return (n + 31) / 32 * 32; };               // every part on a boundary of 128 bytes
     a.joined = scratch;
-    a.stats = a.joined + pairs * rows * 2;
-    a.acc = a.stats + pairs * rows * 2 * a.n_splits;
-    const cudaError_t e = dtype == CML_DTYPE_F32 ? launch_plain<float>(a, (cudaStream_t)stream) : launch_plain<bf16>(a, (cudaStream_t)stream);
+    a.stats = a.joined + room(pairs * rows * 2);
+    a.acc = a.stats + room(pairs * rows * 2 * a.n_splits);
+    a.kept = a.acc + room(out ? pairs * rows * a.n_splits * v_dim : 0);
+    if (((uintptr_t)scratch) & 15) return CML_ERR_BAD_ALIGN;
+    // the tensor cores take rows of q that begin on 16 bytes
+    const bool mma = dtype == CML_DTYPE_BF16 && (k_dim == 64 || k_dim == 128) && (out == nullptr || v_dim == k_dim) &&
+                     (((uintptr_t)q) & 15) == 0 && q_stride % 8 == 0;
+    cudaStream_t s = (cudaStream_t)stream;
+    const cudaError_t e = mma ? (k_dim == 64 ? launch_mma<64>(a, s) : launch_mma<128>(a, s))
+                              : (dtype == CML_DTYPE_F32 ? launch_plain<float>(a, s) : launch_plain<bf16>(a, s));
     if (e != cudaSuccess) return (int)e;
     return cml_launch_status();
 }

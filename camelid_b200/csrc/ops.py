@@ -2029,17 +2029,26 @@ def draws_at(positions: torch.Tensor, seed: torch.Tensor, draws: torch.Tensor):
 # ---------------------------------------------------------------------------------------
 # between two steps: which positions the cache keeps, which drafted tokens stay
 
+ATTN_WEIGHTS_KEPT_ROWS = 16     # rows of a kv head up to which the products q . k are kept for the weights; AK_ROWS in attention_weights.cu
+
+
 @functools.lru_cache(maxsize=512)
 def attn_weights_plan(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int, value_dim: int, dtype: torch.dtype, max_new: int,
                       max_len: int, with_output: bool) -> tuple:
     """(keys of a stretch, float32 numbers of scratch) of ``attn_paged_weights``: a sequence's keys are cut into stretches so that
     the blocks fill the device, none shorter than four pages. Made from sizes alone, without a device."""
     pairs, rows = n_seqs * n_kv_heads, max_new * (n_heads // n_kv_heads)
-    blocks = pairs * ((rows + 7) // 8)
+    if dtype == torch.bfloat16 and head_dim in (64, 128) and value_dim == head_dim:       # rows a block works on together
+        together = (32 if rows > 16 else 16) if with_output or rows <= 16 else 256
+    else:
+        together = 8
+    blocks = pairs * ((rows + together - 1) // together)
     splits = max(1, min((4 * SMS + blocks - 1) // blocks, (max_len + 4 * PAGE - 1) // (4 * PAGE)))
     split_keys = (((max_len + splits - 1) // splits + PAGE - 1) // PAGE) * PAGE
     splits = (max_len + split_keys - 1) // split_keys
-    return split_keys, pairs * rows * 2 * (1 + splits) + (pairs * rows * splits * value_dim if with_output else 0)
+    parts = [pairs * rows * 2, pairs * rows * 2 * splits, pairs * rows * splits * value_dim if with_output else 0,
+             pairs * rows * splits * split_keys if rows <= ATTN_WEIGHTS_KEPT_ROWS else 0]
+    return split_keys, sum((n + 31) // 32 * 32 for n in parts)
 
 
 def attn_weights_floats(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype, max_new: int, max_len: int,
@@ -2080,6 +2089,8 @@ def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, 
         assert out.dtype == q.dtype and out.shape == (rows, n_heads * value_dim) and out.stride(1) == 1
     if max_new < 1 or max_len < 1:
         raise KernelError(f"attn_paged_weights: max_new {max_new} and max_len {max_len} must be at least one")
+    if not 0.0 < scale < float("inf"):
+        raise KernelError(f"attn_paged_weights: the scale must be a positive number, got {scale}")
     split_keys, floats = attn_weights_plan(n_seqs, n_heads, kv_heads, head_dim, value_dim, q.dtype, max_new, max_len, out is not None)
     if scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < floats:
         raise KernelError(f"attn_paged_weights: the scratch must be {floats} contiguous float32 numbers (attn_weights_floats)")

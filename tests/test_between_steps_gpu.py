@@ -107,6 +107,14 @@ def test_weights_of_drafted_steps(cuda, dtype, dim):
 @pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.bfloat16, 80), (torch.float32, 64)])
 def test_weights_of_a_prompts_last_rows(cuda, dtype, dim):
     _attention(cuda, [0, 500, 129], [33, 64, 2], 8, 2, dim, dtype, with_out=False, seed=3)
+    _attention(cuda, [70, 300], [64, 40], 8, 1, dim, dtype, with_out=False, seed=4)
+    _attention(cuda, [70, 0, 5], [20, 3, 1], 4, 2, dim, dtype, with_out=False, seed=5)
+    _attention(cuda, [700], [2], 4, 2, dim, dtype, with_out=False, seed=6)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_weights_of_many_rows_with_output(cuda, dim):
+    _attention(cuda, [70, 300, 0], [9, 4, 12], 16, 2, dim, torch.bfloat16, seed=7)
 
 
 @pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.bfloat16, 112), (torch.float32, 32)])
