@@ -9,20 +9,19 @@
 // before it is rounded (positions reach 2^20, where a float product would be off by 0.06 of a radian); the turn itself is
 // float, and a bfloat16 key is rounded once per move.
 //
-// Two launches. (1) A block per unit finds the score at the border by its digits (four passes of 8 bits over the
-// unit's scores) and lists the places that stay in order. (2) The rows move through shared memory. The out table may be
-// the table itself: place kept[j] >= j, so the rows of an output page come from that page or later ones, and an output
-// page may be written once the rows of every earlier page (and its own) are read. A cluster of blocks shares a unit and
-// goes page by page in rounds; every block waits for its own rows and then at the cluster's barrier before it writes.
+// Two launches. (1) A block per unit finds the score at the border by its digits and lists the places that stay in order.
+// (2) The rows move through registers. The out table may be the table itself: place kept[j] >= j, so the rows of the j-th
+// output place come from there or from later places, and an output row may be written once the rows of every earlier
+// output row (and its own) are read. A cluster of blocks shares a unit and goes through its rows in rounds: every block has
+// its round's rows in registers when it arrives at the cluster's barrier, and writes behind it.
 #include "common.cuh"
 #include <cooperative_groups.h>
 #include <math_constants.h>
 namespace cg = cooperative_groups;
 
-#define EV_SELECT_THREADS 512
-#define EV_MOVE_THREADS 256
+#define EV_MOVE_THREADS 512
+#define EV_ROWS 2               // rows a thread holds at a time
 #define EV_MAX_TEAM 8
-#define EV_STAGES 4             // rounds of rows in flight
 
 struct EvictArgs {
     void* k;
@@ -40,7 +39,6 @@ struct EvictArgs {
     int first, recent;
     const float* inv_freq;       // null: keys keep the angle they have
     int rotary_dim, interleaved;
-    int tile;                    // rows that a block moves in a round (a divisor of the page)
 };
 
 struct Unit {
@@ -65,16 +63,24 @@ __device__ __forceinline__ unsigned int score_key(float s) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__global__ void __launch_bounds__(EV_SELECT_THREADS) evict_select_kernel(EvictArgs a) {
-    __shared__ unsigned int hist[256];
+// (1) The keys of the middle are read once into shared memory where they fit (`cached` of them; beyond it they are read
+// again). Three passes over digits of 11, 11 and 10 bits find the border, then every warp takes a stretch of its own:
+// it counts what stays, the counts are scanned once, and it lists its places without further barriers.
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(EvictArgs a, int cached) {
+    constexpr int WARPS = THREADS / 32, BINS = 2048;
+    extern __shared__ __align__(16) unsigned char raw[];
+    unsigned int* hist = reinterpret_cast<unsigned int*>(raw);
+    unsigned int* keys = hist + BINS;
     __shared__ unsigned int s_prefix, s_need;
-    __shared__ int s_kept[EV_SELECT_THREADS / 32], s_ties[EV_SELECT_THREADS / 32];
+    __shared__ int s_above[WARPS], s_ties[WARPS];
+    __shared__ unsigned int s_sum[32];
     pdl_wait();
     pdl_launch_dependents();
     const Unit x = unit_of(a, blockIdx.x);
     int* kept = a.kept + (size_t)blockIdx.x * a.cap;
     if (x.keep == x.length) {                                     // everything stays
-        for (int j = threadIdx.x; j < x.keep; j += blockDim.x) kept[j] = j;
+        for (int j = threadIdx.x; j < x.keep; j += THREADS) kept[j] = j;
         return;
     }
     const int first = min(a.first, x.keep), recent = min(a.recent, x.keep - first);
@@ -83,236 +89,320 @@ __global__ void __launch_bounds__(EV_SELECT_THREADS) evict_select_kernel(EvictAr
     const int* pages = a.table + (size_t)x.seq * a.width;
     const float* scores = a.scores + (size_t)x.entry * a.n_pages * a.heads * CML_PAGE;
     auto key_at = [&](int place) {
+        if (place < cached) return keys[place];
         const int page = pages[place / CML_PAGE];
         if (page < 0 || page >= a.n_pages) return 0u;
         return score_key(scores[((size_t)page * a.heads + x.head) * CML_PAGE + place % CML_PAGE]);
     };
-    // the key of the want-th largest, digit by digit
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int j = threadIdx.x; j < first; j += THREADS) kept[j] = j;
+    for (int j = threadIdx.x; j < recent; j += THREADS) kept[x.keep - recent + j] = x.length - recent + j;
+    if (want == 0) return;
+    for (int b = threadIdx.x; b < BINS; b += THREADS) hist[b] = 0u;
+    __syncthreads();
     unsigned int prefix = 0u, need = (unsigned int)want;
-    if (want > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int b = threadIdx.x; b < 256; b += blockDim.x) hist[b] = 0u;
-            __syncthreads();
-            const unsigned int mask = shift == 24 ? 0u : (~0u << (shift + 8));
-            for (int p = lo + threadIdx.x; p < hi; p += blockDim.x) {
-                const unsigned int k = key_at(p);
-                if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1u);
-            }
-            __syncthreads();
-            if (threadIdx.x < 32) {                               // a lane sums eight bins from the top
-                const int lane = threadIdx.x;
-                unsigned int mine = 0u;
-                for (int b = 0; b < 8; ++b) mine += hist[255 - (lane * 8 + b)];
-                unsigned int incl = mine;
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : BINS;
+        if (pass == 0) {
+            // a warp reads whole pages, two places a lane and four pages in flight
+            const int n_pages = (hi + CML_PAGE - 1) / CML_PAGE;
+            for (int p0 = lo / CML_PAGE + warp; p0 < n_pages; p0 += 4 * WARPS) {
+                float2 v[4];
+                bool there[4];
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const unsigned int t = __shfl_up_sync(0xffffffffu, incl, o);
-                    if (lane >= o) incl += t;
+                for (int u = 0; u < 4; ++u) {
+                    const int page = pages[min(p0 + u * WARPS, n_pages - 1)];
+                    there[u] = page >= 0 && page < a.n_pages;
+                    v[u] = *reinterpret_cast<const float2*>(scores + ((size_t)(there[u] ? page : 0) * a.heads + x.head) * CML_PAGE + 2 * lane);
                 }
-                const unsigned int who = __ballot_sync(0xffffffffu, incl >= need);
-                if (who != 0u && lane == __ffs(who) - 1) {
-                    unsigned int before = incl - mine;
-                    int b = 0;
-                    for (; b < 7; ++b) {
-                        const unsigned int c = hist[255 - (lane * 8 + b)];
-                        if (before + c >= need) break;
-                        before += c;
-                    }
-                    s_prefix = prefix | ((unsigned int)(255 - (lane * 8 + b)) << shift);
-                    s_need = need - before;                       // how many of the border's digit are still wanted
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int place = (p0 + u * WARPS) * CML_PAGE + 2 * lane;
+                    if (p0 + u * WARPS >= n_pages) break;
+                    const unsigned int k0 = there[u] ? score_key(v[u].x) : 0u, k1 = there[u] ? score_key(v[u].y) : 0u;
+                    if (place < cached) *reinterpret_cast<uint2*>(keys + place) = make_uint2(k0, k1);
+                    if (place >= lo && place < hi) atomicAdd(&hist[k0 >> 21], 1u);
+                    if (place + 1 >= lo && place + 1 < hi) atomicAdd(&hist[k1 >> 21], 1u);
                 }
             }
-            __syncthreads();
-            prefix = s_prefix;
-            need = s_need;
-            __syncthreads();
+        } else {
+            const unsigned int mask = ~0u << (pass == 1 ? 21 : 10);
+#pragma unroll 4
+            for (int p = lo + threadIdx.x; p < hi; p += THREADS) {
+                const unsigned int k = key_at(p);
+                if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
+            }
         }
+        __syncthreads();
+        // the bin in which the need-th largest lies: warps sum equal shares of the bins from the top
+        const int share = bins / 32;                              // bins of a warp's (or, below, lane's) share
+        for (int w = warp; w < 32; w += WARPS) {
+            unsigned int t = 0u;
+            for (int b = lane; b < share; b += 32) t += hist[bins - 1 - (w * share + b)];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            if (lane == 0) s_sum[w] = t;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            unsigned int incl = s_sum[lane];
+            const unsigned int mine = incl;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned int t = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += t;
+            }
+            const int w = __ffs(__ballot_sync(0xffffffffu, incl >= need)) - 1;        // there is one: need <= candidates
+            unsigned int before = __shfl_sync(0xffffffffu, incl - mine, w);
+            const int per = share / 32;                           // one or two bins a lane
+            unsigned int c[2] = {0u, 0u};
+            for (int u = 0; u < per; ++u) c[u] = hist[bins - 1 - (w * share + lane * per + u)];
+            const unsigned int sum = c[0] + c[1];
+            unsigned int run = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned int t = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += t;
+            }
+            const int l = __ffs(__ballot_sync(0xffffffffu, before + run >= need)) - 1;
+            if (lane == l) {
+                before += run - sum;
+                const int u = before + c[0] >= need ? 0 : 1;
+                if (u == 1) before += c[0];
+                s_prefix = prefix | ((unsigned int)(bins - 1 - (w * share + lane * per + u)) << shift);
+                s_need = need - before;                           // how many of the border's digit are still wanted
+            }
+        }
+        __syncthreads();
+        prefix = s_prefix;
+        need = s_need;
+        for (int b = threadIdx.x; b < BINS; b += THREADS) hist[b] = 0u;
+        __syncthreads();
     }
-    // the places that stay, in order; of those at the border the `need` lowest
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    int done = 0, ties_done = 0;
-    for (int p0 = 0; p0 < x.length; p0 += blockDim.x) {
-        const int p = p0 + threadIdx.x;
-        const bool in = p < x.length;
-        const bool outer = in && (p < lo || p >= hi);
-        bool above = false, tie = false;
-        if (in && !outer && want > 0) {
-            const unsigned int k = key_at(p);
-            above = k > prefix;
-            tie = k == prefix;
-        }
+    // a warp's stretch of the middle
+    const int per = (((hi - lo + WARPS - 1) / WARPS) + 31) & ~31;
+    const int begin = min(hi, lo + warp * per), end = min(hi, begin + per);
+    int above = 0, ties = 0;
+#pragma unroll 4
+    for (int p = begin + lane; p < end; p += 32) {
+        const unsigned int k = key_at(p);
+        above += k > prefix;
+        ties += k == prefix;
+    }
+    above = __reduce_add_sync(0xffffffffu, above);
+    ties = __reduce_add_sync(0xffffffffu, ties);
+    if (lane == 0) s_above[warp] = above, s_ties[warp] = ties;
+    __syncthreads();
+    int at = first, ties_before = 0;                              // of the border's equals the `need` lowest places stay
+    for (int w = 0; w < warp; ++w) {
+        at += s_above[w] + max(0, min(s_ties[w], (int)need - ties_before));
+        ties_before += s_ties[w];
+    }
+    const int stop = x.keep - recent;
+    const unsigned int before = (1u << lane) - 1u;
+#pragma unroll 2
+    for (int p0 = begin; p0 < end; p0 += 32) {
+        const int p = p0 + lane;
+        const unsigned int k = p < end ? key_at(p) : 0u;
+        const bool tie = p < end && k == prefix;
+        bool stays = p < end && k > prefix;
         const unsigned int tie_mask = __ballot_sync(0xffffffffu, tie);
-        if (lane == 0) s_ties[warp] = __popc(tie_mask);
-        __syncthreads();
-        int ties_before = ties_done + __popc(tie_mask & ((1u << lane) - 1u)), ties_all = 0;
-        for (int w = 0; w < nw; ++w) {
-            if (w < warp) ties_before += s_ties[w];
-            ties_all += s_ties[w];
+        if (tie_mask) {
+            stays = stays || (tie && ties_before + __popc(tie_mask & before) < (int)need);
+            ties_before += __popc(tie_mask);
         }
-        const bool stays = outer || above || (tie && ties_before < (int)need);
         const unsigned int mask = __ballot_sync(0xffffffffu, stays);
-        if (lane == 0) s_kept[warp] = __popc(mask);
-        __syncthreads();
-        int at = done + __popc(mask & ((1u << lane) - 1u)), all = 0;
-        for (int w = 0; w < nw; ++w) {
-            if (w < warp) at += s_kept[w];
-            all += s_kept[w];
-        }
-        if (stays && at < x.keep) kept[at] = p;
-        done += all;
-        ties_done += ties_all;
-        __syncthreads();
+        const int j = at + __popc(mask & before);
+        if (stays && j < stop) kept[j] = p;
+        at += __popc(mask);
     }
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+template <typename T> struct Chunk { static constexpr int N = 16 / sizeof(T); };       // elements of 16 bytes of a row
+
+// An angle of one place, in turns, as 64 bits behind the point: its product with a whole number of places wraps by itself,
+// and the upper 32 bits of that are the angle to 2^-32 of a turn.
+__device__ __forceinline__ uint2 turns_of(float freq) {
+    const double t = (double)freq * 0.15915494309189535;
+    const unsigned long long f = (unsigned long long)((t - floor(t)) * 18446744073709551616.0);
+    return make_uint2((unsigned int)f, (unsigned int)(f >> 32));
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ float phase_of(unsigned int places, uint2 turns) {
+    return (float)(int)(__umulhi(places, turns.x) + places * turns.y);        // 2^-32 turns, from -2^31 to 2^31
+}
+template <typename T> __device__ __forceinline__ void sine_cosine(unsigned int places, uint2 turns, float* sn, float* cs);
+template <> __device__ __forceinline__ void sine_cosine<float>(unsigned int places, uint2 turns, float* sn, float* cs) {
+    sincospif(phase_of(places, turns) * 4.656612873077393e-10f, sn, cs);      // 2^-31: half turns
+}
+// bfloat16 keys take the fast functions: off by 2^-20.9, an eighth of a percent of their rounding
+template <> __device__ __forceinline__ void sine_cosine<bf16>(unsigned int places, uint2 turns, float* sn, float* cs) {
+    const float x = phase_of(places, turns) * 1.4629180792671596e-09f;        // 2 pi 2^-32
+    asm("sin.approx.ftz.f32 %0, %1;" : "=f"(*sn) : "f"(x));
+    asm("cos.approx.ftz.f32 %0, %1;" : "=f"(*cs) : "f"(x));
+}
+// (l, h) turned back by the angle whose sine and cosine are given (a key moves to a lower place)
+__device__ __forceinline__ void turn_back(float& l, float& h, float sn, float cs) {
+    const float low = l * cs + h * sn;
+    h = h * cs - l * sn;
+    l = low;
+}
+template <typename T> __device__ __forceinline__ void unpack(const uint4& c, float (&e)[Chunk<T>::N]);
+template <> __device__ __forceinline__ void unpack<float>(const uint4& c, float (&e)[4]) {
+    e[0] = __uint_as_float(c.x), e[1] = __uint_as_float(c.y), e[2] = __uint_as_float(c.z), e[3] = __uint_as_float(c.w);
+}
+template <> __device__ __forceinline__ void unpack<bf16>(const uint4& c, float (&e)[8]) {
+    const unsigned int w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[2 * i] = __uint_as_float(w[i] << 16), e[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+template <typename T> __device__ __forceinline__ uint4 pack(const float (&e)[Chunk<T>::N]);
+template <> __device__ __forceinline__ uint4 pack<float>(const float (&e)[4]) {
+    return make_uint4(__float_as_uint(e[0]), __float_as_uint(e[1]), __float_as_uint(e[2]), __float_as_uint(e[3]));
+}
+template <> __device__ __forceinline__ uint4 pack<bf16>(const float (&e)[8]) {
+    unsigned int w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(e[2 * i], e[2 * i + 1]);
+        w[i] = *reinterpret_cast<const unsigned int*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
-template <typename T> struct Chunk {                              // 16 bytes of a row
-    static constexpr int N = 16 / sizeof(T);
-    T e[N];
-};
-
+// (2) A thread owns a column of a row's keys and one of its values, two 16-byte chunks each: of the rotary part the two whose
+// elements are turned together (with neighbours as pairs any two), else one of each half of the rest. So all threads turn
+// keys and all copy values. A round's rows wait in registers for the barrier; the next round's are asked for right behind
+// it, and the places and pages of the two rounds after that are on their way, so that no load waits for another.
 template <typename T>
 __global__ void __launch_bounds__(EV_MOVE_THREADS) evict_move_kernel(EvictArgs a) {
-    constexpr int N = Chunk<T>::N;
+    constexpr int N = Chunk<T>::N, UNROLL = EV_ROWS;
     extern __shared__ __align__(16) unsigned char raw[];
+    uint2* turns = reinterpret_cast<uint2*>(raw);                 // [element of a chunk][columns], or by pair where pairs are neighbours
     pdl_wait();
     pdl_launch_dependents();
     const int team = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank();
     const int u = blockIdx.x / team;
     const Unit x = unit_of(a, u);
+    const int k_cols = a.k_dim / N / 2, v_cols = a.v ? a.v_dim / N / 2 : 0, cols = max(k_cols, v_cols);
+    const int rot_cols = a.inv_freq != nullptr ? a.rotary_dim / N / 2 : 0;
+    for (int i = threadIdx.x; i < rot_cols * N; i += EV_MOVE_THREADS)
+        turns[a.interleaved ? i : i % N * rot_cols + i / N] = turns_of(a.inv_freq[i]);
+    __syncthreads();
     const int* kept = a.kept + (size_t)u * a.cap;
     const int* pages = a.table + (size_t)x.seq * a.width;
     const int* out_pages = a.out_table + (size_t)x.seq * a.out_width;
-    const size_t head_rows = (size_t)a.heads * CML_PAGE;
+    const int head_rows = a.heads * CML_PAGE;
     const size_t entry_rows = (size_t)x.entry * a.n_pages * head_rows;
-    T* const k = (T*)a.k + entry_rows * a.k_dim;
-    T* const v = a.v ? (T*)a.v + entry_rows * a.v_dim : nullptr;
     float* const scores = a.scores + entry_rows;
-    const int k_chunks = a.k_dim / N, v_chunks = v ? a.v_dim / N : 0, chunks = k_chunks + v_chunks;
-    const int stage_bytes = a.tile * (chunks * 16 + 8);           // rows, then a score and a source place each
-    const int n_tiles = (x.keep + a.tile - 1) / a.tile;
-    const int rounds = (n_tiles + team - 1) / team;               // the same for every block of the cluster
-    const uint32_t smem = (uint32_t)__cvta_generic_to_shared(raw);
-    auto row_at = [&](int place) -> long long {                   // row of the entry's pages, -1: no such page
+    const int per_pass = EV_MOVE_THREADS / cols;                  // rows that the block moves in a pass
+    const int my_row = threadIdx.x / cols, col = threadIdx.x - my_row * cols;
+    const bool has_k = col < k_cols, has_v = col < v_cols, rotates = col < rot_cols;
+    const int d0 = rotates ? col * N : a.rotary_dim * (rot_cols > 0) + (col - rot_cols) * N;
+    const int d1 = d0 + (rotates ? a.rotary_dim / 2 : (k_cols - rot_cols) * N);
+    T* const k = (T*)a.k + entry_rows * a.k_dim + d0;
+    T* const v = (T*)a.v + entry_rows * a.v_dim + col * N;
+    const int k_step = d1 - d0, v_step = v_cols * N;
+    const int tile = per_pass * UNROLL;
+    const int rounds = (x.keep + tile * team - 1) / (tile * team);            // the same for every block of the cluster
+    auto place_of = [&](int round, int i) {                       // the source place of this thread's i-th row, -1: none
+        const int j = (round * team + rank) * tile + i * per_pass + my_row;
+        return my_row < per_pass && j < x.keep ? kept[j] : -1;
+    };
+    auto row_of = [&](int place) {                                // its row in the entry's pages, -1: none
+        if (place < 0) return -1;
         const int page = pages[place / CML_PAGE];
-        return page < 0 || page >= a.n_pages ? -1ll : (long long)((size_t)page * head_rows + (size_t)x.head * CML_PAGE + place % CML_PAGE);
+        return page < 0 || page >= a.n_pages ? -1 : page * head_rows + x.head * CML_PAGE + place % CML_PAGE;
     };
-    auto fetch = [&](int round) {
-        const int j0 = (round * team + rank) * a.tile;            // the first output place of this block's rows
-        const int rows = round < rounds ? min(a.tile, x.keep - j0) : 0;
-        unsigned char* st = raw + (size_t)(round % EV_STAGES) * stage_bytes;
-        const uint32_t dst = smem + (uint32_t)(round % EV_STAGES) * stage_bytes;
-        for (int c = threadIdx.x; c < rows * chunks; c += blockDim.x) {
-            const int j = c / chunks, cc = c - j * chunks;
-            const int place = kept[j0 + j];
-            const long long row = row_at(place);
-            if (row < 0) continue;
-            const T* src = cc < k_chunks ? k + row * a.k_dim + cc * N : v + row * a.v_dim + (cc - k_chunks) * N;
-            cp_async16(dst + (uint32_t)c * 16, src);
-        }
-        for (int j = threadIdx.x; j < rows; j += blockDim.x) {
-            const int place = kept[j0 + j];
-            const long long row = row_at(place);
-            float* tail = reinterpret_cast<float*>(st + (size_t)a.tile * chunks * 16);
-            tail[2 * j] = row >= 0 ? scores[row] : 0.f;
-            reinterpret_cast<int*>(tail)[2 * j + 1] = row >= 0 ? place : -1;
-        }
-        cp_async_commit();
+    struct Row {
+        uint4 k0, k1, v0, v1;
+        float score;
     };
-    constexpr int ahead = EV_STAGES - 1;
-    for (int r = 0; r < ahead; ++r) fetch(r);
-    const int half = a.rotary_dim / 2;
+    auto ask = [&](Row& r, int row) {
+        if (row < 0) return;
+        if (has_k) {
+            const T* src = k + (size_t)row * a.k_dim;
+            r.k0 = *reinterpret_cast<const uint4*>(src);
+            r.k1 = *reinterpret_cast<const uint4*>(src + k_step);
+        }
+        if (has_v) {
+            const T* src = v + (size_t)row * a.v_dim;
+            r.v0 = *reinterpret_cast<const uint4*>(src);
+            r.v1 = *reinterpret_cast<const uint4*>(src + v_step);
+        }
+        if (col == 0) r.score = scores[row];
+    };
+    int place[UNROLL], place1[UNROLL], place2[UNROLL], row[UNROLL], row1[UNROLL];         // of this round, the next, the one after
+    Row now[UNROLL], next[UNROLL];
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) place[i] = place_of(0, i), place1[i] = place_of(1, i), place2[i] = place_of(2, i);
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) row[i] = row_of(place[i]), row1[i] = row_of(place1[i]);
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) ask(now[i], row[i]);
     for (int round = 0; round < rounds; ++round) {
-        fetch(round + ahead);
-        asm volatile("cp.async.wait_group 3;" ::: "memory");      // this round's rows: all groups but the three newest
-        cg::this_cluster().sync();                                // ... and those of the cluster's other blocks
-        const int j0 = (round * team + rank) * a.tile;
-        const int rows = min(a.tile, x.keep - j0);
-        const unsigned char* st = raw + (size_t)(round % EV_STAGES) * stage_bytes;
-        const float* tail = reinterpret_cast<const float*>(st + (size_t)a.tile * chunks * 16);
-        const int to = rows > 0 ? out_pages[j0 / CML_PAGE] : -1;
-        if (to >= 0 && to < a.n_pages) {
-            const size_t out_row0 = (size_t)to * head_rows + (size_t)x.head * CML_PAGE + j0 % CML_PAGE;
-            for (int c = threadIdx.x; c < rows * chunks; c += blockDim.x) {
-                const int j = c / chunks, cc = c - j * chunks;
-                const int place = reinterpret_cast<const int*>(tail)[2 * j + 1];
-                if (place < 0) continue;
-                const int move = j0 + j - place;
-                const size_t row = out_row0 + j;
-                Chunk<T> w = *reinterpret_cast<const Chunk<T>*>(st + (size_t)c * 16);
-                if (cc < k_chunks) {
-                    const int d0 = cc * N;
-                    if (a.inv_freq != nullptr && d0 < a.rotary_dim && move != 0) {
-                        if (a.interleaved) {
+        // Every row of this round has been read when the barrier lets go: arriving there orders a thread's loads before
+        // the others' stores behind it.
+        if (team > 1) cg::this_cluster().sync();
+        else __syncthreads();
+        int row2[UNROLL], place3[UNROLL];
 #pragma unroll
-                            for (int e = 0; e < N; e += 2) {
-                                const double t = (double)move * (double)a.inv_freq[(d0 + e) / 2] * 0.15915494309189535;
-                                float sn, cs;
-                                sincospif(2.0f * (float)(t - rint(t)), &sn, &cs);
-                                const float p = to_f32(w.e[e]), q = to_f32(w.e[e + 1]);
-                                w.e[e] = from_f32<T>(p * cs - q * sn);
-                                w.e[e + 1] = from_f32<T>(q * cs + p * sn);
-                            }
-                        } else {
-                            const bool low = d0 < half;
-                            const Chunk<T> o = *reinterpret_cast<const Chunk<T>*>(st + ((size_t)j * chunks + (low ? d0 + half : d0 - half) / N) * 16);
+        for (int i = 0; i < UNROLL; ++i) ask(next[i], row1[i]);
 #pragma unroll
-                            for (int e = 0; e < N; ++e) {
-                                const double t = (double)move * (double)a.inv_freq[(low ? d0 : d0 - half) + e] * 0.15915494309189535;
-                                float sn, cs;
-                                sincospif(2.0f * (float)(t - rint(t)), &sn, &cs);
-                                const float p = to_f32(w.e[e]), q = to_f32(o.e[e]);
-                                w.e[e] = from_f32<T>(low ? p * cs - q * sn : p * cs + q * sn);
-                            }
-                        }
-                    }
-                    *reinterpret_cast<Chunk<T>*>(k + row * a.k_dim + d0) = w;
-                } else {
-                    *reinterpret_cast<Chunk<T>*>(v + row * a.v_dim + (cc - k_chunks) * N) = w;
-                }
+        for (int i = 0; i < UNROLL; ++i) row2[i] = row_of(place2[i]), place3[i] = place_of(round + 3, i);
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) {
+            if (row[i] < 0) continue;
+            const int j = (round * team + rank) * tile + i * per_pass + my_row;
+            const int to = out_pages[j / CML_PAGE];
+            if (to < 0 || to >= a.n_pages) continue;
+            const int out_row = to * head_rows + x.head * CML_PAGE + j % CML_PAGE;
+            if (has_v) {
+                T* dst = v + (size_t)out_row * a.v_dim;
+                *reinterpret_cast<uint4*>(dst) = now[i].v0;
+                *reinterpret_cast<uint4*>(dst + v_step) = now[i].v1;
             }
-            for (int j = threadIdx.x; j < rows; j += blockDim.x)
-                if (reinterpret_cast<const int*>(tail)[2 * j + 1] >= 0) scores[out_row0 + j] = tail[2 * j];
+            const unsigned int back = (unsigned int)(place[i] - j);           // places that the row moves down
+            if (rotates && back != 0u) {
+                float p[N], q[N], sn, cs;
+                unpack<T>(now[i].k0, p);
+                unpack<T>(now[i].k1, q);
+                if (a.interleaved) {
+#pragma unroll
+                    for (int e = 0; e < N; e += 2) {
+                        sine_cosine<T>(back, turns[(d0 + e) / 2], &sn, &cs);
+                        turn_back(p[e], p[e + 1], sn, cs);
+                        sine_cosine<T>(back, turns[(d1 + e) / 2], &sn, &cs);
+                        turn_back(q[e], q[e + 1], sn, cs);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        sine_cosine<T>(back, turns[e * rot_cols + col], &sn, &cs);
+                        turn_back(p[e], q[e], sn, cs);
+                    }
+                }
+                now[i].k0 = pack<T>(p);
+                now[i].k1 = pack<T>(q);
+            }
+            if (has_k) {
+                T* dst = k + (size_t)out_row * a.k_dim;
+                *reinterpret_cast<uint4*>(dst) = now[i].k0;
+                *reinterpret_cast<uint4*>(dst + k_step) = now[i].k1;
+            }
+            if (col == 0) scores[out_row] = now[i].score;
         }
-        __syncthreads();                                          // the stage is fetched into again next
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) {
+            now[i] = next[i];
+            place[i] = place1[i], row[i] = row1[i];
+            place1[i] = place2[i], row1[i] = row2[i];
+            place2[i] = place3[i];
+        }
     }
 }
 
-extern "C" int cml_evict_positions(void* k, void* v, float* scores, int dtype, const int* table, int width, const int* out_table,
-                                   int out_width, const int* lengths, const int* keeps, int* kept, int cap, int entries,
-                                   int n_pages, int n_seqs, int heads, int k_dim, int v_dim, int first, int recent,
-                                   const float* inv_freq, int rotary_dim, int interleaved, void* stream) {
-    if (dtype != CML_DTYPE_F32 && dtype != CML_DTYPE_BF16) return CML_ERR_BAD_DTYPE;
-    if (n_seqs <= 0 || entries <= 0 || cap <= 0) return 0;
-    const int n = dtype == CML_DTYPE_F32 ? 4 : 8;
-    if (heads <= 0 || n_pages <= 0 || width <= 0 || out_width <= 0 || width > (1 << 24) || out_width > (1 << 24)) return CML_ERR_BAD_SIZE;
-    if (k_dim <= 0 || k_dim % n || v_dim % n || k_dim + v_dim > 1024 || first < 0 || recent < 0) return CML_ERR_BAD_SIZE;
-    if (inv_freq != nullptr && (rotary_dim <= 0 || rotary_dim > k_dim || rotary_dim % (2 * n))) return CML_ERR_BAD_SIZE;
-    if (((uintptr_t)k | (uintptr_t)v) & 15) return CML_ERR_BAD_ALIGN;
-    const long long units = (long long)entries * n_seqs * heads;
-    if (units * EV_MAX_TEAM > 0x7fffffffLL) return CML_ERR_BAD_SIZE;
-    EvictArgs a = {};
-    a.k = k; a.v = v; a.scores = scores; a.table = table; a.width = width; a.out_table = out_table; a.out_width = out_width;
-    a.lengths = lengths; a.keeps = keeps; a.kept = kept; a.cap = cap; a.entries = entries; a.n_pages = n_pages;
-    a.n_seqs = n_seqs; a.heads = heads; a.k_dim = k_dim; a.v_dim = v != nullptr ? v_dim : 0; a.first = first; a.recent = recent;
-    a.inv_freq = inv_freq; a.rotary_dim = rotary_dim; a.interleaved = interleaved;
-    cudaStream_t s = (cudaStream_t)stream;
-    cudaError_t e = launch_pdl(evict_select_kernel, dim3((unsigned)units), dim3(EV_SELECT_THREADS), 0, s, a);
-    if (e != cudaSuccess) return (int)e;
-    // blocks that share a unit: enough for every multiprocessor, none without an output page
-    const int out_pages = min(out_width, (cap + CML_PAGE - 1) / CML_PAGE);
-    int team = 1;
-    while (team < EV_MAX_TEAM && units * team < cml_sm_count() && team < out_pages) team *= 2;
-    const size_t row = (size_t)(a.k_dim + a.v_dim) / n * 16 + 8;
-    a.tile = CML_PAGE;
-    while (row * a.tile * EV_STAGES > 200 * 1024) a.tile /= 2;     // rows of at most 4 KB: 8 of them at least
-    const size_t smem = row * a.tile * EV_STAGES;
-    e = dtype == CML_DTYPE_F32 ? cml_allow_smem<evict_move_kernel<float>>(smem) : cml_allow_smem<evict_move_kernel<bf16>>(smem);
-    if (e != cudaSuccess) return (int)e;
+template <typename T>
+static cudaError_t launch_move(const EvictArgs& a, long long units, int team, size_t smem, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(units * team));
     cfg.blockDim = dim3(EV_MOVE_THREADS);
@@ -327,7 +417,49 @@ extern "C" int cml_evict_positions(void* k, void* v, float* scores, int dtype, c
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cml_pdl_enabled() ? 2 : 1;
-    e = dtype == CML_DTYPE_F32 ? cudaLaunchKernelEx(&cfg, evict_move_kernel<float>, a) : cudaLaunchKernelEx(&cfg, evict_move_kernel<bf16>, a);
+    return cudaLaunchKernelEx(&cfg, evict_move_kernel<T>, a);
+}
+
+extern "C" int cml_evict_positions(void* k, void* v, float* scores, int dtype, const int* table, int width, const int* out_table,
+                                   int out_width, const int* lengths, const int* keeps, int* kept, int cap, int entries,
+                                   int n_pages, int n_seqs, int heads, int k_dim, int v_dim, int first, int recent,
+                                   const float* inv_freq, int rotary_dim, int interleaved, void* stream) {
+    if (dtype != CML_DTYPE_F32 && dtype != CML_DTYPE_BF16) return CML_ERR_BAD_DTYPE;
+    if (n_seqs <= 0 || entries <= 0 || cap <= 0) return 0;
+    const int n = dtype == CML_DTYPE_F32 ? 4 : 8;
+    if (heads <= 0 || n_pages <= 0 || width <= 0 || out_width <= 0 || width > (1 << 24) || out_width > (1 << 24)) return CML_ERR_BAD_SIZE;
+    if (k_dim <= 0 || k_dim % 16 || v_dim % 16 || k_dim + v_dim > 1024 || first < 0 || recent < 0) return CML_ERR_BAD_SIZE;
+    if (inv_freq != nullptr && (rotary_dim <= 0 || rotary_dim > k_dim || rotary_dim % 16)) return CML_ERR_BAD_SIZE;
+    if (((uintptr_t)k | (uintptr_t)v) & 15) return CML_ERR_BAD_ALIGN;
+    if ((long long)n_pages * heads * CML_PAGE > 0x7fffffffLL) return CML_ERR_BAD_SIZE;       // an entry's rows are counted in 32 bits
+    const long long units = (long long)entries * n_seqs * heads;
+    if (units * EV_MAX_TEAM > 0x7fffffffLL) return CML_ERR_BAD_SIZE;
+    EvictArgs a = {};
+    a.k = k; a.v = v; a.scores = scores; a.table = table; a.width = width; a.out_table = out_table; a.out_width = out_width;
+    a.lengths = lengths; a.keeps = keeps; a.kept = kept; a.cap = cap; a.entries = entries; a.n_pages = n_pages;
+    a.n_seqs = n_seqs; a.heads = heads; a.k_dim = k_dim; a.v_dim = v != nullptr ? v_dim : 0; a.first = first; a.recent = recent;
+    a.inv_freq = inv_freq; a.rotary_dim = rotary_dim; a.interleaved = interleaved;
+    cudaStream_t s = (cudaStream_t)stream;
+    // A unit's scores fit the shared memory up to 48 k places. Short sequences take small blocks, of which many run at once.
+    const long long longest = (long long)width * CML_PAGE;
+    const int cached = (int)(longest < 49152 ? longest : 49152);
+    const size_t select_smem = (2048 + (size_t)cached) * 4;
+    cudaError_t e;
+    if (longest <= 4096) {
+        e = cml_allow_smem<evict_select_kernel<256>>(select_smem);
+        if (e == cudaSuccess) e = launch_pdl(evict_select_kernel<256>, dim3((unsigned)units), dim3(256), select_smem, s, a, cached);
+    } else {
+        e = cml_allow_smem<evict_select_kernel<1024>>(select_smem);
+        if (e == cudaSuccess) e = launch_pdl(evict_select_kernel<1024>, dim3((unsigned)units), dim3(1024), select_smem, s, a, cached);
+    }
+    if (e != cudaSuccess) return (int)e;
+    // blocks that share a unit: one for every multiprocessor in all, none without rows to move
+    const long long most = out_width * (long long)CML_PAGE < cap ? out_width * (long long)CML_PAGE : cap;
+    const int cols = (k_dim > a.v_dim ? k_dim : a.v_dim) / n / 2, tile = EV_MOVE_THREADS / cols * EV_ROWS;
+    int team = 1;
+    while (team < EV_MAX_TEAM && units * team * 2 <= cml_sm_count() && (long long)team * tile < most) team *= 2;
+    const size_t smem = (size_t)rotary_dim / 2 * 8;
+    e = dtype == CML_DTYPE_F32 ? launch_move<float>(a, units, team, smem, s) : launch_move<bf16>(a, units, team, smem, s);
     if (e != cudaSuccess) return (int)e;
     return cml_launch_status();
 }
