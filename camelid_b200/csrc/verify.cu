@@ -15,13 +15,13 @@
 // Everything that a decision rests on is computed in double, because a rounding of 2^-24 in a sum over 128,256 tokens
 // would move one draw in a hundred to a neighbouring token: exp((l - max) / T), its sums, the thresholds.
 //
-// Two launches, three with filters: (1) the maximum and the sum of every row, in parts of 8,192 columns, or, with
+// Two launches, three with filters: (1) the maximum and the sum of every row, in parts of 4,096 columns, or, with
 // filters, the same of the candidates, by a cluster per row (row_select.cuh); (2) a cluster per sequence decides how
 // many tokens stay, adds up the one row that the next token is drawn from, warp by warp, and walks the warp's stretch
 // in which the crossing lies.
 #include "row_select.cuh"
 
-#define VF_PART 8192            // columns of a row that one block adds up
+#define VF_PART 4096            // columns of a row that one block adds up
 #define VF_PART_THREADS 256
 #define VF_THREADS 512          // threads of a block that decides
 #define VF_WARPS (VF_THREADS / 32)
@@ -64,14 +64,46 @@ struct VerifyArgs {
     int parts;
 };
 
+// exp((l - max) / T) in double to 2e-12 of itself: 2^(z / 32) with z = (l - max) 32 log2(e) / T cut into a whole number,
+// whose upper bits are the exponent and whose lower five choose from a table, and a rest of at most a half, whose power is a
+// polynomial of degree four ((ln 2 / 64)^5 / 120 = 1.2e-12). Eleven operations in double instead of the library
+// function's eighteen among seventy instructions; 32 entries are two rows of the banks, so a warp's look-up takes two turns.
+struct Exponential {
+    double c, max;               // z = (l - max) c; the difference of two floats is exact enough at any temperature
+    float least;                 // below this the result is no longer a normal number: zero
+};
+__device__ __forceinline__ Exponential exponential_of(float max, float temperature) {
+    Exponential e;
+    e.c = 46.166241308446828 / (double)temperature;
+    e.max = (double)max;
+    e.least = (float)((double)max - 700.0 * (double)temperature);
+    return e;
+}
+__device__ __forceinline__ void fill_table(double* table) {       // by the first warp; a barrier follows
+    if (threadIdx.x < 32) table[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
+}
+__device__ __forceinline__ double weight_of(float l, const Exponential& e, const double* table) {
+    const double d = (double)l - e.max;
+    const double shifted = fma(d, e.c, 6755399441055744.0);       // 1.5 * 2^52: the whole number in the low bits
+    const double r = fma(d, e.c, -(shifted - 6755399441055744.0));
+    const int k = __double2loint(shifted);
+    constexpr double C1 = 0.021660849392498290, C2 = C1 * C1 / 2, C3 = C1 * C1 * C1 / 6, C4 = C1 * C1 * C1 * C1 / 24;
+    const double p = fma(r, fma(r, fma(r, fma(r, C4, C3), C2), C1), 1.0);
+    const double t = table[k & 31];
+    const double scaled = __hiloint2double(__double2hiint(t) + ((k >> 5) << 20), __double2loint(t));
+    return l < e.least ? 0.0 : scaled * p;
+}
+
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < CUDART_INF_F; }
 
-// (1a) without filters. A thread keeps its 32 columns in registers, so the row is read once; the block's maximum is the
+// (1a) without filters. A thread keeps its 16 columns in registers, so the row is read once; the block's maximum is the
 // reference of its exponentials, and the parts are joined where they are read.
 __global__ void __launch_bounds__(VF_PART_THREADS) verify_stats_kernel(VerifyArgs a) {
     __shared__ float fred[33];
     __shared__ double dred[33];
     __shared__ int ired[33];
+    __shared__ double table[32];
+    fill_table(table);
     pdl_wait();
     pdl_launch_dependents();
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
@@ -114,14 +146,14 @@ __global__ void __launch_bounds__(VF_PART_THREADS) verify_stats_kernel(VerifyArg
     if ((threadIdx.x & 31) == 0) ired[threadIdx.x >> 5] = at;
     double s = 0.0;
     if (a.temperature > 0.f) {
-        const double inv_t = 1.0 / (double)a.temperature, m = (double)bmax;
+        const Exponential ex = exponential_of(bmax, a.temperature);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = begin + 4 * (u * VF_PART_THREADS + (int)threadIdx.x);
             const float e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                if (i + k < end) s += exp(((double)e[k] - m) * inv_t);
+                if (i + k < end) s += weight_of(e[k], ex, table);
         }
     }
     s = block_sum_double(s, dred);
@@ -145,6 +177,9 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
     __shared__ SelectShared sh;
     __shared__ TeamSlots ts;
     __shared__ float fred[33];
+    __shared__ double table[32];
+    fill_table(table);
+    cg::this_cluster().sync();                                    // every block has started before its memory is written
     pdl_wait();
     pdl_launch_dependents();
     Team tm;
@@ -190,13 +225,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
         tm.sync();
         return;
     }
-    const double inv_t = 1.0 / (double)a.temperature, m = (double)mx;
+    const Exponential ex = exponential_of(mx, a.temperature);
     // the place of a value in the order: never negative, monotone, and finite (masks of the type's lowest value are
     // all put at one far place, where their weight is zero)
-    const float inv_tf = (float)fmin(inv_t, 1e30), far = 1e30f;
-    auto xof = [=](float v) { return fminf(fmaxf((float)((m - (double)v) * (double)inv_tf), 0.f), far); };
+    const float inv_t = fminf(1.0f / a.temperature, 1e30f), far = 1e30f;
+    auto xof = [=](float v) { return fminf((mx - v) * inv_t, far); };
     const float x_max = xof(mn);
-    auto raw_weight = [=](float v, int) { return exp(((double)v - m) * inv_t); };
+    auto raw_weight = [=](float v, int) { return weight_of(v, ex, table); };
     unsigned long long floor_key = 0ull, key;
     double cum;
     auto select_slow = [&](unsigned long long floor, double target, int strict, auto weight) {
@@ -271,37 +306,47 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
 }
 
 struct RowStat {
-    double max, total;               // the maximum as a double, and the sum against it
+    double total;                    // the sum against the maximum
+    float max;
     int arg;
-    bool bad;
+    int bad;
 };
 
-// The parts of a row joined, in their order.
-__device__ RowStat join_parts(const VerifyArgs& a, int row) {
+// The parts of a row joined by a warp, the lanes in their order: the same in every lane.
+__device__ __forceinline__ RowStat join_parts(const VerifyArgs& a, int row, const double* table) {
+    const int lane = threadIdx.x & 31;
+    const PartStat* s = a.stats + (size_t)row * a.parts;
     RowStat r;
     float mx = -CUDART_INF_F;
-    r.bad = false;
-    r.arg = 0;
-    const PartStat* s = a.stats + (size_t)row * a.parts;
-    for (int p = 0; p < a.parts; ++p) {
+    int arg = 0x7fffffff;
+    bool bad = false;
+    for (int p = lane; p < a.parts; p += 32) {
         const float m = s[p].max;
-        if (!finite(m)) r.bad = true;
-        if (m > mx) mx = m, r.arg = s[p].arg;
+        if (!finite(m)) bad = true;
+        if (m > mx) mx = m, arg = s[p].arg;
     }
-    r.max = (double)mx;
+    r.max = warp_max(mx);
+    r.arg = __reduce_min_sync(0xffffffffu, mx == r.max ? arg : 0x7fffffff);
+    r.bad = __any_sync(0xffffffffu, bad) ? 1 : 0;
     r.total = 0.0;
     if (a.temperature > 0.f && !r.bad) {
-        const double inv_t = 1.0 / (double)a.temperature;
-        for (int p = 0; p < a.parts; ++p) r.total += s[p].sum * exp(((double)s[p].max - r.max) * inv_t);
+        const Exponential ex = exponential_of(r.max, a.temperature);
+        for (int p = lane; p < a.parts; p += 32) r.total += s[p].sum * weight_of(s[p].max, ex, table);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) r.total += __shfl_xor_sync(0xffffffffu, r.total, o);
     }
     return r;
 }
 
 // (2) a cluster per sequence.
+#define VF_ROWS 32                   // rows whose joined parts a block remembers
 __global__ void __launch_bounds__(VF_THREADS) verify_decide_kernel(VerifyArgs a) {
-    __shared__ double warp_sums[SAMPLE_MAX_TEAM * VF_WARPS];      // block 0's: every block's warps, in order
+    __shared__ double table[32];
+    __shared__ double warp_sums[2][VF_WARPS], block_sums[2][SAMPLE_MAX_TEAM];     // of two rounds
+    __shared__ RowStat stats[VF_ROWS];
     __shared__ int first_bad, row_bad, err_bits;
-    __shared__ RowStat chosen;
+    fill_table(table);
+    if (threadIdx.x == 0) first_bad = 0x7fffffff, row_bad = 0, err_bits = 0;
     pdl_wait();
     pdl_launch_dependents();
     const int team = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank();
@@ -310,8 +355,6 @@ __global__ void __launch_bounds__(VF_THREADS) verify_decide_kernel(VerifyArgs a)
     const int len = max(0, min(a.lens[seq], a.width)), row0 = a.row0[seq];
     const int vocab = a.vocab;
     const bool greedy = !(a.temperature > 0.f), filtered = a.floors != nullptr;
-    const double inv_t = greedy ? 0.0 : 1.0 / (double)a.temperature;
-    double* sums0 = cg::this_cluster().map_shared_rank(&warp_sums[0], 0);
     int* out = a.tokens + (size_t)seq * (a.width + 1);
     if (row0 < 0 || row0 > a.n_rows - 1 - len) {                  // the same in every block of the cluster
         if (rank == 0) {
@@ -320,40 +363,52 @@ __global__ void __launch_bounds__(VF_THREADS) verify_decide_kernel(VerifyArgs a)
         }
         return;
     }
-    if (threadIdx.x == 0) first_bad = len, row_bad = 0, err_bits = 0;
     __syncthreads();
-    // every draft by a thread of its own: is it accepted?
-    for (int j = threadIdx.x; j <= len; j += blockDim.x) {
-        const RowStat r = join_parts(a, row0 + j);
-        int bits = r.bad ? VF_ERR_NONFINITE : (!greedy && !(r.total > 0.0) ? VF_ERR_EMPTY : 0);
-        if (bits) atomicOr(&row_bad, 1);
+    // the cluster's other blocks have started once all have arrived here: their memory is written only after the wait below
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    // every draft by a warp of its own: is it accepted?
+    for (int j = warp; j <= len; j += VF_WARPS) {
+        // what the decision reads beside the parts does not wait for them
+        int x = 0;
+        float q = 1.f, l = 0.f, u = 0.f;
+        bool known = false;
         if (j < len) {
-            const int x = a.drafts[(long long)seq * a.drafts_ld + j];
-            bool ok = false;
-            if (x < 0 || x >= vocab) bits |= VF_ERR_DRAFT;
-            else if (!r.bad) {
-                const float q = a.probs ? a.probs[(long long)seq * a.probs_seq + (long long)j * a.probs_step + x] : 1.f;
-                if (!(q >= 0.f) || !finite(q)) bits |= VF_ERR_DRAFT;
-                const double u = (double)a.accept[(long long)seq * a.accept_ld + j];
-                double p;
-                if (greedy) p = x == r.arg ? 1.0 : 0.0;
-                else {
-                    const float l = a.logits[(long long)(row0 + j) * a.ld + x];
-                    const bool in = !filtered || composite_key(l, x) >= a.floors[row0 + j];
-                    p = in ? exp(((double)l - r.max) * inv_t) / r.total : 0.0;
-                }
-                ok = u * (double)q < p;
+            x = a.drafts[(long long)seq * a.drafts_ld + j];
+            u = a.accept[(long long)seq * a.accept_ld + j];
+            known = x >= 0 && x < vocab;
+            if (known) {
+                if (a.probs) q = a.probs[(long long)seq * a.probs_seq + (long long)j * a.probs_step + x];
+                l = a.logits[(long long)(row0 + j) * a.ld + x];
             }
-            if (!ok) atomicMin(&first_bad, j);
         }
-        if (bits) atomicOr(&err_bits, bits);
+        const RowStat r = join_parts(a, row0 + j, table);
+        if (lane == 0) {
+            if (j < VF_ROWS) stats[j] = r;
+            int bits = r.bad ? VF_ERR_NONFINITE : (!greedy && !(r.total > 0.0) ? VF_ERR_EMPTY : 0);
+            if (bits) atomicOr(&row_bad, 1);
+            if (j < len) {
+                bool ok = false;
+                if (!known) bits |= VF_ERR_DRAFT;
+                else if (!r.bad) {
+                    if (!(q >= 0.f) || !finite(q)) bits |= VF_ERR_DRAFT;
+                    double p;
+                    if (greedy) p = x == r.arg ? 1.0 : 0.0;
+                    else {
+                        const bool in = !filtered || composite_key(l, x) >= a.floors[row0 + j];
+                        p = in ? weight_of(l, exponential_of(r.max, a.temperature), table) / r.total : 0.0;
+                    }
+                    ok = (double)u * (double)q < p;
+                }
+                if (!ok) atomicMin(&first_bad, j);
+            }
+            if (bits) atomicOr(&err_bits, bits);
+        }
     }
     __syncthreads();
-    const int count = row_bad ? 0 : first_bad;
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    const int count = row_bad ? 0 : min(first_bad, len);
     const int row = row0 + count;
-    if (threadIdx.x == 0) chosen = join_parts(a, row);
-    __syncthreads();
-    const RowStat st = chosen;
+    const RowStat st = count < VF_ROWS ? stats[count] : join_parts(a, row, table);
     if (rank == 0) {
         if (threadIdx.x == 0) {
             a.counts[seq] = count;
@@ -372,77 +427,132 @@ __global__ void __launch_bounds__(VF_THREADS) verify_decide_kernel(VerifyArgs a)
     const float* q = (rejected && a.probs) ? a.probs + (long long)seq * a.probs_seq + (long long)count * a.probs_step : nullptr;
     const int without = (rejected && !a.probs) ? a.drafts[(long long)seq * a.drafts_ld + count] : -1;
     const unsigned long long floor_key = filtered ? a.floors[row] : 0ull;
+    const Exponential ex = exponential_of(st.max, a.temperature);
     const double inv_total = 1.0 / st.total;
     bool bad_q = false;
     bool plain = false;                                           // nothing is left of p - q: draw from p
-    auto weight = [&](int i) {
-        const float l = r[i];
-        if (filtered && composite_key(l, i) < floor_key) return 0.0;
-        const double p = exp(((double)l - st.max) * inv_t) * inv_total;
-        if (plain) return p;
-        if (q) {
-            const float qi = q[i];
-            if (!(qi >= 0.f)) bad_q = true;
-            const double d = p - (double)qi;
-            return d > 0.0 ? d : 0.0;
-        }
-        return i == without ? 0.0 : p;
-    };
-    // stretches of whole tiles of 32 columns, one a warp, in ascending order over the blocks of the cluster
+    // stretches of whole tiles of 128 columns, one a warp, in ascending order over the blocks of the cluster
     const int warps = team * VF_WARPS;
-    const int per = (((vocab + warps - 1) / warps) + 31) & ~31;
-    const int mine = rank * VF_WARPS + warp;
-    const int begin = min(vocab, mine * per), end = min(vocab, begin + per);
-    int owner = -1;
-    double before = 0.0, total = 0.0, target = 0.0;
-    for (int round = 0; round < 2; ++round) {
+    const int per = (((vocab + warps - 1) / warps) + 127) & ~127;
+    const int begin = min(vocab, (rank * VF_WARPS + warp) * per), end = min(vocab, begin + per);
+    const bool vec = (((uintptr_t)r) & 15) == 0 && (q == nullptr || (((uintptr_t)q) & 15) == 0);
+    // four columns of a tile in a lane, ascending over the lanes
+    auto load4 = [&](const float* from, int i, float (&v)[4]) {
+        if (vec && i + 4 <= end) {
+            const float4 t = *reinterpret_cast<const float4*>(from + i);
+            v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = i + k < end ? from[i + k] : 0.f;
+        }
+    };
+    auto weigh = [&](int i, const float (&l)[4], const float (&qi)[4], double (&w)[4]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            double p = weight_of(l[k], ex, table) * inv_total;
+            if (filtered && composite_key(l[k], i + k) < floor_key) p = 0.0;
+            if (!plain) {
+                if (q) {
+                    bad_q = bad_q || !(qi[k] >= 0.f);
+                    p -= (double)qi[k];
+                }
+                if (i + k == without) p = 0.0;
+            }
+            w[k] = i + k < end && p > 0.0 ? p : 0.0;
+        }
+    };
+    double total = 0.0, target, before = 0.0;
+    int owner = -1, round = 0;
+    for (; round < 2; ++round) {
         double s = 0.0;
-        for (int i = begin + lane; i < end; i += 32) s += weight(i);
+        for (int i0 = begin + 4 * lane; i0 < end; i0 += 256) {    // two tiles in flight
+            float l0[4], l1[4], q0[4] = {0.f, 0.f, 0.f, 0.f}, q1[4] = {0.f, 0.f, 0.f, 0.f};
+            const int i1 = i0 + 128;
+            load4(r, i0, l0);
+            load4(r, i1, l1);
+            if (q) load4(q, i0, q0), load4(q, i1, q1);
+            double w[4];
+            weigh(i0, l0, q0, w);
+            s += (w[0] + w[1]) + (w[2] + w[3]);
+            weigh(i1, l1, q1, w);
+            s += (w[0] + w[1]) + (w[2] + w[3]);
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) sums0[mine] = s;
-        cg::this_cluster().sync();
+        if (lane == 0) warp_sums[round][warp] = s;
+        __syncthreads();
+        if ((int)threadIdx.x < team) {                            // this block's sum to every block of the cluster
+            double b = 0.0;
+#pragma unroll
+            for (int w = 0; w < VF_WARPS; ++w) b += warp_sums[round][w];
+            cg::this_cluster().map_shared_rank(&block_sums[round][0], threadIdx.x)[rank] = b;
+        }
+        cg::this_cluster().sync();                                // the last access to another block's memory of this round
         total = 0.0;
-        for (int w = 0; w < warps; ++w) total += sums0[w];
+        for (int b = 0; b < team; ++b) total += block_sums[round][b];
         if (total > 0.0 || round == 1) break;
         plain = true;
-        cg::this_cluster().sync();                                // before the sums are written again
     }
     target = (double)a.draws[seq] * total;
     {
         double run = 0.0;
-        for (int w = 0; w < warps; ++w) {
-            const double s = sums0[w];
-            if (s > 0.0) owner = w, before = run;                 // never reached: the last stretch with any weight
+        for (int b = 0; b < team; ++b) {
+            const double s = block_sums[round][b];
+            if (s > 0.0) owner = b, before = run;                 // never reached: the last stretch with any weight
             run += s;
             if (run > target) break;
         }
     }
-    if (mine == owner) {
+    if (owner == rank) {
+        int mine = -1;
         double run = before;
-        int found = -1, last = -1;
-        for (int i0 = begin; i0 < end; i0 += 32) {
-            const int i = i0 + lane;
-            const double w = i < end ? weight(i) : 0.0;
-            double incl = w;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double t = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += t;
-            }
-            const unsigned int some = __ballot_sync(0xffffffffu, w > 0.0);
-            const unsigned int hit = __ballot_sync(0xffffffffu, w > 0.0 && run + incl > target);
-            if (hit) { found = i0 + __ffs(hit) - 1; break; }
-            if (some) last = i0 + 31 - __clz(some);
-            run += __shfl_sync(0xffffffffu, incl, 31);
+        for (int w = 0; w < VF_WARPS; ++w) {
+            const double s = warp_sums[round][w];
+            if (s > 0.0) mine = w, before = run;
+            run += s;
+            if (run > target) break;
         }
-        if (lane == 0) out[count] = found >= 0 ? found : last;
+        if (warp == mine) {
+            run = before;
+            int found = -1, last = -1;
+            for (int i0 = begin; i0 < end; i0 += 128) {
+                const int i = i0 + 4 * lane;
+                float l[4], qi[4] = {0.f, 0.f, 0.f, 0.f};
+                double w[4];
+                load4(r, i, l);
+                if (q) load4(q, i, qi);
+                weigh(i, l, qi, w);
+                const double s = (w[0] + w[1]) + (w[2] + w[3]);
+                double incl = s;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double t = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += t;
+                }
+                const unsigned int some = __ballot_sync(0xffffffffu, s > 0.0);
+                const unsigned int hit = __ballot_sync(0xffffffffu, s > 0.0 && run + incl > target);
+                if (some) {                                       // the lane of the crossing, or the last with any weight
+                    const int who = hit ? __ffs(hit) - 1 : 31 - __clz(some);
+                    double c = run + (incl - s);
+                    int at = -1;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        c += w[k];
+                        if (w[k] > 0.0) at = i + k;
+                        if (hit && w[k] > 0.0 && c > target) break;
+                    }
+                    last = __shfl_sync(0xffffffffu, at, who);
+                    if (hit) { found = last; break; }
+                }
+                run += __shfl_sync(0xffffffffu, incl, 31);
+            }
+            if (lane == 0) out[count] = found >= 0 ? found : last;
+        }
     } else if (owner < 0 && rank == 0 && threadIdx.x == 0) {      // not a number in the sums
         out[count] = st.arg;
         atomicOr(a.err, VF_ERR_EMPTY);
     }
-    if (__syncthreads_or(bad_q ? 1 : 0) && threadIdx.x == 0) atomicOr(a.err, VF_ERR_DRAFT);
-    cg::this_cluster().sync();                                    // block 0's sums stay until every block has read them
+    if (bad_q) atomicOr(a.err, VF_ERR_DRAFT);
 }
 
 static int verify_parts(int vocab) { return (vocab + VF_PART - 1) / VF_PART; }
@@ -466,7 +576,7 @@ static cudaError_t launch_cluster(K kernel, int blocks, int threads, size_t smem
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-// `scratch`: 16 bytes a row and part of 8,192 columns, then 8 bytes a row (16-byte aligned).
+// `scratch`: 16 bytes a row and part of 4,096 columns, then 8 bytes a row (16-byte aligned).
 extern "C" int cml_verify_drafts(const float* logits, long long ld, int n_rows, int vocab, const int* row0, const int* lens,
                                  const int* drafts, long long drafts_ld, const float* probs, long long probs_seq,
                                  long long probs_step, const float* accept, long long accept_ld, const float* draws, int n_seqs,
@@ -488,14 +598,16 @@ extern "C" int cml_verify_drafts(const float* logits, long long ld, int n_rows, 
     a.parts = filters ? 1 : verify_parts(vocab);
     if ((long long)n_rows * max(a.parts, 8) > 0x7fffffffLL || (long long)n_seqs * 8 > 0x7fffffffLL) return CML_ERR_BAD_SIZE;
     cudaStream_t s = (cudaStream_t)stream;
-    int team = vocab >= 32768 ? 8 : (vocab >= 8192 ? 4 : 1);
+    const int team = vocab >= 32768 ? 8 : (vocab >= 8192 ? 4 : 1);
     if (n_rows > 0) {
         cudaError_t e;
         if (filters) {
+            int share = team;                                      // a block takes a multiprocessor to itself
+            while (share > 1 && (long long)n_rows * share > cml_sm_count()) share /= 2;
             a.floors = (unsigned long long*)((char*)scratch + 16ll * n_rows * verify_parts(vocab));
             e = cml_allow_smem<verify_floor_kernel>(sizeof(FastSharedOf<double>));
             if (e != cudaSuccess) return (int)e;
-            e = launch_cluster(verify_floor_kernel, n_rows * team, SAMPLE_THREADS, sizeof(FastSharedOf<double>), team, s, a);
+            e = launch_cluster(verify_floor_kernel, n_rows * share, SAMPLE_THREADS, sizeof(FastSharedOf<double>), share, s, a);
         } else {
             e = launch_pdl(verify_stats_kernel, dim3((unsigned)(n_rows * a.parts)), dim3(VF_PART_THREADS), 0, s, a);
         }
