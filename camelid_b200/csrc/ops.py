@@ -2139,7 +2139,7 @@ def evict_positions(k_pages, v_pages, scores, block_table, out_table, lengths, k
         _p(inv_freq), rotary_dim, 1 if interleaved else 0, _stream()), "evict_positions", 2)
 
 
-VERIFY_PART = 4096              # columns of a row of logits that a block adds up; VF_PART in verify.cu
+VERIFY_PART = 1024              # columns of a row of logits that a warp adds up; VF_PART in verify.cu
 
 
 def verify_bytes(rows: int, n_seqs: int, vocab: int) -> int:

@@ -15,14 +15,15 @@
 // Everything that a decision rests on is computed in double, because a rounding of 2^-24 in a sum over 128,256 tokens
 // would move one draw in a hundred to a neighbouring token: exp((l - max) / T), its sums, the thresholds.
 //
-// Two launches, three with filters: (1) the maximum and the sum of every row, in parts of 4,096 columns, or, with
+// Two launches, three with filters: (1) the maximum and the sum of every row, in parts of 1,024 columns, or, with
 // filters, the same of the candidates, by a cluster per row (row_select.cuh); (2) a cluster per sequence decides how
 // many tokens stay, adds up the one row that the next token is drawn from, warp by warp, and walks the warp's stretch
 // in which the crossing lies.
 #include "row_select.cuh"
 
-#define VF_PART 4096            // columns of a row that one block adds up
+#define VF_PART 1024            // columns of a row that one warp adds up
 #define VF_PART_THREADS 256
+#define VF_PART_BLOCKS 3        // a multiprocessor: two (127 registers) are 8% slower over 449 rows, four (64) 3%
 #define VF_THREADS 512          // threads of a block that decides
 #define VF_WARPS (VF_THREADS / 32)
 
@@ -76,13 +77,14 @@ __device__ __forceinline__ Exponential exponential_of(float max, float temperatu
     Exponential e;
     e.c = 46.166241308446828 / (double)temperature;
     e.max = (double)max;
-    e.least = (float)((double)max - 700.0 * (double)temperature);
+    e.least = fmaxf((float)((double)max - 700.0 * (double)temperature), -3.402823466e38f);
     return e;
 }
 __device__ __forceinline__ void fill_table(double* table) {       // by the first warp; a barrier follows
     if (threadIdx.x < 32) table[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
 }
-__device__ __forceinline__ double weight_of(float l, const Exponential& e, const double* table) {
+// `l` at least e.least: what lies below stands for e^-700, which adds nothing to a sum of one or more
+__device__ __forceinline__ double power_of(float l, const Exponential& e, const double* table) {
     const double d = (double)l - e.max;
     const double shifted = fma(d, e.c, 6755399441055744.0);       // 1.5 * 2^52: the whole number in the low bits
     const double r = fma(d, e.c, -(shifted - 6755399441055744.0));
@@ -90,81 +92,78 @@ __device__ __forceinline__ double weight_of(float l, const Exponential& e, const
     constexpr double C1 = 0.021660849392498290, C2 = C1 * C1 / 2, C3 = C1 * C1 * C1 / 6, C4 = C1 * C1 * C1 * C1 / 24;
     const double p = fma(r, fma(r, fma(r, fma(r, C4, C3), C2), C1), 1.0);
     const double t = table[k & 31];
-    const double scaled = __hiloint2double(__double2hiint(t) + ((k >> 5) << 20), __double2loint(t));
-    return l < e.least ? 0.0 : scaled * p;
+    return __hiloint2double(__double2hiint(t) + ((k << 15) & 0xfff00000), __double2loint(t)) * p;
+}
+// the same, and exactly zero below
+__device__ __forceinline__ double weight_of(float l, const Exponential& e, const double* table) {
+    const double w = power_of(fmaxf(l, e.least), e, table);
+    return l < e.least ? 0.0 : w;
 }
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < CUDART_INF_F; }
 
-// (1a) without filters. A thread keeps its 16 columns in registers, so the row is read once; the block's maximum is the
-// reference of its exponentials, and the parts are joined where they are read.
-__global__ void __launch_bounds__(VF_PART_THREADS) verify_stats_kernel(VerifyArgs a) {
-    __shared__ float fred[33];
-    __shared__ double dred[33];
-    __shared__ int ired[33];
+// (1a) without filters. A warp takes a part at a time and keeps its 32 columns a lane in registers, so that the row is read
+// once. The part's maximum is the reference of its exponentials; the parts are joined where they are read. No barriers;
+// the blocks stay, so the table is made once.
+__global__ void __launch_bounds__(VF_PART_THREADS, VF_PART_BLOCKS) verify_stats_kernel(VerifyArgs a) {
     __shared__ double table[32];
     fill_table(table);
+    __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
-    const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
-    const float* r = a.logits + (long long)row * a.ld;
-    const int begin = part * VF_PART, end = min(a.vocab, begin + VF_PART);
-    constexpr int U = VF_PART / (4 * VF_PART_THREADS);
-    float4 v[U];
-    const bool vec = (((uintptr_t)r) & 15) == 0;
+    const int lane = threadIdx.x & 31;
+    const int warps = gridDim.x * (VF_PART_THREADS / 32), items = a.n_rows * a.parts;
+    constexpr int U = VF_PART / 32;
+    constexpr float LOWEST = -3.402823466e38f;                    // what stands in the columns behind a row
+    for (int item = blockIdx.x * (VF_PART_THREADS / 32) + (threadIdx.x >> 5); item < items; item += warps) {
+        const int row = item / a.parts, begin = (item - row * a.parts) * VF_PART, n = min(VF_PART, a.vocab - begin);
+        const float* r = a.logits + (long long)row * a.ld + begin;
+        const bool vec = (((uintptr_t)r) & 15) == 0;
+        float v[U];
+        if (vec) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int i = begin + 4 * (u * VF_PART_THREADS + (int)threadIdx.x);
-        if (vec && i + 4 <= end) v[u] = *reinterpret_cast<const float4*>(r + i);
-        else {
-            v[u].x = i < end ? r[i] : -CUDART_INF_F;
-            v[u].y = i + 1 < end ? r[i + 1] : -CUDART_INF_F;
-            v[u].z = i + 2 < end ? r[i + 2] : -CUDART_INF_F;
-            v[u].w = i + 3 < end ? r[i + 3] : -CUDART_INF_F;
-        }
-    }
-    float mx = -CUDART_INF_F;
-    int arg = 0x7fffffff;
-    bool bad = false;
+            for (int g = 0; g < U / 4; ++g) {
+                const int i = g * 128 + 4 * lane;
+                if (i + 4 <= n) {
+                    const float4 t = *reinterpret_cast<const float4*>(r + i);
+                    v[4 * g] = t.x, v[4 * g + 1] = t.y, v[4 * g + 2] = t.z, v[4 * g + 3] = t.w;
+                } else {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int i = begin + 4 * (u * VF_PART_THREADS + (int)threadIdx.x);
-        const float e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (i + k < end) {
-                bad = bad || !finite(e[k]);
-                if (e[k] > mx || (arg == 0x7fffffff)) mx = e[k], arg = i + k;
+                    for (int k = 0; k < 4; ++k) v[4 * g + k] = i + k < n ? r[i + k] : LOWEST;
+                }
             }
-        }
-    }
-    const float bmax = block_max(mx, fred);
-    // the lowest place of the maximum (a thread's places ascend, and it keeps the first)
-    int at = mx == bmax ? arg : 0x7fffffff;
+        } else {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
-    if ((threadIdx.x & 31) == 0) ired[threadIdx.x >> 5] = at;
-    double s = 0.0;
-    if (a.temperature > 0.f) {
-        const Exponential ex = exponential_of(bmax, a.temperature);
+            for (int u = 0; u < U; ++u) v[u] = u * 32 + lane < n ? r[u * 32 + lane] : LOWEST;
+        }
+        float mx = LOWEST, check = 0.f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = begin + 4 * (u * VF_PART_THREADS + (int)threadIdx.x);
-            const float e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (i + k < end) s += weight_of(e[k], ex, table);
+            mx = fmaxf(mx, v[u]);
+            check = fmaf(v[u], 0.f, check);                       // not a number once a logit is not finite
         }
-    }
-    s = block_sum_double(s, dred);
-    const int any_bad = __syncthreads_or(bad ? 1 : 0);
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < VF_PART_THREADS / 32; ++w) at = min(at, ired[w]);
         PartStat st;
-        st.sum = s;
-        st.max = any_bad ? CUDART_NAN_F : bmax;
-        st.arg = at;
-        a.stats[(size_t)row * a.parts + part] = st;
+        st.max = warp_max(mx);
+        st.sum = 0.0;
+        st.arg = 0;
+        if (a.temperature > 0.f) {
+            const Exponential ex = exponential_of(st.max, a.temperature);
+            double s[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+            for (int u = 0; u < U; ++u) s[u & 3] += power_of(fmaxf(v[u], ex.least), ex, table);
+            double t = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            st.sum = t;
+        } else {
+            int at = 0x7fffffff;                                  // the lowest place of the maximum
+#pragma unroll
+            for (int u = U - 1; u >= 0; --u)
+                if (v[u] == st.max) at = vec ? (u / 4) * 128 + 4 * lane + (u & 3) : u * 32 + lane;
+            st.arg = begin + __reduce_min_sync(0xffffffffu, at);
+        }
+        if (__any_sync(0xffffffffu, check != 0.f)) st.max = CUDART_NAN_F;
+        if (lane == 0) a.stats[item] = st;
     }
 }
 
@@ -340,7 +339,8 @@ __device__ __forceinline__ RowStat join_parts(const VerifyArgs& a, int row, cons
 
 // (2) a cluster per sequence.
 #define VF_ROWS 32                   // rows whose joined parts a block remembers
-__global__ void __launch_bounds__(VF_THREADS) verify_decide_kernel(VerifyArgs a) {
+#define VF_GROUPS 8
+__global__ void __launch_bounds__(VF_THREADS, 2) verify_decide_kernel(VerifyArgs a) {
     __shared__ double table[32];
     __shared__ double warp_sums[2][VF_WARPS], block_sums[2][SAMPLE_MAX_TEAM];     // of two rounds
     __shared__ RowStat stats[VF_ROWS];
@@ -431,10 +431,11 @@ __global__ void __launch_bounds__(VF_THREADS) verify_decide_kernel(VerifyArgs a)
     const double inv_total = 1.0 / st.total;
     bool bad_q = false;
     bool plain = false;                                           // nothing is left of p - q: draw from p
-    // stretches of whole tiles of 128 columns, one a warp, in ascending order over the blocks of the cluster
+    // stretches of VF_GROUPS groups of whole tiles of 128 columns, a stretch a warp, in ascending order over the cluster's blocks
     const int warps = team * VF_WARPS;
-    const int per = (((vocab + warps - 1) / warps) + 127) & ~127;
-    const int begin = min(vocab, (rank * VF_WARPS + warp) * per), end = min(vocab, begin + per);
+    const int group = (vocab + warps * VF_GROUPS * 128 - 1) / (warps * VF_GROUPS * 128) * 128, per = group * VF_GROUPS;
+    const long long first = (long long)(rank * VF_WARPS + warp) * per;
+    const int begin = (int)min((long long)vocab, first), end = (int)min((long long)vocab, first + per);
     const bool vec = (((uintptr_t)r) & 15) == 0 && (q == nullptr || (((uintptr_t)q) & 15) == 0);
     // four columns of a tile in a lane, ascending over the lanes
     auto load4 = [&](const float* from, int i, float (&v)[4]) {
@@ -462,20 +463,27 @@ __global__ void __launch_bounds__(VF_THREADS) verify_decide_kernel(VerifyArgs a)
         }
     };
     double total = 0.0, target, before = 0.0;
+    double groups[VF_GROUPS];                                     // this lane's share of every group's sum
     int owner = -1, round = 0;
     for (; round < 2; ++round) {
         double s = 0.0;
-        for (int i0 = begin + 4 * lane; i0 < end; i0 += 256) {    // two tiles in flight
-            float l0[4], l1[4], q0[4] = {0.f, 0.f, 0.f, 0.f}, q1[4] = {0.f, 0.f, 0.f, 0.f};
-            const int i1 = i0 + 128;
-            load4(r, i0, l0);
-            load4(r, i1, l1);
-            if (q) load4(q, i0, q0), load4(q, i1, q1);
-            double w[4];
-            weigh(i0, l0, q0, w);
-            s += (w[0] + w[1]) + (w[2] + w[3]);
-            weigh(i1, l1, q1, w);
-            s += (w[0] + w[1]) + (w[2] + w[3]);
+#pragma unroll
+        for (int g = 0; g < VF_GROUPS; g += 2) {                  // two groups in flight
+            double s0 = 0.0, s1 = 0.0;
+            for (int i = 0; i < group; i += 128) {
+                const int i0 = begin + g * group + i + 4 * lane, i1 = i0 + group;
+                float l0[4], l1[4], q0[4] = {0.f, 0.f, 0.f, 0.f}, q1[4] = {0.f, 0.f, 0.f, 0.f};
+                load4(r, i0, l0);
+                load4(r, i1, l1);
+                if (q) load4(q, i0, q0), load4(q, i1, q1);
+                double w[4];
+                weigh(i0, l0, q0, w);
+                s0 += (w[0] + w[1]) + (w[2] + w[3]);
+                weigh(i1, l1, q1, w);
+                s1 += (w[0] + w[1]) + (w[2] + w[3]);
+            }
+            groups[g] = s0, groups[g + 1] = s1;
+            s += s0 + s1;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -513,9 +521,21 @@ __global__ void __launch_bounds__(VF_THREADS) verify_decide_kernel(VerifyArgs a)
             if (run > target) break;
         }
         if (warp == mine) {
+            // the group of the crossing from the sums in registers, then its columns
+            int in = -1;
+            run = before;
+#pragma unroll
+            for (int g = 0; g < VF_GROUPS; ++g) {
+                double s = groups[g];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                if (s > 0.0 && (in < 0 || !(run > target))) in = g, before = run;
+                run += s;
+            }
             run = before;
             int found = -1, last = -1;
-            for (int i0 = begin; i0 < end; i0 += 128) {
+            const int g_begin = begin + in * group, g_end = min(end, g_begin + group);
+            for (int i0 = g_begin; i0 < g_end; i0 += 128) {
                 const int i = i0 + 4 * lane;
                 float l[4], qi[4] = {0.f, 0.f, 0.f, 0.f};
                 double w[4];
@@ -576,14 +596,14 @@ static cudaError_t launch_cluster(K kernel, int blocks, int threads, size_t smem
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-// `scratch`: 16 bytes a row and part of 4,096 columns, then 8 bytes a row (16-byte aligned).
+// `scratch`: 16 bytes a row and part of 1,024 columns, then 8 bytes a row (16-byte aligned).
 extern "C" int cml_verify_drafts(const float* logits, long long ld, int n_rows, int vocab, const int* row0, const int* lens,
                                  const int* drafts, long long drafts_ld, const float* probs, long long probs_seq,
                                  long long probs_step, const float* accept, long long accept_ld, const float* draws, int n_seqs,
                                  int width, float temperature, int top_k, float top_p, float min_p, int* counts, int* tokens,
                                  int* err, void* scratch, void* stream) {
     if (n_seqs <= 0) return 0;
-    if (vocab <= 0 || vocab > 0x7fffff00 || n_rows < 0 || width < 0 || width > 65535 || !(temperature >= 0.f) ||
+    if (vocab <= 0 || vocab > (1 << 30) || n_rows < 0 || width < 0 || width > 65535 || !(temperature >= 0.f) ||
         !(temperature < __builtin_inff()))
         return CML_ERR_BAD_SIZE;
     if (((uintptr_t)scratch) & 15) return CML_ERR_BAD_ALIGN;
@@ -596,7 +616,7 @@ extern "C" int cml_verify_drafts(const float* logits, long long ld, int n_rows, 
     a.counts = counts; a.tokens = tokens; a.err = err;
     a.stats = (PartStat*)scratch;
     a.parts = filters ? 1 : verify_parts(vocab);
-    if ((long long)n_rows * max(a.parts, 8) > 0x7fffffffLL || (long long)n_seqs * 8 > 0x7fffffffLL) return CML_ERR_BAD_SIZE;
+    if ((long long)n_rows * (a.parts > 8 ? a.parts : 8) > 0x3fffffffLL || (long long)n_seqs * 8 > 0x7fffffffLL) return CML_ERR_BAD_SIZE;
     cudaStream_t s = (cudaStream_t)stream;
     const int team = vocab >= 32768 ? 8 : (vocab >= 8192 ? 4 : 1);
     if (n_rows > 0) {
@@ -609,7 +629,9 @@ extern "C" int cml_verify_drafts(const float* logits, long long ld, int n_rows, 
             if (e != cudaSuccess) return (int)e;
             e = launch_cluster(verify_floor_kernel, n_rows * share, SAMPLE_THREADS, sizeof(FastSharedOf<double>), share, s, a);
         } else {
-            e = launch_pdl(verify_stats_kernel, dim3((unsigned)(n_rows * a.parts)), dim3(VF_PART_THREADS), 0, s, a);
+            const long long blocks = ((long long)n_rows * a.parts + VF_PART_THREADS / 32 - 1) / (VF_PART_THREADS / 32);
+            const long long most = (long long)VF_PART_BLOCKS * cml_sm_count();
+            e = launch_pdl(verify_stats_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(VF_PART_THREADS), 0, s, a);
         }
         if (e != cudaSuccess) return (int)e;
     }
