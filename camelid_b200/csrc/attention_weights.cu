@@ -12,7 +12,9 @@
 // (3) the products q . k are made again and every key's weights summed, in a fixed order of the rows. Products,
 // softmax and sums are float.
 #include "common.cuh"
+#include <cooperative_groups.h>
 #include <math_constants.h>
+namespace cg = cooperative_groups;
 
 #define AW_THREADS 128
 #define AW_ROWS 8               // rows (token, head) a block works on together
@@ -39,7 +41,8 @@ struct WeightArgs {
     float* stats;                // [seqs * kv heads][splits][rows][2]: maximum and sum of a stretch
     float* joined;               // [seqs * kv heads][rows][2]: maximum and 1 / sum of all
     float* acc;                  // [seqs * kv heads][splits][rows][v_dim]
-    float* kept;                 // [seqs * kv heads][rows][splits * split_keys]: q . k, scaled, of steps of few rows
+    float* kept;                 // [seqs * kv heads][rows][kept_stride]: q . k of steps of few rows
+    long long kept_stride;       // max_len rounded up to a page
 };
 
 struct Seq {
@@ -344,21 +347,28 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src
 #define AM_WARPS 4
 #define AM_STAGES 3
 
-// (1) a stretch of keys for up to 16 * MT rows of a (sequence, kv head); grid (stretches, pairs, row chunks). A warp takes every
-// fourth tile of TILE keys with a ring of its own in shared memory, and the warps' ranges are joined at the end in
-// their order. OUT: with values and output. KEEP: the scaled products are kept for (3).
-template <int HD, int MT, bool OUT, bool KEEP>
+// Up to 16 * MT rows of a (sequence, kv head). A warp takes every eighth tile of TILE keys of the block's stretch with a ring of
+// its own in shared memory, and the warps' ranges are joined at the end in their order. OUT: with values and output.
+// ALL (grid: cluster, pairs): the blocks of a cluster share all keys of a sequence, exchange their rows' maxima and sums over
+// distributed shared memory, join the output and sum the weights of their own keys, whose products they kept: one
+// launch does it all. Otherwise (grid: stretches, pairs, row chunks) this is step (1).
+template <int HD, int MT, bool OUT, bool ALL>
 __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightArgs a) {
     constexpr int TILE = HD == 128 ? 16 : 32;
     constexpr int LDS = HD + 8, KS = HD / 16, DT = HD / 8, NT = TILE / 8, KK = TILE / 16, CH = HD / 8;
     constexpr int HALF = TILE * LDS * 2, STAGE = HALF * (OUT ? 2 : 1);        // bytes
+    constexpr int TEAM = MT == 1 ? 16 : 8;                                    // blocks of a cluster at most
     extern __shared__ __align__(16) unsigned char raw[];
     pdl_wait();
     pdl_launch_dependents();
     const int split = blockIdx.x, seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads, m0 = blockIdx.z * 16 * MT;
     const Seq s = seq_of(a, seq);
-    const int first = split * a.split_keys, last = min(s.length, first + a.split_keys);
-    if (first >= last || m0 >= s.rows) return;
+    if (m0 >= s.rows) return;                                                 // the same for a whole cluster
+    const int team = ALL ? (int)gridDim.x : 1;
+    const int share = ALL ? (s.length + team * TILE - 1) / (team * TILE) * TILE : a.split_keys;
+    const int first = split * share, last = min(s.length, first + share);
+    if (ALL) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");        // started: waited for before remote stores
+    else if (first >= last) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = a.heads / a.kv_heads;
     const int* pages = a.table + (size_t)seq * a.width;
@@ -367,30 +377,47 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
     unsigned char* mine = raw + (size_t)warp * AM_STAGES * STAGE;
     const uint32_t mine32 = (uint32_t)__cvta_generic_to_shared(mine);
     const int t_first = first / TILE, t_last = (last + TILE - 1) / TILE;
-    const int n_mine = (t_last - t_first - warp + AM_WARPS - 1) / AM_WARPS;
-    auto page_of = [&](int t) { return pages[t * TILE / CML_PAGE]; };
+    const int n_mine = max(0, t_last - t_first - warp + AM_WARPS - 1) / AM_WARPS;
     auto there = [&](int page) { return page >= 0 && page < a.n_pages; };
-    int page_next = 0 < n_mine ? page_of(t_first + warp) : -1;               // a tile's page is looked up a tile ahead
-    auto issue = [&](int it) {
-        if (it < n_mine) {
-            const int t = t_first + warp + it * AM_WARPS;
-            const int page = page_next;
-            if (it + 1 < n_mine) page_next = page_of(t + AM_WARPS);
+    int page_next = 0 < n_mine ? pages[(t_first + warp) * TILE / CML_PAGE] : -1;         // a tile's page is looked up a tile ahead
+    unsigned int missing = 0u;                                                // a bit for each stage: its page is none
+    // this lane's 16 bytes of a tile's first rows, in the page and in the stage; the others lie at constant distances
+    const int lane_row = lane / CH, lane_in = lane_row * HD + lane % CH * 8;
+    const uint32_t lane_out = mine32 + (uint32_t)(lane_row * LDS + lane % CH * 8) * 2;
+    const bf16* const k_lane = kp + (size_t)kvh * CML_PAGE * HD + lane_in;
+    const bf16* const v_lane = OUT ? vp + (size_t)kvh * CML_PAGE * HD + lane_in : nullptr;
+    const size_t page_elems = (size_t)a.kv_heads * CML_PAGE * HD;
+    int next_tile = t_first + warp, next_stage = 0, to_issue = n_mine;
+    auto issue = [&]() {
+        if (to_issue > 0) {
+            const int t = next_tile, page = page_next;
+            next_tile += AM_WARPS;
+            if (--to_issue > 0) page_next = pages[next_tile * TILE / CML_PAGE];
             const bool ok = there(page);
-            const size_t base = (((size_t)(ok ? page : 0) * a.kv_heads + kvh) * CML_PAGE + (t * TILE) % CML_PAGE) * HD;
-            const uint32_t dst = mine32 + (uint32_t)(it % AM_STAGES) * STAGE;
+            const size_t at = (size_t)(ok ? page : 0) * page_elems + (size_t)(t * TILE % CML_PAGE) * HD;
+            const uint32_t dst = lane_out + (uint32_t)next_stage * STAGE;
             const int valid = ok ? last - t * TILE : 0;
+            missing = ok ? missing & ~(1u << next_stage) : missing | (1u << next_stage);
+            if (valid >= TILE) {
 #pragma unroll
-            for (int c0 = 0; c0 < TILE * CH; c0 += 32) {
-                const int c = c0 + lane, r = c / CH, cc = c % CH;
-                cp_async16_or_zero(dst + (uint32_t)(r * LDS + cc * 8) * 2, kp + base + (size_t)r * HD + cc * 8, r < valid);
-                if (OUT) cp_async16_or_zero(dst + HALF + (uint32_t)(r * LDS + cc * 8) * 2, vp + base + (size_t)r * HD + cc * 8, r < valid);
+                for (int c = 0; c < TILE * CH / 32; ++c) {
+                    cp_async16(dst + c * (32 / CH) * LDS * 2, k_lane + at + c * (32 / CH) * HD);
+                    if (OUT) cp_async16(dst + HALF + c * (32 / CH) * LDS * 2, v_lane + at + c * (32 / CH) * HD);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < TILE * CH / 32; ++c) {
+                    const bool in = lane_row + c * (32 / CH) < valid;
+                    cp_async16_or_zero(dst + c * (32 / CH) * LDS * 2, k_lane + at + c * (32 / CH) * HD, in);
+                    if (OUT) cp_async16_or_zero(dst + HALF + c * (32 / CH) * LDS * 2, v_lane + at + c * (32 / CH) * HD, in);
+                }
             }
+            next_stage = next_stage + 1 == AM_STAGES ? 0 : next_stage + 1;
         }
         cp_async_commit();
     };
 #pragma unroll
-    for (int i = 0; i < AM_STAGES - 1; ++i) issue(i);
+    for (int i = 0; i < AM_STAGES - 1; ++i) issue();
     // the rows of q as A fragments (zero where there is no row); a thread holds rows lane / 4 and + 8 of each 16
     uint32_t qa[MT][KS][4];
     int pos[MT][2];                                                           // the last place a row sees, -1: no row
@@ -420,15 +447,18 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
     }
     const int mat = lane >> 3, rr = lane & 7;
     const int group_rows = a.max_new * group;
-    float* const kept = KEEP ? a.kept + (size_t)blockIdx.y * group_rows * a.n_splits * a.split_keys : nullptr;
-    for (int it = 0; it < n_mine; ++it) {
-        const int t = t_first + warp + it * AM_WARPS;
+    float* const kept = ALL ? a.kept + (size_t)blockIdx.y * group_rows * a.kept_stride : nullptr;
+    int stage = 0;
+    const uint32_t k_frag = mine32 + (uint32_t)(((mat >> 1) * 8 + rr) * LDS + (mat & 1) * 8) * 2;
+    const uint32_t v_frag = mine32 + HALF + (uint32_t)(((mat & 1) * 8 + rr) * LDS + (mat >> 1) * 8) * 2;
+    for (int place0 = (t_first + warp) * TILE; place0 < last; place0 += AM_WARPS * TILE) {
         cp_async_wait<AM_STAGES - 2>();
         __syncwarp();
-        const bool ok = there(page_of(t));
-        issue(it + AM_STAGES - 1);
-        const uint32_t k32 = mine32 + (uint32_t)(it % AM_STAGES) * STAGE, v32 = k32 + HALF;
-        const int place0 = t * TILE;
+        const bool ok = (missing >> stage & 1u) == 0u;
+        issue();
+        const uint32_t k32 = k_frag + (uint32_t)stage * STAGE, v32 = v_frag + (uint32_t)stage * STAGE;
+        unsigned char* const here = mine + (size_t)stage * STAGE;
+        stage = stage + 1 == AM_STAGES ? 0 : stage + 1;
         float x[MT][NT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -439,78 +469,107 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
 #pragma unroll
             for (int np = 0; np < NT / 2; ++np) {
                 uint32_t b0, b1, b2, b3;
-                ldsm_x4(k32 + (uint32_t)((np * 16 + (mat >> 1) * 8 + rr) * LDS + ks * 16 + (mat & 1) * 8) * 2, b0, b1, b2, b3);
+                ldsm_x4(k32 + (np * 16 * LDS + ks * 16) * 2, b0, b1, b2, b3);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     mma_bf16(x[mt][np * 2], qa[mt][ks], b0, b1);
                     mma_bf16(x[mt][np * 2 + 1], qa[mt][ks], b2, b3);
                 }
             }
-        // scale, mask, running maximum
+        // mask; the products are kept
         const int key0 = place0 + 2 * (lane & 3);
+        const bool whole = ok && place0 + TILE - 1 <= s.start && place0 + TILE <= last;     // every row sees every key
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            float now[2] = {top[mt][0], top[mt][1]};
+            if (!whole) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = key0 + n * 8 + (i & 1);
-                    x[mt][n][i] = ok && key < last && key <= pos[mt][i >> 1] ? x[mt][n][i] * a.scale : -CUDART_INF_F;
-                    now[i >> 1] = fmaxf(now[i >> 1], x[mt][n][i]);
-                }
-            if (KEEP) {
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = key0 + n * 8 + (i & 1);
+                        if (!(ok && key < last && key <= pos[mt][i >> 1])) x[mt][n][i] = -CUDART_INF_F;
+                    }
+            }
+            if (ALL) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
                     if (pos[mt][h] >= 0) {
-                        float* row = kept + (size_t)(m0 + mt * 16 + (lane >> 2) + 8 * h) * a.n_splits * a.split_keys + key0;
+                        float* row = kept + (size_t)(mt * 16 + (lane >> 2) + 8 * h) * a.kept_stride + key0;
 #pragma unroll
                         for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(row + n * 8) = make_float2(x[mt][n][2 * h], x[mt][n][2 * h + 1]);
                     }
             }
+        }
+        // The reference of the exponentials moves only when a row passes it by a factor of 2^6: a vote, seldom more.
+        float now[MT][2];
+        bool passed = false;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                now[h] = fmaxf(now[h], __shfl_xor_sync(0xffffffffu, now[h], 1));
-                now[h] = fmaxf(now[h], __shfl_xor_sync(0xffffffffu, now[h], 2));
+                now[mt][h] = x[mt][0][2 * h];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) now[mt][h] = fmaxf(now[mt][h], fmaxf(x[mt][n][2 * h], x[mt][n][2 * h + 1]));
+                now[mt][h] *= a.scale;
+                passed = passed || now[mt][h] > top[mt][h] + 6.f;
             }
-            if (__any_sync(0xffffffffu, now[0] != top[mt][0] || now[1] != top[mt][1])) {
+        if (__any_sync(0xffffffffu, passed)) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float corr = top[mt][h] == -CUDART_INF_F ? 0.f : fast_exp2(top[mt][h] - now[h]);
-                    top[mt][h] = now[h];
+                    float next = fmaxf(now[mt][h], __shfl_xor_sync(0xffffffffu, now[mt][h], 1));
+                    next = fmaxf(top[mt][h], fmaxf(next, __shfl_xor_sync(0xffffffffu, next, 2)));
+                    const float corr = top[mt][h] == -CUDART_INF_F ? 0.f : fast_exp2(top[mt][h] - next);
+                    top[mt][h] = next;
                     sum[mt][h] *= corr;
 #pragma unroll
                     for (int d = 0; d < (OUT ? DT : 1); ++d) o[mt][d][2 * h] *= corr, o[mt][d][2 * h + 1] *= corr;
                 }
-            }
-            const float ref[2] = {top[mt][0] == -CUDART_INF_F ? 0.f : top[mt][0], top[mt][1] == -CUDART_INF_F ? 0.f : top[mt][1]};
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[mt][n][i] = fast_exp2(x[mt][n][i] - ref[i >> 1]);
-                    sum[mt][i >> 1] += x[mt][n][i];
-                }
         }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float ref = top[mt][h] == -CUDART_INF_F ? 0.f : top[mt][h];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        x[mt][n][2 * h + i] = fast_exp2(fmaf(x[mt][n][2 * h + i], a.scale, -ref));
+                        sum[mt][h] += x[mt][n][2 * h + i];
+                    }
+            }
         if (OUT) {
-            bf16* vs = reinterpret_cast<bf16*>(mine + (size_t)(it % AM_STAGES) * STAGE + HALF);
+            bf16* vs = reinterpret_cast<bf16*>(here + HALF);
             if (s.fresh > 1 && place0 + TILE > s.start + 1) {
                 // New places that not every row sees: a probability of zero times what such a place holds must stay zero even
                 // where that is infinite, so their products are made apart, and the tensor cores get zeros.
+                // The probabilities pass through the room of the tile's keys, which are done.
+                float* ps = reinterpret_cast<float*>(here);                   // [16 * MT rows][TILE]
+                __syncwarp();
 #pragma unroll
-                for (int kk = 0; kk < TILE; ++kk) {
-                    const int place = place0 + kk;
-                    if (place <= s.start || place >= last) continue;          // the same in the whole warp
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            *reinterpret_cast<float2*>(ps + (mt * 16 + (lane >> 2) + 8 * h) * TILE + n * 8 + 2 * (lane & 3)) =
+                                make_float2(x[mt][n][2 * h], x[mt][n][2 * h + 1]);
+                __syncwarp();
+#pragma unroll 1
+                for (int kk = max(0, s.start + 1 - place0); kk < TILE && place0 + kk < last; ++kk) {
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const float p = __shfl_sync(0xffffffffu, x[mt][kk / 8][2 * h + (kk & 1)], (lane & ~3) | ((kk & 7) >> 1));
+                            const float p = ps[(mt * 16 + (lane >> 2) + 8 * h) * TILE + kk];
                             if (p != 0.f) {
 #pragma unroll
                                 for (int d = 0; d < DT; ++d) {
-                                    o[mt][d][2 * h] += p * to_f32(vs[kk * LDS + d * 8 + 2 * (lane & 3)]);
-                                    o[mt][d][2 * h + 1] += p * to_f32(vs[kk * LDS + d * 8 + 2 * (lane & 3) + 1]);
+                                    const uint32_t w = *reinterpret_cast<const uint32_t*>(vs + kk * LDS + d * 8 + 2 * (lane & 3));
+                                    o[mt][d][2 * h] = fmaf(p, __uint_as_float(w << 16), o[mt][d][2 * h]);
+                                    o[mt][d][2 * h + 1] = fmaf(p, __uint_as_float(w & 0xffff0000u), o[mt][d][2 * h + 1]);
                                 }
                             }
                         }
@@ -534,7 +593,7 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
 #pragma unroll
                 for (int dp = 0; dp < DT / 2; ++dp) {
                     uint32_t b0, b1, b2, b3;
-                    ldsm_x4_t(v32 + (uint32_t)((kk * 16 + (mat & 1) * 8 + rr) * LDS + dp * 16 + (mat >> 1) * 8) * 2, b0, b1, b2, b3);
+                    ldsm_x4_t(v32 + (kk * 16 * LDS + dp * 16) * 2, b0, b1, b2, b3);
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
                         mma_bf16(o[mt][dp * 2], pa[mt], b0, b1);
@@ -574,6 +633,11 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
     const size_t base = ((size_t)blockIdx.y * a.n_splits + split) * group_rows + m0;
     const int rows = min(16 * MT, s.rows - m0);
     constexpr int PER = OUT ? HD / 4 : 1;
+    float* const own = red + (size_t)AM_WARPS * 16 * MT * RW;                 // ALL: [16 * MT rows][HD], the block's output
+    __shared__ float2 stat_s[ALL ? TEAM * 16 * MT : 1];                // ALL: [blocks][rows] maximum and sum, of the whole cluster
+    __shared__ float factor_s[ALL ? TEAM * 16 * MT : 1];               // ALL: what a block's output counts in the joined one
+    __shared__ float2 join_s[ALL ? 16 * MT : 1];                              // ALL: [rows] maximum and 1 / sum of all keys
+    if (ALL) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     for (int i = threadIdx.x; i < rows * PER; i += AM_WARPS * 32) {
         const int m = i / PER, d = i % PER * 4;
         float most = -CUDART_INF_F, f[AM_WARPS], l = 0.f;
@@ -592,112 +656,110 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
                 const float4 t = *reinterpret_cast<const float4*>(red + ((size_t)w * 16 * MT + m) * RW + 4 + d);
                 v.x += f[w] * t.x; v.y += f[w] * t.y; v.z += f[w] * t.z; v.w += f[w] * t.w;
             }
-            *reinterpret_cast<float4*>(a.acc + (base + m) * HD + d) = v;
+            *reinterpret_cast<float4*>(ALL ? own + m * HD + d : a.acc + (base + m) * HD + d) = v;
         }
         if (d == 0) {
-            a.stats[(base + m) * 2] = most;
-            a.stats[(base + m) * 2 + 1] = l;
+            if (ALL) {
+                for (int c = 0; c < team; ++c) cg::this_cluster().map_shared_rank(&stat_s[0], c)[split * 16 * MT + m] = make_float2(most, l);
+            } else {
+                a.stats[(base + m) * 2] = most;
+                a.stats[(base + m) * 2 + 1] = l;
+            }
         }
     }
-}
-
-// (2 and 3) of steps whose products are kept: the first blocks of a pair sum the weights of 256 keys each, the others join
-// the output of a row each. Grid (key blocks + rows, pairs).
-#define AK_THREADS 256
-#define AK_ROWS 16
-template <typename T, int HD>
-__global__ void __launch_bounds__(AK_THREADS) weights_finish_kernel(WeightArgs a, int key_blocks) {
-    __shared__ float top_s[AK_ROWS], inv_s[AK_ROWS];
-    pdl_wait();
-    pdl_launch_dependents();
-    const int seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
-    const Seq s = seq_of(a, seq);
-    const int group = a.heads / a.kv_heads, group_rows = a.max_new * group;
-    const int splits = (s.length + a.split_keys - 1) / a.split_keys;
-    const size_t base = (size_t)blockIdx.y * a.n_splits * group_rows;
-    const bool keys = (int)blockIdx.x < key_blocks;
-    const int key0 = blockIdx.x * AK_THREADS, row = (int)blockIdx.x - key_blocks;
-    if (keys ? key0 >= s.length : row >= s.rows) return;
-    // a warp joins a row's stretches: lanes take every 32nd, then a tree over the lanes
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int m = keys ? warp : row; m < (keys ? s.rows : row + 1); m += AK_THREADS / 32) {
-        float top = -CUDART_INF_F, sum = 0.f;
-        for (int i = lane; i < splits; i += 32) {
-            const float2 t = *reinterpret_cast<const float2*>(a.stats + (base + (size_t)i * group_rows + m) * 2);
-            const float now = fmaxf(top, t.x);
-            if (now != -CUDART_INF_F) sum = sum * exp2f(top - now) + exp2f(t.x - now) * t.y;
-            top = now;
+    if (!ALL) return;
+    cg::this_cluster().sync();
+    if ((int)threadIdx.x < rows) {
+        const int m = threadIdx.x;
+        float most = -CUDART_INF_F, l = 0.f;
+        for (int c = 0; c < team; ++c) most = fmaxf(most, stat_s[c * 16 * MT + m].x);
+        for (int c = 0; c < team; ++c) {
+            const float2 t = stat_s[c * 16 * MT + m];
+            const float f = t.x == -CUDART_INF_F ? 0.f : fast_exp2(t.x - most);
+            factor_s[c * 16 * MT + m] = f;
+            l += f * t.y;
         }
-        const float most = warp_max(top);
-        sum = most == -CUDART_INF_F ? 0.f : warp_sum(sum * exp2f(top - most));
-        if (lane == 0) {
-            top_s[m & (AK_ROWS - 1)] = most == -CUDART_INF_F ? 0.f : most;
-            inv_s[m & (AK_ROWS - 1)] = most == -CUDART_INF_F ? 0.f : 1.f / sum;
-        }
-        if (!keys) break;
+        join_s[m] = most == -CUDART_INF_F ? make_float2(0.f, 0.f) : make_float2(most, 1.f / l);
     }
     __syncthreads();
-    if (keys) {
-        const int place = key0 + threadIdx.x;
-        if (place >= s.length) return;
-        const int page = a.table[(size_t)seq * a.width + place / CML_PAGE];
-        if (page < 0 || page >= a.n_pages) return;
-        const size_t at = ((size_t)page * a.kv_heads + kvh) * CML_PAGE + place % CML_PAGE;
-        const float old = place < s.start ? a.scores[at] : 0.f;
-        const size_t stride = (size_t)a.n_splits * a.split_keys;
-        const float* x = a.kept + (size_t)blockIdx.y * group_rows * stride + place;
-        float gained = 0.f;
+    if (OUT) {                                                                // the output's elements in equal shares, the blocks in their order
+        const int pairs2 = rows * HD / 2;
+        for (int i = split * AM_WARPS * 32 + threadIdx.x; i < pairs2; i += team * AM_WARPS * 32) {
+            const int m = i / (HD / 2), d = i % (HD / 2) * 2;
+            float x = 0.f, y = 0.f;
 #pragma unroll 4
-        for (int m = 0; m < s.rows; ++m) gained += fast_exp2(x[m * stride] - top_s[m]) * inv_s[m];
-        a.scores_out[at] = old + gained;
-    } else {
-        const float top = top_s[row & (AK_ROWS - 1)], inv = inv_s[row & (AK_ROWS - 1)];
-        T* out = (T*)a.out + (long long)(s.row0 + row / group) * a.out_stride + (long long)(kvh * group + row % group) * HD;
-        for (int d = threadIdx.x; d < HD; d += AK_THREADS) {
-            float x = 0.f;
-            for (int i = 0; i < splits; ++i) {
-                const float t = a.stats[(base + (size_t)i * group_rows + row) * 2];
-                x += fast_exp2(t - top) * a.acc[(base + (size_t)i * group_rows + row) * HD + d];
+            for (int c = 0; c < team; ++c) {
+                const float2 t = *reinterpret_cast<const float2*>(cg::this_cluster().map_shared_rank(own, c) + m * HD + d);
+                const float f = factor_s[c * 16 * MT + m];
+                x += f * t.x, y += f * t.y;
             }
-            out[d] = from_f32<T>(x * inv);
+            const float inv = join_s[m].y;
+            bf16* dst = (bf16*)a.out + (long long)(s.row0 + m / group) * a.out_stride + (long long)(kvh * group + m % group) * HD + d;
+            if ((a.out_stride & 1) == 0 && (((uintptr_t)a.out) & 3) == 0) *reinterpret_cast<uint32_t*>(dst) = pack_bf16(x * inv, y * inv);
+            else dst[0] = __float2bfloat16_rn(x * inv), dst[1] = __float2bfloat16_rn(y * inv);
         }
     }
-}
-
-template <typename T>
-static cudaError_t launch_plain(WeightArgs& a, cudaStream_t s) {
-    const unsigned pairs = (unsigned)a.n_seqs * (unsigned)a.kv_heads;
-    const int group_rows = a.max_new * (a.heads / a.kv_heads);
-    const size_t k_page = (size_t)CML_PAGE * (a.k_dim * sizeof(T) + 16), v_page = a.out ? (size_t)CML_PAGE * a.v_dim * sizeof(T) : 0;
-    const size_t rows = (size_t)AW_ROWS * a.k_dim * 4;
-    const size_t rest = rows + AW_ROWS * CML_PAGE * 4 + 3 * AW_ROWS * 4, smem3 = k_page + rows;
-    a.stages = 2 * (k_page + v_page) + rest <= 227 * 1024 ? 2 : 1;
-    const size_t smem1 = a.stages * (k_page + v_page) + rest;
-    cudaError_t e = cml_allow_smem<weights_part_kernel<T>>(smem1);
-    if (e == cudaSuccess) e = cml_allow_smem<weights_sum_kernel<T>>(smem3);
-    if (e != cudaSuccess) return e;
-    e = launch_pdl(weights_part_kernel<T>, dim3((unsigned)a.n_splits, pairs, (unsigned)((group_rows + AW_ROWS - 1) / AW_ROWS)), dim3(AW_THREADS),
-                   smem1, s, a);
-    if (e != cudaSuccess) return e;
-    e = launch_pdl(weights_join_kernel<T>, dim3((unsigned)group_rows, pairs), dim3(AW_THREADS), 0, s, a);
-    if (e != cudaSuccess) return e;
-    return launch_pdl(weights_sum_kernel<T>, dim3((unsigned)((a.max_len + CML_PAGE - 1) / CML_PAGE), pairs), dim3(AW_THREADS), smem3, s, a);
+    // the weights of this block's keys, two groups of four keys a thread in flight
+    for (int group0 = first + 4 * (int)threadIdx.x; group0 < last; group0 += 2 * AM_WARPS * 128) {
+        float g[2][4], old[2][4];
+        size_t at[2];
+        bool has[2];
+        const float* x[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int place = group0 + u * AM_WARPS * 128;
+            const int page = place < last ? pages[place / CML_PAGE] : -1;
+            has[u] = there(page);
+            at[u] = ((size_t)(has[u] ? page : 0) * a.kv_heads + kvh) * CML_PAGE + place % CML_PAGE;
+            const float4 t = *reinterpret_cast<const float4*>(a.scores + at[u]);
+            old[u][0] = t.x, old[u][1] = t.y, old[u][2] = t.z, old[u][3] = t.w;
+            x[u] = kept + (has[u] ? place : first);
+            g[u][0] = g[u][1] = g[u][2] = g[u][3] = 0.f;
+        }
+#pragma unroll 4
+        for (int m = 0; m < rows; ++m) {
+            const float2 j = join_s[m];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const float4 t = *reinterpret_cast<const float4*>(x[u] + (size_t)m * a.kept_stride);
+                g[u][0] = fmaf(fast_exp2(fmaf(t.x, a.scale, -j.x)), j.y, g[u][0]);
+                g[u][1] = fmaf(fast_exp2(fmaf(t.y, a.scale, -j.x)), j.y, g[u][1]);
+                g[u][2] = fmaf(fast_exp2(fmaf(t.z, a.scale, -j.x)), j.y, g[u][2]);
+                g[u][3] = fmaf(fast_exp2(fmaf(t.w, a.scale, -j.x)), j.y, g[u][3]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (!has[u]) continue;
+            const int place = group0 + u * AM_WARPS * 128;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) g[u][k] += place + k < s.start ? old[u][k] : 0.f;
+            if (place + 4 <= last) *reinterpret_cast<float4*>(a.scores_out + at[u]) = make_float4(g[u][0], g[u][1], g[u][2], g[u][3]);
+            else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (place + k < last) a.scores_out[at[u] + k] = g[u][k];
+            }
+        }
+    }
+    if (OUT) cg::this_cluster().sync();                                       // a block's output stays until every block has read it
 }
 
 // (1) without output, for many rows (a prompt's last ones): a warp keeps 64 rows of q in registers and lets the keys pass;
 // grid (stretches, pairs, row chunks). The block's warps share the rows (`row_warps` of them) and the 16-key pieces of
 // a page. A thread keeps a maximum and a sum of its own for each of its eight rows, the maximum moves only when it is passed
 // by a factor of 2^6, and lanes and warps meet at the end. The exponentials (one a row and key) bound this kernel.
+#define AR_WARPS 4
 #define AR_STAGES 4
 template <int HD>
-__global__ void __launch_bounds__(AM_WARPS * 32, 2) weights_rows_mma_kernel(WeightArgs a, int row_warps) {
+__global__ void __launch_bounds__(AR_WARPS * 32, 2) weights_rows_mma_kernel(WeightArgs a, int row_warps) {
     constexpr int LDS = HD + 8, KS = HD / 16, CH = HD / 8, STAGE = CML_PAGE * LDS * 2;
     extern __shared__ __align__(16) unsigned char raw[];
     pdl_wait();
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = blockIdx.x, seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
-    const int m0 = ((int)blockIdx.z * row_warps + warp % row_warps) * 64, key_group = warp / row_warps, key_groups = AM_WARPS / row_warps;
+    const int m0 = ((int)blockIdx.z * row_warps + warp % row_warps) * 64, key_group = warp / row_warps, key_groups = AR_WARPS / row_warps;
     const Seq s = seq_of(a, seq);
     const int first = split * a.split_keys, last = min(s.length, first + a.split_keys);
     if (first >= last || (int)blockIdx.z * row_warps * 64 >= s.rows) return;
@@ -715,7 +777,7 @@ __global__ void __launch_bounds__(AM_WARPS * 32, 2) weights_rows_mma_kernel(Weig
             const bf16* src = (const bf16*)a.k + ((size_t)(valid ? pages[p] : 0) * a.kv_heads + kvh) * CML_PAGE * HD;
             const uint32_t dst = raw32 + (uint32_t)((p - p_first) % AR_STAGES) * STAGE;
 #pragma unroll
-            for (int c0 = 0; c0 < CML_PAGE * CH; c0 += AM_WARPS * 32) {
+            for (int c0 = 0; c0 < CML_PAGE * CH; c0 += AR_WARPS * 32) {
                 const int c = c0 + threadIdx.x, r = c / CH, cc = c % CH;
                 cp_async16_or_zero(dst + (uint32_t)(r * LDS + cc * 8) * 2, src + (size_t)r * HD + cc * 8, r < valid);
             }
@@ -833,7 +895,7 @@ __global__ void __launch_bounds__(AM_WARPS * 32, 2) weights_rows_mma_kernel(Weig
         }
     __syncthreads();
     const size_t base = ((size_t)blockIdx.y * a.n_splits + split) * group_rows;
-    for (int i = threadIdx.x; i < row_warps * 64; i += AM_WARPS * 32) {
+    for (int i = threadIdx.x; i < row_warps * 64; i += AR_WARPS * 32) {
         const int m = (int)blockIdx.z * row_warps * 64 + i;
         if (m >= s.rows) break;
         float t = -CUDART_INF_F, l = 0.f;
@@ -851,8 +913,8 @@ __global__ void __launch_bounds__(AM_WARPS * 32, 2) weights_rows_mma_kernel(Weig
 #define AC_ROWS 32              // rows of q in a stage
 #define AC_STAGES 4
 template <int HD>
-__global__ void __launch_bounds__(AM_WARPS * 32, 2) weights_keys_mma_kernel(WeightArgs a) {
-    constexpr int LDS = HD + 8, KS = HD / 16, CH = HD / 8, KEYS = AM_WARPS * 64;
+__global__ void __launch_bounds__(AR_WARPS * 32, 2) weights_keys_mma_kernel(WeightArgs a) {
+    constexpr int LDS = HD + 8, KS = HD / 16, CH = HD / 8, KEYS = AR_WARPS * 64;
     constexpr int QSTAGE = AC_ROWS * LDS * 2 + AC_ROWS * 16;                  // rows, then (maximum, 1 / sum, last place) of each
     extern __shared__ __align__(16) unsigned char raw[];
     pdl_wait();
@@ -896,7 +958,7 @@ __global__ void __launch_bounds__(AM_WARPS * 32, 2) weights_keys_mma_kernel(Weig
             unsigned char* st = raw + (size_t)(c % AC_STAGES) * QSTAGE;
             const uint32_t dst = raw32 + (uint32_t)(c % AC_STAGES) * QSTAGE;
 #pragma unroll
-            for (int c0 = 0; c0 < AC_ROWS * CH; c0 += AM_WARPS * 32) {
+            for (int c0 = 0; c0 < AC_ROWS * CH; c0 += AR_WARPS * 32) {
                 const int i = c0 + threadIdx.x, r = i / CH, cc = i % CH, m = c * AC_ROWS + r;
                 const bool in = m < s.rows;
                 const bf16* src = (const bf16*)a.q + (long long)(s.row0 + (in ? m / group : 0)) * a.q_stride + (long long)(kvh * group + (in ? m % group : 0)) * HD + cc * 8;
@@ -978,6 +1040,53 @@ __global__ void __launch_bounds__(AM_WARPS * 32, 2) weights_keys_mma_kernel(Weig
         }
 }
 
+template <typename T>
+static cudaError_t launch_plain(WeightArgs& a, cudaStream_t s) {
+    const unsigned pairs = (unsigned)a.n_seqs * (unsigned)a.kv_heads;
+    const int group_rows = a.max_new * (a.heads / a.kv_heads);
+    const size_t k_page = (size_t)CML_PAGE * (a.k_dim * sizeof(T) + 16), v_page = a.out ? (size_t)CML_PAGE * a.v_dim * sizeof(T) : 0;
+    const size_t rows = (size_t)AW_ROWS * a.k_dim * 4;
+    const size_t rest = rows + AW_ROWS * CML_PAGE * 4 + 3 * AW_ROWS * 4, smem3 = k_page + rows;
+    a.stages = 2 * (k_page + v_page) + rest <= 227 * 1024 ? 2 : 1;
+    const size_t smem1 = a.stages * (k_page + v_page) + rest;
+    cudaError_t e = cml_allow_smem<weights_part_kernel<T>>(smem1);
+    if (e == cudaSuccess) e = cml_allow_smem<weights_sum_kernel<T>>(smem3);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(weights_part_kernel<T>, dim3((unsigned)a.n_splits, pairs, (unsigned)((group_rows + AW_ROWS - 1) / AW_ROWS)), dim3(AW_THREADS),
+                   smem1, s, a);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(weights_join_kernel<T>, dim3((unsigned)group_rows, pairs), dim3(AW_THREADS), 0, s, a);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(weights_sum_kernel<T>, dim3((unsigned)((a.max_len + CML_PAGE - 1) / CML_PAGE), pairs), dim3(AW_THREADS), smem3, s, a);
+}
+
+template <int HD, int MT, bool OUT>
+static cudaError_t launch_all(const WeightArgs& a, unsigned pairs, int team, size_t smem, cudaStream_t s) {
+    const auto kernel = weights_part_mma_kernel<HD, MT, OUT, true>;
+    static bool wide = false;                                     // clusters of 16 blocks have to be asked for, once
+    cudaError_t e = cml_allow_smem<weights_part_mma_kernel<HD, MT, OUT, true>>(smem);
+    if (e == cudaSuccess && !wide) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        wide = e == cudaSuccess;
+    }
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)team, pairs);
+    cfg.blockDim = dim3(AM_WARPS * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)team;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cml_pdl_enabled() ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
 template <int HD>
 static cudaError_t launch_mma(const WeightArgs& a, cudaStream_t s) {
     constexpr int TILE = HD == 128 ? 16 : 32;
@@ -985,41 +1094,39 @@ static cudaError_t launch_mma(const WeightArgs& a, cudaStream_t s) {
     const int rows = a.max_new * (a.heads / a.kv_heads);
     constexpr size_t ring = (size_t)AM_WARPS * AM_STAGES * TILE * (HD + 8) * 2;
     cudaError_t e;
-#define AW_PART(MT, OUT, KEEP)                                                                                                   \
-    do {                                                                                                                         \
-        const size_t smem = ring * (OUT ? 2 : 1);                                                                                \
-        e = cml_allow_smem<weights_part_mma_kernel<HD, MT, OUT, KEEP>>(smem);                                                    \
-        if (e == cudaSuccess)                                                                                                    \
-            e = launch_pdl(weights_part_mma_kernel<HD, MT, OUT, KEEP>,                                                           \
-                           dim3((unsigned)a.n_splits, pairs, (unsigned)((rows + 16 * MT - 1) / (16 * MT))), dim3(AM_WARPS * 32), \
-                           smem, s, a);                                                                                          \
-    } while (0)
-    if (rows <= AK_ROWS) {
-        if (a.out) AW_PART(1, true, true);
-        else AW_PART(1, false, true);
-        if (e != cudaSuccess) return e;
-        const int key_blocks = (a.max_len + AK_THREADS - 1) / AK_THREADS;
-        return launch_pdl(weights_finish_kernel<bf16, HD>, dim3((unsigned)(key_blocks + (a.out ? rows : 0)), pairs), dim3(AK_THREADS), 0, s, a, key_blocks);
+    if (rows <= 32) {
+        // Where the blocks of all sequences run at the same time, more of them; beyond that up to twice as many, for sequences of
+        // unequal lengths, while a block has 768 keys (8 sequences of up to 8,191 keys: 34.6 us with eight blocks, 43 with four;
+        // 64 of up to 1,047: 24.0 with one, 35 with two); none without a tile of keys for each warp. Long sequences of which there are
+        // few take clusters of sixteen (one of 32,001 keys and eight kv heads: 41.6 us for 52.4; at 2,047 keys they are equal).
+        const long long slots = 2ll * cml_sm_count();
+        int team = 1;
+        while (team < 8 && (pairs * team * 2 <= slots || (pairs * team * 2 <= 2 * slots && a.max_len >= team * 2 * 768)) && team * 128 < a.max_len) team *= 2;
+        if (rows <= 16 && team == 8 && pairs * 16 <= (unsigned)cml_sm_count() && a.max_len >= 4096) team = 16;
+        if (rows <= 16) return a.out ? launch_all<HD, 1, true>(a, pairs, team, 2 * ring, s) : launch_all<HD, 1, false>(a, pairs, team, ring, s);
+        return a.out ? launch_all<HD, 2, true>(a, pairs, team, 2 * ring, s) : launch_all<HD, 2, false>(a, pairs, team, ring, s);
     }
     if (a.out) {
-        AW_PART(2, true, false);
+        e = cml_allow_smem<weights_part_mma_kernel<HD, 2, true, false>>(2 * ring);
+        if (e == cudaSuccess)
+            e = launch_pdl(weights_part_mma_kernel<HD, 2, true, false>, dim3((unsigned)a.n_splits, pairs, (unsigned)((rows + 31) / 32)),
+                           dim3(AM_WARPS * 32), 2 * ring, s, a);
     } else {
         const int row_warps = rows <= 64 ? 1 : (rows <= 128 ? 2 : 4);
         constexpr size_t smem = (size_t)AR_STAGES * CML_PAGE * (HD + 8) * 2;
         e = cml_allow_smem<weights_rows_mma_kernel<HD>>(smem);
         if (e == cudaSuccess)
             e = launch_pdl(weights_rows_mma_kernel<HD>, dim3((unsigned)a.n_splits, pairs, (unsigned)((rows + 64 * row_warps - 1) / (64 * row_warps))),
-                           dim3(AM_WARPS * 32), smem, s, a, row_warps);
+                           dim3(AR_WARPS * 32), smem, s, a, row_warps);
     }
     if (e != cudaSuccess) return e;
     e = launch_pdl(weights_join_kernel<bf16>, dim3((unsigned)rows, pairs), dim3(AW_THREADS), 0, s, a);
     if (e != cudaSuccess) return e;
-    constexpr size_t keys = (size_t)AM_WARPS * 64 * (HD + 8) * 2, stages = (size_t)AC_STAGES * AC_ROWS * ((HD + 8) * 2 + 16);
+    constexpr size_t keys = (size_t)AR_WARPS * 64 * (HD + 8) * 2, stages = (size_t)AC_STAGES * AC_ROWS * ((HD + 8) * 2 + 16);
     constexpr size_t smem = keys > stages ? keys : stages;
     e = cml_allow_smem<weights_keys_mma_kernel<HD>>(smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(weights_keys_mma_kernel<HD>, dim3((unsigned)((a.max_len + AM_WARPS * 64 - 1) / (AM_WARPS * 64)), pairs), dim3(AM_WARPS * 32), smem, s, a);
-#undef AW_PART
+    return launch_pdl(weights_keys_mma_kernel<HD>, dim3((unsigned)((a.max_len + AR_WARPS * 64 - 1) / (AR_WARPS * 64)), pairs), dim3(AR_WARPS * 32), smem, s, a);
 }
 
 extern "C" int cml_attn_paged_weights(const void* q, int dtype, long long q_stride, void* out, long long out_stride, const void* k,
@@ -1046,8 +1153,9 @@ extern "C" int cml_attn_paged_weights(const void* q, int dtype, long long q_stri
     a.joined = scratch;
     a.stats = a.joined + room(pairs * rows * 2);
     a.acc = a.stats + room(pairs * rows * 2 * a.n_splits);
+    a.kept_stride = ((long long)max_len + CML_PAGE - 1) / CML_PAGE * CML_PAGE;
     a.kept = a.acc + room(out ? pairs * rows * a.n_splits * v_dim : 0);
-    if (((uintptr_t)scratch) & 15) return CML_ERR_BAD_ALIGN;
+    if ((((uintptr_t)scratch) & 15) || (((uintptr_t)scores | (uintptr_t)scores_out) & 15)) return CML_ERR_BAD_ALIGN;
     // the tensor cores take rows of q that begin on 16 bytes
     const bool mma = dtype == CML_DTYPE_BF16 && (k_dim == 64 || k_dim == 128) && (out == nullptr || v_dim == k_dim) &&
                      (((uintptr_t)q) & 15) == 0 && q_stride % 8 == 0;

@@ -2029,7 +2029,7 @@ def draws_at(positions: torch.Tensor, seed: torch.Tensor, draws: torch.Tensor):
 # ---------------------------------------------------------------------------------------
 # between two steps: which positions the cache keeps, which drafted tokens stay
 
-ATTN_WEIGHTS_KEPT_ROWS = 16     # rows of a kv head up to which the products q . k are kept for the weights; AK_ROWS in attention_weights.cu
+ATTN_WEIGHTS_KEPT_ROWS = 32     # rows of a kv head up to which the products q . k are kept for the weights
 
 
 @functools.lru_cache(maxsize=512)
@@ -2047,7 +2047,7 @@ def attn_weights_plan(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int,
     split_keys = (((max_len + splits - 1) // splits + PAGE - 1) // PAGE) * PAGE
     splits = (max_len + split_keys - 1) // split_keys
     parts = [pairs * rows * 2, pairs * rows * 2 * splits, pairs * rows * splits * value_dim if with_output else 0,
-             pairs * rows * splits * split_keys if rows <= ATTN_WEIGHTS_KEPT_ROWS else 0]
+             pairs * rows * ((max_len + PAGE - 1) // PAGE * PAGE) if rows <= ATTN_WEIGHTS_KEPT_ROWS else 0]
     return split_keys, sum((n + 31) // 32 * 32 for n in parts)
 
 
