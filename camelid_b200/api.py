@@ -34,8 +34,12 @@ class LanguageModel:
     def config(self):
         return self.model.typed_config
 
-    def new_cache(self, max_tokens: int, max_slots: int | None = None):
-        return self.model.new_cache(max_tokens, max_slots)
+    def new_cache(self, max_tokens: int, max_slots: int | None = None, track_weights: bool = False):
+        return self.model.new_cache(max_tokens, max_slots, track_weights)
+
+    def evict(self, cache, slots, keep: int, *, first: int = 4, recent: int | None = None) -> list:
+        """Cut sequences to ``keep`` positions by the attention they received; see DecoderModel.evict."""
+        return self.model.evict(cache, slots, keep, first=first, recent=recent)
 
     def step(self, cache, entries) -> torch.Tensor:
         """``entries``: StepEntry(slot, tokens, want) or such tuples; see DecoderModel.step."""
@@ -57,9 +61,11 @@ class LanguageModel:
     def generate(self, prompts, max_tokens: int = 128, *, temperature: float = 0.0, top_k=None, top_p=None,
                  min_p=None, seed=None, presence_penalty: float = 0.0, frequency_penalty: float = 0.0,
                  repeat_penalty: float = 1.0, logit_bias=(), stop_token_ids=None, max_batch: int | None = None,
-                 cache=None, details: bool = False, on_step=None):
+                 cache=None, details: bool = False, on_step=None, drafter=None):
         """Generate for a list of prompts (lists of token ids). Returns the generated ids per
-        prompt (the stop token included), or ``GenerationResult`` objects with ``details``."""
+        prompt (the stop token included), or ``GenerationResult`` objects with ``details``. ``drafter``: a callable
+        that gives the tokens it expects after a history (``PromptLookup``, a smaller model): a step then brings them along
+        and keeps those that the model would have drawn; greedy tokens are the same with it."""
         single = bool(prompts) and isinstance(prompts[0], int)
         if single:
             prompts = [prompts]
@@ -70,7 +76,7 @@ class LanguageModel:
         stops = self.stop_token_ids if stop_token_ids is None else tuple(stop_token_ids)
         cache = cache if cache is not None else self._cache_for(prompts, max_tokens, max_batch)
         results = _generate(self.model, cache, sampler, prompts, max_tokens, stop_ids=stops, max_batch=max_batch,
-                            on_step=on_step)
+                            on_step=on_step, drafter=drafter)
         sampler.check()
         self.model.check_device_errors()
         out = results if details else [r.tokens for r in results]

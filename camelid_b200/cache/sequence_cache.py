@@ -25,7 +25,7 @@ _STATE_DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "int32": 
 
 class SequenceCache:
     def __init__(self, entry_specs: list, entry_sources: list, *, max_tokens: int, max_position: int,
-                 dtype: torch.dtype, device, max_slots: Optional[int] = None):
+                 dtype: torch.dtype, device, max_slots: Optional[int] = None, track_weights: bool = False):
         n_pages = max(1, (int(max_tokens) + PAGE - 1) // PAGE)
         n_slots = int(max_slots) if max_slots else n_pages
         self.dtype = dtype
@@ -69,8 +69,12 @@ class SequenceCache:
                 if self.entry_kv[src] is None:
                     raise CacheError(f"schedule entry {i} reads the keys of entry {src}, which keeps none")
                 self.entry_kv[i] = self.entry_kv[src]
+        if track_weights and (state_specs or not kv_specs or any(s.forgets for s in kv_specs)):
+            raise CacheError("attention weights are kept only by caches that keep all keys and no per-sequence state of fixed size")
         self.book = CacheBook(kv_specs, n_pages, n_slots, max_position)
         need = self.bytes_needed(kv_specs, counts_kv, state_specs, counts_state, n_pages, n_slots, dtype)
+        if track_weights:
+            need += sum(self.score_bytes(s, c, n_pages) for s, c in zip(kv_specs, counts_kv))
         if self.device.type == "cuda":
             free, _total = torch.cuda.mem_get_info(self.device)
             if need > free:
@@ -84,7 +88,16 @@ class SequenceCache:
                   for g, s in enumerate(kv_specs)]
         self.state = [torch.zeros((counts_state[g], n_slots) + tuple(s.shape), dtype=_STATE_DTYPES[s.dtype],
                                   device=self.device) for g, s in enumerate(state_specs)]
+        # with ``track_weights``: what every position was weighed by the queries since, float32 [entries, pages, kv_heads, 64] a
+        # group (attention sets a position's score when it writes its key, so pages need no clearing); else None
+        self.scores = None
+        if track_weights:
+            self.scores = [torch.zeros(t.shape[:-1], dtype=torch.float32, device=self.device) for t in self.k]
         self.bytes = need
+
+    @staticmethod
+    def score_bytes(spec: KVSpec, entries: int, n_pages: int) -> int:
+        return 4 * entries * n_pages * spec.n_kv_heads * PAGE
 
     @staticmethod
     def bytes_needed(kv_specs, counts_kv, state_specs, counts_state, n_pages, n_slots, dtype) -> int:
@@ -129,6 +142,11 @@ class SequenceCache:
             raise CacheError(f"schedule entry {entry} keeps no keys and values")
         g, i = where
         return g, self.k[g][i], self.v[g][i]
+
+    def scores_of(self, entry: int):
+        """The kept attention weights [pages, kv_heads, 64] of a schedule entry (None if the cache keeps none)."""
+        where = self.entry_kv[entry]
+        return None if self.scores is None or where is None else self.scores[where[0]][where[1]]
 
     def state_of(self, entry: int, name: str | None = None) -> torch.Tensor:
         """[slots, *shape] state of a schedule entry; ``name`` picks one where the entry keeps several."""

@@ -2,7 +2,7 @@
 // cached position gains the attention weight that the step's rows gave it, summed over the query heads of its kv head.
 //
 //   s = scale q . k      w = exp(s - max s) / sum exp(s - max s)      out = sum w v
-//   scores'[place] = (place was cached before the step ? scores[place] : 0) + sum over rows and heads of w
+//   scores'[place] = (place was cached before ? scores[place] : 0) + sum over rows and heads of w
 //
 // A step's rows are packed: sequence i owns rows row0[i] .. row0[i] + new[i], its row j stands at place start[i] + j and
 // sees the places up to its own. Without an output only the scores are made (what a prompt's last rows look at).
@@ -33,6 +33,7 @@ struct WeightArgs {
     const int* row0;
     const int* start;
     const int* fresh;            // new tokens of each sequence
+    const int* cached;           // places of each sequence whose scores count from before (null: those below `start`)
     int n_seqs, n_rows, heads, kv_heads, k_dim, v_dim;
     int max_new, max_len;
     float scale;                 // of the scores, times log2(e): the softmax is taken in powers of two
@@ -47,11 +48,13 @@ struct WeightArgs {
 
 struct Seq {
     int start, fresh, length, row0, rows;      // rows: (token, head) pairs that share a kv head
+    int old;                                   // places below this keep the score they have and gain
 };
 __device__ __forceinline__ Seq seq_of(const WeightArgs& a, int i) {
     Seq s;
     s.start = max(0, min(a.start[i], 1 << 30));
     s.row0 = a.row0[i];
+    s.old = a.cached != nullptr ? min(a.cached[i], s.start) : s.start;
     s.fresh = max(0, min(a.fresh[i], a.max_new));
     if (s.row0 < 0 || s.row0 > a.n_rows - s.fresh) s.fresh = 0;
     s.length = min(min(s.start + s.fresh, a.max_len), a.width * CML_PAGE);
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(AW_THREADS) weights_sum_kernel(WeightArgs a) {
     __syncthreads();
     if (half == 0 && key < valid) {
         const int place = p * CML_PAGE + key;
-        a.scores_out[at + key] = (place < s.start ? a.scores[at + key] : 0.f) + (gained + other[key]);
+        a.scores_out[at + key] = (place < s.old ? a.scores[at + key] : 0.f) + (gained + other[key]);
     }
 }
 
@@ -733,7 +736,7 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
             if (!has[u]) continue;
             const int place = group0 + u * AM_WARPS * 128;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) g[u][k] += place + k < s.start ? old[u][k] : 0.f;
+            for (int k = 0; k < 4; ++k) g[u][k] += place + k < s.old ? old[u][k] : 0.f;
             if (place + 4 <= last) *reinterpret_cast<float4*>(a.scores_out + at[u]) = make_float4(g[u][0], g[u][1], g[u][2], g[u][3]);
             else {
 #pragma unroll
@@ -1036,7 +1039,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, 2) weights_keys_mma_kernel(Weig
             g += __shfl_xor_sync(0xffffffffu, g, 1);
             g += __shfl_xor_sync(0xffffffffu, g, 2);
             const int key = mt * 16 + (lane >> 2) + 8 * h;
-            if ((lane & 3) == 0 && key < valid) a.scores_out[at + key] = (place0 + key < s.start ? a.scores[at + key] : 0.f) + g;
+            if ((lane & 3) == 0 && key < valid) a.scores_out[at + key] = (place0 + key < s.old ? a.scores[at + key] : 0.f) + g;
         }
 }
 
@@ -1131,7 +1134,7 @@ static cudaError_t launch_mma(const WeightArgs& a, cudaStream_t s) {
 
 extern "C" int cml_attn_paged_weights(const void* q, int dtype, long long q_stride, void* out, long long out_stride, const void* k,
                                       const void* v, const float* scores, float* scores_out, const int* table, int width, int n_pages,
-                                      const int* row0, const int* start, const int* fresh, int n_seqs, int n_rows, int heads,
+                                      const int* row0, const int* start, const int* fresh, const int* cached, int n_seqs, int n_rows, int heads,
                                       int kv_heads, int k_dim, int v_dim, int max_new, int max_len, float scale, int split_keys,
                                       float* scratch, void* stream) {
     if (dtype != CML_DTYPE_F32 && dtype != CML_DTYPE_BF16) return CML_ERR_BAD_DTYPE;
@@ -1145,7 +1148,7 @@ extern "C" int cml_attn_paged_weights(const void* q, int dtype, long long q_stri
     if (((uintptr_t)k | (uintptr_t)(out ? v : nullptr)) & 15) return CML_ERR_BAD_ALIGN;
     WeightArgs a = {};
     a.q = q; a.q_stride = q_stride; a.out = out; a.out_stride = out_stride; a.k = k; a.v = v; a.scores = scores; a.scores_out = scores_out;
-    a.table = table; a.width = width; a.n_pages = n_pages; a.row0 = row0; a.start = start; a.fresh = fresh; a.n_seqs = n_seqs;
+    a.table = table; a.width = width; a.n_pages = n_pages; a.row0 = row0; a.start = start; a.fresh = fresh; a.cached = cached; a.n_seqs = n_seqs;
     a.n_rows = n_rows; a.heads = heads; a.kv_heads = kv_heads; a.k_dim = k_dim; a.v_dim = v_dim; a.max_new = max_new; a.max_len = max_len;
     a.scale = scale * 1.4426950408889634f; a.split_keys = split_keys;
     a.n_splits = (max_len + split_keys - 1) / split_keys;

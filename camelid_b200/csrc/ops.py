@@ -200,8 +200,8 @@ _SIGNATURES = {
     ("gemm_few", "cml_gemm_few_experts"): [c_void_p, c_long, c_int, c_int, c_void_p, c_long, c_int, c_int, c_int, c_void_p, c_long, c_int,
                                            c_void_p, c_void_p, c_void_p],
     ("attention_weights", "cml_attn_paged_weights"): [c_void_p, c_int, c_long, c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_void_p,
-                                                      c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
-                                                      c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p],
+                                                      c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                                                      c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p],
     ("eviction", "cml_evict_positions"): [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                           c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p],
     ("verify", "cml_verify_drafts"): [c_void_p, c_long, c_int, c_int, c_void_p, c_void_p, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p,
@@ -2059,18 +2059,19 @@ def attn_weights_floats(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: in
 
 
 def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, seq_start, seq_new, n_heads: int, max_new: int,
-                       max_len: int, scale: float, scratch, scores_out=None):
+                       max_len: int, scale: float, scratch, scores_out=None, seq_cached=None):
     """Attention of a step's rows over the paged cache that keeps what it weighed. Sequence i owns the rows
     seq_row0[i] .. + seq_new[i] of ``q`` [rows, heads * head_dim]; its row j stands at place seq_start[i] + j and sees the
     places up to its own (keys and values of the new places are in the cache already). ``out`` [rows, heads * value_dim] gets the
     attention output (None, with ``v_pages`` None: scores only, for the last rows of a prompt). ``scores`` (float32 [pages, kv
     heads, 64]) gain every place's weight, summed over the rows and the query heads of its kv head; new places start from
-    zero, whatever their page held. The new scores go to ``scores_out`` (None: in place), where nothing but the sequences'
+    zero, whatever their page held (``seq_cached``: int32 [sequences], places that count as cached where fewer than seq_start do,
+    because the same step brought the others). The new scores go to ``scores_out`` (None: in place), where nothing but the sequences'
     places is written. ``max_new`` and ``max_len`` bound the sequences' new tokens and lengths (rows and places beyond them are
     left out); ``scratch``: float32, ``attn_weights_floats`` numbers, free again when the call's work is done. No page
     stands in two rows of the table."""
     scores_out = scores if scores_out is None else scores_out
-    _here(q, out, k_pages, v_pages, scores, scores_out, block_table, seq_row0, seq_start, seq_new, scratch)
+    _here(q, out, k_pages, v_pages, scores, scores_out, block_table, seq_row0, seq_start, seq_new, scratch, seq_cached)
     n_pages, kv_heads, page, head_dim = k_pages.shape
     n_seqs, width = block_table.shape
     rows = q.shape[0]
@@ -2081,6 +2082,7 @@ def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, 
     assert block_table.dtype == torch.int32 and block_table.is_contiguous()
     for t in (seq_row0, seq_start, seq_new):
         assert t.dtype == torch.int32 and t.numel() == n_seqs and t.is_contiguous()
+    assert seq_cached is None or (seq_cached.dtype == torch.int32 and seq_cached.numel() == n_seqs and seq_cached.is_contiguous())
     assert (out is None) == (v_pages is None), "an output needs values, and values an output"
     value_dim = head_dim
     if out is not None:
@@ -2096,8 +2098,8 @@ def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, 
         raise KernelError(f"attn_paged_weights: the scratch must be {floats} contiguous float32 numbers (attn_weights_floats)")
     _check(_fn("attention_weights", "cml_attn_paged_weights")(
         _p(q), dtype_code(q.dtype), q.stride(0), _p(out), 0 if out is None else out.stride(0), _p(k_pages), _p(v_pages), _p(scores),
-        _p(scores_out), _p(block_table), width, n_pages, _p(seq_row0), _p(seq_start), _p(seq_new), n_seqs, rows, n_heads, kv_heads,
-        head_dim, value_dim, int(max_new), int(max_len), float(scale), split_keys, _p(scratch), _stream()), "attn_paged_weights", 3)
+        _p(scores_out), _p(block_table), width, n_pages, _p(seq_row0), _p(seq_start), _p(seq_new), _p(seq_cached), n_seqs, rows, n_heads,
+        kv_heads, head_dim, value_dim, int(max_new), int(max_len), float(scale), split_keys, _p(scratch), _stream()), "attn_paged_weights", 3)
 
 
 def evict_positions(k_pages, v_pages, scores, block_table, out_table, lengths, keeps, kept, first: int, recent: int, inv_freq=None,

@@ -102,6 +102,7 @@ class StepContext:
         self.pending = None             # float32 [splits, rows, hidden] still to be added to the residual stream
         self.deferred = None            # (x, w, residual): a product into the residual stream not yet launched
         self.row_scale = None           # ops.RowScale: what the rows of the last norm's output still lack
+        self.observed = None            # (tokens, row0, start, new): each sequence's last rows of the step, see observed_rows
         self.rows_copy = None           # (stream, rows): the stream's rows in the compute type as its last writer left them
         # host-side knowledge (filled by the constructors below)
         self.h_slots: list = []
@@ -231,6 +232,18 @@ class StepContext:
         """[slots, *shape] fixed-size state of the running entry (``name`` picks one where the entry
         keeps several); index it with ``seq_slot``."""
         return self.cache.state_of(self.entry, name)
+
+    def scores(self):
+        """Where the running entry keeps the attention weights of its positions (None: it keeps none, or borrows its keys)."""
+        return None if self.cache_source is not None else self.cache.scores_of(self.entry)
+
+    def observed_rows(self, tokens: int):
+        """(row0, start, new) of every sequence's last rows of the step, ``tokens`` at most: made once a step on the device."""
+        if self.observed is None or self.observed[0] != tokens:
+            new = torch.clamp(self.seq_new, max=tokens)
+            skipped = self.seq_new - new
+            self.observed = (tokens, self.seq_row0 + skipped, self.seq_start + skipped, new)
+        return self.observed[1:]
 
     def query_tiles(self, rows_per_tile):
         """Tiles of at most ``rows_per_tile`` consecutive new rows of one sequence:

@@ -168,10 +168,82 @@ def run_batch(model, cache, sampler, prompts: list, budgets: list, requested: li
     return results
 
 
+def _drafts_of(drafter, history: list, most: int) -> tuple:
+    """(tokens, probabilities or None) that ``drafter`` expects after ``history``, ``most`` at most."""
+    if most <= 0:
+        return [], None
+    given = drafter(list(history))
+    tokens, probs = given if isinstance(given, tuple) else (given, None)
+    tokens = [int(t) for t in _to_list(tokens)][:most]
+    return tokens, probs[:len(tokens)] if probs is not None and tokens else None
+
+
+def run_drafted_batch(model, cache, sampler, drafter, prompts: list, budgets: list, requested: list, stop_ids: set,
+                      on_step=None) -> list:
+    """``run_batch`` with drafted tokens: every step brings a sequence's last token and what ``drafter`` expects behind it, the
+    sampler verifies the drafts against the step's logits, and the rejected ones leave the cache again. A step yields
+    one token more than it accepts drafts."""
+    n = len(prompts)
+    results = [GenerationResult(prompt_tokens=len(p)) for p in prompts]
+    slots = [None] * n
+    histories = [list(p) for p in prompts]
+    live = []
+    try:
+        for i in range(n):
+            if budgets[i] <= 0:
+                results[i].finish_reason = "capacity" if requested[i] > 0 else "length"
+                continue
+            slots[i] = cache.alloc_slot()
+            live.append(i)
+        fed = {i: list(prompts[i]) for i in live}                        # what the next step brings before the drafts
+        while live:
+            drafts, probs = [], []
+            for i in live:
+                # a token more than the drafts may come out of a step, and none behind the budget
+                d, p = _drafts_of(drafter, histories[i], budgets[i] - len(results[i].tokens) - 1)
+                for t in d:
+                    if not 0 <= t < sampler.vocab_size:
+                        raise StepError(f"slot {slots[i]}: the drafted token {t} is outside the vocabulary of {sampler.vocab_size}")
+                drafts.append(d)
+                probs.append(p)
+            entries = [StepEntry(slots[i], fed[i] + d, list(range(len(fed[i]) - 1, len(fed[i]) + len(d)))) for i, d in zip(live, drafts)]
+            logits = model.step(cache, entries)
+            counts, nexts = sampler.verify(logits, drafts, [histories[i] for i in live], probs)
+            if on_step is not None:
+                on_step(len(live))
+            still = []
+            for i, d, count, token in zip(live, drafts, counts, nexts):
+                new = d[:count] + [int(token)]
+                for at, t in enumerate(new):
+                    if t in stop_ids:
+                        new = new[:at + 1]
+                        break
+                results[i].tokens.extend(new)
+                histories[i].extend(new)
+                if new[-1] in stop_ids:
+                    results[i].finish_reason = "stop"
+                elif len(results[i].tokens) >= budgets[i]:
+                    results[i].finish_reason = "length" if budgets[i] >= requested[i] else "capacity"
+                if results[i].finish_reason:
+                    cache.free_slot(slots[i])
+                    slots[i] = None
+                else:
+                    if count < len(d):
+                        cache.truncate(slots[i], cache.length(slots[i]) - (len(d) - count))
+                    fed[i] = [int(token)]
+                    still.append(i)
+            live = still
+    finally:
+        for s in slots:
+            if s is not None:
+                cache.free_slot(s)
+    return results
+
+
 def generate(model, cache, sampler, prompts: list, max_tokens, *, stop_ids=(), max_batch: int | None = None,
-             on_step=None) -> list:
+             on_step=None, drafter=None) -> list:
     """Generate for every prompt; ``max_tokens`` is one number or one per prompt. Returns a
-    ``GenerationResult`` per prompt, in the order given."""
+    ``GenerationResult`` per prompt, in the order given. ``drafter``: see ``run_drafted_batch`` and ``sampling/drafts.py``."""
     if not prompts:
         return []
     per = list(max_tokens) if isinstance(max_tokens, (list, tuple)) else [int(max_tokens)] * len(prompts)
@@ -183,6 +255,9 @@ def generate(model, cache, sampler, prompts: list, max_tokens, *, stop_ids=(), m
         if per[i] < 0:
             raise StepError(f"prompt {i}: max_tokens must not be negative")
     book = cache.book
+    if drafter is not None and (getattr(cache, "state", None) or any(s.forgets for s in book.kv_specs)):
+        raise StepError("drafted tokens need a cache that can be rolled back: this model keeps per-sequence state of fixed size "
+                        "or gives old positions back")
     lens = [len(p) for p in prompts]
     for i, n in enumerate(lens):
         if n > book.max_position:
@@ -190,8 +265,8 @@ def generate(model, cache, sampler, prompts: list, max_tokens, *, stop_ids=(), m
     budgets = [token_budget(n, m, book.max_position, book.n_pages) for n, m in zip(lens, per)]
     results = [None] * len(prompts)
     for batch in plan_batches(lens, budgets, book.n_pages, book.n_slots, max_batch):
-        out = run_batch(model, cache, sampler, [list(prompts[i]) for i in batch], [budgets[i] for i in batch],
-                        [per[i] for i in batch], set(stop_ids), on_step)
+        what = ([list(prompts[i]) for i in batch], [budgets[i] for i in batch], [per[i] for i in batch], set(stop_ids), on_step)
+        out = run_batch(model, cache, sampler, *what) if drafter is None else run_drafted_batch(model, cache, sampler, drafter, *what)
         for i, r in zip(batch, out):
             results[i] = r
     return results

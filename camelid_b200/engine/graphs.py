@@ -118,13 +118,14 @@ class DecodeGraph:
     def capture(self):
         """Warm up eagerly on the buffer's present contents, then capture. The warm-up runs the
         step once for real: keys and values it writes are written again, identically, by the
-        first replay, but per-sequence state of fixed size would be advanced twice, so it is put
-        back as it was."""
+        first replay, but per-sequence state of fixed size would be advanced twice and kept attention
+        weights added twice, so both are put back as they were."""
         tokens_before = self.ctx.tokens.clone()
-        state_before = [t.clone() for t in self.cache.state]
+        kept = self.cache.state + (self.cache.scores or [])
+        state_before = [t.clone() for t in kept]
         self._forward()
         self.ctx.tokens.copy_(tokens_before)
-        for t, saved in zip(self.cache.state, state_before):
+        for t, saved in zip(kept, state_before):
             t.copy_(saved)
         torch.cuda.synchronize()
         before = ops.launch_count()

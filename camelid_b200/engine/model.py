@@ -23,7 +23,7 @@ import torch
 from ..cache.sequence_cache import SequenceCache
 from ..config.plan import ModelPlan
 from ..config.registry import load_config
-from ..errors import ConfigError, KernelError, StepError
+from ..errors import CacheError, ConfigError, KernelError, StepError
 from ..options import KernelOptions
 from ..parts import build_block, build_part
 from ..weights.loader import check_tensors
@@ -87,6 +87,7 @@ class DecoderModel:
                               and all(p.graph_safe_any_step for p in self._single_parts()))
         self._seen_layouts = weakref.WeakKeyDictionary()   # cache -> {key: times seen}
         self._step_graphs = weakref.WeakKeyDictionary()    # cache -> {key: StepGraph}, oldest first
+        self._turnings: dict = {}                           # position encoding -> what evict has to know of it
 
     # ---- construction ----
     @classmethod
@@ -167,17 +168,74 @@ class DecoderModel:
     def entry_cache_sources(self) -> list:
         return [e.cache_source for e in self.schedule] + [None]
 
-    def new_cache(self, max_tokens: int, max_slots: int | None = None) -> SequenceCache:
+    def new_cache(self, max_tokens: int, max_slots: int | None = None, track_weights: bool = False) -> SequenceCache:
         """A cache for at most ``max_tokens`` live tokens (each sequence's count rounded up to
-        a multiple of 64) and ``max_slots`` live sequences (default: one per page)."""
+        a multiple of 64) and ``max_slots`` live sequences (default: one per page). ``track_weights``: the cache also keeps, for
+        every position, the attention weight it received (``evict`` goes by it): of single-token steps and steps of up to 8 tokens
+        from all rows, of longer ones from a sequence's last 32."""
         from ..memory import device_free_bytes
+        if track_weights:
+            for i, e in enumerate(self.schedule):
+                if not getattr(getattr(self.blocks[e.layer], "mixer", None), "keeps_weights", False):
+                    raise ConfigError("track_weights", f"the mixer of schedule entry {i} does not keep attention weights")
+                if self.blocks[e.layer].mixer.position.rotary_dim % 16:
+                    raise ConfigError("track_weights", f"the keys of schedule entry {i} cannot be turned: their rotary size "
+                                      f"{self.blocks[e.layer].mixer.position.rotary_dim} is no multiple of 16")
         free = device_free_bytes(self.device)
         if free is not None:
             self.memory_plan(max_tokens, max_slots).check(free, f"a cache for {max_tokens} tokens on {self.device}",
                                                           parts=("cache", "workspace"))
         return SequenceCache(self.entry_cache_specs(), self.entry_cache_sources(),
                              max_tokens=max_tokens, max_position=self.plan.max_position, dtype=self.dtype,
-                             device=self.device, max_slots=max_slots)
+                             device=self.device, max_slots=max_slots, track_weights=track_weights)
+
+    def evict(self, cache: SequenceCache, slots: list, keep: int, *, first: int = 4, recent: int | None = None) -> list:
+        """Cut the sequences in ``slots`` that are longer than ``keep`` to that many positions, in place: of every layer and kv head the
+        ``first`` positions stay, the ``recent`` last ones (default: a quarter of ``keep``) and those that received the most
+        attention. They close up, their keys are turned by the way they move, and the sequence goes on as one of length ``keep``:
+        the next token stands at position ``keep``. The cache must have been made with ``track_weights``. Returns the
+        new lengths; nothing changes if a check fails."""
+        from ..csrc import ops
+        if cache.scores is None:
+            raise CacheError("the cache keeps no attention weights: make it with new_cache(..., track_weights=True)")
+        slots = [int(s) for s in slots]
+        recent = keep // 4 if recent is None else int(recent)
+        if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
+            raise CacheError(f"cannot keep {keep} positions with the first {first} and the last {recent} among them")
+        if len(set(slots)) != len(slots):
+            raise CacheError("a slot occurs twice")
+        lengths = {s: cache.length(s) for s in slots}
+        cut = [s for s in slots if lengths[s] > keep]
+        if cut:
+            book, n = cache.book, len(cut)
+            ints = torch.tensor([lengths[s] for s in cut] + [keep] * n, dtype=torch.int32).to(self.device)
+            for g, spec in enumerate(book.kv_specs):
+                table = torch.tensor(book.block_table(g, cut), dtype=torch.int32).to(self.device)
+                entries = [(i, cache.entry_kv[i][1], self.blocks[e.layer].mixer.position) for i, e in enumerate(self.schedule)
+                           if e.cache_source is None and cache.entry_kv[i][0] == g]
+                # entries whose positions turn alike move together
+                alike: dict = {}
+                for _, at, pos in sorted(entries, key=lambda x: x[1]):
+                    alike.setdefault(self._turning(pos), []).append((at, pos))
+                for group in alike.values():
+                    ats, pos = [at for at, _ in group], group[0][1]
+                    whole = ats == list(range(cache.k[g].shape[0]))
+                    for at in [slice(None)] if whole else [slice(a, a + 1) for a in ats]:
+                        k, scores = cache.k[g][at], cache.scores[g][at]
+                        kept = torch.empty((k.shape[0], n, spec.n_kv_heads, keep), dtype=torch.int32, device=self.device)
+                        ops.evict_positions(k, cache.v[g][at], scores, table, table, ints[:n], ints[n:], kept, first, recent,
+                                            inv_freq=pos.inv_freq if pos.rotary_dim else None, interleaved=self._turning(pos)[0])
+            for s in cut:
+                book.truncate(s, keep)
+        return [min(lengths[s], keep) for s in slots]
+
+    def _turning(self, position) -> tuple:
+        """(pairs are neighbours, frequencies) of a position encoding, as numbers: read from the device once."""
+        known = self._turnings.get(position)
+        if known is None:
+            known = (getattr(position, "pairing", "split") == "interleaved", tuple(position.inv_freq.tolist()))
+            self._turnings[position] = known
+        return known
 
     # ---- the step ----
     def _validate(self, cache: SequenceCache, entries: list) -> list:
@@ -390,6 +448,7 @@ class DecoderModel:
         ctx.deferred = None
         ctx.row_scale = None
         ctx.rows_copy = None
+        ctx.observed = None
         h = ctx.buffer("hidden", (ctx.n_rows, self.hidden_size), torch.float32)
         ctx.entry = len(self.schedule)                      # the embedding's own entry of the cache
         ctx.cache_source = None

@@ -30,6 +30,13 @@ class GroupedQueryAttention(Part):
     graph_safe_any_step = True
     handles_pending = True
     accepts_row_scale = True
+    keeps_weights = True
+    keeps_weights_in = ("forward",)
+
+    # In a cache that keeps attention weights: steps of up to ``weighed_tokens`` new tokens a sequence run the attention that keeps
+    # them; of longer ones (prompts) the last ``observed_tokens`` rows of every sequence are asked what they look at.
+    weighed_tokens = 8
+    observed_tokens = 32
 
     def __init__(self, params, prefix=""):
         super().__init__(params, prefix)
@@ -94,8 +101,9 @@ class GroupedQueryAttention(Part):
         if part is not None:
             row_scale = None
         out = ctx.buffer("attn_out", (n, self.q_width))
+        scores = ctx.scores()
         splits = self._decode_splits(ctx, n, 1, True) if ctx.decode else 1
-        if (part is not None and ctx.decode and ctx.options.decode_attention == "fused" and (splits <= 8 or ctx.max_len <= 8192)
+        if (scores is None and part is not None and ctx.decode and ctx.options.decode_attention == "fused" and (splits <= 8 or ctx.max_len <= 8192)
                 and ops.attn_decode_fused_usable(part, out, self.head_dim, self.num_heads, self.num_kv_heads)):
             # decode: one launch sums the product's splits, rotates, writes the cache and attends
             ops.attn_decode_fused(part, out, ctx.row_pos, ctx.row_seq, table, k_pages, v_pages, pos.inv_freq,
@@ -115,6 +123,12 @@ class GroupedQueryAttention(Part):
             ops.rope_kv_write(qkv, ctx.row_pos, ctx.row_seq, table, k_pages, v_pages, pos.inv_freq, pos.rotary_dim,
                               self.num_heads, self.num_kv_heads, self.head_dim, write_kv=not borrow)
             q = qkv[:, :self.q_width]
+        if scores is not None:
+            few = ctx.max_new <= self.weighed_tokens
+            self._weigh(ctx, q, out if few else None, k_pages, v_pages, scores, table, self.weighed_tokens if few else self.observed_tokens)
+            if few:
+                linear.add_into_residual(ctx, out, self.w_o, residual, "o_partial")
+                return
         # prefill: bfloat16 with a head size of 64 or 128 on the tcgen05 kernel, everything else in
         # float on the CUDA cores; decode (where the fused kernel did not take it): mma.sync tiles
         # for those head sizes, split over blocks
@@ -129,6 +143,16 @@ class GroupedQueryAttention(Part):
         else:
             self._attend(ctx, q, out, k_pages, v_pages, table, tensor_cores=False)
         linear.add_into_residual(ctx, out, self.w_o, residual, "o_partial")
+
+    def _weigh(self, ctx, q, out, k_pages, v_pages, scores, table, tokens: int):
+        """The step's rows (``out``: with their attention output), or the last ``tokens`` of each sequence, add their weights to the
+        kept scores. Lengths are bounded by the block table, so a captured step serves any of them."""
+        max_new, max_len = min(ctx.max_new, tokens), table.shape[1] * PAGE
+        row0, start, new = (ctx.seq_row0, ctx.seq_start, ctx.seq_new) if ctx.max_new <= tokens else ctx.observed_rows(tokens)
+        scratch = ctx.buffer("attn_weights", (ops.attn_weights_floats(ctx.n_seqs, self.num_heads, self.num_kv_heads, self.head_dim, q.dtype,
+                                                                      max_new, max_len, out is not None),), torch.float32)
+        ops.attn_paged_weights(q, out, k_pages, v_pages if out is not None else None, scores, table, row0, start, new, self.num_heads, max_new,
+                               max_len, self.scale, scratch, seq_cached=ctx.seq_start)
 
     def _decode_splits(self, ctx, n_tiles: int, chunks: int, tensor_cores: bool) -> int:
         """Blocks that share the keys of one (row, kv head) in a decode step: enough for all SMs

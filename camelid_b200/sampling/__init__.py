@@ -1,6 +1,7 @@
+from .drafts import PromptLookup
 from .options import SamplingOptions, splitmix64, unit_draw
 
-__all__ = ["SamplingOptions", "splitmix64", "unit_draw", "Sampler"]
+__all__ = ["PromptLookup", "SamplingOptions", "splitmix64", "unit_draw", "Sampler"]
 
 
 def __getattr__(name):

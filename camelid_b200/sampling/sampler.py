@@ -14,7 +14,7 @@ import torch
 
 from ..csrc import ops
 from ..errors import SamplingError
-from .options import SamplingOptions, unit_draw
+from .options import SamplingOptions, splitmix64, unit_draw
 
 
 class Sampler:
@@ -81,6 +81,56 @@ class Sampler:
                             o.min_p or 0.0, draws, out, self._err)
         return out
 
+    def verify(self, logits: torch.Tensor, drafts: list, histories: list, draft_probs: list | None = None) -> tuple:
+        """Which drafted tokens stay, and the token behind them. ``logits``: float32 on the device, for every sequence a row for each
+        of its ``drafts`` (a list of tokens) and one more, packed (adjusted in place when penalties or biases are set);
+        ``histories``: per sequence the tokens before its drafts; ``draft_probs``: per sequence the drafter's probabilities
+        (float32 [drafts, vocabulary] on the device), or None where it was certain of its tokens. Returns (accepted drafts,
+        next tokens), two lists. The draws come from the sampler's seed and the history's length: the next token's
+        from the stream of ``sample``, the acceptances' from one of their own."""
+        o = self.options
+        n, room = len(drafts), max([len(d) for d in drafts] + [1])
+        rows = sum(len(d) + 1 for d in drafts)
+        if logits.shape[0] != rows or len(histories) != n:
+            raise SamplingError(f"{n} sequences with {rows - n} drafts need {rows} rows of logits and {n} histories, got "
+                                f"{logits.shape[0]} and {len(histories)}")
+        if o.adjusts:
+            entries, biases = self._adjust_entries([list(h) + list(d[:j]) for h, d in zip(histories, drafts) for j in range(len(d) + 1)])
+            if entries:
+                e = torch.tensor(entries, dtype=torch.int32).to(self.device, non_blocking=True)
+                b = torch.tensor(biases, dtype=torch.float32).to(self.device, non_blocking=True)
+                ops.adjust_logits(logits, e, b, o.repeat_penalty, o.presence_penalty, o.frequency_penalty)
+        seed = o.seed or 0
+        own = splitmix64(seed ^ 0x5851F42D4C957F2D)                  # the acceptances' stream
+        row0, at = [], 0
+        for d in drafts:
+            row0.append(at)
+            at += len(d) + 1
+        ints = torch.tensor([row0, [len(d) for d in drafts]], dtype=torch.int32).to(self.device, non_blocking=True)
+        tokens = torch.tensor([list(d) + [0] * (room - len(d)) for d in drafts], dtype=torch.int32).to(self.device, non_blocking=True)
+        accept = torch.tensor([[unit_draw(own, len(h) + j) for j in range(room)] for h in histories], dtype=torch.float32)
+        accept = accept.to(self.device, non_blocking=True)
+        draws = torch.tensor([unit_draw(seed, len(h)) for h in histories], dtype=torch.float32).to(self.device, non_blocking=True)
+        probs = None
+        if draft_probs is not None and any(p is not None for p in draft_probs):
+            probs = torch.zeros((n, room, self.vocab_size), dtype=torch.float32, device=self.device)
+            for i, (p, d) in enumerate(zip(draft_probs, drafts)):
+                if p is not None:
+                    if tuple(p.shape) != (len(d), self.vocab_size):
+                        raise SamplingError(f"sequence {i}: {len(d)} drafts need probabilities [{len(d)}, {self.vocab_size}], got {list(p.shape)}")
+                    probs[i, :len(d)] = p
+                else:                                                # certain drafts among others with probabilities
+                    for j, t in enumerate(d):
+                        probs[i, j, int(t)] = 1.0
+        out = torch.empty((n, room + 2), dtype=torch.int32, device=self.device)
+        counts, chosen = torch.empty(n, dtype=torch.int32, device=self.device), torch.empty((n, room + 1), dtype=torch.int32, device=self.device)
+        scratch = torch.empty(ops.verify_bytes(rows, n, self.vocab_size), dtype=torch.uint8, device=self.device)
+        ops.verify_drafts(logits, ints[0], ints[1], tokens, probs, accept, draws, o.temperature, o.top_k or 0,
+                          o.top_p if o.top_p is not None else 1.0, o.min_p or 0.0, counts, chosen, self._err, scratch)
+        out[:, 0], out[:, 1:] = counts, chosen
+        host = out.tolist()
+        return [r[0] for r in host], [r[1 + r[0]] for r in host]
+
     def check(self) -> None:
         """Synchronising read of the error word: non-finite logits are an error
         (src/inference.rs:5890-5907)."""
@@ -88,4 +138,4 @@ class Sampler:
         if code:
             self._err.zero_()
             raise SamplingError("sampler logits contain a non-finite value" if code & 1
-                                else "sampler softmax produced an invalid normalisation sum")
+                                else "a drafted token is outside the vocabulary or its probabilities are none" if code & 4 else "sampler softmax produced an invalid normalisation sum")
