@@ -256,16 +256,13 @@ def _dev(*tensors):
 
 def _here(*tensors):
     """All given tensors stand on the current device, whose current stream the kernels run on."""
-    now = None
+    now = _device_now() if _raw_stream is not None and torch.cuda.is_initialized() else -2
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise KernelError("camelid_b200 kernels run on CUDA tensors only; there is no CPU path")
-        if now is None:
-            now = torch.cuda.current_device()
-        if t.device.index != now:
-            raise KernelError(f"a tensor stands on {t.device}, the current device is cuda:{now}")
+        if t is not None and t.get_device() != now:
+            if not t.is_cuda:
+                raise KernelError("camelid_b200 kernels run on CUDA tensors only; there is no CPU path")
+            if t.device.index != torch.cuda.current_device():
+                raise KernelError(f"a tensor stands on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
 def _p(t):
@@ -2072,34 +2069,38 @@ def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, 
     stands in two rows of the table."""
     scores_out = scores if scores_out is None else scores_out
     _here(q, out, k_pages, v_pages, scores, scores_out, block_table, seq_row0, seq_start, seq_new, scratch, seq_cached)
-    n_pages, kv_heads, page, head_dim = k_pages.shape
+    n_pages, kv_heads, page, head_dim = shape = k_pages.shape
     n_seqs, width = block_table.shape
-    rows = q.shape[0]
-    assert page == PAGE and k_pages.dtype == q.dtype and k_pages.is_contiguous() and q.dim() == 2 and q.stride(1) == 1
-    assert n_heads % kv_heads == 0 and q.shape[1] == n_heads * head_dim
-    assert scores.dtype == torch.float32 and scores.shape == (n_pages, kv_heads, PAGE) and scores.is_contiguous()
-    assert scores_out.dtype == torch.float32 and scores_out.shape == scores.shape and scores_out.is_contiguous()
-    assert block_table.dtype == torch.int32 and block_table.is_contiguous()
-    for t in (seq_row0, seq_start, seq_new):
-        assert t.dtype == torch.int32 and t.numel() == n_seqs and t.is_contiguous()
+    rows, q_width = q.shape
+    q_stride, q_step = q.stride()
+    dtype = q.dtype
+    assert page == PAGE and k_pages.dtype == dtype and k_pages.is_contiguous() and q_step == 1
+    assert n_heads % kv_heads == 0 and q_width == n_heads * head_dim
+    assert scores.dtype == torch.float32 and scores.shape == shape[:3] and scores.is_contiguous()
+    assert scores_out is scores or (scores_out.dtype == torch.float32 and scores_out.shape == shape[:3] and scores_out.is_contiguous())
+    assert block_table.dtype == seq_row0.dtype == seq_start.dtype == seq_new.dtype == torch.int32
+    assert block_table.is_contiguous() and seq_row0.is_contiguous() and seq_start.is_contiguous() and seq_new.is_contiguous()
+    assert seq_row0.numel() == seq_start.numel() == seq_new.numel() == n_seqs
     assert seq_cached is None or (seq_cached.dtype == torch.int32 and seq_cached.numel() == n_seqs and seq_cached.is_contiguous())
     assert (out is None) == (v_pages is None), "an output needs values, and values an output"
-    value_dim = head_dim
+    value_dim, out_stride = head_dim, 0
     if out is not None:
         value_dim = v_pages.shape[3]
-        assert v_pages.shape == (n_pages, kv_heads, PAGE, value_dim) and v_pages.dtype == q.dtype and v_pages.is_contiguous()
-        assert out.dtype == q.dtype and out.shape == (rows, n_heads * value_dim) and out.stride(1) == 1
+        out_stride, out_step = out.stride()
+        assert v_pages.dtype == out.dtype == dtype and v_pages.is_contiguous() and out_step == 1
+        assert v_pages.shape == (n_pages, kv_heads, PAGE, value_dim) and out.shape == (rows, n_heads * value_dim)
     if max_new < 1 or max_len < 1:
         raise KernelError(f"attn_paged_weights: max_new {max_new} and max_len {max_len} must be at least one")
     if not 0.0 < scale < float("inf"):
         raise KernelError(f"attn_paged_weights: the scale must be a positive number, got {scale}")
-    split_keys, floats = attn_weights_plan(n_seqs, n_heads, kv_heads, head_dim, value_dim, q.dtype, max_new, max_len, out is not None)
-    if scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < floats:
+    split_keys, floats = attn_weights_plan(n_seqs, n_heads, kv_heads, head_dim, value_dim, dtype, max_new, max_len, out is not None)
+    if scratch.dtype != torch.float32 or scratch.numel() < floats or not scratch.is_contiguous():
         raise KernelError(f"attn_paged_weights: the scratch must be {floats} contiguous float32 numbers (attn_weights_floats)")
     _check(_fn("attention_weights", "cml_attn_paged_weights")(
-        _p(q), dtype_code(q.dtype), q.stride(0), _p(out), 0 if out is None else out.stride(0), _p(k_pages), _p(v_pages), _p(scores),
-        _p(scores_out), _p(block_table), width, n_pages, _p(seq_row0), _p(seq_start), _p(seq_new), _p(seq_cached), n_seqs, rows, n_heads,
-        kv_heads, head_dim, value_dim, int(max_new), int(max_len), float(scale), split_keys, _p(scratch), _stream()), "attn_paged_weights", 3)
+        q.data_ptr(), dtype_code(dtype), q_stride, _p(out), out_stride, k_pages.data_ptr(), _p(v_pages), scores.data_ptr(),
+        scores_out.data_ptr(), block_table.data_ptr(), width, n_pages, seq_row0.data_ptr(), seq_start.data_ptr(), seq_new.data_ptr(),
+        _p(seq_cached), n_seqs, rows, n_heads, kv_heads, head_dim, value_dim, max_new, max_len, scale, split_keys, scratch.data_ptr(),
+        _stream()), "attn_paged_weights", 3)
 
 
 def evict_positions(k_pages, v_pages, scores, block_table, out_table, lengths, keeps, kept, first: int, recent: int, inv_freq=None,
@@ -2117,28 +2118,30 @@ def evict_positions(k_pages, v_pages, scores, block_table, out_table, lengths, k
     if k_pages.dim() == 4:
         k_pages, scores, kept = k_pages.unsqueeze(0), scores.unsqueeze(0), kept.unsqueeze(0)
         v_pages = v_pages.unsqueeze(0) if v_pages is not None else None
-    entries, n_pages, heads, page, k_dim = k_pages.shape
+    entries, n_pages, heads, page, k_dim = shape = k_pages.shape
     n_seqs, width = block_table.shape
+    out_rows, out_width = out_table.shape
+    dtype = k_pages.dtype
     assert page == PAGE and k_pages.is_contiguous()
-    assert scores.dtype == torch.float32 and scores.shape == (entries, n_pages, heads, PAGE) and scores.is_contiguous()
-    v_dim = 0
+    assert scores.dtype == torch.float32 and scores.shape == shape[:4] and scores.is_contiguous()
+    v_dim, v = 0, None
     if v_pages is not None:
-        v_dim = v_pages.shape[-1]
-        assert v_pages.dtype == k_pages.dtype and v_pages.shape == (entries, n_pages, heads, PAGE, v_dim) and v_pages.is_contiguous()
-    assert block_table.dtype == torch.int32 and block_table.is_contiguous()
-    assert out_table.dtype == torch.int32 and out_table.is_contiguous() and out_table.dim() == 2 and out_table.shape[0] == n_seqs
-    assert lengths.dtype == torch.int32 and lengths.numel() == n_seqs and keeps.dtype == torch.int32 and keeps.numel() == n_seqs
-    assert kept.dtype == torch.int32 and kept.is_contiguous() and kept.dim() == 4 and kept.shape[:3] == (entries, n_seqs, heads)
+        v_dim, v = v_pages.shape[4], v_pages.data_ptr()
+        assert v_pages.dtype == dtype and v_pages.shape[:4] == shape[:4] and v_pages.is_contiguous()
+    assert block_table.dtype == out_table.dtype == lengths.dtype == keeps.dtype == kept.dtype == torch.int32
+    assert block_table.is_contiguous() and out_table.is_contiguous() and lengths.is_contiguous() and keeps.is_contiguous() and kept.is_contiguous()
+    kept_entries, kept_seqs, kept_heads, room = kept.shape
+    assert out_rows == lengths.numel() == keeps.numel() == kept_seqs == n_seqs and kept_entries == entries and kept_heads == heads
     if first < 0 or recent < 0:
         raise KernelError(f"evict_positions: first {first} and recent {recent} must not be negative")
-    rotary_dim = 0
+    rotary_dim, freq = 0, None
     if inv_freq is not None:
-        rotary_dim = 2 * inv_freq.numel()
+        rotary_dim, freq = 2 * inv_freq.numel(), inv_freq.data_ptr()
         assert inv_freq.dtype == torch.float32 and inv_freq.is_contiguous() and 0 < rotary_dim <= k_dim
     _check(_fn("eviction", "cml_evict_positions")(
-        _p(k_pages), _p(v_pages), _p(scores), dtype_code(k_pages.dtype), _p(block_table), width, _p(out_table), out_table.shape[1],
-        _p(lengths), _p(keeps), _p(kept), kept.shape[3], entries, n_pages, n_seqs, heads, k_dim, v_dim, int(first), int(recent),
-        _p(inv_freq), rotary_dim, 1 if interleaved else 0, _stream()), "evict_positions", 2)
+        k_pages.data_ptr(), v, scores.data_ptr(), dtype_code(dtype), block_table.data_ptr(), width, out_table.data_ptr(), out_width,
+        lengths.data_ptr(), keeps.data_ptr(), kept.data_ptr(), room, entries, n_pages, n_seqs, heads, k_dim, v_dim, first, recent, freq,
+        rotary_dim, 1 if interleaved else 0, _stream()), "evict_positions", 2)
 
 
 VERIFY_PART = 1024              # columns of a row of logits that a warp adds up; VF_PART in verify.cu
@@ -2164,26 +2167,30 @@ def verify_drafts(logits, row0, lens, drafts, draft_probs, accept_draws, next_dr
     or a negative or not finite probability, 8 for rows that do not exist (no token at all). ``scratch``: uint8, ``verify_bytes``."""
     _here(logits, row0, lens, drafts, draft_probs, accept_draws, next_draws, counts, tokens, err, scratch)
     rows, vocab = logits.shape
-    n, room = drafts.shape
-    assert logits.dtype == torch.float32 and logits.stride(1) == 1
-    assert drafts.dtype == torch.int32 and (room < 2 or drafts.stride(1) == 1)
-    assert accept_draws.dtype == torch.float32 and accept_draws.shape == (n, room) and (room < 2 or accept_draws.stride(1) == 1)
-    assert next_draws.dtype == torch.float32 and next_draws.numel() == n and next_draws.is_contiguous()
-    for t in (row0, lens, counts):
-        assert t.dtype == torch.int32 and t.numel() == n and t.is_contiguous()
-    assert tokens.dtype == torch.int32 and tokens.shape == (n, room + 1) and tokens.is_contiguous() and err.dtype == torch.int32
+    n, room = shape = drafts.shape
+    ld, step = logits.stride()
+    drafts_ld, drafts_step = drafts.stride()
+    accept_ld, accept_step = accept_draws.stride()
+    assert logits.dtype == accept_draws.dtype == next_draws.dtype == torch.float32 and step == 1
+    assert accept_draws.shape == shape and (room < 2 or drafts_step == accept_step == 1)
+    assert row0.dtype == lens.dtype == drafts.dtype == counts.dtype == tokens.dtype == err.dtype == torch.int32
+    assert row0.numel() == lens.numel() == counts.numel() == next_draws.numel() == n
+    assert row0.is_contiguous() and lens.is_contiguous() and counts.is_contiguous() and next_draws.is_contiguous()
+    assert tokens.shape == (n, room + 1) and tokens.is_contiguous()
+    probs, probs_seq, probs_step = None, 0, 0
     if draft_probs is not None:
-        assert draft_probs.dtype == torch.float32 and draft_probs.shape == (n, room, vocab) and draft_probs.stride(2) == 1
+        probs_seq, probs_step, one = draft_probs.stride()
+        probs = draft_probs.data_ptr()
+        assert draft_probs.dtype == torch.float32 and draft_probs.shape == (n, room, vocab) and (one == 1 or vocab == 1)
     if not (0.0 <= temperature < float("inf")) or top_k < 0 or not top_p > 0.0 or not 0.0 <= min_p <= 1.0:
         raise KernelError(f"verify_drafts: temperature {temperature}, top_k {top_k}, top_p {top_p} or min_p {min_p} is outside its range")
     need = verify_bytes(rows, n, vocab)
-    if scratch.dtype != torch.uint8 or not scratch.is_contiguous() or scratch.numel() < need:
+    if scratch.dtype != torch.uint8 or scratch.numel() < need or not scratch.is_contiguous():
         raise KernelError(f"verify_drafts: the scratch must be {need} contiguous bytes (verify_bytes)")
     _check(_fn("verify", "cml_verify_drafts")(
-        _p(logits), logits.stride(0), rows, vocab, _p(row0), _p(lens), _p(drafts), drafts.stride(0), _p(draft_probs),
-        0 if draft_probs is None else draft_probs.stride(0), 0 if draft_probs is None else draft_probs.stride(1), _p(accept_draws),
-        accept_draws.stride(0), _p(next_draws), n, room, float(temperature), int(top_k), float(top_p), float(min_p), _p(counts),
-        _p(tokens), _p(err), _p(scratch), _stream()), "verify_drafts", 2)
+        logits.data_ptr(), ld, rows, vocab, row0.data_ptr(), lens.data_ptr(), drafts.data_ptr(), drafts_ld, probs, probs_seq, probs_step,
+        accept_draws.data_ptr(), accept_ld, next_draws.data_ptr(), n, room, temperature, top_k, top_p, min_p, counts.data_ptr(),
+        tokens.data_ptr(), err.data_ptr(), scratch.data_ptr(), _stream()), "verify_drafts", 2)
 
 
 class NativeDecodeLoop:
