@@ -16,8 +16,9 @@
 #include <math_constants.h>
 namespace cg = cooperative_groups;
 
-#define AW_THREADS 128
+#define AW_THREADS 256
 #define AW_ROWS 8               // rows (token, head) a block works on together
+#define AW_TEAM 8               // blocks of a cluster at most (sixteen were 7% to 40% slower here)
 
 struct WeightArgs {
     const void* q;
@@ -74,10 +75,13 @@ template <typename T>
 __device__ __forceinline__ void fetch_page(unsigned char* dst, int stride, const T* src, int dim, int valid) {
     const int chunks = dim * (int)sizeof(T) / 16;
     const uint32_t at = (uint32_t)__cvta_generic_to_shared(dst);
-    for (int c = threadIdx.x; c < CML_PAGE * chunks; c += AW_THREADS) {
-        const int r = c / chunks, cc = c - r * chunks;
+    int r = (int)threadIdx.x / chunks, cc = (int)threadIdx.x - r * chunks;    // walked without further divisions
+    const int r_step = AW_THREADS / chunks, c_step = AW_THREADS - r_step * chunks;
+    while (r < CML_PAGE) {
         if (r < valid) cp_async16(at + (uint32_t)(r * stride + cc * 16), (const unsigned char*)src + ((size_t)r * dim) * sizeof(T) + cc * 16);
         else *reinterpret_cast<uint4*>(dst + r * stride + cc * 16) = make_uint4(0, 0, 0, 0);
+        r += r_step, cc += c_step;
+        if (cc >= chunks) cc -= chunks, ++r;
     }
 }
 
@@ -96,11 +100,11 @@ template <> __device__ __forceinline__ float dot_chunk<bf16>(const unsigned char
     return s;
 }
 
-// q of AW_ROWS rows as float into shared memory (zeros where there is no row).
-template <typename T>
+// q of R rows as float into shared memory (zeros where there is no row).
+template <typename T, int R>
 __device__ __forceinline__ void load_q(const WeightArgs& a, const Seq& s, int kvh, int m0, float* q_s) {
     const int group = a.heads / a.kv_heads;
-    for (int c = threadIdx.x; c < AW_ROWS * a.k_dim; c += AW_THREADS) {
+    for (int c = threadIdx.x; c < R * a.k_dim; c += AW_THREADS) {
         const int m = m0 + c / a.k_dim, d = c % a.k_dim;
         float x = 0.f;
         if (m < s.rows) x = to_f32(((const T*)a.q)[(long long)(s.row0 + m / group) * a.q_stride + (long long)(kvh * group + m % group) * a.k_dim + d]);
@@ -108,43 +112,58 @@ __device__ __forceinline__ void load_q(const WeightArgs& a, const Seq& s, int kv
     }
 }
 
-// The scores of this thread's key (threadIdx.x & 63) for four of the block's rows (threadIdx.x >> 6), scaled and masked.
-template <typename T>
-__device__ __forceinline__ void score4(const WeightArgs& a, const Seq& s, int m0, int place, bool there, const unsigned char* k_row,
-                                       const float* q_s, float (&out)[4]) {
+// The scores of this thread's key (threadIdx.x & 63) for a quarter of the block's R rows (threadIdx.x >> 6), scaled and masked.
+template <typename T, int R>
+__device__ __forceinline__ void score_rows(const WeightArgs& a, const Seq& s, int m0, int place, bool there, const unsigned char* k_row,
+                                           const float* q_s, float (&out)[R / 4]) {
     constexpr int N = 16 / sizeof(T);
-    const int group = a.heads / a.kv_heads, half = threadIdx.x >> 6;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    const float* q = q_s + half * 4 * a.k_dim;
+    const int group = a.heads / a.kv_heads, quarter = threadIdx.x >> 6;
+    float acc[R / 4];
+#pragma unroll
+    for (int m = 0; m < R / 4; ++m) acc[m] = 0.f;
+    const float* q = q_s + quarter * (R / 4) * a.k_dim;
+#pragma unroll 4
     for (int d = 0; d < a.k_dim; d += N)
 #pragma unroll
-        for (int m = 0; m < 4; ++m) acc[m] += dot_chunk<T>(k_row + d * sizeof(T), q + m * a.k_dim + d);
+        for (int m = 0; m < R / 4; ++m) acc[m] += dot_chunk<T>(k_row + d * sizeof(T), q + m * a.k_dim + d);
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-        const int r = m0 + half * 4 + m;
+    for (int m = 0; m < R / 4; ++m) {
+        const int r = m0 + quarter * (R / 4) + m;
         out[m] = there && r < s.rows && place <= s.start + r / group ? acc[m] * a.scale : -CUDART_INF_F;
     }
 }
 
-// (1) a stretch of keys: grid (stretches, sequences * kv heads, row tiles)
-template <typename T>
+// R rows and a stretch of keys, in float on the CUDA cores: a page of keys and values at a time, a quarter of the rows and
+// a key a thread for the scores, a channel (of half the keys, up to 128 channels) for the output. ALL (grid: cluster, pairs; for steps of at most R rows): the blocks of a cluster share all
+// keys of a sequence and finish by themselves, as on the tensor cores below. Otherwise (grid: stretches, pairs, row tiles)
+// this is step (1).
+template <typename T, int R, bool ALL>
 __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) {
     extern __shared__ __align__(16) unsigned char raw[];
-    const int split = blockIdx.x, seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads, m0 = blockIdx.z * AW_ROWS;
+    __shared__ float2 stat_s[ALL ? AW_TEAM * R : 1];              // ALL: [blocks][rows] maximum and sum, of the whole cluster
+    __shared__ float2 join_s[ALL ? R : 1];                        // ALL: [rows] maximum and 1 / sum of all keys
+    const int split = blockIdx.x, seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads, m0 = blockIdx.z * R;
     pdl_wait();
     pdl_launch_dependents();
     const Seq s = seq_of(a, seq);
-    const int first = split * a.split_keys, last = min(s.length, first + a.split_keys);
-    if (first >= last || m0 >= s.rows) return;
+    if (m0 >= s.rows) return;                                     // the same for a whole cluster
+    const int team = ALL ? (int)gridDim.x : 1;
+    const int share = ALL ? (s.length + team * CML_PAGE - 1) / (team * CML_PAGE) * CML_PAGE : a.split_keys;
+    const int first = split * share, last = min(s.length, first + share);
+    if (ALL) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");        // started: waited for before remote stores
+    else if (first >= last) return;
     const int k_stride = a.k_dim * (int)sizeof(T) + 16, v_stride = a.out ? a.v_dim * (int)sizeof(T) : 0;
     const int page_bytes = CML_PAGE * (k_stride + v_stride);
     float* q_s = reinterpret_cast<float*>(raw + a.stages * page_bytes);
-    float* p_s = q_s + AW_ROWS * a.k_dim;                          // [rows][page]
-    float* m_s = p_s + AW_ROWS * CML_PAGE;
-    float* l_s = m_s + AW_ROWS;
-    float* c_s = l_s + AW_ROWS;
+    float* p_s = q_s + R * a.k_dim;                               // [page][rows]
+    float* m_s = p_s + R * CML_PAGE;
+    float* l_s = m_s + R;
+    float* c_s = l_s + R;
+    float* own = c_s + R;                                         // [rows][v_dim], the block's output
     const int* pages = a.table + (size_t)seq * a.width;
     const int p_first = first / CML_PAGE, p_last = (last + CML_PAGE - 1) / CML_PAGE;
+    const int group_rows = a.max_new * (a.heads / a.kv_heads);
+    float* const kept = ALL ? a.kept + (size_t)blockIdx.y * group_rows * a.kept_stride : nullptr;
     auto valid_of = [&](int p) {
         const int page = p < p_last ? pages[p] : -1;
         return page < 0 || page >= a.n_pages ? 0 : min(CML_PAGE, last - p * CML_PAGE);
@@ -160,12 +179,16 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
         cp_async_commit();
     };
     fetch(p_first);
-    load_q<T>(a, s, kvh, m0, q_s);
-    if (threadIdx.x < AW_ROWS) m_s[threadIdx.x] = -CUDART_INF_F, l_s[threadIdx.x] = 0.f;
-    float o[AW_ROWS][2];
+    load_q<T, R>(a, s, kvh, m0, q_s);
+    if (threadIdx.x < R) m_s[threadIdx.x] = -CUDART_INF_F, l_s[threadIdx.x] = 0.f;
+    float o[R];
 #pragma unroll
-    for (int m = 0; m < AW_ROWS; ++m) o[m][0] = o[m][1] = 0.f;
+    for (int m = 0; m < R; ++m) o[m] = 0.f;
+    const bool halves = a.v_dim <= AW_THREADS / 2;
+    const int d = halves ? threadIdx.x & (AW_THREADS / 2 - 1) : threadIdx.x;
+    const int kk_first = halves ? (threadIdx.x / (AW_THREADS / 2)) * (CML_PAGE / 2) : 0, kk_last = halves ? kk_first + CML_PAGE / 2 : CML_PAGE;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rows = min(R, s.rows - m0);
     for (int p = p_first; p < p_last; ++p) {
         if (a.stages > 1) fetch(p + 1);
         else if (p > p_first) fetch(p);
@@ -173,67 +196,124 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
         else cp_async_wait<0>();
         __syncthreads();
         const unsigned char* ks = raw + (size_t)((p - p_first) & (a.stages - 1)) * page_bytes;
-        const int key = threadIdx.x & 63;
-        float sc[4];
-        score4<T>(a, s, m0, p * CML_PAGE + key, key < valid_of(p), ks + key * k_stride, q_s, sc);
+        const int key = threadIdx.x & 63, quarter = threadIdx.x >> 6;
+        float sc[R / 4];
+        score_rows<T, R>(a, s, m0, p * CML_PAGE + key, key < valid_of(p), ks + key * k_stride, q_s, sc);
 #pragma unroll
-        for (int m = 0; m < 4; ++m) p_s[((threadIdx.x >> 6) * 4 + m) * CML_PAGE + key] = sc[m];
+        for (int m = 0; m < R / 4; ++m) {
+            p_s[key * R + quarter * (R / 4) + m] = sc[m];
+            if (ALL && quarter * (R / 4) + m < rows) kept[(size_t)(quarter * (R / 4) + m) * a.kept_stride + p * CML_PAGE + key] = sc[m];
+        }
         __syncthreads();
-#pragma unroll
-        for (int mm = 0; mm < 2; ++mm) {
-            const int m = warp * 2 + mm;
-            const float a0 = p_s[m * CML_PAGE + lane], a1 = p_s[m * CML_PAGE + lane + 32];
+        for (int m = warp; m < rows; m += AW_THREADS / 32) {
+            const float a0 = p_s[lane * R + m], a1 = p_s[(lane + 32) * R + m];
             const float old = m_s[m], now = fmaxf(old, warp_max(fmaxf(a0, a1)));
             const float e0 = a0 == -CUDART_INF_F ? 0.f : exp2f(a0 - now), e1 = a1 == -CUDART_INF_F ? 0.f : exp2f(a1 - now);
             const float corr = old == -CUDART_INF_F ? 0.f : exp2f(old - now);
             const float sum = warp_sum(e0 + e1);
-            p_s[m * CML_PAGE + lane] = e0;
-            p_s[m * CML_PAGE + lane + 32] = e1;
+            p_s[lane * R + m] = e0;
+            p_s[(lane + 32) * R + m] = e1;
             __syncwarp();
             if (lane == 0) m_s[m] = now, l_s[m] = l_s[m] * corr + sum, c_s[m] = corr;
         }
         __syncthreads();
-        if (a.out) {
+        if (a.out && d < a.v_dim) {
             const T* vs = reinterpret_cast<const T*>(ks + CML_PAGE * k_stride);
+            float t[R];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int d = threadIdx.x + h * AW_THREADS;
-                if (d >= a.v_dim) break;
-                float t[AW_ROWS];
-#pragma unroll
-                for (int m = 0; m < AW_ROWS; ++m) t[m] = 0.f;
-                for (int kk = 0; kk < CML_PAGE; ++kk) {
+            for (int m = 0; m < R; ++m) t[m] = 0.f;
+            if (s.fresh > 1 && (p + 1) * CML_PAGE > s.start + 1) {
+                // where rows do not all see the same places, one that a row does not see adds nothing, whatever it holds
+                for (int kk = kk_first; kk < kk_last; ++kk) {
                     const float val = to_f32(vs[kk * a.v_dim + d]);
 #pragma unroll
-                    for (int m = 0; m < AW_ROWS; ++m) {
-                        const float w = p_s[m * CML_PAGE + kk];
-                        if (w != 0.f) t[m] += w * val;             // a place that a row does not see adds nothing, whatever it holds
+                    for (int m = 0; m < R; ++m) {
+                        const float w = p_s[kk * R + m];
+                        if (w != 0.f) t[m] = fmaf(w, val, t[m]);
                     }
                 }
+            } else {
+#pragma unroll 8
+                for (int kk = kk_first; kk < kk_last; ++kk) {
+                    const float val = to_f32(vs[kk * a.v_dim + d]);
 #pragma unroll
-                for (int m = 0; m < AW_ROWS; ++m) o[m][h] = o[m][h] * c_s[m] + t[m];
+                    for (int m = 0; m < R; m += 4) {
+                        const float4 w = *reinterpret_cast<const float4*>(p_s + kk * R + m);
+                        t[m] = fmaf(w.x, val, t[m]);
+                        t[m + 1] = fmaf(w.y, val, t[m + 1]);
+                        t[m + 2] = fmaf(w.z, val, t[m + 2]);
+                        t[m + 3] = fmaf(w.w, val, t[m + 3]);
+                    }
+                }
             }
+#pragma unroll
+            for (int m = 0; m < R; ++m)
+                if (m < rows) o[m] = o[m] * c_s[m] + t[m];
         }
         __syncthreads();
     }
     cp_async_wait<0>();
-    const int group_rows = a.max_new * (a.heads / a.kv_heads);
-    const size_t base = ((size_t)blockIdx.y * a.n_splits + split) * group_rows;
-    if (threadIdx.x < AW_ROWS && m0 + threadIdx.x < s.rows) {
-        a.stats[(base + m0 + threadIdx.x) * 2] = m_s[threadIdx.x];
-        a.stats[(base + m0 + threadIdx.x) * 2 + 1] = l_s[threadIdx.x];
+    __syncthreads();
+    if (a.out && d < a.v_dim && (!halves || kk_first > 0)) {
+#pragma unroll
+        for (int m = 0; m < R; ++m) own[m * a.v_dim + d] = o[m];
     }
-    if (a.out) {
+    __syncthreads();
+    if (a.out && halves && kk_first == 0 && d < a.v_dim) {        // the first half of the keys, then the second
 #pragma unroll
-        for (int m = 0; m < AW_ROWS; ++m) {
-            if (m0 + m >= s.rows) break;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int d = threadIdx.x + h * AW_THREADS;
-                if (d < a.v_dim) a.acc[(base + m0 + m) * a.v_dim + d] = o[m][h];
-            }
+        for (int m = 0; m < R; ++m) own[m * a.v_dim + d] = o[m] + own[m * a.v_dim + d];
+    }
+    if (!ALL) {
+        const size_t base = ((size_t)blockIdx.y * a.n_splits + split) * group_rows + m0;
+        if ((int)threadIdx.x < rows) {
+            a.stats[(base + threadIdx.x) * 2] = m_s[threadIdx.x];
+            a.stats[(base + threadIdx.x) * 2 + 1] = l_s[threadIdx.x];
+        }
+        __syncthreads();
+        if (a.out)
+            for (int i = threadIdx.x; i < rows * a.v_dim; i += AW_THREADS) a.acc[base * a.v_dim + i] = own[i];
+        return;
+    }
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if ((int)threadIdx.x < rows)
+        for (int c = 0; c < team; ++c) cg::this_cluster().map_shared_rank(&stat_s[0], c)[split * R + threadIdx.x] = make_float2(m_s[threadIdx.x], l_s[threadIdx.x]);
+    cg::this_cluster().sync();
+    if ((int)threadIdx.x < rows) {
+        const int m = threadIdx.x;
+        float most = -CUDART_INF_F, l = 0.f;
+        for (int c = 0; c < team; ++c) most = fmaxf(most, stat_s[c * R + m].x);
+        for (int c = 0; c < team; ++c) {
+            const float2 t = stat_s[c * R + m];
+            const float f = t.x == -CUDART_INF_F ? 0.f : exp2f(t.x - most);
+            stat_s[c * R + m].x = f;                              // from here on: what a block's output counts in the joined one
+            l += f * t.y;
+        }
+        join_s[m] = most == -CUDART_INF_F ? make_float2(0.f, 0.f) : make_float2(most, 1.f / l);
+    }
+    __syncthreads();
+    if (a.out) {                                                  // the output's elements in equal shares, the blocks in their order
+        const int group = a.heads / a.kv_heads;
+        for (int i = split * AW_THREADS + threadIdx.x; i < rows * a.v_dim; i += team * AW_THREADS) {
+            const int m = i / a.v_dim, d = i - m * a.v_dim;
+            float x = 0.f;
+#pragma unroll 4
+            for (int c = 0; c < team; ++c) x += stat_s[c * R + m].x * cg::this_cluster().map_shared_rank(own, c)[m * a.v_dim + d];
+            ((T*)a.out)[(long long)(s.row0 + m / group) * a.out_stride + (long long)(kvh * group + m % group) * a.v_dim + d] = from_f32<T>(x * join_s[m].y);
         }
     }
+    // the weights of this block's keys
+    for (int place = first + (int)threadIdx.x; place < last; place += AW_THREADS) {
+        const int page = pages[place / CML_PAGE];
+        if (page < 0 || page >= a.n_pages) continue;
+        const size_t at = ((size_t)page * a.kv_heads + kvh) * CML_PAGE + place % CML_PAGE;
+        float gained = 0.f;
+        const float old = a.scores[at];
+#pragma unroll
+        for (int m = 0; m < R; ++m)
+            if (m < rows) gained += exp2f(kept[(size_t)m * a.kept_stride + place] - join_s[m].x) * join_s[m].y;
+        a.scores_out[at] = (place < s.old ? old : 0.f) + gained;
+    }
+    if (a.out) cg::this_cluster().sync();                         // a block's output stays until every block has read it
 }
 
 // (2) the stretches of a row joined in their order: grid (rows that share a kv head, sequences * kv heads)
@@ -275,7 +355,7 @@ __global__ void __launch_bounds__(AW_THREADS) weights_join_kernel(WeightArgs a) 
 template <typename T>
 __global__ void __launch_bounds__(AW_THREADS) weights_sum_kernel(WeightArgs a) {
     extern __shared__ __align__(16) unsigned char raw[];
-    __shared__ float other[CML_PAGE];
+    __shared__ float other[3][CML_PAGE];
     pdl_wait();
     pdl_launch_dependents();
     const int p = blockIdx.x, seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
@@ -289,29 +369,29 @@ __global__ void __launch_bounds__(AW_THREADS) weights_sum_kernel(WeightArgs a) {
     const size_t at = ((size_t)page * a.kv_heads + kvh) * CML_PAGE;
     fetch_page<T>(raw, k_stride, (const T*)a.k + at * a.k_dim, a.k_dim, valid);
     cp_async_commit();
-    const int key = threadIdx.x & 63, half = threadIdx.x >> 6;
+    const int key = threadIdx.x & 63, quarter = threadIdx.x >> 6;
     const int group_rows = a.max_new * (a.heads / a.kv_heads);
     float gained = 0.f;
     for (int m0 = 0; m0 < s.rows; m0 += AW_ROWS) {
         __syncthreads();
-        load_q<T>(a, s, kvh, m0, q_s);
+        load_q<T, AW_ROWS>(a, s, kvh, m0, q_s);
         cp_async_wait<0>();
         __syncthreads();
-        float sc[4];
-        score4<T>(a, s, m0, p * CML_PAGE + key, key < valid, raw + key * k_stride, q_s, sc);
+        float sc[AW_ROWS / 4];
+        score_rows<T, AW_ROWS>(a, s, m0, p * CML_PAGE + key, key < valid, raw + key * k_stride, q_s, sc);
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const int r = m0 + half * 4 + m;
+        for (int m = 0; m < AW_ROWS / 4; ++m) {
+            const int r = m0 + quarter * (AW_ROWS / 4) + m;
             if (r >= s.rows || sc[m] == -CUDART_INF_F) continue;
             const float* j = a.joined + ((size_t)blockIdx.y * group_rows + r) * 2;
             gained += exp2f(sc[m] - j[0]) * j[1];
         }
     }
-    if (half == 1) other[key] = gained;
+    if (quarter > 0) other[quarter - 1][key] = gained;
     __syncthreads();
-    if (half == 0 && key < valid) {
+    if (quarter == 0 && key < valid) {
         const int place = p * CML_PAGE + key;
-        a.scores_out[at + key] = (place < s.old ? a.scores[at + key] : 0.f) + (gained + other[key]);
+        a.scores_out[at + key] = (place < s.old ? a.scores[at + key] : 0.f) + (((gained + other[0][key]) + other[1][key]) + other[2][key]);
     }
 }
 
@@ -1043,39 +1123,12 @@ __global__ void __launch_bounds__(AR_WARPS * 32, 2) weights_keys_mma_kernel(Weig
         }
 }
 
-template <typename T>
-static cudaError_t launch_plain(WeightArgs& a, cudaStream_t s) {
-    const unsigned pairs = (unsigned)a.n_seqs * (unsigned)a.kv_heads;
-    const int group_rows = a.max_new * (a.heads / a.kv_heads);
-    const size_t k_page = (size_t)CML_PAGE * (a.k_dim * sizeof(T) + 16), v_page = a.out ? (size_t)CML_PAGE * a.v_dim * sizeof(T) : 0;
-    const size_t rows = (size_t)AW_ROWS * a.k_dim * 4;
-    const size_t rest = rows + AW_ROWS * CML_PAGE * 4 + 3 * AW_ROWS * 4, smem3 = k_page + rows;
-    a.stages = 2 * (k_page + v_page) + rest <= 227 * 1024 ? 2 : 1;
-    const size_t smem1 = a.stages * (k_page + v_page) + rest;
-    cudaError_t e = cml_allow_smem<weights_part_kernel<T>>(smem1);
-    if (e == cudaSuccess) e = cml_allow_smem<weights_sum_kernel<T>>(smem3);
-    if (e != cudaSuccess) return e;
-    e = launch_pdl(weights_part_kernel<T>, dim3((unsigned)a.n_splits, pairs, (unsigned)((group_rows + AW_ROWS - 1) / AW_ROWS)), dim3(AW_THREADS),
-                   smem1, s, a);
-    if (e != cudaSuccess) return e;
-    e = launch_pdl(weights_join_kernel<T>, dim3((unsigned)group_rows, pairs), dim3(AW_THREADS), 0, s, a);
-    if (e != cudaSuccess) return e;
-    return launch_pdl(weights_sum_kernel<T>, dim3((unsigned)((a.max_len + CML_PAGE - 1) / CML_PAGE), pairs), dim3(AW_THREADS), smem3, s, a);
-}
-
-template <int HD, int MT, bool OUT>
-static cudaError_t launch_all(const WeightArgs& a, unsigned pairs, int team, size_t smem, cudaStream_t s) {
-    const auto kernel = weights_part_mma_kernel<HD, MT, OUT, true>;
-    static bool wide = false;                                     // clusters of 16 blocks have to be asked for, once
-    cudaError_t e = cml_allow_smem<weights_part_mma_kernel<HD, MT, OUT, true>>(smem);
-    if (e == cudaSuccess && !wide) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        wide = e == cudaSuccess;
-    }
-    if (e != cudaSuccess) return e;
+// A launch of clusters of `team` blocks, one for each pair.
+template <typename K>
+static cudaError_t launch_team(K kernel, const WeightArgs& a, unsigned pairs, int team, int threads, size_t smem, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)team, pairs);
-    cfg.blockDim = dim3(AM_WARPS * 32);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -1088,6 +1141,57 @@ static cudaError_t launch_all(const WeightArgs& a, unsigned pairs, int team, siz
     cfg.attrs = attr;
     cfg.numAttrs = cml_pdl_enabled() ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+// Clusters of sixteen blocks have to be asked for, once a kernel.
+template <auto Kernel>
+static cudaError_t allow_wide_clusters() {
+    static bool allowed = false;
+    if (allowed) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    allowed = e == cudaSuccess;
+    return e;
+}
+
+template <typename T, int R>
+static cudaError_t launch_plain_all(const WeightArgs& a, unsigned pairs, size_t smem, cudaStream_t s) {
+    cudaError_t e = cml_allow_smem<weights_part_kernel<T, R, true>>(smem);
+    if (e == cudaSuccess) e = allow_wide_clusters<weights_part_kernel<T, R, true>>();
+    if (e != cudaSuccess) return e;
+    int team = 1;                                                 // two blocks for every multiprocessor, none without a page of keys
+    while (team < AW_TEAM && (long long)pairs * team < 2ll * cml_sm_count() && team * CML_PAGE < a.max_len) team *= 2;
+    return launch_team(weights_part_kernel<T, R, true>, a, pairs, team, AW_THREADS, smem, s);
+}
+
+template <typename T>
+static cudaError_t launch_plain(WeightArgs& a, cudaStream_t s) {
+    const unsigned pairs = (unsigned)a.n_seqs * (unsigned)a.kv_heads;
+    const int group_rows = a.max_new * (a.heads / a.kv_heads);
+    const size_t k_page = (size_t)CML_PAGE * (a.k_dim * sizeof(T) + 16), v_page = a.out ? (size_t)CML_PAGE * a.v_dim * sizeof(T) : 0;
+    auto rest = [&](int rows) { return (size_t)rows * (a.k_dim + CML_PAGE + 3 + (a.out ? a.v_dim : 0)) * 4; };
+    a.stages = 2 * (k_page + v_page) + rest(AW_ROWS) <= 220 * 1024 ? 2 : 1;
+    const size_t ring = a.stages * (k_page + v_page);
+    if (group_rows <= 4) return launch_plain_all<T, 4>(a, pairs, ring + rest(4), s);
+    if (group_rows <= AW_ROWS) return launch_plain_all<T, AW_ROWS>(a, pairs, ring + rest(AW_ROWS), s);
+    const size_t smem1 = ring + rest(AW_ROWS), smem3 = k_page + (size_t)AW_ROWS * a.k_dim * 4;
+    cudaError_t e = cml_allow_smem<weights_part_kernel<T, AW_ROWS, false>>(smem1);
+    if (e == cudaSuccess) e = cml_allow_smem<weights_sum_kernel<T>>(smem3);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(weights_part_kernel<T, AW_ROWS, false>, dim3((unsigned)a.n_splits, pairs, (unsigned)((group_rows + AW_ROWS - 1) / AW_ROWS)), dim3(AW_THREADS),
+                   smem1, s, a);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(weights_join_kernel<T>, dim3((unsigned)group_rows, pairs), dim3(AW_THREADS), 0, s, a);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(weights_sum_kernel<T>, dim3((unsigned)((a.max_len + CML_PAGE - 1) / CML_PAGE), pairs), dim3(AW_THREADS), smem3, s, a);
+}
+
+template <int HD, int MT, bool OUT>
+static cudaError_t launch_all(const WeightArgs& a, unsigned pairs, int team, size_t smem, cudaStream_t s) {
+    const auto kernel = weights_part_mma_kernel<HD, MT, OUT, true>;
+    cudaError_t e = cml_allow_smem<weights_part_mma_kernel<HD, MT, OUT, true>>(smem);
+    if (e == cudaSuccess) e = allow_wide_clusters<weights_part_mma_kernel<HD, MT, OUT, true>>();
+    if (e != cudaSuccess) return e;
+    return launch_team(kernel, a, pairs, team, AM_WARPS * 32, smem, s);
 }
 
 template <int HD>
