@@ -111,20 +111,23 @@ struct TeamSlots {
 };
 
 // Every element of this block's slice to `f(value, index)`, a thread's elements in ascending index order. Rows
-// that start on a 16-byte boundary are read 16 bytes at a time, two such loads in flight per thread (a scan with
+// that start on a 16-byte boundary are read 16 bytes at a time, FLIGHT such loads in flight per thread (a scan with
 // one 4-byte load at a time is bound by the loads' round trips).
-template <typename F>
+template <int FLIGHT = 2, typename F>
 __device__ __forceinline__ void for_each_in_slice(const float* __restrict__ row, const Team& tm, F f) {
     const int begin = tm.begin, end = tm.end;
     if ((((uintptr_t)row) & 15) == 0) {
         const int g_begin = begin >> 2, g_end = end >> 2;          // whole groups of four within the slice
         const float4* r4 = reinterpret_cast<const float4*>(row);
-        for (int g0 = g_begin + threadIdx.x; g0 < g_end; g0 += 2 * blockDim.x) {
-            const int g1 = g0 + blockDim.x;
-            const float4 a = r4[g0];
-            const float4 b = r4[min(g1, g_end - 1)];
-            f(a.x, 4 * g0); f(a.y, 4 * g0 + 1); f(a.z, 4 * g0 + 2); f(a.w, 4 * g0 + 3);
-            if (g1 < g_end) { f(b.x, 4 * g1); f(b.y, 4 * g1 + 1); f(b.z, 4 * g1 + 2); f(b.w, 4 * g1 + 3); }
+        for (int g0 = g_begin + threadIdx.x; g0 < g_end; g0 += FLIGHT * blockDim.x) {
+            float4 v[FLIGHT];
+#pragma unroll
+            for (int u = 0; u < FLIGHT; ++u) v[u] = r4[min(g0 + u * (int)blockDim.x, g_end - 1)];
+#pragma unroll
+            for (int u = 0; u < FLIGHT; ++u) {
+                const int g = g0 + u * (int)blockDim.x;
+                if (g < g_end) { f(v[u].x, 4 * g); f(v[u].y, 4 * g + 1); f(v[u].z, 4 * g + 2); f(v[u].w, 4 * g + 3); }
+            }
         }
         for (int i = max(begin, 4 * g_end) + threadIdx.x; i < end; i += blockDim.x) f(row[i], i);
     } else {
@@ -190,7 +193,7 @@ __device__ __forceinline__ float value_of_key(unsigned long long key) {
 // Returns true and the choice if the fast way settled it, false if the caller has to run select_by_mass.
 // `xof(v)` is the place of a value in the order (smaller first, monotone in v), `weight(v, i)` as above,
 // `approx(x)` a cheap estimate of the weight of a value at place x, good enough to find the bin.
-template <typename W, typename XFn, typename WeightFn, typename ApproxFn>
+template <int FLIGHT = 2, typename W, typename XFn, typename WeightFn, typename ApproxFn>
 __device__ bool select_fast(const float* row, Team& tm, unsigned long long floor_key, double target, int strict,
                             XFn xof, float x_max, WeightFn weight, ApproxFn approx, FastSharedOf<W>* fs, TeamSlots* ts,
                             unsigned long long* out_key, double* out_cum) {
@@ -212,7 +215,7 @@ __device__ bool select_fast(const float* row, Team& tm, unsigned long long floor
         auto bin_of = [&](float v) { return bin_at(xof(v)); };
         const bool has_floor = floor_key != 0ull;
         double head = 0.0;                               // weight ordered before the range
-        for_each_in_slice(row, tm, [&](float v, int i) {
+        for_each_in_slice<FLIGHT>(row, tm, [&](float v, int i) {
             if (has_floor && composite_key(v, i) < floor_key) return;
             const float x = xof(v);
             const int b = bin_at(x);
@@ -285,7 +288,7 @@ __device__ bool select_fast(const float* row, Team& tm, unsigned long long floor
             const int bsel = fs0->bin;
             double before = 0.0;
             unsigned int after = 0u;
-            for_each_in_slice(row, tm, [&](float v, int i) {
+            for_each_in_slice<FLIGHT>(row, tm, [&](float v, int i) {
                 if (has_floor && composite_key(v, i) < floor_key) return;
                 const int b = bin_of(v);
                 if (b < bsel) before += (double)weight(v, i);

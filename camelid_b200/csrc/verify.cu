@@ -100,6 +100,9 @@ __device__ __forceinline__ double weight_of(float l, const Exponential& e, const
     return l < e.least ? 0.0 : w;
 }
 
+// a call instead of a copy, for kernels whose many loops would not fit the instruction cache with a copy for every element
+__device__ __noinline__ double weight_call(float l, Exponential e, const double* table) { return weight_of(l, e, table); }
+
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < CUDART_INF_F; }
 
 // (1a) without filters. A warp takes a part at a time and keeps its 32 columns a lane in registers, so that the row is read
@@ -178,6 +181,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
     __shared__ float fred[33];
     __shared__ double table[32];
     fill_table(table);
+    if (threadIdx.x == 0) fs.n_list = 0u;
     cg::this_cluster().sync();                                    // every block has started before its memory is written
     pdl_wait();
     pdl_launch_dependents();
@@ -196,7 +200,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
     const float* row = a.logits + (long long)row_index * a.ld;
     float mx = -CUDART_INF_F, mn = CUDART_INF_F;
     bool bad = false;
-    for_each_in_slice(row, tm, [&](float v, int) {
+    for_each_in_slice<8>(row, tm, [&](float v, int) {
         if (!finite(v)) bad = true;
         mx = fmaxf(mx, v);
         mn = fminf(mn, v);
@@ -230,7 +234,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
     const float inv_t = fminf(1.0f / a.temperature, 1e30f), far = 1e30f;
     auto xof = [=](float v) { return fminf((mx - v) * inv_t, far); };
     const float x_max = xof(mn);
-    auto raw_weight = [=](float v, int) { return weight_of(v, ex, table); };
+    const double* const powers = table;
+    auto raw_weight = [=](float v, int) { return weight_call(v, ex, powers); };
     unsigned long long floor_key = 0ull, key;
     double cum;
     auto select_slow = [&](unsigned long long floor, double target, int strict, auto weight) {
@@ -254,9 +259,79 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
     }
     // min_p: the weight of the maximum is one, so a candidate's own weight is compared
     const double least = (double)a.min_p;
+    // (only places near enough are weighed: past -ln(min_p), with room for its rounding, nothing stays)
+    const float near = least > 0.0 ? -logf(a.min_p) * 1.001f + 0.01f : CUDART_INF_F;
+    // Few candidates, the usual case where there is a min_p or a top_k: their keys are collected in one pass, sorted by block 0, and
+    // the rest of the way goes along that list.
+    if (floor_key != 0ull || least > 0.0) {
+        if (a.top_k > 0 && a.top_k < vocab) {                     // the selection left its own list there
+            if (writer) fs.n_list = 0u;
+            tm.sync();
+        }
+        for_each_in_slice<4>(row, tm, [&](float v, int i) {
+            if (xof(v) > near) return;
+            const unsigned long long ck = composite_key(v, i);
+            if (ck < floor_key || (least > 0.0 && raw_weight(v, i) < least)) return;
+            const unsigned int slot = atomicAdd(&fs0->n_list, 1u);
+            if (slot < FS_CAP) fs0->list[slot] = ck;
+        });
+        tm.sync();
+        const unsigned int n = fs0->n_list;
+        if (n <= FS_CAP) {                                        // the same in every block
+            if (tm.rank == 0) {
+                unsigned int m = 1u;
+                while (m < n) m <<= 1;
+                for (unsigned int i = n + threadIdx.x; i < m; i += blockDim.x) fs.list[i] = 0ull;
+                __syncthreads();
+                for (unsigned int k = 2; k <= m; k <<= 1) {
+                    for (unsigned int j = k >> 1; j > 0; j >>= 1) {
+                        for (unsigned int i = threadIdx.x; i < m; i += blockDim.x) {
+                            const unsigned int l = i ^ j;
+                            if (l > i) {
+                                const unsigned long long x = fs.list[i], y = fs.list[l];
+                                if ((i & k) == 0 ? x < y : x > y) { fs.list[i] = y; fs.list[l] = x; }
+                            }
+                        }
+                        __syncthreads();
+                    }
+                }
+                if (threadIdx.x < 32) {                           // one warp adds up, 32 candidates at a time, in their order
+                    const int lane = threadIdx.x;
+                    double sum = 0.0;
+                    for (unsigned int i0 = 0; i0 < n; i0 += 32) {
+                        double w = i0 + lane < n ? raw_weight(value_of_key(fs.list[i0 + lane]), 0) : 0.0;
+#pragma unroll
+                        for (int o = 1; o < 32; o <<= 1) {
+                            const double t = __shfl_up_sync(0xffffffffu, w, o);
+                            if (lane >= o) w += t;
+                        }
+                        fs.lp[i0 + lane] = sum + w;               // cumulative; the list has room for whole warps
+                        sum = __shfl_sync(0xffffffffu, sum + w, 31);
+                    }
+                    unsigned int stay = n;                        // candidates that stay: up to the first that reaches top_p
+                    if (a.top_p < 1.f) {
+                        const double target = (double)a.top_p * sum;
+                        for (unsigned int i0 = 0; i0 < n; i0 += 32) {
+                            const unsigned int hit = __ballot_sync(0xffffffffu, i0 + lane < n && fs.lp[i0 + lane] >= target);
+                            if (hit) { stay = i0 + __ffs(hit); break; }
+                        }
+                    }
+                    if (lane == 0) {
+                        st.sum = fs.lp[stay - 1];
+                        st.max = mx;
+                        a.stats[row_index] = st;
+                        a.floors[row_index] = fs.list[stay - 1];
+                    }
+                }
+            }
+            tm.sync();                                            // block 0's memory stays until every block has read it
+            return;
+        }
+    }
     double part = 0.0;
     unsigned long long kmin = ~0ull;
     for_each_in_slice(row, tm, [&](float v, int i) {
+        if (xof(v) > near) return;
         const unsigned long long ck = composite_key(v, i);
         if (ck < floor_key) return;
         const double w = raw_weight(v, i);
