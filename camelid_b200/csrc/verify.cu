@@ -268,13 +268,41 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
             if (writer) fs.n_list = 0u;
             tm.sync();
         }
-        for_each_in_slice<4>(row, tm, [&](float v, int i) {
-            if (xof(v) > near) return;
+        // Sixteen columns a thread are compared, and the few that are near enough looked at one by one.
+        auto consider = [&](int i) {
+            const float v = row[i];
             const unsigned long long ck = composite_key(v, i);
             if (ck < floor_key || (least > 0.0 && raw_weight(v, i) < least)) return;
             const unsigned int slot = atomicAdd(&fs0->n_list, 1u);
             if (slot < FS_CAP) fs0->list[slot] = ck;
-        });
+        };
+        const bool vec = (((uintptr_t)row) & 15) == 0;
+        const int whole = vec ? tm.end & ~3 : tm.end;             // up to here in whole groups of four
+        for (int g0 = tm.begin + (vec ? 4 : 1) * (int)threadIdx.x; g0 < whole; g0 += 16 * SAMPLE_THREADS) {
+            unsigned int some = 0u;
+            if (vec) {
+                float4 t[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) t[u] = *reinterpret_cast<const float4*>(row + min(g0 + u * 4 * SAMPLE_THREADS, whole - 4));
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    some |= (xof(t[u].x) <= near ? 1u : 0u) << (4 * u);
+                    some |= (xof(t[u].y) <= near ? 2u : 0u) << (4 * u);
+                    some |= (xof(t[u].z) <= near ? 4u : 0u) << (4 * u);
+                    some |= (xof(t[u].w) <= near ? 8u : 0u) << (4 * u);
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < 16; ++u) some |= (xof(row[min(g0 + u * SAMPLE_THREADS, whole - 1)]) <= near ? 1u : 0u) << u;
+            }
+            while (some) {
+                const int u = __ffs(some) - 1;
+                some &= some - 1u;
+                const int i = vec ? g0 + (u >> 2) * 4 * SAMPLE_THREADS + (u & 3) : g0 + u * SAMPLE_THREADS;
+                if (i < whole) consider(i);
+            }
+        }
+        if ((int)threadIdx.x < tm.end - whole && xof(row[whole + threadIdx.x]) <= near) consider(whole + threadIdx.x);
         tm.sync();
         const unsigned int n = fs0->n_list;
         if (n <= FS_CAP) {                                        // the same in every block
@@ -701,8 +729,8 @@ extern "C" int cml_verify_drafts(const float* logits, long long ld, int n_rows, 
     if (n_rows > 0) {
         cudaError_t e;
         if (filters) {
-            int share = team;                                      // a block takes a multiprocessor to itself
-            while (share > 1 && (long long)n_rows * share > cml_sm_count()) share /= 2;
+            // a block takes a multiprocessor to itself: as many share a row as all rows leave room for
+            const int share = max(1, min(team, cml_sm_count() / n_rows));
             a.floors = (unsigned long long*)((char*)scratch + 16ll * n_rows * verify_parts(vocab));
             e = cml_allow_smem<verify_floor_kernel>(sizeof(FastSharedOf<double>));
             if (e != cudaSuccess) return (int)e;
