@@ -1194,8 +1194,13 @@ static cudaError_t launch_all(const WeightArgs& a, unsigned pairs, int team, siz
     return launch_team(kernel, a, pairs, team, AM_WARPS * 32, smem, s);
 }
 
+#include "attention_weights_tc.cuh"
+
+// Rows of a kv head from which their weights alone are made on tcgen05 (up to 512), and the same as the plan of the scratch says.
+#define AW_TC_ROWS 64
+
 template <int HD>
-static cudaError_t launch_mma(const WeightArgs& a, cudaStream_t s) {
+static cudaError_t launch_mma(const WeightArgs& a, int* err, cudaStream_t s) {
     constexpr int TILE = HD == 128 ? 16 : 32;
     const unsigned pairs = (unsigned)a.n_seqs * (unsigned)a.kv_heads;
     const int rows = a.max_new * (a.heads / a.kv_heads);
@@ -1213,6 +1218,9 @@ static cudaError_t launch_mma(const WeightArgs& a, cudaStream_t s) {
         if (rows <= 16) return a.out ? launch_all<HD, 1, true>(a, pairs, team, 2 * ring, s) : launch_all<HD, 1, false>(a, pairs, team, ring, s);
         return a.out ? launch_all<HD, 2, true>(a, pairs, team, 2 * ring, s) : launch_all<HD, 2, false>(a, pairs, team, ring, s);
     }
+    if (a.out == nullptr && err != nullptr && rows >= AW_TC_ROWS && rows <= 512 && a.split_keys % WT_KEYS == 0 &&
+        (long long)a.n_pages * a.kv_heads * CML_PAGE <= 0x7fffffffLL)
+        return launch_tc<HD>(a, err, s);
     if (a.out) {
         e = cml_allow_smem<weights_part_mma_kernel<HD, 2, true, false>>(2 * ring);
         if (e == cudaSuccess)
@@ -1240,7 +1248,7 @@ extern "C" int cml_attn_paged_weights(const void* q, int dtype, long long q_stri
                                       const void* v, const float* scores, float* scores_out, const int* table, int width, int n_pages,
                                       const int* row0, const int* start, const int* fresh, const int* cached, int n_seqs, int n_rows, int heads,
                                       int kv_heads, int k_dim, int v_dim, int max_new, int max_len, float scale, int split_keys,
-                                      float* scratch, void* stream) {
+                                      float* scratch, int* err, void* stream) {
     if (dtype != CML_DTYPE_F32 && dtype != CML_DTYPE_BF16) return CML_ERR_BAD_DTYPE;
     if (n_seqs <= 0 || n_rows <= 0) return 0;
     if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || k_dim < 16 || k_dim > 256 || k_dim % 16 || v_dim < 16 || v_dim > 256 || v_dim % 16)
@@ -1267,7 +1275,7 @@ extern "C" int cml_attn_paged_weights(const void* q, int dtype, long long q_stri
     const bool mma = dtype == CML_DTYPE_BF16 && (k_dim == 64 || k_dim == 128) && (out == nullptr || v_dim == k_dim) &&
                      (((uintptr_t)q) & 15) == 0 && q_stride % 8 == 0;
     cudaStream_t s = (cudaStream_t)stream;
-    const cudaError_t e = mma ? (k_dim == 64 ? launch_mma<64>(a, s) : launch_mma<128>(a, s))
+    const cudaError_t e = mma ? (k_dim == 64 ? launch_mma<64>(a, err, s) : launch_mma<128>(a, err, s))
                               : (dtype == CML_DTYPE_F32 ? launch_plain<float>(a, s) : launch_plain<bf16>(a, s));
     if (e != cudaSuccess) return (int)e;
     return cml_launch_status();

@@ -1,0 +1,359 @@
+// The weights of a prompt's last rows on tcgen05: many rows (token, head) of q against all cached keys, without output.
+// Included by attention_weights.cu, whose arguments it takes.
+//
+// Both passes are one kernel. The rows of q stay in shared memory (up to 512 of them), the keys pass by in tiles of 128 that TMA
+// brings from the pages, and every (tile, 128 rows) is one product of 128 x 128 in tensor memory, of which two are in flight.
+//
+//   SUM false: S = Q K^T, a thread a row (and half of the tile's keys): its running maximum and sum over a stretch of keys
+//   SUM true:  S = K Q^T, a thread a key (and half of the rows): the sum of its weights 2^(s - max) / sum over the rows,
+//              kept in one register; the stretches' statistics are joined by every block for itself
+//
+// One exponential a row and key in each pass bounds the kernel (16 a cycle and multiprocessor): a product of 128 x 128 x 128 takes
+// half as long. Eight warps of exponentials, one that brings keys, one that issues products.
+#pragma once
+#include <cuda.h>
+
+#define WT_KEYS 128
+#define WT_WORKERS 256                 // threads that work on scores
+#define WT_THREADS (WT_WORKERS + 64)
+#define WT_WAIT_CYCLES 2000000000ll
+
+__device__ __forceinline__ void wt_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void wt_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void wt_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool wt_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Every wait has an end: past it the flag is set, and all roles run through to the block's last barrier without working.
+__device__ __forceinline__ bool wt_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+    if (wt_try(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (true) {
+        if (wt_try(bar, parity)) return true;
+        if (*gave_up) return false;
+        if (clock64() - t0 > WT_WAIT_CYCLES) {
+            *gave_up = 1;
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ void wt_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"((uint64_t)map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void wt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wt_fence_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void wt_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void wt_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+// 32 columns of this thread's lane, without waiting.
+__device__ __forceinline__ void wt_read32(uint32_t addr, float* r) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(r);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+          "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+          "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void wt_read_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Rows of 128 bytes, 128-byte swizzle, 1,024 bytes between groups of eight rows: as TMA writes the keys and the workers q.
+__device__ __forceinline__ uint64_t wt_desc(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void wt_workers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(WT_WORKERS) : "memory"); }
+
+template <int HD, int RT> struct WtPlan {
+    static constexpr int KB = HD / 64;                                        // 64-channel blocks of a row
+    static constexpr uint32_t TILE = 128u * 128u * KB;                        // 128 rows or keys
+    static constexpr int STAGES = RT * KB >= 8 ? 2 : 3;
+    static constexpr size_t SMEM = 1024 + (size_t)TILE * (RT + STAGES) + 256 + RT * 128 * 16 + 2 * 128 * 4;
+};
+
+// grid (stretches, pairs). RT: tiles of 128 rows.
+template <int HD, int RT, bool SUM>
+__global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_constant__ CUtensorMap map, WeightArgs a, int* err) {
+    using P = WtPlan<HD, RT>;
+    constexpr int KB = P::KB, STAGES = P::STAGES;
+    constexpr uint32_t TILE = P::TILE, BLOCK = 128u * 128u;
+    extern __shared__ uint8_t wt_raw[];
+    const uint32_t base = ((uint32_t)__cvta_generic_to_shared(wt_raw) + 1023u) & ~1023u;
+    uint8_t* const gbase = wt_raw + (base - (uint32_t)__cvta_generic_to_shared(wt_raw));
+    const uint32_t sQ = base, sK = sQ + RT * TILE, bars = sK + STAGES * TILE;
+    uint8_t* const tail = gbase + (bars - base);
+    uint32_t* const slot = reinterpret_cast<uint32_t*>(tail + 16 * 8);
+    volatile int* const gave_up = reinterpret_cast<volatile int*>(slot + 1);
+    float4* const rows_s = reinterpret_cast<float4*>(tail + 256);             // [RT * 128]: SUM (maximum, 1 / sum, last place, -); else results
+    float* const half_s = reinterpret_cast<float*>(rows_s + RT * 128);        // SUM: [2][128] the second half's sums
+    auto k_full = [&](int s) { return bars + 8u * s; };
+    auto k_empty = [&](int s) { return bars + 8u * (STAGES + s); };
+    auto s_full = [&](int b) { return bars + 8u * (2 * STAGES + b); };
+    auto s_empty = [&](int b) { return bars + 8u * (2 * STAGES + 2 + b); };
+    const uint32_t q_ready = bars + 8u * (2 * STAGES + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int split = blockIdx.x, seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
+    const Seq s = seq_of(a, seq);
+    const int first = split * a.split_keys, last = min(s.length, first + a.split_keys);
+    if (first >= last) return;                                                // the same for the whole block
+    const int group = a.heads / a.kv_heads, group_rows = a.max_new * group;
+    const int n_tiles = (last - first + WT_KEYS - 1) / WT_KEYS;
+    const int row_tiles = (s.rows + 127) / 128;                               // at most RT
+    const int* const pages = a.table + (size_t)seq * a.width;
+    auto page_at = [&](int key) {                                             // the page of a key of this stretch, -1: none
+        const int page = key < last ? pages[key / CML_PAGE] : -1;
+        return page < a.n_pages ? page : -1;
+    };
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) wt_init(k_full(i), 1), wt_init(k_empty(i), 1);
+        for (int i = 0; i < 2; ++i) wt_init(s_full(i), 1), wt_init(s_empty(i), WT_WORKERS);
+        wt_init(q_ready, WT_WORKERS);
+        *gave_up = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        wt_fence_smem();
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(slot)), "r"(256u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    wt_fence_before();
+    __syncthreads();
+    wt_fence_after();
+    const uint32_t tmem = *slot;
+
+    if (warp == 8) {
+        if (lane == 0) {
+            int issued = 0;
+            for (int t = 0; t < n_tiles; ++t) {
+                const int st = t % STAGES;
+                if (!wt_wait(k_empty(st), ((uint32_t)(t / STAGES) & 1u) ^ 1u, gave_up)) break;
+                wt_expect(k_full(st), TILE);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {                                 // a page that is none: any, its keys are masked
+                    const int y = (max(page_at(first + t * WT_KEYS + h * CML_PAGE), 0) * a.kv_heads + kvh) * CML_PAGE;
+#pragma unroll
+                    for (int b = 0; b < KB; ++b) wt_load(sK + st * TILE + b * BLOCK + h * (BLOCK / 2), &map, k_full(st), b * 64, y);
+                }
+                issued = t + 1;
+            }
+            if (*gave_up) {                                                   // copies in flight land before the block ends
+                for (int t = max(0, issued - STAGES); t < issued; ++t) {
+                    const long long t0 = clock64();
+                    while (!wt_try(k_full(t % STAGES), (uint32_t)(t / STAGES) & 1u) && clock64() - t0 < 20000000ll) {}
+                }
+            }
+        }
+    } else if (warp == 9) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+            bool ok = wt_wait(q_ready, 0, gave_up);
+            int it = 0;
+            for (int t = 0; t < n_tiles && ok; ++t) {
+                const int st = t % STAGES;
+                ok = wt_wait(k_full(st), (uint32_t)(t / STAGES) & 1u, gave_up);
+                for (int rt = 0; rt < row_tiles && ok; ++rt, ++it) {
+                    ok = wt_wait(s_empty(it & 1), ((uint32_t)(it >> 1) & 1u) ^ 1u, gave_up);
+                    if (!ok) break;
+                    wt_fence_after();
+#pragma unroll
+                    for (int b = 0; b < KB; ++b) {
+                        const uint64_t q = wt_desc(sQ + rt * TILE + b * BLOCK), k = wt_desc(sK + st * TILE + b * BLOCK);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            wt_mma(tmem + (it & 1) * 128, (SUM ? k : q) + (uint64_t)(c * 2), (SUM ? q : k) + (uint64_t)(c * 2), idesc, (b | c) ? 1u : 0u);
+                    }
+                    wt_commit(s_full(it & 1));
+                }
+                if (ok) wt_commit(k_empty(st));
+            }
+        }
+    } else {
+        // q into its tiles, zeros where there is no row
+        for (int c = threadIdx.x; c < row_tiles * 128 * KB * 8; c += WT_WORKERS) {
+            const int m = c / (KB * 8), cc = c % (KB * 8), b = cc / 8, r = m % 128;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (m < s.rows) v = *reinterpret_cast<const uint4*>((const bf16*)a.q + (long long)(s.row0 + m / group) * a.q_stride + (long long)(kvh * group + m % group) * HD + cc * 8);
+            *reinterpret_cast<uint4*>(gbase + (m / 128) * TILE + b * BLOCK + (r >> 3) * 1024 + (r & 7) * 128 + (((cc & 7) ^ (r & 7)) << 4)) = v;
+        }
+        if (SUM) {                                                            // the stretches of every row joined, in their order
+            const int splits = (s.length + a.split_keys - 1) / a.split_keys;
+            for (int m = threadIdx.x; m < RT * 128; m += WT_WORKERS) {
+                float top = -CUDART_INF_F, sum = 0.f;
+                if (m < s.rows) {
+                    const float* st = a.stats + ((size_t)blockIdx.y * a.n_splits * group_rows + m) * 2;
+                    for (int i = 0; i < splits; ++i) top = fmaxf(top, st[(size_t)i * group_rows * 2]);
+                    for (int i = 0; i < splits; ++i) {
+                        const float2 x = *reinterpret_cast<const float2*>(st + (size_t)i * group_rows * 2);
+                        if (x.x != -CUDART_INF_F) sum += exp2f(x.x - top) * x.y;
+                    }
+                }
+                const bool none = top == -CUDART_INF_F;
+                rows_s[m] = make_float4(none ? 0.f : top, none ? 0.f : 1.f / sum, __int_as_float(m < s.rows ? s.start + m / group : -1), 0.f);
+            }
+        }
+        wt_fence_smem();
+        wt_arrive(q_ready);
+        wt_workers_sync();                                                    // rows_s is whole
+        const int half = warp >> 2, mine = (warp & 3) * 32 + lane;            // this thread's lane of tensor memory
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        float top[RT], sum[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) top[r] = -CUDART_INF_F, sum[r] = 0.f;
+        bool ok = true;
+        int it = 0;
+        for (int t = 0; t < n_tiles; ++t) {
+            const int key0 = first + t * WT_KEYS;
+            const int page0 = page_at(key0), page1 = page_at(key0 + CML_PAGE);
+            // every row sees every key of the tile
+            const bool whole = page0 >= 0 && page1 >= 0 && key0 + WT_KEYS <= last && key0 + WT_KEYS - 1 <= s.start;
+            float gained = 0.f;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                if (rt >= row_tiles) break;
+                if (ok) ok = wt_wait(s_full(it & 1), (uint32_t)(it >> 1) & 1u, gave_up);
+                if (ok) {
+                    wt_fence_after();
+                    float x[64];
+                    wt_read32(tmem + (it & 1) * 128 + lanes + half * 64, x);
+                    wt_read32(tmem + (it & 1) * 128 + lanes + half * 64 + 32, x + 32);
+                    wt_read_wait();
+                    wt_fence_before();
+                    wt_arrive(s_empty(it & 1));
+                    if (!SUM) {                                               // this thread's row, the keys of one page
+                        if (!whole) {
+                            const int seen = (half ? page1 : page0) < 0 ? -1 : min(last - 1, s.start + (rt * 128 + mine) / group) - key0 - half * 64;
+#pragma unroll
+                            for (int c = 0; c < 64; ++c) x[c] = c <= seen ? x[c] : -CUDART_INF_F;
+                        }
+                        float most = x[0];
+#pragma unroll
+                        for (int c = 1; c < 64; ++c) most = fmaxf(most, x[c]);
+                        most *= a.scale;
+                        if (most > top[rt] + 6.f) {                           // the reference moves only when it is passed by 2^6
+                            sum[rt] *= fast_exp2(top[rt] - most);
+                            top[rt] = most;
+                        }
+                        const float ref = top[rt] == -CUDART_INF_F ? 0.f : top[rt];
+                        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int c = 0; c < 64; ++c) part[c & 3] += fast_exp2(fmaf(x[c], a.scale, -ref));
+                        sum[rt] += (part[0] + part[1]) + (part[2] + part[3]);
+                    } else {                                                  // this thread's key, half of the tile's rows
+                        const float4* const rows = rows_s + rt * 128 + half * 64;
+                        float part[4] = {0.f, 0.f, 0.f, 0.f};
+                        if (whole) {
+#pragma unroll
+                            for (int c = 0; c < 64; ++c) {
+                                const float2 r = *reinterpret_cast<const float2*>(rows + c);
+                                part[c & 3] = fmaf(fast_exp2(fmaf(x[c], a.scale, -r.x)), r.y, part[c & 3]);
+                            }
+                        } else {
+                            const int key = key0 + mine;
+#pragma unroll
+                            for (int c = 0; c < 64; ++c) {
+                                const float4 r = rows[c];
+                                if (key <= __float_as_int(r.z)) part[c & 3] = fmaf(fast_exp2(fmaf(x[c], a.scale, -r.x)), r.y, part[c & 3]);
+                            }
+                        }
+                        gained += (part[0] + part[1]) + (part[2] + part[3]);
+                    }
+                }
+                ++it;
+            }
+            if (SUM) {                                                        // the two halves of the rows, then the key's score
+                if (half) half_s[(t & 1) * 128 + mine] = gained;
+                wt_workers_sync();
+                const int key = key0 + mine, page = mine < CML_PAGE ? page0 : page1;
+                if (!half && ok && key < last && page >= 0) {
+                    const size_t at = ((size_t)page * a.kv_heads + kvh) * CML_PAGE + key % CML_PAGE;
+                    a.scores_out[at] = (key < s.old ? a.scores[at] : 0.f) + (gained + half_s[(t & 1) * 128 + mine]);
+                }
+            }
+        }
+        if (!SUM) {
+            if (half) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) rows_s[r * 128 + mine] = make_float4(top[r], sum[r], 0.f, 0.f);
+            }
+            wt_workers_sync();
+            if (!half) {
+                float* const out = a.stats + ((size_t)blockIdx.y * a.n_splits + split) * group_rows * 2;
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const int m = r * 128 + mine;
+                    if (m >= s.rows) break;
+                    const float4 o = rows_s[m];
+                    const float most = fmaxf(top[r], o.x);
+                    float l = 0.f;
+                    if (top[r] != -CUDART_INF_F) l += fast_exp2(top[r] - most) * sum[r];
+                    if (o.x != -CUDART_INF_F) l += fast_exp2(o.x - most) * o.y;
+                    *reinterpret_cast<float2*>(out + m * 2) = make_float2(most, l);
+                }
+            }
+        }
+    }
+    wt_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        wt_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
+    }
+    if (threadIdx.x == 0 && *gave_up) atomicExch(err, 4);
+}
+
+typedef CUresult (*WtEncode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static WtEncode wt_encode() {
+    static WtEncode fn = nullptr;
+    if (!fn) {
+        void* q = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &r) == cudaSuccess && r == cudaDriverEntryPointSuccess) fn = (WtEncode)q;
+    }
+    return fn;
+}
+
+template <int HD, int RT>
+static cudaError_t launch_tc_rows(const CUtensorMap& map, const WeightArgs& a, int* err, cudaStream_t s) {
+    constexpr size_t smem = WtPlan<HD, RT>::SMEM;
+    cudaError_t e = cml_allow_smem<weights_tc_kernel<HD, RT, false>>(smem);
+    if (e == cudaSuccess) e = cml_allow_smem<weights_tc_kernel<HD, RT, true>>(smem);
+    if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned)a.n_splits, (unsigned)a.n_seqs * (unsigned)a.kv_heads);
+    e = launch_pdl(weights_tc_kernel<HD, RT, false>, grid, dim3(WT_THREADS), smem, s, map, a, err);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(weights_tc_kernel<HD, RT, true>, grid, dim3(WT_THREADS), smem, s, map, a, err);
+}
+
+template <int HD>
+static cudaError_t launch_tc(const WeightArgs& a, int* err, cudaStream_t s) {
+    const WtEncode encode = wt_encode();
+    if (!encode) return cudaErrorNotSupported;
+    CUtensorMap map;                                                          // the pool as a matrix [pages * kv heads * 64, HD], boxes of a page and 64 channels
+    const cuuint64_t dims[2] = {(cuuint64_t)HD, (cuuint64_t)a.n_pages * a.kv_heads * CML_PAGE}, strides[1] = {(cuuint64_t)HD * 2};
+    const cuuint32_t box[2] = {64, CML_PAGE}, steps[2] = {1, 1};
+    if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(a.k), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return cudaErrorInvalidValue;
+    const int rows = a.max_new * (a.heads / a.kv_heads);
+    return rows <= 128 ? launch_tc_rows<HD, 1>(map, a, err, s) : rows <= 256 ? launch_tc_rows<HD, 2>(map, a, err, s) : launch_tc_rows<HD, 4>(map, a, err, s);
+}

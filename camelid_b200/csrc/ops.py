@@ -201,7 +201,7 @@ _SIGNATURES = {
                                            c_void_p, c_void_p, c_void_p],
     ("attention_weights", "cml_attn_paged_weights"): [c_void_p, c_int, c_long, c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_void_p,
                                                       c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
-                                                      c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p],
+                                                      c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p, c_void_p],
     ("eviction", "cml_evict_positions"): [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                           c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p],
     ("verify", "cml_verify_drafts"): [c_void_p, c_long, c_int, c_int, c_void_p, c_void_p, c_void_p, c_long, c_void_p, c_long, c_long, c_void_p,
@@ -2026,6 +2026,7 @@ def draws_at(positions: torch.Tensor, seed: torch.Tensor, draws: torch.Tensor):
 # ---------------------------------------------------------------------------------------
 # between two steps: which positions the cache keeps, which drafted tokens stay
 
+ATTN_WEIGHTS_TC_ROWS = 64, 512  # rows of a kv head whose weights alone are made on tcgen05; AW_TC_ROWS in attention_weights.cu
 ATTN_WEIGHTS_KEPT_ROWS = 32     # rows of a kv head up to which the products q . k are kept for the weights
 
 
@@ -2035,13 +2036,16 @@ def attn_weights_plan(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int,
     """(keys of a stretch, float32 numbers of scratch) of ``attn_paged_weights``: a sequence's keys are cut into stretches so that
     the blocks fill the device, none shorter than four pages. Made from sizes alone, without a device."""
     pairs, rows = n_seqs * n_kv_heads, max_new * (n_heads // n_kv_heads)
-    if dtype == torch.bfloat16 and head_dim in (64, 128) and value_dim == head_dim:       # rows a block works on together
-        together = (32 if rows > 16 else 16) if with_output or rows <= 16 else 256
+    fast = dtype == torch.bfloat16 and head_dim in (64, 128) and value_dim == head_dim
+    if fast and not with_output and ATTN_WEIGHTS_TC_ROWS[0] <= rows <= ATTN_WEIGHTS_TC_ROWS[1]:
+        # tcgen05: blocks with a multiprocessor (or half of one) to themselves, tiles of 128 keys
+        splits = max(1, min((2 * SMS + pairs - 1) // pairs, (max_len + 511) // 512))
+        split_keys = (((max_len + splits - 1) // splits + 127) // 128) * 128
     else:
-        together = 8
-    blocks = pairs * ((rows + together - 1) // together)
-    splits = max(1, min((4 * SMS + blocks - 1) // blocks, (max_len + 4 * PAGE - 1) // (4 * PAGE)))
-    split_keys = (((max_len + splits - 1) // splits + PAGE - 1) // PAGE) * PAGE
+        together = 8 if not fast else 32 if with_output else 256                          # rows a block works on together
+        blocks = pairs * ((rows + together - 1) // together)
+        splits = max(1, min((4 * SMS + blocks - 1) // blocks, (max_len + 4 * PAGE - 1) // (4 * PAGE)))
+        split_keys = (((max_len + splits - 1) // splits + PAGE - 1) // PAGE) * PAGE
     splits = (max_len + split_keys - 1) // split_keys
     parts = [pairs * rows * 2, pairs * rows * 2 * splits, pairs * rows * splits * value_dim if with_output else 0,
              pairs * rows * ((max_len + PAGE - 1) // PAGE * PAGE) if rows <= ATTN_WEIGHTS_KEPT_ROWS else 0]
@@ -2056,7 +2060,7 @@ def attn_weights_floats(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: in
 
 
 def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, seq_start, seq_new, n_heads: int, max_new: int,
-                       max_len: int, scale: float, scratch, scores_out=None, seq_cached=None):
+                       max_len: int, scale: float, scratch, scores_out=None, seq_cached=None, err=None):
     """Attention of a step's rows over the paged cache that keeps what it weighed. Sequence i owns the rows
     seq_row0[i] .. + seq_new[i] of ``q`` [rows, heads * head_dim]; its row j stands at place seq_start[i] + j and sees the
     places up to its own (keys and values of the new places are in the cache already). ``out`` [rows, heads * value_dim] gets the
@@ -2065,8 +2069,9 @@ def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, 
     zero, whatever their page held (``seq_cached``: int32 [sequences], places that count as cached where fewer than seq_start do,
     because the same step brought the others). The new scores go to ``scores_out`` (None: in place), where nothing but the sequences'
     places is written. ``max_new`` and ``max_len`` bound the sequences' new tokens and lengths (rows and places beyond them are
-    left out); ``scratch``: float32, ``attn_weights_floats`` numbers, free again when the call's work is done. No page
-    stands in two rows of the table."""
+    left out); ``scratch``: float32, ``attn_weights_floats`` numbers, free again when the call's work is done. ``err``
+    (int32 [1]; by default ``simt_error_word``) is set if one of the kernels' bounded waits runs out. No page stands in two rows of
+    the table."""
     scores_out = scores if scores_out is None else scores_out
     _here(q, out, k_pages, v_pages, scores, scores_out, block_table, seq_row0, seq_start, seq_new, scratch, seq_cached)
     n_pages, kv_heads, page, head_dim = shape = k_pages.shape
@@ -2094,13 +2099,15 @@ def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, 
     if not 0.0 < scale < float("inf"):
         raise KernelError(f"attn_paged_weights: the scale must be a positive number, got {scale}")
     split_keys, floats = attn_weights_plan(n_seqs, n_heads, kv_heads, head_dim, value_dim, dtype, max_new, max_len, out is not None)
+    if err is None and out is None:             # only the kernels without output wait on barriers
+        err = simt_error_word(q.device)
     if scratch.dtype != torch.float32 or scratch.numel() < floats or not scratch.is_contiguous():
         raise KernelError(f"attn_paged_weights: the scratch must be {floats} contiguous float32 numbers (attn_weights_floats)")
     _check(_fn("attention_weights", "cml_attn_paged_weights")(
         q.data_ptr(), dtype_code(dtype), q_stride, _p(out), out_stride, k_pages.data_ptr(), _p(v_pages), scores.data_ptr(),
         scores_out.data_ptr(), block_table.data_ptr(), width, n_pages, seq_row0.data_ptr(), seq_start.data_ptr(), seq_new.data_ptr(),
         _p(seq_cached), n_seqs, rows, n_heads, kv_heads, head_dim, value_dim, max_new, max_len, scale, split_keys, scratch.data_ptr(),
-        _stream()), "attn_paged_weights", 3)
+        _p(err), _stream()), "attn_paged_weights", 3)
 
 
 def evict_positions(k_pages, v_pages, scores, block_table, out_table, lengths, keeps, kept, first: int, recent: int, inv_freq=None,

@@ -152,7 +152,7 @@ class GroupedQueryAttention(Part):
         scratch = ctx.buffer("attn_weights", (ops.attn_weights_floats(ctx.n_seqs, self.num_heads, self.num_kv_heads, self.head_dim, q.dtype,
                                                                       max_new, max_len, out is not None),), torch.float32)
         ops.attn_paged_weights(q, out, k_pages, v_pages if out is not None else None, scores, table, row0, start, new, self.num_heads, max_new,
-                               max_len, self.scale, scratch, seq_cached=ctx.seq_start)
+                               max_len, self.scale, scratch, seq_cached=ctx.seq_start, err=linear._err_word(q.device))
 
     def _decode_splits(self, ctx, n_tiles: int, chunks: int, tensor_cores: bool) -> int:
         """Blocks that share the keys of one (row, kv head) in a decode step: enough for all SMs

@@ -38,7 +38,7 @@ def test_kernel_entries_refuse_sizes_before_they_launch():
     """The C entries return the error of a size or type without touching a device."""
     att = ops._fn("attention_weights", "cml_attn_paged_weights")
     good = dict(q=4096, dtype=0, qs=64, out=4096, os=64, k=4096, v=4096, s=4096, so=4096, table=4096, width=1, pages=1, row0=4096, start=4096,
-                new=4096, cached=None, n=1, rows=1, heads=1, kv=1, kd=64, vd=64, max_new=1, max_len=1, scale=1.0, split=64, scratch=4096, stream=None)
+                new=4096, cached=None, n=1, rows=1, heads=1, kv=1, kd=64, vd=64, max_new=1, max_len=1, scale=1.0, split=64, scratch=4096, err=None, stream=None)
     for change, code in (({"dtype": 7}, -2), ({"kd": 24}, -3), ({"kd": 272}, -3), ({"vd": 8}, -3), ({"heads": 3, "kv": 2}, -3), ({"kv": 0}, -3),
                          ({"max_new": 0}, -3), ({"max_len": 0}, -3), ({"split": 0}, -3), ({"split": 63}, -3), ({"scale": 0.0}, -3),
                          ({"scale": float("nan")}, -3), ({"scale": float("inf")}, -3), ({"width": 0}, -3), ({"pages": 0}, -3),
