@@ -76,7 +76,6 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(EvictArgs a, int 
     __shared__ int s_above[WARPS], s_ties[WARPS];
     __shared__ unsigned int s_sum[32];
     pdl_wait();
-    pdl_launch_dependents();
     const Unit x = unit_of(a, blockIdx.x);
     int* kept = a.kept + (size_t)blockIdx.x * a.cap;
     if (x.keep == x.length) {                                     // everything stays
@@ -279,7 +278,6 @@ __global__ void __launch_bounds__(EV_MOVE_THREADS) evict_move_kernel(EvictArgs a
     extern __shared__ __align__(16) unsigned char raw[];
     uint2* turns = reinterpret_cast<uint2*>(raw);                 // [element of a chunk][columns], or by pair where pairs are neighbours
     pdl_wait();
-    pdl_launch_dependents();
     const int team = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank();
     const int u = blockIdx.x / team;
     const Unit x = unit_of(a, u);
