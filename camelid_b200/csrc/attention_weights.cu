@@ -144,7 +144,6 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
     __shared__ float2 join_s[ALL ? R : 1];                        // ALL: [rows] maximum and 1 / sum of all keys
     const int split = blockIdx.x, seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads, m0 = blockIdx.z * R;
     pdl_wait();
-    pdl_launch_dependents();
     const Seq s = seq_of(a, seq);
     if (m0 >= s.rows) return;                                     // the same for a whole cluster
     const int team = ALL ? (int)gridDim.x : 1;
@@ -254,6 +253,7 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
     }
     cp_async_wait<0>();
     __syncthreads();
+    pdl_launch_dependents();
     if (a.out && d < a.v_dim && (!halves || kk_first > 0)) {
 #pragma unroll
         for (int m = 0; m < R; ++m) own[m * a.v_dim + d] = o[m];
@@ -443,7 +443,6 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
     constexpr int TEAM = MT == 1 ? 16 : 8;                                    // blocks of a cluster at most
     extern __shared__ __align__(16) unsigned char raw[];
     pdl_wait();
-    pdl_launch_dependents();
     const int split = blockIdx.x, seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads, m0 = blockIdx.z * 16 * MT;
     const Seq s = seq_of(a, seq);
     if (m0 >= s.rows) return;                                                 // the same for a whole cluster
@@ -695,6 +694,8 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
             sum[mt][h] += __shfl_xor_sync(0xffffffffu, sum[mt][h], 2);
         }
     __syncthreads();                                                          // every warp is done with its ring
+    // The next kernel may begin beside what is left: earlier it only took room (16 long sequences 348 us for 345).
+    pdl_launch_dependents();
     // the warps' ranges: [warp][16 * MT rows][maximum, sum, output]
     constexpr int RW = OUT ? HD + 4 : 4;
     float* red = reinterpret_cast<float*>(raw);

@@ -455,7 +455,6 @@ __global__ void __launch_bounds__(VF_THREADS, PER_SM) verify_decide_kernel(Verif
     fill_table(table);
     if (threadIdx.x == 0) first_bad = 0x7fffffff, row_bad = 0, err_bits = 0;
     pdl_wait();
-    pdl_launch_dependents();
     const int team = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank();
     const int seq = blockIdx.x / team;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
