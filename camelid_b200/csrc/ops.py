@@ -2035,7 +2035,7 @@ def attn_weights_plan(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int,
                       max_len: int, with_output: bool) -> tuple:
     """(keys of a stretch, float32 numbers of scratch) of ``attn_paged_weights``: a sequence's keys are cut into stretches so that
     the blocks fill the device, none shorter than four pages. Made from sizes alone, without a device."""
-    pairs, rows = n_seqs * n_kv_heads, max_new * (n_heads // n_kv_heads)
+    pairs, rows = max(1, n_seqs) * n_kv_heads, max_new * (n_heads // n_kv_heads)
     fast = dtype == torch.bfloat16 and head_dim in (64, 128) and value_dim == head_dim
     if fast and not with_output and ATTN_WEIGHTS_TC_ROWS[0] <= rows <= ATTN_WEIGHTS_TC_ROWS[1]:
         # tcgen05: a block for every multiprocessor (a second round of blocks costs as much as the first: one sequence of 32,001
@@ -2101,6 +2101,8 @@ def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, 
         raise KernelError(f"attn_paged_weights: the scale must be a positive number, got {scale}")
     split_keys, floats = attn_weights_plan(n_seqs, n_heads, kv_heads, head_dim, value_dim, dtype, max_new, max_len, out is not None)
     if err is None and out is None:             # only the kernels without output wait on barriers
+        if q.device not in _simt_err and torch.cuda.is_current_stream_capturing():
+            raise KernelError("attn_paged_weights: the default error word is made by a first call outside of a graph's capture (or pass err)")
         err = simt_error_word(q.device)
     if scratch.dtype != torch.float32 or scratch.numel() < floats or not scratch.is_contiguous():
         raise KernelError(f"attn_paged_weights: the scratch must be {floats} contiguous float32 numbers (attn_weights_floats)")
@@ -2115,7 +2117,7 @@ def evict_positions(k_pages, v_pages, scores, block_table, out_table, lengths, k
                     interleaved: bool = False):
     """Keep min(keeps[i], lengths[i]) places of every sequence i, chosen for each cache entry and kv head: its ``first`` places, its
     ``recent`` last ones (cut to what is kept in all) and those of the largest ``scores``, the lower place among equals (a
-    score that is not a number counts as the lowest). They move, in order, to the places 0.. of the pages in
+    score that is not a number counts as the lowest). No page stands in two rows of the table. They move, in order, to the places 0.. of the pages in
     ``out_table``, which is ``block_table`` itself (the cache closes its gaps in place) or names pages that ``block_table``
     does not. Keys, values and scores: [pages, kv heads, 64(, size)] or, for several entries with one table, [entries, pages, ...];
     ``v_pages`` None: values live in the key rows. ``kept`` int32 [(entries,) sequences, kv heads, room] gets the old places in order

@@ -206,13 +206,22 @@ def run_drafted_batch(model, cache, sampler, drafter, prompts: list, budgets: li
                         raise StepError(f"slot {slots[i]}: the drafted token {t} is outside the vocabulary of {sampler.vocab_size}")
                 drafts.append(d)
                 probs.append(p)
-            entries = [StepEntry(slots[i], fed[i] + d, list(range(len(fed[i]) - 1, len(fed[i]) + len(d)))) for i, d in zip(live, drafts)]
+            # Every sequence brings as many rows as the one with the most drafts, where its budget lets it: steps of few layouts come
+            # back and are captured. What stands behind a sequence's drafts is not looked at and leaves the cache with the rest.
+            most = max(len(d) for d in drafts)
+            entries, row0, at = [], [], 0
+            for i, d in zip(live, drafts):
+                rows = max(len(d), min(most, budgets[i] - len(results[i].tokens) - 1))
+                tokens = fed[i] + d + [fed[i][-1]] * (rows - len(d))
+                entries.append(StepEntry(slots[i], tokens, list(range(len(fed[i]) - 1, len(tokens)))))
+                row0.append(at)
+                at += rows + 1
             logits = model.step(cache, entries)
-            counts, nexts = sampler.verify(logits, drafts, [histories[i] for i in live], probs)
+            counts, nexts = sampler.verify(logits, drafts, [histories[i] for i in live], probs, row0)
             if on_step is not None:
                 on_step(len(live))
             still = []
-            for i, d, count, token in zip(live, drafts, counts, nexts):
+            for i, d, count, token, entry in zip(live, drafts, counts, nexts, entries):
                 new = d[:count] + [int(token)]
                 for at, t in enumerate(new):
                     if t in stop_ids:
@@ -228,8 +237,9 @@ def run_drafted_batch(model, cache, sampler, drafter, prompts: list, budgets: li
                     cache.free_slot(slots[i])
                     slots[i] = None
                 else:
-                    if count < len(d):
-                        cache.truncate(slots[i], cache.length(slots[i]) - (len(d) - count))
+                    stale = len(entry.tokens) - len(fed[i]) - count
+                    if stale:
+                        cache.truncate(slots[i], cache.length(slots[i]) - stale)
                     fed[i] = [int(token)]
                     still.append(i)
             live = still

@@ -81,31 +81,35 @@ class Sampler:
                             o.min_p or 0.0, draws, out, self._err)
         return out
 
-    def verify(self, logits: torch.Tensor, drafts: list, histories: list, draft_probs: list | None = None) -> tuple:
+    def verify(self, logits: torch.Tensor, drafts: list, histories: list, draft_probs: list | None = None, row0: list | None = None) -> tuple:
         """Which drafted tokens stay, and the token behind them. ``logits``: float32 on the device, for every sequence a row for each
-        of its ``drafts`` (a list of tokens) and one more, packed (adjusted in place when penalties or biases are set);
-        ``histories``: per sequence the tokens before its drafts; ``draft_probs``: per sequence the drafter's probabilities
+        of its ``drafts`` (a list of tokens) and one more, packed or from the rows ``row0`` on (adjusted in place when penalties or
+        biases are set); ``histories``: per sequence the tokens before its drafts; ``draft_probs``: per sequence the drafter's probabilities
         (float32 [drafts, vocabulary] on the device), or None where it was certain of its tokens. Returns (accepted drafts,
         next tokens), two lists. The draws come from the sampler's seed and the history's length: the next token's
         from the stream of ``sample``, the acceptances' from one of their own."""
         o = self.options
         n, room = len(drafts), max([len(d) for d in drafts] + [1])
-        rows = sum(len(d) + 1 for d in drafts)
-        if logits.shape[0] != rows or len(histories) != n:
-            raise SamplingError(f"{n} sequences with {rows - n} drafts need {rows} rows of logits and {n} histories, got "
-                                f"{logits.shape[0]} and {len(histories)}")
+        if row0 is None:
+            row0, at = [], 0
+            for d in drafts:
+                row0.append(at)
+                at += len(d) + 1
+        rows = logits.shape[0]
+        if len(histories) != n or len(row0) != n or any(not 0 <= r <= rows - len(d) - 1 for r, d in zip(row0, drafts)):
+            raise SamplingError(f"{n} sequences with {sum(len(d) for d in drafts)} drafts do not fit {rows} rows of logits and "
+                                f"{len(histories)} histories")
         if o.adjusts:
-            entries, biases = self._adjust_entries([list(h) + list(d[:j]) for h, d in zip(histories, drafts) for j in range(len(d) + 1)])
+            # a row's history ends with the drafts before it; rows that no sequence names are left alone
+            named = {r + j: list(h) + list(d[:j]) for r, h, d in zip(row0, histories, drafts) for j in range(len(d) + 1)}
+            entries, biases = self._adjust_entries(list(named.values()))
             if entries:
-                e = torch.tensor(entries, dtype=torch.int32).to(self.device, non_blocking=True)
+                at = list(named)
+                e = torch.tensor([(at[r], t, c) for r, t, c in entries], dtype=torch.int32).to(self.device, non_blocking=True)
                 b = torch.tensor(biases, dtype=torch.float32).to(self.device, non_blocking=True)
                 ops.adjust_logits(logits, e, b, o.repeat_penalty, o.presence_penalty, o.frequency_penalty)
         seed = o.seed or 0
         own = splitmix64(seed ^ 0x5851F42D4C957F2D)                  # the acceptances' stream
-        row0, at = [], 0
-        for d in drafts:
-            row0.append(at)
-            at += len(d) + 1
         ints = torch.tensor([row0, [len(d) for d in drafts]], dtype=torch.int32).to(self.device, non_blocking=True)
         tokens = torch.tensor([list(d) + [0] * (room - len(d)) for d in drafts], dtype=torch.int32).to(self.device, non_blocking=True)
         accept = torch.tensor([[unit_draw(own, len(h) + j) for j in range(room)] for h in histories], dtype=torch.float32)

@@ -177,6 +177,55 @@ def test_weights_with_missing_pages(cuda):
         assert bool(((s_dev.cpu().double() - ref_scores).abs() <= tol_scores + 1e-30).all())
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_window_at_the_limits_of_its_kernels(cuda, dim):
+    """Rows just below, at and beyond what the tensor-memory kernels take, and stretches that end inside a tile."""
+    for heads, new in ((16, 4), (16, 3), (21, 3), (16, 32), (16, 33), (9, 30), (16, 8), (16, 16)):
+        _attention(cuda, [200, 5], [new, min(new, 2)], heads, 1, dim, torch.bfloat16, with_out=False, seed=heads + new)
+    _attention(cuda, [2100, 1279, 0], [20, 1, 20], 8, 2, dim, torch.bfloat16, with_out=False, seed=8, in_place=False, spoil=float("nan"))
+    _attention(cuda, [300, 40], [16, 9], 8, 2, dim, torch.bfloat16, with_out=False, loose=True, q_pad=8)
+
+
+def test_window_with_missing_pages(cuda):
+    from camelid_b200.csrc import ops
+    for dim in (64, 128):
+        gen = torch.Generator().manual_seed(6)
+        k = torch.randn(5, 1, PAGE, dim, generator=gen).to(torch.bfloat16)
+        q = torch.randn(40, 4 * dim, generator=gen).to(torch.bfloat16)
+        table = [[-1, 1, 3, 99, 0], [2, -1, -1, -1, -1]]
+        start, new, row0 = [260, 100], [20, 20], [0, 20]
+        scores = torch.rand(5, 1, PAGE, generator=gen)
+        ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)    # noqa: E731
+        scratch = torch.empty(ops.attn_weights_floats(2, 4, 1, dim, torch.bfloat16, 20, 280, False), device=cuda)
+        s_dev = scores.to(cuda)
+        ops.attn_paged_weights(q.to(cuda), None, k.to(cuda), None, s_dev, ints(table), ints(row0), ints(start), ints(new), 4, 20, 280, dim ** -0.5,
+                               scratch)
+        _, ref, _, tol = pb.weights(q, k, None, scores, table, row0, start, new, 4, dim ** -0.5)
+        assert bool(((s_dev.cpu().double() - ref).abs() <= tol + 1e-30).all())
+
+
+@pytest.mark.parametrize("dtype,dim,new", [(torch.bfloat16, 64, 1), (torch.bfloat16, 128, 6), (torch.bfloat16, 64, 40), (torch.float32, 48, 1),
+                                           (torch.float32, 64, 9)])
+def test_places_that_the_same_step_brought_start_from_zero(cuda, dtype, dim, new):
+    """``seq_cached``: the places between it and the rows' own were written by this step, whatever score their page held."""
+    from camelid_b200.csrc import ops
+    gen = torch.Generator().manual_seed(new)
+    with_out = new < 30
+    k, v = (torch.randn(4, 2, PAGE, dim, generator=gen).to(dtype) for _ in range(2))
+    q = torch.randn(2 * new, 8 * dim, generator=gen).to(dtype)
+    scores = torch.rand(4, 2, PAGE, generator=gen)
+    table, start, cached = [[0, 2], [3, 1]], [80, 70], [30, 70]
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)        # noqa: E731
+    scratch = torch.empty(ops.attn_weights_floats(2, 8, 2, dim, dtype, new, 120, with_out), device=cuda)
+    s_dev, out = scores.to(cuda), torch.empty(2 * new, 8 * dim, dtype=dtype, device=cuda)
+    ops.attn_paged_weights(q.to(cuda), out if with_out else None, k.to(cuda), v.to(cuda) if with_out else None, s_dev, ints(table), ints([0, new]),
+                           ints(start), ints([new, new]), 8, new, 120, dim ** -0.5, scratch, seq_cached=ints(cached))
+    for p in range(30, 80):
+        scores[table[0][p // PAGE], :, p % PAGE] = 0
+    _, ref, _, tol = pb.weights(q, k, v if with_out else None, scores, table, [0, new], start, [new, new], 8, dim ** -0.5)
+    assert bool(((s_dev.cpu().double() - ref).abs() <= tol + 1e-30).all())
+
+
 def test_weights_of_large_scores(cuda):
     """Scores of hundreds: nothing overflows, one place takes everything."""
     for dtype, dim in ((torch.bfloat16, 64), (torch.float32, 64), (torch.bfloat16, 128)):
@@ -354,6 +403,14 @@ def test_verify_with_the_samplers_filters(cuda, vocab, filters):
         assert _verify(cuda, vocab, [3, 0, 5], 0.8, with_probs, seed=vocab, **filters)[2] == 0
 
 
+def test_verify_without_room_for_drafts(cuda):
+    """No drafts at all: the next token of every sequence."""
+    for vocab in (500, 40000):
+        for filters in ({}, {"top_p": 0.8}):
+            _verify(cuda, vocab, [0, 0, 0], 0.9, False, room=0, **filters)
+            _verify(cuda, vocab, [0, 0, 0], 0.0, True, room=0)
+
+
 def test_verify_strided_rows(cuda):
     for pad in (1, 3, 4):
         _verify(cuda, 1000, [3, 2], 0.9, True, pad=pad, room=6)
@@ -434,3 +491,80 @@ def test_verify_keeps_the_targets_distribution(cuda):
     share = torch.bincount(tokens[:, 0].cpu().long(), minlength=vocab).double() / n
     p = torch.softmax(p_logits.double(), 0)
     assert bool(((share - p).abs() <= 5 * torch.sqrt(p * (1 - p) / n)).all())       # five standard deviations
+
+
+# ---- captured, replayed, on other streams -------------------------------------------------------------------------------
+def _calls(cuda):
+    """(names, what each call changes, the calls) on buffers of their own, of all kernels of the three operators."""
+    from camelid_b200.csrc import ops
+    gen = torch.Generator().manual_seed(1)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)        # noqa: E731
+    calls = []
+    for dtype, dim, new, with_out in ((torch.bfloat16, 64, 1, True), (torch.bfloat16, 128, 6, True), (torch.bfloat16, 128, 20, True),
+                                      (torch.bfloat16, 64, 6, False), (torch.bfloat16, 64, 40, False), (torch.float32, 32, 1, True),
+                                      (torch.float32, 32, 5, True)):
+        k, v = (torch.randn(9, 2, PAGE, dim, generator=gen).to(dtype).to(cuda) for _ in range(2))
+        q = torch.randn(2 * new, 8 * dim, generator=gen).to(dtype).to(cuda)
+        old, s, out = torch.rand(9, 2, PAGE, generator=gen).to(cuda), torch.zeros(9, 2, PAGE, device=cuda), torch.zeros_like(q)
+        scratch = torch.empty(ops.attn_weights_floats(2, 8, 2, dim, dtype, new, 300, with_out), device=cuda)
+        args = (q, out if with_out else None, k, v if with_out else None, old, ints([[0, 1, 2, 3, 4], [5, 6, 7, 8, -1]]), ints([0, new]),
+                ints([250, 200]), ints([new, new]), 8, new, 300, 0.1, scratch)
+        calls.append(([s, out], lambda args=args, s=s: ops.attn_paged_weights(*args, scores_out=s)))
+    for dtype in (torch.bfloat16, torch.float32):
+        k, v = (torch.randn(2, 12, 2, PAGE, 32, generator=gen).to(dtype).to(cuda) for _ in range(2))
+        s = torch.rand(2, 12, 2, PAGE, generator=gen).to(cuda)
+        kept = torch.zeros(2, 2, 2, 100, dtype=torch.int32, device=cuda)
+        args = (k, v, s, ints([[0, 1, 2, 3], [4, 5, 6, -1]]), ints([[7, 8], [9, 10]]), ints([250, 180]), ints([100, 70]), kept, 2, 10)
+        freq = torch.full((16,), 0.3, device=cuda)
+        calls.append(([k, v, s, kept], lambda args=args, freq=freq: ops.evict_positions(*args, inv_freq=freq)))
+    for filters in ((0, 1.0, 0.0), (20, 0.9, 0.0), (0, 0.8, 0.01), (0, 0.7, 0.0)):
+        logits = (3 * torch.randn(7, 9000, generator=gen)).to(cuda)
+        counts, tokens, err = ints([0, 0]), torch.zeros(2, 4, dtype=torch.int32, device=cuda), ints([0])
+        scratch = torch.empty(ops.verify_bytes(7, 2, 9000), dtype=torch.uint8, device=cuda)
+        args = (logits, ints([0, 4]), ints([3, 2]), logits.argmax(-1).int()[torch.tensor([[0, 1, 2], [4, 5, 6]], device=cuda)], None,
+                torch.rand(2, 3, generator=gen).to(cuda), torch.rand(2, generator=gen).to(cuda), 0.8, *filters, counts, tokens, err, scratch)
+        calls.append(([counts, tokens, err], lambda args=args: ops.verify_drafts(*args)))
+    return calls
+
+
+def test_captured_and_replayed_and_on_another_stream(cuda):
+    want = []
+    for changed, call in _calls(cuda):
+        call()
+        want.append([t.clone() for t in changed])
+    for i, (changed, call) in enumerate(_calls(cuda)):      # buffers of their own: made anew from the same numbers
+        torch.cuda.synchronize()
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            call()
+        stream.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(changed, want[i])), i
+    for i, (changed, call) in enumerate(_calls(cuda)):
+        start = [t.clone() for t in changed]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call()                                          # kernels are loaded and their limits set before a capture
+        torch.cuda.current_stream().wait_stream(side)
+        for t, s in zip(changed, start):
+            t.copy_(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
+        for _ in range(3):
+            for t, s in zip(changed, start):
+                t.copy_(s)
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(changed, want[i])), i
+
+
+def test_the_same_call_twice_gives_the_same_bits(cuda):
+    calls = _calls(cuda)
+    for i, (changed, call) in enumerate(calls):
+        call()
+        first = [t.clone() for t in changed]
+        for _ in range(5):
+            call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(changed, first)), i
