@@ -1219,7 +1219,7 @@ static cudaError_t launch_mma(const WeightArgs& a, int* err, cudaStream_t s) {
         if (rows <= 16) return a.out ? launch_all<HD, 1, true>(a, pairs, team, 2 * ring, s) : launch_all<HD, 1, false>(a, pairs, team, ring, s);
         return a.out ? launch_all<HD, 2, true>(a, pairs, team, 2 * ring, s) : launch_all<HD, 2, false>(a, pairs, team, ring, s);
     }
-    if (a.out == nullptr && err != nullptr && rows >= AW_TC_ROWS && rows <= 512 && a.split_keys % WT_KEYS == 0 &&
+    if (a.out == nullptr && err != nullptr && rows >= AW_TC_ROWS && rows <= 512 &&
         (long long)a.n_pages * a.kv_heads * CML_PAGE <= 0x7fffffffLL)
         return launch_tc<HD>(a, err, s);
     if (a.out) {

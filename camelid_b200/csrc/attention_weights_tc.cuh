@@ -88,7 +88,54 @@ template <int HD, int RT> struct WtPlan {
     static constexpr size_t SMEM = 1024 + (size_t)TILE * (RT + STAGES) + 256 + RT * 128 * 16 + 2 * 128 * 4;
 };
 
-// grid (stretches, pairs). RT: tiles of 128 rows.
+// Which stretch a block has. All sequences' key tiles are cut into stretches of the same number of tiles, the smallest for which they
+// are no more than the blocks of a kv head (and none has more than the statistics have room for): sequences of unequal
+// lengths keep all multiprocessors busy to the end (four prompts of 9,001 to 16,384: 142 us with stretches of one length
+// made for the longest, 119 with these).
+struct WtShare {
+    int seq, split, tiles, splits;             // tiles: of a stretch; splits: stretches of the sequence
+};
+__device__ __forceinline__ WtShare wt_share(const WeightArgs& a, int block, int blocks) {        // by a whole warp, the same in every lane
+    const int lane = threadIdx.x & 31;
+    auto look_up = [&](int i) { return i < a.n_seqs ? (seq_of(a, i).length + WT_KEYS - 1) / WT_KEYS : 0; };
+    const int own = look_up(lane);             // the first 32 sequences are looked up once
+    auto tiles_of = [&](int i) { return i < 32 ? own : look_up(i); };
+    int total = 0;
+    for (int i = lane; i < a.n_seqs; i += 32) total += tiles_of(i);
+    total = __reduce_add_sync(0xffffffffu, total);
+    int tiles = max(1, (total + blocks - 1) / blocks);
+    while (true) {                             // ends: stretches as long as the longest sequence make one of each
+        int n = 0, most = 0;
+        for (int i = lane; i < a.n_seqs; i += 32) {
+            const int k = (tiles_of(i) + tiles - 1) / tiles;
+            n += k, most = max(most, k);
+        }
+        if (__reduce_add_sync(0xffffffffu, n) <= blocks && __reduce_max_sync(0xffffffffu, most) <= a.n_splits) break;
+        ++tiles;
+    }
+    WtShare w = {-1, 0, tiles, 0};
+    int before = 0;
+    for (int i0 = 0; i0 < a.n_seqs && w.seq < 0; i0 += 32) {
+        const int k = (tiles_of(i0 + lane) + tiles - 1) / tiles;
+        int incl = k;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += t;
+        }
+        const unsigned int mine = __ballot_sync(0xffffffffu, block >= before + incl - k && block < before + incl);
+        if (mine) {
+            const int who = __ffs(mine) - 1;
+            w.seq = i0 + who;
+            w.split = block - before - __shfl_sync(0xffffffffu, incl - k, who);
+            w.splits = __shfl_sync(0xffffffffu, k, who);
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return w;
+}
+
+// grid (blocks of a kv head, kv heads). RT: tiles of 128 rows.
 template <int HD, int RT, bool SUM>
 __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_constant__ CUtensorMap map, WeightArgs a, int* err) {
     using P = WtPlan<HD, RT>;
@@ -111,10 +158,11 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     pdl_launch_dependents();
-    const int split = blockIdx.x, seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
+    const WtShare share = wt_share(a, blockIdx.x, gridDim.x);                 // every warp for itself
+    if (share.seq < 0) return;                                                // more blocks than stretches: the same for the whole block
+    const int split = share.split, seq = share.seq, kvh = blockIdx.y, pair = seq * a.kv_heads + kvh;
     const Seq s = seq_of(a, seq);
-    const int first = split * a.split_keys, last = min(s.length, first + a.split_keys);
-    if (first >= last) return;                                                // the same for the whole block
+    const int first = split * share.tiles * WT_KEYS, last = min(s.length, first + share.tiles * WT_KEYS);
     const int group = a.heads / a.kv_heads, group_rows = a.max_new * group;
     const int n_tiles = (last - first + WT_KEYS - 1) / WT_KEYS;
     const int row_tiles = (s.rows + 127) / 128;                               // at most RT
@@ -195,11 +243,11 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
             *reinterpret_cast<uint4*>(gbase + (m / 128) * TILE + b * BLOCK + (r >> 3) * 1024 + (r & 7) * 128 + (((cc & 7) ^ (r & 7)) << 4)) = v;
         }
         if (SUM) {                                                            // the stretches of every row joined, in their order
-            const int splits = (s.length + a.split_keys - 1) / a.split_keys;
+            const int splits = share.splits;
             for (int m = threadIdx.x; m < RT * 128; m += WT_WORKERS) {
                 float top = -CUDART_INF_F, sum = 0.f;
                 if (m < s.rows) {
-                    const float* st = a.stats + ((size_t)blockIdx.y * a.n_splits * group_rows + m) * 2;
+                    const float* st = a.stats + ((size_t)pair * a.n_splits * group_rows + m) * 2;
                     for (int i = 0; i < splits; ++i) top = fmaxf(top, st[(size_t)i * group_rows * 2]);
                     for (int i = 0; i < splits; ++i) {
                         const float2 x = *reinterpret_cast<const float2*>(st + (size_t)i * group_rows * 2);
@@ -296,7 +344,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
             }
             wt_workers_sync();
             if (!half) {
-                float* const out = a.stats + ((size_t)blockIdx.y * a.n_splits + split) * group_rows * 2;
+                float* const out = a.stats + ((size_t)pair * a.n_splits + split) * group_rows * 2;
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
                     const int m = r * 128 + mine;
@@ -338,7 +386,8 @@ static cudaError_t launch_tc_rows(const CUtensorMap& map, const WeightArgs& a, i
     cudaError_t e = cml_allow_smem<weights_tc_kernel<HD, RT, false>>(smem);
     if (e == cudaSuccess) e = cml_allow_smem<weights_tc_kernel<HD, RT, true>>(smem);
     if (e != cudaSuccess) return e;
-    const dim3 grid((unsigned)a.n_splits, (unsigned)a.n_seqs * (unsigned)a.kv_heads);
+    // one block for every multiprocessor in all, one for every sequence at least; n_splits of a sequence at most, so that the others have one
+    const dim3 grid((unsigned)(a.n_splits + a.n_seqs - 1), (unsigned)a.kv_heads);
     e = launch_pdl(weights_tc_kernel<HD, RT, false>, grid, dim3(WT_THREADS), smem, s, map, a, err);
     if (e != cudaSuccess) return e;
     return launch_pdl(weights_tc_kernel<HD, RT, true>, grid, dim3(WT_THREADS), smem, s, map, a, err);

@@ -2038,10 +2038,10 @@ def attn_weights_plan(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int,
     pairs, rows = max(1, n_seqs) * n_kv_heads, max_new * (n_heads // n_kv_heads)
     fast = dtype == torch.bfloat16 and head_dim in (64, 128) and value_dim == head_dim
     if fast and not with_output and ATTN_WEIGHTS_TC_ROWS[0] <= rows <= ATTN_WEIGHTS_TC_ROWS[1]:
-        # tcgen05: a block for every multiprocessor (a second round of blocks costs as much as the first: one sequence of 32,001
-        # keys and 8 kv heads 49.6 us with 16 stretches, 64 with 32), none with less than 256 keys
-        splits = max(1, min(SMS // pairs, (max_len + 255) // 256))
-        split_keys = (((max_len + splits - 1) // splits + 127) // 128) * 128
+        # tcgen05: the kernel cuts all sequences into stretches of one length itself, for a block of every multiprocessor; a
+        # sequence has as many as the others leave it
+        splits = max(1, min(SMS // n_kv_heads - max(1, n_seqs) + 1, (max_len + 127) // 128))
+        split_keys = ((max_len + splits - 1) // splits + PAGE - 1) // PAGE * PAGE
     else:
         together = 8 if not fast else 32 if with_output else 256                          # rows a block works on together
         blocks = pairs * ((rows + together - 1) // together)
