@@ -71,13 +71,13 @@ struct VerifyArgs {
 // function's eighteen among seventy instructions; 32 entries are two rows of the banks, so a warp's look-up takes two turns.
 struct Exponential {
     double c, max;               // z = (l - max) c; the difference of two floats is exact enough at any temperature
-    float least;                 // below this the result is no longer a normal number: zero
+    float least;                 // below this the result is no longer a normal number: zero (never below max - 700 T)
 };
 __device__ __forceinline__ Exponential exponential_of(float max, float temperature) {
     Exponential e;
     e.c = 46.166241308446828 / (double)temperature;
     e.max = (double)max;
-    e.least = fmaxf((float)((double)max - 700.0 * (double)temperature), -3.402823466e38f);
+    e.least = fmaxf(__double2float_ru((double)max - 700.0 * (double)temperature), -3.402823466e38f);
     return e;
 }
 __device__ __forceinline__ void fill_table(double* table) {       // by the first warp; a barrier follows
@@ -152,12 +152,20 @@ __global__ void __launch_bounds__(VF_PART_THREADS, VF_PART_BLOCKS) verify_stats_
         if (a.temperature > 0.f) {
             const Exponential ex = exponential_of(st.max, a.temperature);
             double s[4] = {0.0, 0.0, 0.0, 0.0};
+            // What is raised to `least` adds nothing if that lies far below the maximum. Where floats are too coarse for that (their
+            // steps are of 100 T and more), everything but the maximum itself adds less than e^-50.
+            if (ex.least == LOWEST || (double)ex.least - ex.max <= -600.0 * (double)a.temperature) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) s[u & 3] += power_of(fmaxf(v[u], ex.least), ex, table);
+                for (int u = 0; u < U; ++u) s[u & 3] += power_of(fmaxf(v[u], ex.least), ex, table);
+            } else {
+#pragma unroll
+                for (int u = 0; u < U; ++u) s[0] += v[u] == st.max ? 1.0 : 0.0;
+            }
             double t = (s[0] + s[1]) + (s[2] + s[3]);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-            st.sum = t;
+            // what stands behind the row counts where the row's own maximum is the lowest value, or the temperature huge
+            st.sum = n < VF_PART ? t - (VF_PART - n) * weight_of(LOWEST, ex, table) : t;
         } else {
             int at = 0x7fffffff;                                  // the lowest place of the maximum
 #pragma unroll

@@ -429,6 +429,46 @@ def test_verify_logits_at_the_types_lowest(cuda):
             assert err == 0 and all(t == -1 or t % 2 == 1 for t in tokens.flatten().tolist())
 
 
+def test_verify_rows_whose_mask_leaves_nothing(cuda):
+    """Rows of nothing but the lowest value: every token is as likely as the others, in vocabularies that end inside a part too."""
+    for vocab in (700, 1024, 1500, 9001):
+        logits = torch.full((9, vocab), torch.finfo(torch.float32).min)
+        drafts = torch.full((3, 2), vocab - 1, dtype=torch.int32)
+        probs = torch.full((3, 2, vocab), 1.0 / vocab)
+        for temperature in (0.5, 1.0):
+            for seed in (0, 1):
+                assert _verify(cuda, vocab, [2, 2, 2], temperature, True, seed=seed, logits=logits, drafts=drafts, probs=probs)[2] == 0
+        assert _verify(cuda, vocab, [2, 2, 2], 0.0, False, logits=logits)[2] == 0
+    # drafts that a row's share decides: 1 / vocabulary lies just above what the draw asks for
+    from camelid_b200.csrc import ops
+    vocab, n = 1025, 4096
+    ints = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=cuda)        # noqa: E731
+    counts, tokens, err = ints(n), ints(n, 2), ints(1)
+    logits = torch.full((2 * n, vocab), torch.finfo(torch.float32).min, device=cuda)
+    scratch = torch.empty(ops.verify_bytes(2 * n, n, vocab), dtype=torch.uint8, device=cuda)
+    accept = (torch.arange(n, device=cuda)[:, None].float() + 0.5) / n                # accepted while below 1 / vocabulary
+    ops.verify_drafts(logits, 2 * torch.arange(n, device=cuda).int(), ints(n) + 1, ints(n, 1) + 7, None, accept, accept[:, 0].contiguous(), 1.0, 0, 1.0,
+                      0.0, counts, tokens, err, scratch)
+    assert int(err) == 0 and torch.equal(counts, (accept[:, 0].double() < 1.0 / vocab).int())
+
+
+@pytest.mark.parametrize("filters", [{}, {"top_p": 0.9}, {"top_k": 5}])
+def test_verify_temperatures_at_the_edge(cuda, filters):
+    """Temperatures far below the logits' own rounding, logits far above the temperature, and temperatures that level everything."""
+    gen = torch.Generator().manual_seed(12)
+    base = torch.randn(6, 5000, generator=gen) * 4
+    base[:, 40] = base[:, 4000] = base.amax(1) + 0.25                 # two largest of one value
+    for temperature in (1e-30, 1e-10, 3e-10, 1e-9, 3e-9, 1e-8, 1e-6):
+        assert _verify(cuda, 5000, [2, 2], temperature, False, logits=base, **filters)[2] == 0
+    for top in (1e6, 3e7, 1e10, 1e30):
+        logits = base.clone()
+        logits[:, 17] = logits[:, 4500] = top
+        assert _verify(cuda, 5000, [2, 2], 1.0, False, logits=logits, **filters)[2] == 0
+    if not filters:
+        for temperature in (1e6, 1e30, 1e38):
+            assert _verify(cuda, 5000, [2, 2], temperature, True, logits=base)[2] == 0
+
+
 def test_verify_equal_logits(cuda):
     """Ties: the lowest id at temperature 0, the draw's share of the ids otherwise."""
     logits = torch.zeros(2, 40000)
