@@ -55,6 +55,7 @@ struct VerifyArgs {
     const float* draws;
     int n_seqs, width;           // width: drafted tokens a sequence has room for
     float temperature;           // 0: greedy
+    double rate;                 // 32 log2(e) / T
     int top_k;
     float top_p, min_p;
     int* counts;
@@ -69,21 +70,24 @@ struct VerifyArgs {
 // whose upper bits are the exponent and whose lower five choose from a table, and a rest of at most a half, whose power is a
 // polynomial of degree four ((ln 2 / 64)^5 / 120 = 1.2e-12). Eleven operations in double instead of the library
 // function's eighteen among seventy instructions; 32 entries are two rows of the banks, so a warp's look-up takes two turns.
+constexpr float LOWEST = -3.402823466e38f;
 struct Exponential {
     double c, max;               // z = (l - max) c; the difference of two floats is exact enough at any temperature
     float least;                 // below this the result is no longer a normal number: zero (never below max - 700 T)
 };
-__device__ __forceinline__ Exponential exponential_of(float max, float temperature) {
+// A temperature below 2^-30 of the maximum, a 64th of a float's step there, leaves nothing but the maximum (e^-64 of it at most).
+__device__ __forceinline__ bool only_largest(const VerifyArgs& a, float max) { return fabsf(max) * 9.313225746e-10f > a.temperature; }
+__device__ __forceinline__ Exponential exponential_of(const VerifyArgs& a, float max) {
     Exponential e;
-    e.c = 46.166241308446828 / (double)temperature;
+    e.c = a.rate;
     e.max = (double)max;
-    e.least = fmaxf(__double2float_ru((double)max - 700.0 * (double)temperature), -3.402823466e38f);
+    e.least = only_largest(a, max) ? max : fmaxf(__fsub_ru(max, 700.f * a.temperature), LOWEST);
     return e;
 }
 __device__ __forceinline__ void fill_table(double* table) {       // by the first warp; a barrier follows
     if (threadIdx.x < 32) table[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
 }
-// `l` at least e.least: what lies below stands for e^-700, which adds nothing to a sum of one or more
+// `l` at least e.least: what lies below stands for e^-700, which adds nothing to a sum of one or more.
 __device__ __forceinline__ double power_of(float l, const Exponential& e, const double* table) {
     const double d = (double)l - e.max;
     const double shifted = fma(d, e.c, 6755399441055744.0);       // 1.5 * 2^52: the whole number in the low bits
@@ -117,7 +121,6 @@ __global__ void __launch_bounds__(VF_PART_THREADS, VF_PART_BLOCKS) verify_stats_
     const int lane = threadIdx.x & 31;
     const int warps = gridDim.x * (VF_PART_THREADS / 32), items = a.n_rows * a.parts;
     constexpr int U = VF_PART / 32;
-    constexpr float LOWEST = -3.402823466e38f;                    // what stands in the columns behind a row
     for (int item = blockIdx.x * (VF_PART_THREADS / 32) + (threadIdx.x >> 5); item < items; item += warps) {
         const int row = item / a.parts, begin = (item - row * a.parts) * VF_PART, n = min(VF_PART, a.vocab - begin);
         const float* r = a.logits + (long long)row * a.ld + begin;
@@ -150,22 +153,14 @@ __global__ void __launch_bounds__(VF_PART_THREADS, VF_PART_BLOCKS) verify_stats_
         st.sum = 0.0;
         st.arg = 0;
         if (a.temperature > 0.f) {
-            const Exponential ex = exponential_of(st.max, a.temperature);
+            const Exponential ex = exponential_of(a, st.max);
             double s[4] = {0.0, 0.0, 0.0, 0.0};
-            // What is raised to `least` adds nothing if that lies far below the maximum. Where floats are too coarse for that (their
-            // steps are of 100 T and more), everything but the maximum itself adds less than e^-50.
-            if (ex.least == LOWEST || (double)ex.least - ex.max <= -600.0 * (double)a.temperature) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) s[u & 3] += power_of(fmaxf(v[u], ex.least), ex, table);
-            } else {
-#pragma unroll
-                for (int u = 0; u < U; ++u) s[0] += v[u] == st.max ? 1.0 : 0.0;
-            }
+            for (int u = 0; u < U; ++u) s[u & 3] += power_of(fmaxf(v[u], ex.least), ex, table);
             double t = (s[0] + s[1]) + (s[2] + s[3]);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-            // what stands behind the row counts where the row's own maximum is the lowest value, or the temperature huge
-            st.sum = n < VF_PART ? t - (VF_PART - n) * weight_of(LOWEST, ex, table) : t;
+            st.sum = t;
         } else {
             int at = 0x7fffffff;                                  // the lowest place of the maximum
 #pragma unroll
@@ -236,7 +231,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
         tm.sync();
         return;
     }
-    const Exponential ex = exponential_of(mx, a.temperature);
+    const Exponential ex = exponential_of(a, mx);
     // the place of a value in the order: never negative, monotone, and finite (masks of the type's lowest value are
     // all put at one far place, where their weight is zero)
     const float inv_t = fminf(1.0f / a.temperature, 1e30f), far = 1e30f;
@@ -440,8 +435,15 @@ __device__ __forceinline__ RowStat join_parts(const VerifyArgs& a, int row, cons
     r.bad = __any_sync(0xffffffffu, bad) ? 1 : 0;
     r.total = 0.0;
     if (a.temperature > 0.f && !r.bad) {
-        const Exponential ex = exponential_of(r.max, a.temperature);
-        for (int p = lane; p < a.parts; p += 32) r.total += s[p].sum * weight_of(s[p].max, ex, table);
+        const Exponential ex = exponential_of(a, r.max);
+        if (a.floors == nullptr && only_largest(a, r.max)) {      // the parts' sums counted what lies just below as well
+            const float* l = a.logits + (long long)row * a.ld;
+            for (int i = lane; i < a.vocab; i += 32) r.total += l[i] == r.max ? 1.0 : 0.0;
+        } else {
+            for (int p = lane; p < a.parts; p += 32) r.total += s[p].sum * weight_of(s[p].max, ex, table);
+            // LOWEST behind the row's end counts where the temperature is huge
+            if (lane == 31 && a.floors == nullptr) r.total -= (a.parts * VF_PART - a.vocab) * weight_of(LOWEST, ex, table);
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) r.total += __shfl_xor_sync(0xffffffffu, r.total, o);
     }
@@ -509,7 +511,7 @@ __global__ void __launch_bounds__(VF_THREADS, PER_SM) verify_decide_kernel(Verif
                     if (greedy) p = x == r.arg ? 1.0 : 0.0;
                     else {
                         const bool in = !filtered || composite_key(l, x) >= a.floors[row0 + j];
-                        p = in ? weight_of(l, exponential_of(r.max, a.temperature), table) / r.total : 0.0;
+                        p = in ? weight_of(l, exponential_of(a, r.max), table) / r.total : 0.0;
                     }
                     ok = (double)u * (double)q < p;
                 }
@@ -541,7 +543,7 @@ __global__ void __launch_bounds__(VF_THREADS, PER_SM) verify_decide_kernel(Verif
     const float* q = (rejected && a.probs) ? a.probs + (long long)seq * a.probs_seq + (long long)count * a.probs_step : nullptr;
     const int without = (rejected && !a.probs) ? a.drafts[(long long)seq * a.drafts_ld + count] : -1;
     const unsigned long long floor_key = filtered ? a.floors[row] : 0ull;
-    const Exponential ex = exponential_of(st.max, a.temperature);
+    const Exponential ex = exponential_of(a, st.max);
     const double inv_total = 1.0 / st.total;
     bool bad_q = false;
     bool plain = false;                                           // nothing is left of p - q: draw from p
@@ -568,7 +570,7 @@ __global__ void __launch_bounds__(VF_THREADS, PER_SM) verify_decide_kernel(Verif
             if (filtered && composite_key(l[k], i + k) < floor_key) p = 0.0;
             if (!plain) {
                 if (q) {
-                    bad_q = bad_q || !(qi[k] >= 0.f);
+                    bad_q = bad_q || !(qi[k] >= 0.f) || !finite(qi[k]);
                     p -= (double)qi[k];
                 }
                 if (i + k == without) p = 0.0;
@@ -726,7 +728,7 @@ extern "C" int cml_verify_drafts(const float* logits, long long ld, int n_rows, 
     a.logits = logits; a.ld = ld; a.n_rows = n_rows; a.vocab = vocab; a.row0 = row0; a.lens = lens;
     a.drafts = drafts; a.drafts_ld = drafts_ld; a.probs = probs; a.probs_seq = probs_seq; a.probs_step = probs_step;
     a.accept = accept; a.accept_ld = accept_ld; a.draws = draws; a.n_seqs = n_seqs; a.width = width;
-    a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p;
+    a.temperature = temperature; a.rate = 46.166241308446828 / (double)temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p;
     a.counts = counts; a.tokens = tokens; a.err = err;
     a.stats = (PartStat*)scratch;
     a.parts = filters ? 1 : verify_parts(vocab);
