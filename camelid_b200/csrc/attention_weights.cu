@@ -1093,7 +1093,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, 2) weights_keys_mma_kernel(Weig
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float4 row = tail[half * 16 + n * 8 + 2 * (lane & 3) + i];
-                    if (whole) {
+                    if (whole && c * AC_ROWS + AC_ROWS <= s.rows) {           // (rows that are none: zero times an infinite key is no zero)
 #pragma unroll
                         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll

@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
                     } else {                                                  // this thread's key, half of the tile's rows
                         const float4* const rows = rows_s + rt * 128 + half * 64;
                         float part[4] = {0.f, 0.f, 0.f, 0.f};
-                        if (whole) {
+                        if (whole && rt * 128 + half * 64 + 64 <= s.rows) {   // (rows that are none: zero times an infinite key is no zero)
 #pragma unroll
                             for (int c = 0; c < 64; ++c) {
                                 const float2 r = *reinterpret_cast<const float2*>(rows + c);

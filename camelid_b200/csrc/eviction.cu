@@ -428,7 +428,7 @@ extern "C" int cml_evict_positions(void* k, void* v, float* scores, int dtype, c
     if (heads <= 0 || n_pages <= 0 || width <= 0 || out_width <= 0 || width > (1 << 24) || out_width > (1 << 24)) return CML_ERR_BAD_SIZE;
     if (k_dim <= 0 || k_dim % 16 || v_dim % 16 || k_dim + v_dim > 1024 || first < 0 || recent < 0) return CML_ERR_BAD_SIZE;
     if (inv_freq != nullptr && (rotary_dim <= 0 || rotary_dim > k_dim || rotary_dim % 16)) return CML_ERR_BAD_SIZE;
-    if (((uintptr_t)k | (uintptr_t)v) & 15) return CML_ERR_BAD_ALIGN;
+    if ((((uintptr_t)k | (uintptr_t)v) & 15) || (((uintptr_t)scores) & 7)) return CML_ERR_BAD_ALIGN;      // scores are read in pairs
     if ((long long)n_pages * heads * CML_PAGE > 0x7fffffffLL) return CML_ERR_BAD_SIZE;       // an entry's rows are counted in 32 bits
     const long long units = (long long)entries * n_seqs * heads;
     if (units * EV_MAX_TEAM > 0x7fffffffLL) return CML_ERR_BAD_SIZE;

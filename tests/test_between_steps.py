@@ -61,6 +61,12 @@ def test_kernel_entries_refuse_sizes_before_they_launch():
         assert ve(*{**good, **change}.values()) == code, change
 
 
+def test_eviction_refuses_scores_that_do_not_begin_on_eight_bytes():
+    ev = ops._fn("eviction", "cml_evict_positions")
+    args = [4096, 4096, 4100, 0, 4096, 1, 4096, 1, 4096, 4096, 4096, 4, 1, 1, 1, 1, 64, 64, 0, 0, None, 0, 0, None]
+    assert ev(*args) == -4
+
+
 # ---- caches that keep attention weights --------------------------------------------------------------------------------
 def _cache(specs, **kw):
     return SequenceCache(specs, [None] * len(specs), max_tokens=256, max_position=1000, dtype=torch.float32, device="cpu", **kw)

@@ -204,6 +204,30 @@ def test_window_with_missing_pages(cuda):
         assert bool(((s_dev.cpu().double() - ref).abs() <= tol + 1e-30).all())
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [5, 9, 17, 20, 33, 70])
+def test_window_with_an_infinite_key(cuda, dim, new):
+    """A key of minus infinity weighs nothing: its score stays a number, whatever rows fill up a tile."""
+    from camelid_b200.csrc import ops
+    gen = torch.Generator().manual_seed(new)
+    k = torch.randn(9, 1, PAGE, dim, generator=gen).to(torch.bfloat16)
+    q = torch.randn(new, 8 * dim, generator=gen).to(torch.bfloat16)
+    q[:, ::dim] = q[:, ::dim].abs() + 0.1                      # the channel of every head that meets the infinite one
+    k[4, 0, 7, 0] = -math.inf
+    start, scores = 9 * PAGE - new - 3, torch.rand(9, 1, PAGE, generator=gen)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)        # noqa: E731
+    scratch = torch.empty(ops.attn_weights_floats(1, 8, 1, dim, torch.bfloat16, new, start + new, False), device=cuda)
+    s_dev = scores.to(cuda)
+    ops.attn_paged_weights(q.to(cuda), None, k.to(cuda), None, s_dev, ints([list(range(9))]), ints([0]), ints([start]), ints([new]), 8, new,
+                           start + new, dim ** -0.5, scratch)
+    without = k.clone()
+    without[4, 0, 7] = 0.0                                     # the tolerances of the other places
+    _, _, _, tol = pb.weights(q, without, None, scores, [list(range(9))], [0], [start], [new], 8, dim ** -0.5)
+    _, ref, _, _ = pb.weights(q, k, None, scores, [list(range(9))], [0], [start], [new], 8, dim ** -0.5)
+    assert bool(torch.isfinite(ref).all()) and float(s_dev[4, 0, 7]) == float(scores[4, 0, 7])
+    assert bool(((s_dev.cpu().double() - ref).abs() <= 2 * tol + 1e-30).all())
+
+
 @pytest.mark.parametrize("dtype,dim,new", [(torch.bfloat16, 64, 1), (torch.bfloat16, 128, 6), (torch.bfloat16, 64, 40), (torch.float32, 48, 1),
                                            (torch.float32, 64, 9)])
 def test_places_that_the_same_step_brought_start_from_zero(cuda, dtype, dim, new):
@@ -512,6 +536,14 @@ def test_verify_reports_what_it_cannot_use(cuda):
     probs = torch.full((1, 2, 500), -1.0)
     counts, tokens, err = _verify(cuda, 500, [2], 1.0, True, drafts=torch.tensor([[1, 3]], dtype=torch.int32), probs=probs)
     assert err == 4
+
+
+def test_verify_reports_an_infinite_probability_of_another_token(cuda):
+    """The probabilities of the row that the next token is drawn from are all looked at."""
+    probs = torch.full((1, 1, 500), 0.0)
+    probs[0, 0, 3], probs[0, 0, 77] = 1e6, float("inf")        # the draft, token 3, is rejected
+    counts, tokens, err = _verify(cuda, 500, [1], 1.0, True, drafts=torch.tensor([[3]], dtype=torch.int32), probs=probs)
+    assert int(counts) == 0 and int(tokens[0, 0]) not in (3, 77) and err == 4
 
 
 def test_verify_keeps_the_targets_distribution(cuda):
