@@ -2069,7 +2069,8 @@ def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, 
     heads, 64]) gain every place's weight, summed over the rows and the query heads of its kv head; new places start from
     zero, whatever their page held (``seq_cached``: int32 [sequences], places that count as cached where fewer than seq_start do,
     because the same step brought the others). The new scores go to ``scores_out`` (None: in place), where nothing but the sequences'
-    places is written. ``max_new`` and ``max_len`` bound the sequences' new tokens and lengths (rows and places beyond them are
+    places is written; a sequence without new tokens is left alone. A row that sees no place (its pages are missing) gives zeros and
+    weighs nothing. ``max_new`` and ``max_len`` bound the sequences' new tokens and lengths (rows and places beyond them are
     left out); ``scratch``: float32, ``attn_weights_floats`` numbers, free again when the call's work is done. ``err``
     (int32 [1]; by default ``simt_error_word``) is set if one of the kernels' bounded waits runs out. No page stands in two rows of
     the table."""

@@ -181,8 +181,8 @@ def _drafts_of(drafter, history: list, most: int) -> tuple:
 def run_drafted_batch(model, cache, sampler, drafter, prompts: list, budgets: list, requested: list, stop_ids: set,
                       on_step=None) -> list:
     """``run_batch`` with drafted tokens: every step brings a sequence's last token and what ``drafter`` expects behind it, the
-    sampler verifies the drafts against the step's logits, and the rejected ones leave the cache again. A step yields
-    one token more than it accepts drafts."""
+    sampler verifies the drafts against the step's logits, and the rejected ones leave the cache again (what they looked at
+    stays in the scores of a cache that keeps attention weights). A step yields one token more than it accepts drafts."""
     n = len(prompts)
     results = [GenerationResult(prompt_tokens=len(p)) for p in prompts]
     slots = [None] * n
@@ -207,8 +207,9 @@ def run_drafted_batch(model, cache, sampler, drafter, prompts: list, budgets: li
                 drafts.append(d)
                 probs.append(p)
             # Every sequence brings as many rows as the one with the most drafts, where its budget lets it: steps of few layouts come
-            # back and are captured. What stands behind a sequence's drafts is not looked at and leaves the cache with the rest.
-            most = max(len(d) for d in drafts)
+            # back and are captured. What stands behind a sequence's drafts is not looked at and leaves the cache with the rest; a cache
+            # that keeps attention weights would keep those of such rows, so there every sequence brings its own.
+            most = max(len(d) for d in drafts) if getattr(cache, "scores", None) is None else 0
             entries, row0, at = [], [], 0
             for i, d in zip(live, drafts):
                 rows = max(len(d), min(most, budgets[i] - len(results[i].tokens) - 1))

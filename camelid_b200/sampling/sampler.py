@@ -99,6 +99,8 @@ class Sampler:
         if len(histories) != n or len(row0) != n or any(not 0 <= r <= rows - len(d) - 1 for r, d in zip(row0, drafts)):
             raise SamplingError(f"{n} sequences with {sum(len(d) for d in drafts)} drafts do not fit {rows} rows of logits and "
                                 f"{len(histories)} histories")
+        if n == 0:
+            return [], []
         if o.adjusts:
             # a row's history ends with the drafts before it; rows that no sequence names are left alone
             named = {r + j: list(h) + list(d[:j]) for r, h, d in zip(row0, histories, drafts) for j in range(len(d) + 1)}

@@ -232,6 +232,15 @@ def test_drafted_loop_keeps_within_budget_and_cache():
     assert generate(Counting(), Rolling(), Exact(), [[1]], 0, drafter=_expected)[0].tokens == []
 
 
+def test_drafted_loop_brings_no_rows_of_its_own_where_weights_are_kept():
+    """Rows that only make steps of one size would leave their weights in the scores."""
+    model, cache = Counting(), Rolling()
+    cache.scores = [torch.zeros(1)]
+    drafts = {1: [5, 6, 7], 2: [], 3: [9]}
+    generate(model, cache, Exact(), [[1], [2], [3]], 6, drafter=lambda h: drafts[h[0]])
+    assert (4, 1, 2) in model.layouts and (4, 4, 4) not in model.layouts
+
+
 def test_drafted_loop_refusals():
     with pytest.raises(StepError):
         generate(Counting(), Rolling(), Exact(), [[1]], 5, drafter=lambda h: [50])

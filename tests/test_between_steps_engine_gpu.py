@@ -187,6 +187,28 @@ def test_drafted_sampling_is_the_requests_own(cuda, model_folders):
             assert together == alone and all(len(t) == 16 for t in together)
 
 
+def test_verification_of_no_sequences(cuda):
+    from camelid_b200.sampling import Sampler, SamplingOptions
+    for options in (SamplingOptions(), SamplingOptions(temperature=0.5, repeat_penalty=1.2, seed=1)):
+        assert Sampler(options, 100, "cuda").verify(torch.zeros(0, 100, device=cuda), [], []) == ([], [])
+
+
+def test_drafted_generation_over_a_cache_that_keeps_weights(cuda, model_folders):
+    """Drafts that are always right: every row counts once, whatever steps brought it."""
+    import camelid_b200
+    lm = camelid_b200.load(model_folders["tiny_d"], dtype="float32")
+    prompts = [tokens(60 + i, n, 331) for i, n in enumerate([30, 7, 12])]
+    want = lm.generate(prompts, max_tokens=24, stop_token_ids=())
+    known = [list(p) + w for p, w in zip(prompts, want)]
+
+    def right(history):
+        full = next(k for k in known if k[:len(history)] == history)
+        return full[len(history):len(history) + 1 + len(history) % 4]
+    cache = lm.new_cache(1024, track_weights=True)
+    assert lm.generate(prompts, max_tokens=24, stop_token_ids=(), drafter=right, cache=cache) == want
+    cache.book.audit()
+
+
 def test_drafts_verification_and_eviction_together(cuda):
     """A long run as it would be served: prompts, steps with drafts, rejected ones rolled back, eviction over a budget; the captured
     single-token steps in between. With one layer and nothing of the middle kept, a fresh sequence of the positions that
