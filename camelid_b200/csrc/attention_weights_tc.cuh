@@ -2,11 +2,13 @@
 // Included by attention_weights.cu, whose arguments it takes.
 //
 // Both passes are one kernel. The rows of q stay in shared memory (up to 512 of them), the keys pass by in tiles of 128 that TMA
-// brings from the pages, and every (tile, 128 rows) is one product of 128 x 128 in tensor memory, of which two are in flight.
+// brings from the pages, and every (tile, 128 rows) is one product of 128 x 128 in tensor memory. Two sides of four warps take the
+// tiles in turn, so that one side's exponentials run beside the other's reads and maxima (both on halves of one tile: 58 and 66 us
+// for the two passes over four prompts of 9,001 to 16,384 keys, TODO).
 //
-//   SUM false: S = Q K^T, a thread a row (and half of the tile's keys): its running maximum and sum over a stretch of keys
-//   SUM true:  S = K Q^T, a thread a key (and half of the rows): the sum of its weights 2^(s - max) / sum over the rows,
-//              kept in one register; the stretches' statistics are joined by every block for itself
+//   SUM false: S = Q K^T, a thread a row: its running maximum and sum over its side's tiles of a stretch of keys
+//   SUM true:  S = K Q^T, a thread a key: the sum of its weights 2^(s - max - log2 sum) over the rows, in registers; the
+//              stretches' statistics are joined by every block for itself
 //
 // One exponential a row and key in each pass bounds the kernel (16 a cycle and multiprocessor): a product of 128 x 128 x 128 takes
 // half as long. Eight warps of exponentials, one that brings keys, one that issues products.
@@ -14,7 +16,7 @@
 #include <cuda.h>
 
 #define WT_KEYS 128
-#define WT_WORKERS 256                 // threads that work on scores
+#define WT_WORKERS 512                 // threads that work on scores: two sides of two halves of 128
 #define WT_THREADS (WT_WORKERS + 64)
 #define WT_WAIT_CYCLES 2000000000ll
 
@@ -74,7 +76,16 @@ __device__ __forceinline__ void wt_read32(uint32_t addr, float* r) {
           "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
         : "r"(addr));
 }
-__device__ __forceinline__ void wt_read_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The loads of these 32 columns are there; nothing uses them before.
+__device__ __forceinline__ void wt_read_wait(float* r) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(r);
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+        : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]), "+r"(u[4]), "+r"(u[5]), "+r"(u[6]), "+r"(u[7]), "+r"(u[8]),
+          "+r"(u[9]), "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]), "+r"(u[14]), "+r"(u[15]), "+r"(u[16]),
+          "+r"(u[17]), "+r"(u[18]), "+r"(u[19]), "+r"(u[20]), "+r"(u[21]), "+r"(u[22]), "+r"(u[23]), "+r"(u[24]),
+          "+r"(u[25]), "+r"(u[26]), "+r"(u[27]), "+r"(u[28]), "+r"(u[29]), "+r"(u[30]), "+r"(u[31])
+        :: "memory");
+}
 // Rows of 128 bytes, 128-byte swizzle, 1,024 bytes between groups of eight rows: as TMA writes the keys and the workers q.
 __device__ __forceinline__ uint64_t wt_desc(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
@@ -84,8 +95,10 @@ __device__ __forceinline__ void wt_workers_sync() { asm volatile("bar.sync 1, %0
 template <int HD, int RT> struct WtPlan {
     static constexpr int KB = HD / 64;                                        // 64-channel blocks of a row
     static constexpr uint32_t TILE = 128u * 128u * KB;                        // 128 rows or keys
-    static constexpr int STAGES = RT * KB >= 8 ? 2 : 3;
-    static constexpr size_t SMEM = 1024 + (size_t)TILE * (RT + STAGES) + 256 + RT * 128 * 16 + 2 * 128 * 4;
+    static constexpr int ROOM = (227 * 1024 - 1280 - RT * 1024 * 3) / (int)TILE - RT;
+    static constexpr int STAGES = ROOM < 6 ? ROOM : 6;                        // what the rows of q leave room for
+    static constexpr size_t SMEM = 1024 + (size_t)TILE * (RT + STAGES) + 256 + RT * 128 * 8 * 3;
+    static constexpr int BUFS = 2;                                            // products of a side in tensor memory
 };
 
 // Which stretch a block has. All sequences' key tiles are cut into stretches of the same number of tiles, the smallest for which they
@@ -139,22 +152,24 @@ __device__ __forceinline__ WtShare wt_share(const WeightArgs& a, int block, int 
 template <int HD, int RT, bool SUM>
 __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_constant__ CUtensorMap map, WeightArgs a, int* err) {
     using P = WtPlan<HD, RT>;
-    constexpr int KB = P::KB, STAGES = P::STAGES;
+    constexpr int KB = P::KB, STAGES = P::STAGES, BUFS = P::BUFS;
     constexpr uint32_t TILE = P::TILE, BLOCK = 128u * 128u;
     extern __shared__ uint8_t wt_raw[];
     const uint32_t base = ((uint32_t)__cvta_generic_to_shared(wt_raw) + 1023u) & ~1023u;
     uint8_t* const gbase = wt_raw + (base - (uint32_t)__cvta_generic_to_shared(wt_raw));
     const uint32_t sQ = base, sK = sQ + RT * TILE, bars = sK + STAGES * TILE;
     uint8_t* const tail = gbase + (bars - base);
-    uint32_t* const slot = reinterpret_cast<uint32_t*>(tail + 16 * 8);
+    uint32_t* const slot = reinterpret_cast<uint32_t*>(tail + 24 * 8);
     volatile int* const gave_up = reinterpret_cast<volatile int*>(slot + 1);
-    float4* const rows_s = reinterpret_cast<float4*>(tail + 256);             // [RT * 128]: SUM (maximum, 1 / sum, last place, -); else results
-    float* const half_s = reinterpret_cast<float*>(rows_s + RT * 128);        // SUM: [2][128] the second half's sums
+    float* const ref_s = reinterpret_cast<float*>(tail + 256);                // SUM: [RT * 128] maximum + log2 sum of a row, and
+    int* const place_s = reinterpret_cast<int*>(ref_s + RT * 128);            // the last place it sees
+    float* const half_s = reinterpret_cast<float*>(place_s + RT * 128);       // [2 sides][2 tiles][128]: the second half's sums
+    float2* const rows_s = reinterpret_cast<float2*>(tail + 256);             // else: [3][RT * 128] the others' maxima and sums
     auto k_full = [&](int s) { return bars + 8u * s; };
     auto k_empty = [&](int s) { return bars + 8u * (STAGES + s); };
     auto s_full = [&](int b) { return bars + 8u * (2 * STAGES + b); };
-    auto s_empty = [&](int b) { return bars + 8u * (2 * STAGES + 2 + b); };
-    const uint32_t q_ready = bars + 8u * (2 * STAGES + 4);
+    auto s_empty = [&](int b) { return bars + 8u * (2 * STAGES + 2 * BUFS + b); };
+    const uint32_t q_ready = bars + 8u * (2 * STAGES + 4 * BUFS);             // 21 barriers at most
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     pdl_launch_dependents();
@@ -173,14 +188,14 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
     };
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) wt_init(k_full(i), 1), wt_init(k_empty(i), 1);
-        for (int i = 0; i < 2; ++i) wt_init(s_full(i), 1), wt_init(s_empty(i), WT_WORKERS);
+        for (int i = 0; i < 2 * BUFS; ++i) wt_init(s_full(i), 1), wt_init(s_empty(i), WT_WORKERS / 64);
         wt_init(q_ready, WT_WORKERS);
         *gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         wt_fence_smem();
     }
-    if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(slot)), "r"(256u) : "memory");
+    if (warp == WT_WORKERS / 32 + 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(slot)), "r"(256u * BUFS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     wt_fence_before();
@@ -188,7 +203,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
     wt_fence_after();
     const uint32_t tmem = *slot;
 
-    if (warp == 8) {
+    if (warp == WT_WORKERS / 32) {
         if (lane == 0) {
             int issued = 0;
             for (int t = 0; t < n_tiles; ++t) {
@@ -210,150 +225,174 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
                 }
             }
         }
-    } else if (warp == 9) {
+    } else if (warp == WT_WORKERS / 32 + 1) {
         if (lane == 0) {
             constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
             bool ok = wt_wait(q_ready, 0, gave_up);
-            int it = 0;
-            for (int t = 0; t < n_tiles && ok; ++t) {
-                const int st = t % STAGES;
-                ok = wt_wait(k_full(st), (uint32_t)(t / STAGES) & 1u, gave_up);
-                for (int rt = 0; rt < row_tiles && ok; ++rt, ++it) {
-                    ok = wt_wait(s_empty(it & 1), ((uint32_t)(it >> 1) & 1u) ^ 1u, gave_up);
-                    if (!ok) break;
-                    wt_fence_after();
+            int item = 0;                                                     // of a side: (tile, 128 rows) in turn
+            for (int t0 = 0; t0 < n_tiles && ok; t0 += 2) {
+                for (int rt = 0; rt < row_tiles && ok; ++rt, ++item) {
+                    for (int side = 0; side < 2 && t0 + side < n_tiles; ++side) {
+                        const int t = t0 + side, st = t % STAGES, buf = side * BUFS + item % BUFS;
+                        if (rt == 0) ok = wt_wait(k_full(st), (uint32_t)(t / STAGES) & 1u, gave_up);
+                        if (ok) ok = wt_wait(s_empty(buf), ((uint32_t)(item / BUFS) & 1u) ^ 1u, gave_up);
+                        if (!ok) break;
+                        wt_fence_after();
 #pragma unroll
-                    for (int b = 0; b < KB; ++b) {
-                        const uint64_t q = wt_desc(sQ + rt * TILE + b * BLOCK), k = wt_desc(sK + st * TILE + b * BLOCK);
+                        for (int b = 0; b < KB; ++b) {
+                            const uint64_t q = wt_desc(sQ + rt * TILE + b * BLOCK), k = wt_desc(sK + st * TILE + b * BLOCK);
 #pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            wt_mma(tmem + (it & 1) * 128, (SUM ? k : q) + (uint64_t)(c * 2), (SUM ? q : k) + (uint64_t)(c * 2), idesc, (b | c) ? 1u : 0u);
+                            for (int c = 0; c < 4; ++c)
+                                wt_mma(tmem + buf * 128, (SUM ? k : q) + (uint64_t)(c * 2), (SUM ? q : k) + (uint64_t)(c * 2), idesc, (b | c) ? 1u : 0u);
+                        }
+                        wt_commit(s_full(buf));
+                        if (rt == row_tiles - 1) wt_commit(k_empty(st));
                     }
-                    wt_commit(s_full(it & 1));
                 }
-                if (ok) wt_commit(k_empty(st));
             }
         }
     } else {
         // q into its tiles, zeros where there is no row
-        for (int c = threadIdx.x; c < row_tiles * 128 * KB * 8; c += WT_WORKERS) {
-            const int m = c / (KB * 8), cc = c % (KB * 8), b = cc / 8, r = m % 128;
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (m < s.rows) v = *reinterpret_cast<const uint4*>((const bf16*)a.q + (long long)(s.row0 + m / group) * a.q_stride + (long long)(kvh * group + m % group) * HD + cc * 8);
-            *reinterpret_cast<uint4*>(gbase + (m / 128) * TILE + b * BLOCK + (r >> 3) * 1024 + (r & 7) * 128 + (((cc & 7) ^ (r & 7)) << 4)) = v;
+        constexpr int ROW = KB * 8;                                           // 16-byte pieces of a row
+        const int piece = threadIdx.x % ROW, x0 = threadIdx.x / ROW;
+        for (int m = x0; m < row_tiles * 128; m += WT_WORKERS / ROW) {
+            const bool in = m < s.rows;
+            const int j = in ? m / group : 0;
+            const bf16* src = (const bf16*)a.q + (long long)(s.row0 + j) * a.q_stride + (long long)(kvh * group + (in ? m - j * group : 0)) * HD + piece * 8;
+            const int r = m % 128;
+            cp_async16_or_zero(sQ + (m / 128) * TILE + (piece / 8) * BLOCK + (r >> 3) * 1024 + (r & 7) * 128 + (((piece & 7) ^ (r & 7)) << 4), src, in);
         }
+        cp_async_commit();
         if (SUM) {                                                            // the stretches of every row joined, in their order
             const int splits = share.splits;
             for (int m = threadIdx.x; m < RT * 128; m += WT_WORKERS) {
                 float top = -CUDART_INF_F, sum = 0.f;
                 if (m < s.rows) {
                     const float* st = a.stats + ((size_t)pair * a.n_splits * group_rows + m) * 2;
-                    for (int i = 0; i < splits; ++i) top = fmaxf(top, st[(size_t)i * group_rows * 2]);
-                    for (int i = 0; i < splits; ++i) {
-                        const float2 x = *reinterpret_cast<const float2*>(st + (size_t)i * group_rows * 2);
-                        if (x.x != -CUDART_INF_F) sum += exp2f(x.x - top) * x.y;
+                    for (int i0 = 0; i0 < splits; i0 += 8) {                  // eight at a time, which are asked for at once
+                        float2 x[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            x[i] = i0 + i < splits ? *reinterpret_cast<const float2*>(st + (size_t)(i0 + i) * group_rows * 2) : make_float2(-CUDART_INF_F, 0.f);
+                        float most = top;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) most = fmaxf(most, x[i].x);
+                        if (top != -CUDART_INF_F) sum *= exp2f(top - most);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (x[i].x != -CUDART_INF_F) sum += exp2f(x[i].x - most) * x[i].y;
+                        top = most;
                     }
                 }
-                const bool none = top == -CUDART_INF_F;
-                rows_s[m] = make_float4(none ? 0.f : top, none ? 0.f : 1.f / sum, __int_as_float(m < s.rows ? s.start + m / group : -1), 0.f);
+                ref_s[m] = top == -CUDART_INF_F ? CUDART_INF_F : top + log2f(sum);
+                place_s[m] = m < s.rows ? s.start + m / group : -1;
             }
         }
+        cp_async_wait<0>();
         wt_fence_smem();
         wt_arrive(q_ready);
-        wt_workers_sync();                                                    // rows_s is whole
-        const int half = warp >> 2, mine = (warp & 3) * 32 + lane;            // this thread's lane of tensor memory
+        wt_workers_sync();                                                    // ref_s is whole
+        const int side = warp >> 3, half = (warp >> 2) & 1, mine = (warp & 3) * 32 + lane;    // mine: this thread's lane of tensor memory
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         float top[RT], sum[RT];
 #pragma unroll
         for (int r = 0; r < RT; ++r) top[r] = -CUDART_INF_F, sum[r] = 0.f;
         bool ok = true;
-        int it = 0;
-        for (int t = 0; t < n_tiles; ++t) {
+        int item = 0;
+        for (int t = side; t < n_tiles; t += 2) {                             // (after a wait that ran out: without working)
             const int key0 = first + t * WT_KEYS;
             const int page0 = page_at(key0), page1 = page_at(key0 + CML_PAGE);
             // every row sees every key of the tile
             const bool whole = page0 >= 0 && page1 >= 0 && key0 + WT_KEYS <= last && key0 + WT_KEYS - 1 <= s.start;
-            float gained = 0.f;
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 if (rt >= row_tiles) break;
-                if (ok) ok = wt_wait(s_full(it & 1), (uint32_t)(it >> 1) & 1u, gave_up);
-                if (ok) {
-                    wt_fence_after();
-                    float x[64];
-                    wt_read32(tmem + (it & 1) * 128 + lanes + half * 64, x);
-                    wt_read32(tmem + (it & 1) * 128 + lanes + half * 64 + 32, x + 32);
-                    wt_read_wait();
-                    wt_fence_before();
-                    wt_arrive(s_empty(it & 1));
-                    if (!SUM) {                                               // this thread's row, the keys of one page
-                        if (!whole) {
-                            const int seen = (half ? page1 : page0) < 0 ? -1 : min(last - 1, s.start + (rt * 128 + mine) / group) - key0 - half * 64;
+                const int buf = side * BUFS + item % BUFS;
+                ok = ok && __all_sync(0xffffffffu, wt_wait(s_full(buf), (uint32_t)(item / BUFS) & 1u, gave_up));
+                ++item;
+                if (!ok) break;
+                wt_fence_after();
+                float x[64];
+                wt_read32(tmem + buf * 128 + lanes + half * 64, x);
+                wt_read32(tmem + buf * 128 + lanes + half * 64 + 32, x + 32);
+                wt_read_wait(x);
+                wt_read_wait(x + 32);
+                wt_fence_before();
+                __syncwarp();
+                if (lane == 0) wt_arrive(s_empty(buf));                       // read: the next product may come
+                if (!SUM) {                                                   // this thread's row, the keys of one page
+                    if (!whole) {
+                        const int seen = (half ? page1 : page0) < 0 ? -1 : min(last - 1, s.start + (rt * 128 + mine) / group) - key0 - half * 64;
 #pragma unroll
-                            for (int c = 0; c < 64; ++c) x[c] = c <= seen ? x[c] : -CUDART_INF_F;
-                        }
-                        float most = x[0];
-#pragma unroll
-                        for (int c = 1; c < 64; ++c) most = fmaxf(most, x[c]);
-                        most *= a.scale;
-                        if (most > top[rt] + 6.f) {                           // the reference moves only when it is passed by 2^6
-                            sum[rt] *= fast_exp2(top[rt] - most);
-                            top[rt] = most;
-                        }
-                        const float ref = top[rt] == -CUDART_INF_F ? 0.f : top[rt];
-                        float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int c = 0; c < 64; ++c) part[c & 3] += fast_exp2(fmaf(x[c], a.scale, -ref));
-                        sum[rt] += (part[0] + part[1]) + (part[2] + part[3]);
-                    } else {                                                  // this thread's key, half of the tile's rows
-                        const float4* const rows = rows_s + rt * 128 + half * 64;
-                        float part[4] = {0.f, 0.f, 0.f, 0.f};
-                        if (whole && rt * 128 + half * 64 + 64 <= s.rows) {   // (rows that are none: zero times an infinite key is no zero)
-#pragma unroll
-                            for (int c = 0; c < 64; ++c) {
-                                const float2 r = *reinterpret_cast<const float2*>(rows + c);
-                                part[c & 3] = fmaf(fast_exp2(fmaf(x[c], a.scale, -r.x)), r.y, part[c & 3]);
-                            }
-                        } else {
-                            const int key = key0 + mine;
-#pragma unroll
-                            for (int c = 0; c < 64; ++c) {
-                                const float4 r = rows[c];
-                                if (key <= __float_as_int(r.z)) part[c & 3] = fmaf(fast_exp2(fmaf(x[c], a.scale, -r.x)), r.y, part[c & 3]);
-                            }
-                        }
-                        gained += (part[0] + part[1]) + (part[2] + part[3]);
+                        for (int i = 0; i < 64; ++i) x[i] = i <= seen ? x[i] : -CUDART_INF_F;
                     }
+                    float m[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) m[i] = x[i];
+#pragma unroll
+                    for (int i = 4; i < 64; ++i) m[i & 3] = fmaxf(m[i & 3], x[i]);
+                    const float most = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * a.scale;
+                    const bool passed = most > top[rt] + 6.f;
+                    if (__any_sync(0xffffffffu, passed)) {                    // the reference moves only when a row passes it by 2^6
+                        sum[rt] *= passed ? fast_exp2(top[rt] - most) : 1.f;
+                        top[rt] = passed ? most : top[rt];
+                    }
+                    const float ref = top[rt] == -CUDART_INF_F ? 0.f : top[rt];
+                    part[0] = part[1] = part[2] = part[3] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) part[i & 3] += fast_exp2(fmaf(x[i], a.scale, -ref));
+                    sum[rt] += (part[0] + part[1]) + (part[2] + part[3]);
+                } else if (whole && rt * 128 + half * 64 + 64 <= s.rows) {    // this thread's key, 64 rows
+#pragma unroll
+                    for (int i = 0; i < 64; i += 4) {
+                        const float4 ref = *reinterpret_cast<const float4*>(ref_s + rt * 128 + half * 64 + i);
+                        part[0] += fast_exp2(fmaf(x[i], a.scale, -ref.x));
+                        part[1] += fast_exp2(fmaf(x[i + 1], a.scale, -ref.y));
+                        part[2] += fast_exp2(fmaf(x[i + 2], a.scale, -ref.z));
+                        part[3] += fast_exp2(fmaf(x[i + 3], a.scale, -ref.w));
+                    }
+                } else {                                                      // some rows see less (or are none: zero times an infinite key is no zero)
+#pragma unroll
+                    for (int i = 0; i < 64; ++i)
+                        if (key0 + mine <= place_s[rt * 128 + half * 64 + i]) part[i & 3] += fast_exp2(fmaf(x[i], a.scale, -ref_s[rt * 128 + half * 64 + i]));
                 }
-                ++it;
             }
             if (SUM) {                                                        // the two halves of the rows, then the key's score
-                if (half) half_s[(t & 1) * 128 + mine] = gained;
-                wt_workers_sync();
+                const float gained = (part[0] + part[1]) + (part[2] + part[3]);
+                float* const other = half_s + (side * 2 + ((t >> 1) & 1)) * 128 + mine;
+                if (half) *other = gained;
+                if (side) asm volatile("bar.sync 3, %0;" ::"n"(WT_WORKERS / 2) : "memory");
+                else asm volatile("bar.sync 2, %0;" ::"n"(WT_WORKERS / 2) : "memory");
                 const int key = key0 + mine, page = mine < CML_PAGE ? page0 : page1;
                 if (!half && ok && key < last && page >= 0) {
                     const size_t at = ((size_t)page * a.kv_heads + kvh) * CML_PAGE + key % CML_PAGE;
-                    a.scores_out[at] = (key < s.old ? a.scores[at] : 0.f) + (gained + half_s[(t & 1) * 128 + mine]);
+                    a.scores_out[at] = (key < s.old ? a.scores[at] : 0.f) + (gained + *other);
                 }
             }
         }
-        if (!SUM) {
-            if (half) {
+        if (!SUM) {                                                           // the sides' and halves' keys together
+            const int who = warp >> 2;
+            if (who) {
 #pragma unroll
-                for (int r = 0; r < RT; ++r) rows_s[r * 128 + mine] = make_float4(top[r], sum[r], 0.f, 0.f);
+                for (int r = 0; r < RT; ++r) rows_s[((who - 1) * RT + r) * 128 + mine] = make_float2(top[r], sum[r]);
             }
             wt_workers_sync();
-            if (!half) {
+            if (!who) {
                 float* const out = a.stats + ((size_t)pair * a.n_splits + split) * group_rows * 2;
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
                     const int m = r * 128 + mine;
                     if (m >= s.rows) break;
-                    const float4 o = rows_s[m];
-                    const float most = fmaxf(top[r], o.x);
-                    float l = 0.f;
+                    float most = top[r], l = 0.f;
+#pragma unroll
+                    for (int w = 0; w < 3; ++w) most = fmaxf(most, rows_s[(w * RT + r) * 128 + mine].x);
                     if (top[r] != -CUDART_INF_F) l += fast_exp2(top[r] - most) * sum[r];
-                    if (o.x != -CUDART_INF_F) l += fast_exp2(o.x - most) * o.y;
+#pragma unroll
+                    for (int w = 0; w < 3; ++w) {
+                        const float2 o = rows_s[(w * RT + r) * 128 + mine];
+                        if (o.x != -CUDART_INF_F) l += fast_exp2(o.x - most) * o.y;
+                    }
                     *reinterpret_cast<float2*>(out + m * 2) = make_float2(most, l);
                 }
             }
@@ -361,9 +400,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
     }
     wt_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == WT_WORKERS / 32 + 1) {
         wt_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u * BUFS) : "memory");
     }
     if (threadIdx.x == 0 && *gave_up) atomicExch(err, 4);
 }
