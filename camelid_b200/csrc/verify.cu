@@ -417,15 +417,34 @@ struct RowStat {
     int bad;
 };
 
-// The parts of a row joined by a warp, the lanes in their order: the same in every lane.
-__device__ __forceinline__ RowStat join_parts(const VerifyArgs& a, int row, const double* table) {
+// The parts of a row joined by a warp, the lanes in their order: the same in every lane. The first 128 are asked for by
+// themselves, so that they come beside what else a decision reads.
+#define VF_AHEAD 4
+struct Parts {
+    PartStat s[VF_AHEAD];
+};
+__device__ __forceinline__ Parts load_parts(const VerifyArgs& a, int row) {
+    const PartStat* s = a.stats + (size_t)row * a.parts + (threadIdx.x & 31);
+    Parts r;
+#pragma unroll
+    for (int u = 0; u < VF_AHEAD; ++u)
+        if ((int)(threadIdx.x & 31) + 32 * u < a.parts) r.s[u] = s[32 * u];
+        else r.s[u] = {0.0, LOWEST, 0x7fffffff};                  // (no part: what is at the type's lowest anyway adds nothing of its own)
+    return r;
+}
+__device__ __forceinline__ RowStat join_parts(const VerifyArgs& a, int row, const Parts& first, const double* table) {
     const int lane = threadIdx.x & 31;
     const PartStat* s = a.stats + (size_t)row * a.parts;
     RowStat r;
     float mx = -CUDART_INF_F;
     int arg = 0x7fffffff;
     bool bad = false;
-    for (int p = lane; p < a.parts; p += 32) {
+#pragma unroll
+    for (int u = 0; u < VF_AHEAD; ++u) {
+        if (!finite(first.s[u].max)) bad = true;
+        if (first.s[u].max > mx) mx = first.s[u].max, arg = first.s[u].arg;
+    }
+    for (int p = lane + 32 * VF_AHEAD; p < a.parts; p += 32) {
         const float m = s[p].max;
         if (!finite(m)) bad = true;
         if (m > mx) mx = m, arg = s[p].arg;
@@ -440,7 +459,9 @@ __device__ __forceinline__ RowStat join_parts(const VerifyArgs& a, int row, cons
             const float* l = a.logits + (long long)row * a.ld;
             for (int i = lane; i < a.vocab; i += 32) r.total += l[i] == r.max ? 1.0 : 0.0;
         } else {
-            for (int p = lane; p < a.parts; p += 32) r.total += s[p].sum * weight_of(s[p].max, ex, table);
+#pragma unroll
+            for (int u = 0; u < VF_AHEAD; ++u) r.total += first.s[u].sum * weight_of(first.s[u].max, ex, table);
+            for (int p = lane + 32 * VF_AHEAD; p < a.parts; p += 32) r.total += s[p].sum * weight_of(s[p].max, ex, table);
             // LOWEST behind the row's end counts where the temperature is huge
             if (lane == 31 && a.floors == nullptr) r.total -= (a.parts * VF_PART - a.vocab) * weight_of(LOWEST, ex, table);
         }
@@ -452,14 +473,14 @@ __device__ __forceinline__ RowStat join_parts(const VerifyArgs& a, int row, cons
 
 // (2) a cluster per sequence.
 #define VF_ROWS 32                   // rows whose joined parts a block remembers
-#define VF_GROUPS 8
-// PER_SM: blocks that share a multiprocessor. Where all blocks run at the same time anyway, one with twice the registers is faster
-// (8 sequences of 4 drafts with filters 34.9 us for 41.2, one without 15.4 for 16.3); 64 sequences of 7 drafts take 127 us with
-// one and 104 with two.
-template <int PER_SM>
+#define VF_TEAM 16                   // blocks of a cluster at most
+// PER_SM: blocks that share a multiprocessor; one alone has the registers to ask for the next tiles ahead (8 sequences 18.9 us for
+// 23.4; 64 sequences of 7 drafts would take 127 us in several rounds, and take 96).
+// GROUPS: a warp's stretch is cut into as many, whose sums stay in registers.
+template <int PER_SM, int GROUPS>
 __global__ void __launch_bounds__(VF_THREADS, PER_SM) verify_decide_kernel(VerifyArgs a) {
     __shared__ double table[32];
-    __shared__ double warp_sums[2][VF_WARPS], block_sums[2][SAMPLE_MAX_TEAM];     // of two rounds
+    __shared__ double warp_sums[2][VF_WARPS], block_sums[2][VF_TEAM];     // of two rounds
     __shared__ RowStat stats[VF_ROWS];
     __shared__ int first_bad, row_bad, err_bits;
     fill_table(table);
@@ -484,7 +505,7 @@ __global__ void __launch_bounds__(VF_THREADS, PER_SM) verify_decide_kernel(Verif
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     // every draft by a warp of its own: is it accepted?
     for (int j = warp; j <= len; j += VF_WARPS) {
-        // what the decision reads beside the parts does not wait for them
+        const Parts parts = load_parts(a, row0 + j);              // what the decision reads beside them does not wait for them
         int x = 0;
         float q = 1.f, l = 0.f, u = 0.f;
         bool known = false;
@@ -497,7 +518,7 @@ __global__ void __launch_bounds__(VF_THREADS, PER_SM) verify_decide_kernel(Verif
                 l = a.logits[(long long)(row0 + j) * a.ld + x];
             }
         }
-        const RowStat r = join_parts(a, row0 + j, table);
+        const RowStat r = join_parts(a, row0 + j, parts, table);
         if (lane == 0) {
             if (j < VF_ROWS) stats[j] = r;
             int bits = r.bad ? VF_ERR_NONFINITE : (!greedy && !(r.total > 0.0) ? VF_ERR_EMPTY : 0);
@@ -524,7 +545,7 @@ __global__ void __launch_bounds__(VF_THREADS, PER_SM) verify_decide_kernel(Verif
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     const int count = row_bad ? 0 : min(first_bad, len);
     const int row = row0 + count;
-    const RowStat st = count < VF_ROWS ? stats[count] : join_parts(a, row, table);
+    const RowStat st = count < VF_ROWS ? stats[count] : join_parts(a, row, load_parts(a, row), table);
     if (rank == 0) {
         if (threadIdx.x == 0) {
             a.counts[seq] = count;
@@ -547,9 +568,9 @@ __global__ void __launch_bounds__(VF_THREADS, PER_SM) verify_decide_kernel(Verif
     const double inv_total = 1.0 / st.total;
     bool bad_q = false;
     bool plain = false;                                           // nothing is left of p - q: draw from p
-    // stretches of VF_GROUPS groups of whole tiles of 128 columns, a stretch a warp, in ascending order over the cluster's blocks
+    // stretches of GROUPS groups of whole tiles of 128 columns, a stretch a warp, in ascending order over the cluster's blocks
     const int warps = team * VF_WARPS;
-    const int group = (vocab + warps * VF_GROUPS * 128 - 1) / (warps * VF_GROUPS * 128) * 128, per = group * VF_GROUPS;
+    const int group = (vocab + warps * GROUPS * 128 - 1) / (warps * GROUPS * 128) * 128, per = group * GROUPS;
     const long long first = (long long)(rank * VF_WARPS + warp) * per;
     const int begin = (int)min((long long)vocab, first), end = (int)min((long long)vocab, first + per);
     const bool vec = (((uintptr_t)r) & 15) == 0 && (q == nullptr || (((uintptr_t)q) & 15) == 0);
@@ -579,24 +600,35 @@ __global__ void __launch_bounds__(VF_THREADS, PER_SM) verify_decide_kernel(Verif
         }
     };
     double total = 0.0, target, before = 0.0;
-    double groups[VF_GROUPS];                                     // this lane's share of every group's sum
+    double groups[GROUPS];                                     // this lane's share of every group's sum
     int owner = -1, round = 0;
     for (; round < 2; ++round) {
         double s = 0.0;
+        constexpr bool AHEAD = PER_SM == 1;                       // two groups' tiles at a time; the next two on their way where registers allow
+        float l0[4], l1[4], q0[4] = {0.f, 0.f, 0.f, 0.f}, q1[4] = {0.f, 0.f, 0.f, 0.f};
+        auto load_two = [&](int i0, float (&l0)[4], float (&l1)[4], float (&q0)[4], float (&q1)[4]) {       // (behind the row: nothing)
+            load4(r, i0, l0);
+            load4(r, i0 + group, l1);
+            if (q) load4(q, i0, q0), load4(q, i0 + group, q1);
+        };
+        if (AHEAD) load_two(begin + 4 * lane, l0, l1, q0, q1);
 #pragma unroll
-        for (int g = 0; g < VF_GROUPS; g += 2) {                  // two groups in flight
+        for (int g = 0; g < GROUPS; g += 2) {
             double s0 = 0.0, s1 = 0.0;
             for (int i = 0; i < group; i += 128) {
-                const int i0 = begin + g * group + i + 4 * lane, i1 = i0 + group;
-                float l0[4], l1[4], q0[4] = {0.f, 0.f, 0.f, 0.f}, q1[4] = {0.f, 0.f, 0.f, 0.f};
-                load4(r, i0, l0);
-                load4(r, i1, l1);
-                if (q) load4(q, i0, q0), load4(q, i1, q1);
+                const int i0 = begin + g * group + i + 4 * lane;
+                float nl0[4], nl1[4], nq0[4] = {0.f, 0.f, 0.f, 0.f}, nq1[4] = {0.f, 0.f, 0.f, 0.f};
+                if (AHEAD) load_two(i + 128 < group ? i0 + 128 : begin + (g + 2) * group + 4 * lane, nl0, nl1, nq0, nq1);
+                else load_two(i0, l0, l1, q0, q1);
                 double w[4];
                 weigh(i0, l0, q0, w);
                 s0 += (w[0] + w[1]) + (w[2] + w[3]);
-                weigh(i1, l1, q1, w);
+                weigh(i0 + group, l1, q1, w);
                 s1 += (w[0] + w[1]) + (w[2] + w[3]);
+                if (AHEAD) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) l0[k] = nl0[k], l1[k] = nl1[k], q0[k] = nq0[k], q1[k] = nq1[k];
+                }
             }
             groups[g] = s0, groups[g + 1] = s1;
             s += s0 + s1;
@@ -640,11 +672,22 @@ __global__ void __launch_bounds__(VF_THREADS, PER_SM) verify_decide_kernel(Verif
             // the group of the crossing from the sums in registers, then its columns
             int in = -1;
             run = before;
+            // (the groups' sums over the lanes: every exchange halves what a lane holds, 32 / GROUPS lanes have one group's in the end)
 #pragma unroll
-            for (int g = 0; g < VF_GROUPS; ++g) {
-                double s = groups[g];
+            for (int o = 16, n = GROUPS / 2; n > 0; o >>= 1, n >>= 1) {
+                const bool high = (lane & o) != 0;
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                for (int g = 0; g < GROUPS / 2; ++g) {
+                    if (g >= n) break;
+                    const double away = high ? groups[g] : groups[g + n], here = high ? groups[g + n] : groups[g];
+                    groups[g] = here + __shfl_xor_sync(0xffffffffu, away, o);
+                }
+            }
+#pragma unroll
+            for (int o = 16 / GROUPS; o > 0; o >>= 1) groups[0] += __shfl_xor_sync(0xffffffffu, groups[0], o);
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                const double s = __shfl_sync(0xffffffffu, groups[0], g * (32 / GROUPS));
                 if (s > 0.0 && (in < 0 || !(run > target))) in = g, before = run;
                 run += s;
             }
@@ -752,8 +795,23 @@ extern "C" int cml_verify_drafts(const float* logits, long long ld, int n_rows, 
         if (e != cudaSuccess) return (int)e;
     }
     while (team > 1 && n_seqs * team > 2 * cml_sm_count()) team /= 2;          // one round of blocks, two a multiprocessor (64 sequences: 98 us for 104)
-    const cudaError_t e = n_seqs * team <= cml_sm_count() ? launch_cluster(verify_decide_kernel<1>, n_seqs * team, VF_THREADS, 0, team, s, a)
-                                                          : launch_cluster(verify_decide_kernel<2>, n_seqs * team, VF_THREADS, 0, team, s, a);
+    // Where all clusters find room at the same time, a multiprocessor for every block (of clusters of eight 15 do: 15 sequences of
+    // 128,256 tokens 24.6 us for 30.1, 16 would take 34.1 for 31.2).
+    const bool alone = n_seqs * team <= (team < 8 ? cml_sm_count() : cml_sm_count() * 5 / 6);
+    cudaError_t e;
+    if (vocab >= 65536 && n_seqs <= 4) {
+        // few sequences: sixteen blocks each (one of 128,256 tokens 9.4 us for 11.8), which have to be asked for once
+        static bool allowed = false;
+        e = allowed ? cudaSuccess : cudaFuncSetAttribute(verify_decide_kernel<1, 4>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        allowed = e == cudaSuccess;
+        if (allowed) e = launch_cluster(verify_decide_kernel<1, 4>, n_seqs * VF_TEAM, VF_THREADS, 0, VF_TEAM, s, a);
+    } else if (alone && vocab <= team * VF_WARPS * 512) {         // four groups are enough (50,257 tokens: 9.5 us for 12.2 with eight)
+        e = launch_cluster(verify_decide_kernel<1, 4>, n_seqs * team, VF_THREADS, 0, team, s, a);
+    } else if (alone) {
+        e = launch_cluster(verify_decide_kernel<1, 8>, n_seqs * team, VF_THREADS, 0, team, s, a);
+    } else {
+        e = launch_cluster(verify_decide_kernel<2, 8>, n_seqs * team, VF_THREADS, 0, team, s, a);
+    }
     if (e != cudaSuccess) return (int)e;
     return cml_launch_status();
 }
