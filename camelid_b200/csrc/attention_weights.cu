@@ -9,8 +9,18 @@
 //
 // The weights of a key are known only when all keys are seen, so the work is cut in three: (1) blocks take stretches of
 // a sequence's keys and keep the running maximum, sum and output of their rows; (2) the stretches are joined, in order;
-// (3) the products q . k are made again and every key's weights summed, in a fixed order of the rows. Products,
-// softmax and sums are float.
+// (3) every key's weights are summed, in a fixed order of the rows. Steps of few rows (a single token, a drafted step) do all
+// three in one launch: the blocks of a cluster share a sequence and kv head, exchange their rows' maxima and sums over distributed
+// shared memory, and weigh the products q . k again that they kept (4 bytes a row and key, which stay in L2). More rows make
+// the products again in a kernel of their own; without output (a prompt's last rows) on tcgen05 (attention_weights_tc.cuh).
+// Products, softmax and sums are float; on the tensor cores a probability is rounded to bfloat16 where it meets a value, as
+// the values are: the sum over the keys has half a step of each product (2^-8 of it), beside which the output's own rounding is
+// as large (16 sequences of 24,001 to 32,768 keys: 0.0021 from 64 bits in norm, 0.0017 with probabilities in float).
+//
+// Bound by memory where sequences are long: 16 of 24,001 to 32,768 keys with 8 kv heads of 128 (1.9 GB) take 340 us, 5.6 TB/s
+// of 6.6 that a copy reaches; 8 of 300 to 8,191 34.5 us (4.1 TB/s: unequal lengths, and 4 us of joining and weighing at the end);
+// short ones by the launch (12 us a call on the host, 6 on the device for 517 keys). In float: 4 sequences of 700 to 2,047 keys, heads of
+// 96, 20.8 us for 17 MB (a page is worked on in four phases between barriers, 4 us a page; only one page is on its way meanwhile).
 #include "common.cuh"
 #include <cooperative_groups.h>
 #include <math_constants.h>
@@ -829,169 +839,7 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
     if (OUT) cg::this_cluster().sync();                                       // a block's output stays until every block has read it
 }
 
-// (1) without output, for many rows (a prompt's last ones): a warp keeps 64 rows of q in registers and lets the keys pass;
-// grid (stretches, pairs, row chunks). The block's warps share the rows (`row_warps` of them) and the 16-key pieces of
-// a page. A thread keeps a maximum and a sum of its own for each of its eight rows, the maximum moves only when it is passed
-// by a factor of 2^6, and lanes and warps meet at the end. The exponentials (one a row and key) bound this kernel.
 #define AR_WARPS 4
-#define AR_STAGES 4
-template <int HD>
-__global__ void __launch_bounds__(AR_WARPS * 32, 2) weights_rows_mma_kernel(WeightArgs a, int row_warps) {
-    constexpr int LDS = HD + 8, KS = HD / 16, CH = HD / 8, STAGE = CML_PAGE * LDS * 2;
-    extern __shared__ __align__(16) unsigned char raw[];
-    pdl_wait();
-    pdl_launch_dependents();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int split = blockIdx.x, seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y % a.kv_heads;
-    const int m0 = ((int)blockIdx.z * row_warps + warp % row_warps) * 64, key_group = warp / row_warps, key_groups = AR_WARPS / row_warps;
-    const Seq s = seq_of(a, seq);
-    const int first = split * a.split_keys, last = min(s.length, first + a.split_keys);
-    if (first >= last || (int)blockIdx.z * row_warps * 64 >= s.rows) return;
-    const int group = a.heads / a.kv_heads, group_rows = a.max_new * group;
-    const int* pages = a.table + (size_t)seq * a.width;
-    const uint32_t raw32 = (uint32_t)__cvta_generic_to_shared(raw);
-    const int p_first = first / CML_PAGE, p_last = (last + CML_PAGE - 1) / CML_PAGE;
-    auto valid_of = [&](int p) {
-        const int page = pages[p];
-        return page < 0 || page >= a.n_pages ? 0 : min(CML_PAGE, last - p * CML_PAGE);
-    };
-    auto issue = [&](int p) {
-        if (p < p_last) {
-            const int valid = valid_of(p);
-            const bf16* src = (const bf16*)a.k + ((size_t)(valid ? pages[p] : 0) * a.kv_heads + kvh) * CML_PAGE * HD;
-            const uint32_t dst = raw32 + (uint32_t)((p - p_first) % AR_STAGES) * STAGE;
-#pragma unroll
-            for (int c0 = 0; c0 < CML_PAGE * CH; c0 += AR_WARPS * 32) {
-                const int c = c0 + threadIdx.x, r = c / CH, cc = c % CH;
-                cp_async16_or_zero(dst + (uint32_t)(r * LDS + cc * 8) * 2, src + (size_t)r * HD + cc * 8, r < valid);
-            }
-        }
-        cp_async_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < AR_STAGES - 1; ++i) issue(p_first + i);
-    uint32_t qa[4][KS][4];
-    int pos[4][2];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int m = m0 + mt * 16 + (lane >> 2) + 8 * h;
-            const bool in = m < s.rows;
-            const int j = in ? m / group : 0;
-            pos[mt][h] = in ? s.start + j : -1;
-            const bf16* qr = (const bf16*)a.q + (long long)(s.row0 + j) * a.q_stride + (long long)(kvh * group + (in ? m % group : 0)) * HD + 2 * (lane & 3);
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                qa[mt][ks][h] = in ? *reinterpret_cast<const uint32_t*>(qr + ks * 16) : 0u;
-                qa[mt][ks][h + 2] = in ? *reinterpret_cast<const uint32_t*>(qr + ks * 16 + 8) : 0u;
-            }
-        }
-    float top[4][2], sum[4][2];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) top[mt][0] = top[mt][1] = -CUDART_INF_F, sum[mt][0] = sum[mt][1] = 0.f;
-    const int mat = lane >> 3, rr = lane & 7;
-    const bool any_rows = m0 < s.rows;
-    for (int p = p_first; p < p_last; ++p) {
-        cp_async_wait<AR_STAGES - 2>();
-        __syncthreads();
-        issue(p + AR_STAGES - 1);
-        if (!any_rows) continue;
-        const int valid = valid_of(p);
-        const uint32_t k32 = raw32 + (uint32_t)((p - p_first) % AR_STAGES) * STAGE;
-        const bool whole = valid == CML_PAGE && p * CML_PAGE + CML_PAGE - 1 <= s.start;      // every row sees every key
-        for (int c = key_group; c < CML_PAGE / 16; c += key_groups) {
-            float x[4][2][4];
-#pragma unroll
-            for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-                for (int n = 0; n < 2; ++n) x[mt][n][0] = x[mt][n][1] = x[mt][n][2] = x[mt][n][3] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                uint32_t b0, b1, b2, b3;
-                ldsm_x4(k32 + (uint32_t)((c * 16 + (mat >> 1) * 8 + rr) * LDS + ks * 16 + (mat & 1) * 8) * 2, b0, b1, b2, b3);
-#pragma unroll
-                for (int mt = 0; mt < 4; ++mt) {
-                    mma_bf16(x[mt][0], qa[mt][ks], b0, b1);
-                    mma_bf16(x[mt][1], qa[mt][ks], b2, b3);
-                }
-            }
-            if (!whole) {
-                const int at = c * 16 + 2 * (lane & 3);
-#pragma unroll
-                for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int key = at + n * 8 + (i & 1);
-                            if (!(key < valid && p * CML_PAGE + key <= pos[mt][i >> 1])) x[mt][n][i] = -CUDART_INF_F;
-                        }
-            }
-            bool passed = false;
-            float now[4][2];
-#pragma unroll
-            for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float hi = fmaxf(fmaxf(x[mt][0][2 * h], x[mt][0][2 * h + 1]), fmaxf(x[mt][1][2 * h], x[mt][1][2 * h + 1]));
-                    now[mt][h] = hi * a.scale;
-                    passed = passed || now[mt][h] > top[mt][h] + 6.f;
-                }
-            if (__any_sync(0xffffffffu, passed)) {
-#pragma unroll
-                for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float next = fmaxf(top[mt][h], now[mt][h]);
-                        if (next != -CUDART_INF_F) sum[mt][h] *= fast_exp2(top[mt][h] - next);
-                        top[mt][h] = next;
-                    }
-            }
-#pragma unroll
-            for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float ref = top[mt][h] == -CUDART_INF_F ? 0.f : top[mt][h];
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) sum[mt][h] += fast_exp2(fmaf(x[mt][n][2 * h + i], a.scale, -ref));
-                }
-        }
-    }
-    cp_async_wait<0>();
-    __syncthreads();                                                          // the ring is free: the warps' results take its place
-    float2* red = reinterpret_cast<float2*>(raw);                             // [warps][64 rows]
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float t = top[mt][h], l = sum[mt][h];
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                const float t2 = __shfl_xor_sync(0xffffffffu, t, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
-                const float most = fmaxf(t, t2);
-                if (most != -CUDART_INF_F) l = l * fast_exp2(t - most) + l2 * fast_exp2(t2 - most);
-                t = most;
-            }
-            if ((lane & 3) == 0) red[warp * 64 + mt * 16 + (lane >> 2) + 8 * h] = make_float2(t, l);
-        }
-    __syncthreads();
-    const size_t base = ((size_t)blockIdx.y * a.n_splits + split) * group_rows;
-    for (int i = threadIdx.x; i < row_warps * 64; i += AR_WARPS * 32) {
-        const int m = (int)blockIdx.z * row_warps * 64 + i;
-        if (m >= s.rows) break;
-        float t = -CUDART_INF_F, l = 0.f;
-        for (int w = 0; w < key_groups; ++w) t = fmaxf(t, red[(w * row_warps + i / 64) * 64 + i % 64].x);
-        for (int w = 0; w < key_groups; ++w) {
-            const float2 one = red[(w * row_warps + i / 64) * 64 + i % 64];
-            if (one.x != -CUDART_INF_F) l += fast_exp2(one.x - t) * one.y;
-        }
-        *reinterpret_cast<float2*>(a.stats + (base + m) * 2) = make_float2(t, l);
-    }
-}
-
 // (3) for more than 16 rows: a warp keeps 64 keys in registers as the operand of 16 rows and lets the rows of q pass, so that a
 // key's sum over the rows stays in one quad of lanes, in the order of the rows. Grid (256 keys, pairs).
 #define AC_ROWS 32              // rows of q in a stage
@@ -1197,9 +1045,6 @@ static cudaError_t launch_all(const WeightArgs& a, unsigned pairs, int team, siz
 
 #include "attention_weights_tc.cuh"
 
-// Rows of a kv head from which their weights alone are made on tcgen05 (up to 512), and the same as the plan of the scratch says.
-#define AW_TC_ROWS 64
-
 template <int HD>
 static cudaError_t launch_mma(const WeightArgs& a, int* err, cudaStream_t s) {
     constexpr int TILE = HD == 128 ? 16 : 32;
@@ -1219,22 +1064,14 @@ static cudaError_t launch_mma(const WeightArgs& a, int* err, cudaStream_t s) {
         if (rows <= 16) return a.out ? launch_all<HD, 1, true>(a, pairs, team, 2 * ring, s) : launch_all<HD, 1, false>(a, pairs, team, ring, s);
         return a.out ? launch_all<HD, 2, true>(a, pairs, team, 2 * ring, s) : launch_all<HD, 2, false>(a, pairs, team, ring, s);
     }
-    if (a.out == nullptr && err != nullptr && rows >= AW_TC_ROWS && rows <= 512 &&
-        (long long)a.n_pages * a.kv_heads * CML_PAGE <= 0x7fffffffLL)
-        return launch_tc<HD>(a, err, s);
-    if (a.out) {
-        e = cml_allow_smem<weights_part_mma_kernel<HD, 2, true, false>>(2 * ring);
-        if (e == cudaSuccess)
-            e = launch_pdl(weights_part_mma_kernel<HD, 2, true, false>, dim3((unsigned)a.n_splits, pairs, (unsigned)((rows + 31) / 32)),
-                           dim3(AM_WARPS * 32), 2 * ring, s, a);
-    } else {
-        const int row_warps = rows <= 64 ? 1 : (rows <= 128 ? 2 : 4);
-        constexpr size_t smem = (size_t)AR_STAGES * CML_PAGE * (HD + 8) * 2;
-        e = cml_allow_smem<weights_rows_mma_kernel<HD>>(smem);
-        if (e == cudaSuccess)
-            e = launch_pdl(weights_rows_mma_kernel<HD>, dim3((unsigned)a.n_splits, pairs, (unsigned)((rows + 64 * row_warps - 1) / (64 * row_warps))),
-                           dim3(AR_WARPS * 32), smem, s, a, row_warps);
-    }
+    // Without output and beyond the rows whose products are kept: tcgen05, in two launches (four sequences of 4,000 keys, 8 kv heads of
+    // 128: 27.9 us whatever the rows up to 128; the one launch above takes 26.2 with 32 rows, 14.3 with 8, and its split form, which
+    // stood here, 56 with 36 and 94 with 128).
+    if (a.out == nullptr) return launch_tc<HD>(a, err, s);
+    e = cml_allow_smem<weights_part_mma_kernel<HD, 2, true, false>>(2 * ring);
+    if (e == cudaSuccess)
+        e = launch_pdl(weights_part_mma_kernel<HD, 2, true, false>, dim3((unsigned)a.n_splits, pairs, (unsigned)((rows + 31) / 32)), dim3(AM_WARPS * 32),
+                       2 * ring, s, a);
     if (e != cudaSuccess) return e;
     e = launch_pdl(weights_join_kernel<bf16>, dim3((unsigned)rows, pairs), dim3(AW_THREADS), 0, s, a);
     if (e != cudaSuccess) return e;
@@ -1275,6 +1112,7 @@ extern "C" int cml_attn_paged_weights(const void* q, int dtype, long long q_stri
     // the tensor cores take rows of q that begin on 16 bytes
     const bool mma = dtype == CML_DTYPE_BF16 && (k_dim == 64 || k_dim == 128) && (out == nullptr || v_dim == k_dim) &&
                      (((uintptr_t)q) & 15) == 0 && q_stride % 8 == 0;
+    if (mma && out == nullptr && (err == nullptr || (long long)n_pages * kv_heads * CML_PAGE > 0x7fffffffLL)) return CML_ERR_BAD_SIZE;      // rows of TMA's matrix
     cudaStream_t s = (cudaStream_t)stream;
     const cudaError_t e = mma ? (k_dim == 64 ? launch_mma<64>(a, err, s) : launch_mma<128>(a, err, s))
                               : (dtype == CML_DTYPE_F32 ? launch_plain<float>(a, s) : launch_plain<bf16>(a, s));

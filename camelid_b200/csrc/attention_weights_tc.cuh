@@ -2,16 +2,19 @@
 // Included by attention_weights.cu, whose arguments it takes.
 //
 // Both passes are one kernel. The rows of q stay in shared memory (up to 512 of them), the keys pass by in tiles of 128 that TMA
-// brings from the pages, and every (tile, 128 rows) is one product of 128 x 128 in tensor memory. Two sides of four warps take the
-// tiles in turn, so that one side's exponentials run beside the other's reads and maxima (both on halves of one tile: 58 and 66 us
-// for the two passes over four prompts of 9,001 to 16,384 keys, TODO).
+// brings from the pages, and every (tile, 128 rows) is one product of 128 x 128 in tensor memory, of which four are in flight.
 //
-//   SUM false: S = Q K^T, a thread a row: its running maximum and sum over its side's tiles of a stretch of keys
-//   SUM true:  S = K Q^T, a thread a key: the sum of its weights 2^(s - max - log2 sum) over the rows, in registers; the
-//              stretches' statistics are joined by every block for itself
+//   SUM false: S = Q K^T, a thread a row (and half of a tile's keys): its running maximum and sum over a stretch of keys
+//   SUM true:  S = K Q^T, a thread a key (and half of the rows): the sum of its weights 2^(s - max - log2 sum) over the rows,
+//              in registers; the stretches' statistics are joined by every block for itself
 //
-// One exponential a row and key in each pass bounds the kernel (16 a cycle and multiprocessor): a product of 128 x 128 x 128 takes
-// half as long. Eight warps of exponentials, one that brings keys, one that issues products.
+// Sixteen warps of exponentials, in two sides that take the tiles in turn, one warp that brings keys, one that issues products.
+// With eight warps on halves of one tile, all were in the same phase and the exponentials' unit idled half of the time. Measured
+// over 64 rows (256 with their heads) of four prompts of 9,001 to 16,384 keys and 8 kv heads: 300 us on mma.sync, 145 with eight
+// warps here, 119 with stretches of equal work, 94 with sixteen warps and a ring as deep as shared memory allows. What bounds it:
+// the exponentials of both passes take 48 us (16 a cycle and multiprocessor), the products, whose two operands pass through
+// shared memory, 57 without them, the start of both kernels 21 (the passes alone, without exponentials and maxima, take 78 us,
+// with exponentials and one product in eight 84).
 #pragma once
 #include <cuda.h>
 
@@ -108,9 +111,13 @@ template <int HD, int RT> struct WtPlan {
 struct WtShare {
     int seq, split, tiles, splits;             // tiles: of a stretch; splits: stretches of the sequence
 };
-__device__ __forceinline__ WtShare wt_share(const WeightArgs& a, int block, int blocks) {        // by a whole warp, the same in every lane
+__device__ __forceinline__ WtShare wt_share(const WeightArgs& a, int m0, int block, int blocks) {        // by a whole warp, the same in every lane
     const int lane = threadIdx.x & 31;
-    auto look_up = [&](int i) { return i < a.n_seqs ? (seq_of(a, i).length + WT_KEYS - 1) / WT_KEYS : 0; };
+    auto look_up = [&](int i) {
+        if (i >= a.n_seqs) return 0;
+        const Seq s = seq_of(a, i);
+        return m0 < s.rows ? (s.length + WT_KEYS - 1) / WT_KEYS : 0;
+    };
     const int own = look_up(lane);             // the first 32 sequences are looked up once
     auto tiles_of = [&](int i) { return i < 32 ? own : look_up(i); };
     int total = 0;
@@ -148,9 +155,9 @@ __device__ __forceinline__ WtShare wt_share(const WeightArgs& a, int block, int 
     return w;
 }
 
-// grid (blocks of a kv head, kv heads). RT: tiles of 128 rows.
+// grid (blocks of a kv head, kv heads). RT: tiles of 128 rows, from row m0 of a sequence on.
 template <int HD, int RT, bool SUM>
-__global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_constant__ CUtensorMap map, WeightArgs a, int* err) {
+__global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_constant__ CUtensorMap map, WeightArgs a, int m0, int* err) {
     using P = WtPlan<HD, RT>;
     constexpr int KB = P::KB, STAGES = P::STAGES, BUFS = P::BUFS;
     constexpr uint32_t TILE = P::TILE, BLOCK = 128u * 128u;
@@ -173,14 +180,14 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     pdl_launch_dependents();
-    const WtShare share = wt_share(a, blockIdx.x, gridDim.x);                 // every warp for itself
+    const WtShare share = wt_share(a, m0, blockIdx.x, gridDim.x);                 // every warp for itself
     if (share.seq < 0) return;                                                // more blocks than stretches: the same for the whole block
     const int split = share.split, seq = share.seq, kvh = blockIdx.y, pair = seq * a.kv_heads + kvh;
     const Seq s = seq_of(a, seq);
     const int first = split * share.tiles * WT_KEYS, last = min(s.length, first + share.tiles * WT_KEYS);
     const int group = a.heads / a.kv_heads, group_rows = a.max_new * group;
     const int n_tiles = (last - first + WT_KEYS - 1) / WT_KEYS;
-    const int row_tiles = (s.rows + 127) / 128;                               // at most RT
+    const int rows = min(s.rows - m0, RT * 128), row_tiles = (rows + 127) / 128;
     const int* const pages = a.table + (size_t)seq * a.width;
     auto page_at = [&](int key) {                                             // the page of a key of this stretch, -1: none
         const int page = key < last ? pages[key / CML_PAGE] : -1;
@@ -256,9 +263,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
         constexpr int ROW = KB * 8;                                           // 16-byte pieces of a row
         const int piece = threadIdx.x % ROW, x0 = threadIdx.x / ROW;
         for (int m = x0; m < row_tiles * 128; m += WT_WORKERS / ROW) {
-            const bool in = m < s.rows;
-            const int j = in ? m / group : 0;
-            const bf16* src = (const bf16*)a.q + (long long)(s.row0 + j) * a.q_stride + (long long)(kvh * group + (in ? m - j * group : 0)) * HD + piece * 8;
+            const bool in = m < rows;
+            const int j = in ? (m0 + m) / group : 0;
+            const bf16* src = (const bf16*)a.q + (long long)(s.row0 + j) * a.q_stride + (long long)(kvh * group + (in ? m0 + m - j * group : 0)) * HD + piece * 8;
             const int r = m % 128;
             cp_async16_or_zero(sQ + (m / 128) * TILE + (piece / 8) * BLOCK + (r >> 3) * 1024 + (r & 7) * 128 + (((piece & 7) ^ (r & 7)) << 4), src, in);
         }
@@ -267,8 +274,8 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
             const int splits = share.splits;
             for (int m = threadIdx.x; m < RT * 128; m += WT_WORKERS) {
                 float top = -CUDART_INF_F, sum = 0.f;
-                if (m < s.rows) {
-                    const float* st = a.stats + ((size_t)pair * a.n_splits * group_rows + m) * 2;
+                if (m < rows) {
+                    const float* st = a.stats + ((size_t)pair * a.n_splits * group_rows + m0 + m) * 2;
                     for (int i0 = 0; i0 < splits; i0 += 8) {                  // eight at a time, which are asked for at once
                         float2 x[8];
 #pragma unroll
@@ -285,7 +292,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
                     }
                 }
                 ref_s[m] = top == -CUDART_INF_F ? CUDART_INF_F : top + log2f(sum);
-                place_s[m] = m < s.rows ? s.start + m / group : -1;
+                place_s[m] = m < rows ? s.start + (m0 + m) / group : -1;
             }
         }
         cp_async_wait<0>();
@@ -323,7 +330,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
                 if (lane == 0) wt_arrive(s_empty(buf));                       // read: the next product may come
                 if (!SUM) {                                                   // this thread's row, the keys of one page
                     if (!whole) {
-                        const int seen = (half ? page1 : page0) < 0 ? -1 : min(last - 1, s.start + (rt * 128 + mine) / group) - key0 - half * 64;
+                        const int seen = (half ? page1 : page0) < 0 ? -1 : min(last - 1, s.start + (m0 + rt * 128 + mine) / group) - key0 - half * 64;
 #pragma unroll
                         for (int i = 0; i < 64; ++i) x[i] = i <= seen ? x[i] : -CUDART_INF_F;
                     }
@@ -343,7 +350,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
 #pragma unroll
                     for (int i = 0; i < 64; ++i) part[i & 3] += fast_exp2(fmaf(x[i], a.scale, -ref));
                     sum[rt] += (part[0] + part[1]) + (part[2] + part[3]);
-                } else if (whole && rt * 128 + half * 64 + 64 <= s.rows) {    // this thread's key, 64 rows
+                } else if (whole && rt * 128 + half * 64 + 64 <= rows) {    // this thread's key, 64 rows
 #pragma unroll
                     for (int i = 0; i < 64; i += 4) {
                         const float4 ref = *reinterpret_cast<const float4*>(ref_s + rt * 128 + half * 64 + i);
@@ -367,7 +374,8 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
                 const int key = key0 + mine, page = mine < CML_PAGE ? page0 : page1;
                 if (!half && ok && key < last && page >= 0) {
                     const size_t at = ((size_t)page * a.kv_heads + kvh) * CML_PAGE + key % CML_PAGE;
-                    a.scores_out[at] = (key < s.old ? a.scores[at] : 0.f) + (gained + *other);
+                    const float old = m0 ? a.scores_out[at] : key < s.old ? a.scores[at] : 0.f;      // (earlier rows' weights are there)
+                    a.scores_out[at] = old + (gained + *other);
                 }
             }
         }
@@ -379,11 +387,11 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
             }
             wt_workers_sync();
             if (!who) {
-                float* const out = a.stats + ((size_t)pair * a.n_splits + split) * group_rows * 2;
+                float* const out = a.stats + (((size_t)pair * a.n_splits + split) * group_rows + m0) * 2;
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
                     const int m = r * 128 + mine;
-                    if (m >= s.rows) break;
+                    if (m >= rows) break;
                     float most = top[r], l = 0.f;
 #pragma unroll
                     for (int w = 0; w < 3; ++w) most = fmaxf(most, rows_s[(w * RT + r) * 128 + mine].x);
@@ -420,16 +428,16 @@ static WtEncode wt_encode() {
 }
 
 template <int HD, int RT>
-static cudaError_t launch_tc_rows(const CUtensorMap& map, const WeightArgs& a, int* err, cudaStream_t s) {
+static cudaError_t launch_tc_rows(const CUtensorMap& map, const WeightArgs& a, int m0, int* err, cudaStream_t s) {
     constexpr size_t smem = WtPlan<HD, RT>::SMEM;
     cudaError_t e = cml_allow_smem<weights_tc_kernel<HD, RT, false>>(smem);
     if (e == cudaSuccess) e = cml_allow_smem<weights_tc_kernel<HD, RT, true>>(smem);
     if (e != cudaSuccess) return e;
     // one block for every multiprocessor in all, one for every sequence at least; n_splits of a sequence at most, so that the others have one
     const dim3 grid((unsigned)(a.n_splits + a.n_seqs - 1), (unsigned)a.kv_heads);
-    e = launch_pdl(weights_tc_kernel<HD, RT, false>, grid, dim3(WT_THREADS), smem, s, map, a, err);
+    e = launch_pdl(weights_tc_kernel<HD, RT, false>, grid, dim3(WT_THREADS), smem, s, map, a, m0, err);
     if (e != cudaSuccess) return e;
-    return launch_pdl(weights_tc_kernel<HD, RT, true>, grid, dim3(WT_THREADS), smem, s, map, a, err);
+    return launch_pdl(weights_tc_kernel<HD, RT, true>, grid, dim3(WT_THREADS), smem, s, map, a, m0, err);
 }
 
 template <int HD>
@@ -442,6 +450,12 @@ static cudaError_t launch_tc(const WeightArgs& a, int* err, cudaStream_t s) {
     if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(a.k), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaErrorInvalidValue;
+    // up to 512 rows at a time: as many as shared memory holds beside the keys
     const int rows = a.max_new * (a.heads / a.kv_heads);
-    return rows <= 128 ? launch_tc_rows<HD, 1>(map, a, err, s) : rows <= 256 ? launch_tc_rows<HD, 2>(map, a, err, s) : launch_tc_rows<HD, 4>(map, a, err, s);
+    cudaError_t e = cudaSuccess;
+    for (int m0 = 0; m0 < rows && e == cudaSuccess; m0 += 512) {
+        const int left = rows - m0;
+        e = left <= 128 ? launch_tc_rows<HD, 1>(map, a, m0, err, s) : left <= 256 ? launch_tc_rows<HD, 2>(map, a, m0, err, s) : launch_tc_rows<HD, 4>(map, a, m0, err, s);
+    }
+    return e;
 }

@@ -2026,7 +2026,6 @@ def draws_at(positions: torch.Tensor, seed: torch.Tensor, draws: torch.Tensor):
 # ---------------------------------------------------------------------------------------
 # between two steps: which positions the cache keeps, which drafted tokens stay
 
-ATTN_WEIGHTS_TC_ROWS = 64, 512  # rows of a kv head whose weights alone are made on tcgen05; AW_TC_ROWS in attention_weights.cu
 ATTN_WEIGHTS_KEPT_ROWS = 32     # rows of a kv head up to which the products q . k are kept for the weights
 
 
@@ -2037,13 +2036,13 @@ def attn_weights_plan(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int,
     the blocks fill the device, none shorter than four pages. Made from sizes alone, without a device."""
     pairs, rows = max(1, n_seqs) * n_kv_heads, max_new * (n_heads // n_kv_heads)
     fast = dtype == torch.bfloat16 and head_dim in (64, 128) and value_dim == head_dim
-    if fast and not with_output and ATTN_WEIGHTS_TC_ROWS[0] <= rows <= ATTN_WEIGHTS_TC_ROWS[1]:
+    if fast and not with_output and rows > ATTN_WEIGHTS_KEPT_ROWS:
         # tcgen05: the kernel cuts all sequences into stretches of one length itself, for a block of every multiprocessor; a
         # sequence has as many as the others leave it
         splits = max(1, min(SMS // n_kv_heads - max(1, n_seqs) + 1, (max_len + 127) // 128))
         split_keys = ((max_len + splits - 1) // splits + PAGE - 1) // PAGE * PAGE
     else:
-        together = 8 if not fast else 32 if with_output else 256                          # rows a block works on together
+        together = 32 if fast else 8                                                      # rows a block works on together
         blocks = pairs * ((rows + together - 1) // together)
         splits = max(1, min((4 * SMS + blocks - 1) // blocks, (max_len + 4 * PAGE - 1) // (4 * PAGE)))
         split_keys = (((max_len + splits - 1) // splits + PAGE - 1) // PAGE) * PAGE
