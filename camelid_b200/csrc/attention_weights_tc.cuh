@@ -120,18 +120,22 @@ __device__ __forceinline__ WtShare wt_share(const WeightArgs& a, int m0, int blo
     };
     const int own = look_up(lane);             // the first 32 sequences are looked up once
     auto tiles_of = [&](int i) { return i < 32 ? own : look_up(i); };
-    int total = 0;
-    for (int i = lane; i < a.n_seqs; i += 32) total += tiles_of(i);
+    int total = 0, longest = 0;
+    for (int i = lane; i < a.n_seqs; i += 32) {
+        const int k = tiles_of(i);
+        total += k, longest = max(longest, k);
+    }
     total = __reduce_add_sync(0xffffffffu, total);
-    int tiles = max(1, (total + blocks - 1) / blocks);
-    while (true) {                             // ends: stretches as long as the longest sequence make one of each
+    int tiles = max(1, (total + blocks - 1) / blocks), most_tiles = max(tiles, __reduce_max_sync(0xffffffffu, longest));
+    while (tiles < most_tiles) {               // halved: stretches as long as the longest sequence, one of each, always fit
+        const int half = (tiles + most_tiles) / 2;
         int n = 0, most = 0;
         for (int i = lane; i < a.n_seqs; i += 32) {
-            const int k = (tiles_of(i) + tiles - 1) / tiles;
+            const int k = (tiles_of(i) + half - 1) / half;
             n += k, most = max(most, k);
         }
-        if (__reduce_add_sync(0xffffffffu, n) <= blocks && __reduce_max_sync(0xffffffffu, most) <= a.n_splits) break;
-        ++tiles;
+        if (__reduce_add_sync(0xffffffffu, n) <= blocks && __reduce_max_sync(0xffffffffu, most) <= a.n_splits) most_tiles = half;
+        else tiles = half + 1;
     }
     WtShare w = {-1, 0, tiles, 0};
     int before = 0;
