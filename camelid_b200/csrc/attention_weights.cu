@@ -20,7 +20,7 @@
 // Bound by memory where sequences are long: 16 of 24,001 to 32,768 keys with 8 kv heads of 128 (1.9 GB) take 340 us, 5.6 TB/s
 // of 6.6 that a copy reaches; 8 of 300 to 8,191 34.5 us (4.1 TB/s: unequal lengths, and 4 us of joining and weighing at the end);
 // short ones by the launch (12 us a call on the host, 6 on the device for 517 keys). In float: 4 sequences of 700 to 2,047 keys, heads of
-// 96, 20.8 us for 17 MB (a page is worked on in four phases between barriers, 4 us a page; only one page is on its way meanwhile).
+// 96, 18.2 us for 17 MB (a page is worked on in phases between barriers, and only one is on its way meanwhile).
 #include "common.cuh"
 #include <cooperative_groups.h>
 #include <math_constants.h>
@@ -110,15 +110,21 @@ template <> __device__ __forceinline__ float dot_chunk<bf16>(const unsigned char
     return s;
 }
 
-// q of R rows as float into shared memory (zeros where there is no row).
+// q of R rows as float into shared memory (zeros where there is no row); a channel's rows are asked for at once.
 template <typename T, int R>
 __device__ __forceinline__ void load_q(const WeightArgs& a, const Seq& s, int kvh, int m0, float* q_s) {
     const int group = a.heads / a.kv_heads;
-    for (int c = threadIdx.x; c < R * a.k_dim; c += AW_THREADS) {
-        const int m = m0 + c / a.k_dim, d = c % a.k_dim;
-        float x = 0.f;
-        if (m < s.rows) x = to_f32(((const T*)a.q)[(long long)(s.row0 + m / group) * a.q_stride + (long long)(kvh * group + m % group) * a.k_dim + d]);
-        q_s[c] = x;
+    for (int d = threadIdx.x; d < a.k_dim; d += AW_THREADS) {
+        float x[R];
+#pragma unroll
+        for (int m = 0; m < R; ++m) {
+            const bool in = m0 + m < s.rows;
+            const int j = in ? (m0 + m) / group : 0, h = in ? m0 + m - j * group : 0;
+            x[m] = to_f32(((const T*)a.q)[(long long)(s.row0 + j) * a.q_stride + (long long)(kvh * group + h) * a.k_dim + d]);
+            if (!in) x[m] = 0.f;
+        }
+#pragma unroll
+        for (int m = 0; m < R; ++m) q_s[m * a.k_dim + d] = x[m];
     }
 }
 
@@ -143,10 +149,23 @@ __device__ __forceinline__ void score_rows(const WeightArgs& a, const Seq& s, in
     }
 }
 
-// R rows and a stretch of keys, in float on the CUDA cores: a page of keys and values at a time, a quarter of the rows and
-// a key a thread for the scores, a channel (of half the keys, up to 128 channels) for the output. ALL (grid: cluster, pairs; for steps of at most R rows): the blocks of a cluster share all
-// keys of a sequence and finish by themselves, as on the tensor cores below. Otherwise (grid: stretches, pairs, row tiles)
-// this is step (1).
+template <typename T> __device__ __forceinline__ void four_of(const T* p, float (&v)[4]);
+template <> __device__ __forceinline__ void four_of<float>(const float* p, float (&v)[4]) {
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+}
+template <> __device__ __forceinline__ void four_of<bf16>(const bf16* p, float (&v)[4]) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(x.x << 16), v[1] = __uint_as_float(x.x & 0xffff0000u), v[2] = __uint_as_float(x.y << 16), v[3] = __uint_as_float(x.y & 0xffff0000u);
+}
+
+// R rows and a stretch of keys, in float on the CUDA cores, a page of keys and values at a time. For the scores a thread has a key, all
+// rows and a quarter of the channels, so that a key is read from shared memory once; for the output four channels of the keys that its
+// group of v_dim / 4 threads takes in turn with the others, so that no thread is idle; the groups meet once, behind the keys. (With a
+// row a thread over all channels, and a channel a thread over half of the keys, 4 sequences of 700 to 2,047 keys took 20.8 us for 18.2
+// with heads of 96, two of 4,000 68 for 50 with heads of 256; rings of four pages leave room for one block and took 23.6.)
+// ALL (grid: cluster, pairs; for steps of at most R rows): the blocks of a cluster share all keys of a sequence and finish by
+// themselves, as on the tensor cores below. Otherwise (grid: stretches, pairs, row tiles) this is step (1).
 template <typename T, int R, bool ALL>
 __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) {
     extern __shared__ __align__(16) unsigned char raw[];
@@ -163,9 +182,11 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
     else if (first >= last) return;
     const int k_stride = a.k_dim * (int)sizeof(T) + 16, v_stride = a.out ? a.v_dim * (int)sizeof(T) : 0;
     const int page_bytes = CML_PAGE * (k_stride + v_stride);
-    float* q_s = reinterpret_cast<float*>(raw + a.stages * page_bytes);
+    // (the ring's room holds the output of all groups of threads in the end, so it is as large as that at least)
+    float* q_s = reinterpret_cast<float*>(raw + max(a.stages * page_bytes, a.out ? R * AW_THREADS * 16 : 0));
     float* p_s = q_s + R * a.k_dim;                               // [page][rows]
-    float* m_s = p_s + R * CML_PAGE;
+    float* part_s = p_s + R * CML_PAGE;                           // [quarters][rows][page] the quarters' products
+    float* m_s = part_s + 4 * R * CML_PAGE;
     float* l_s = m_s + R;
     float* c_s = l_s + R;
     float* own = c_s + R;                                         // [rows][v_dim], the block's output
@@ -190,14 +211,13 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
     fetch(p_first);
     load_q<T, R>(a, s, kvh, m0, q_s);
     if (threadIdx.x < R) m_s[threadIdx.x] = -CUDART_INF_F, l_s[threadIdx.x] = 0.f;
-    float o[R];
+    float o[R][4];
 #pragma unroll
-    for (int m = 0; m < R; ++m) o[m] = 0.f;
-    const bool halves = a.v_dim <= AW_THREADS / 2;
-    const int d = halves ? threadIdx.x & (AW_THREADS / 2 - 1) : threadIdx.x;
-    const int kk_first = halves ? (threadIdx.x / (AW_THREADS / 2)) * (CML_PAGE / 2) : 0, kk_last = halves ? kk_first + CML_PAGE / 2 : CML_PAGE;
+    for (int m = 0; m < R; ++m) o[m][0] = o[m][1] = o[m][2] = o[m][3] = 0.f;
+    const int quads = a.out ? a.v_dim / 4 : AW_THREADS, groups = AW_THREADS / quads;          // groups of threads that share the keys
+    const int kk_first = threadIdx.x / quads, d = (threadIdx.x - kk_first * quads) * 4;       // (a thread behind the groups has no keys)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rows = min(R, s.rows - m0);
+    const int rows = min(R, s.rows - m0), group = a.heads / a.kv_heads;
     for (int p = p_first; p < p_last; ++p) {
         if (a.stages > 1) fetch(p + 1);
         else if (p > p_first) fetch(p);
@@ -206,16 +226,32 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
         __syncthreads();
         const unsigned char* ks = raw + (size_t)((p - p_first) & (a.stages - 1)) * page_bytes;
         const int key = threadIdx.x & 63, quarter = threadIdx.x >> 6;
-        float sc[R / 4];
-        score_rows<T, R>(a, s, m0, p * CML_PAGE + key, key < valid_of(p), ks + key * k_stride, q_s, sc);
+        {
+            constexpr int N = 16 / sizeof(T);
+            const int chunks = a.k_dim / N;
+            float acc[R];
 #pragma unroll
-        for (int m = 0; m < R / 4; ++m) {
-            p_s[key * R + quarter * (R / 4) + m] = sc[m];
-            if (ALL && quarter * (R / 4) + m < rows) kept[(size_t)(quarter * (R / 4) + m) * a.kept_stride + p * CML_PAGE + key] = sc[m];
+            for (int m = 0; m < R; ++m) acc[m] = 0.f;
+#pragma unroll 4
+            for (int c = quarter; c < chunks; c += 4)
+#pragma unroll
+                for (int m = 0; m < R; ++m) acc[m] += dot_chunk<T>(ks + key * k_stride + c * 16, q_s + m * a.k_dim + c * N);
+#pragma unroll
+            for (int m = 0; m < R; ++m) part_s[(quarter * R + m) * CML_PAGE + key] = acc[m];
         }
         __syncthreads();
+        const int valid = valid_of(p);
         for (int m = warp; m < rows; m += AW_THREADS / 32) {
-            const float a0 = p_s[lane * R + m], a1 = p_s[(lane + 32) * R + m];
+            const int sees = min(valid - 1, s.start + (m0 + m) / group - p * CML_PAGE);       // the last key of the page that the row sees
+            float x[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float* const from = part_s + m * CML_PAGE + lane + 32 * h;
+                x[h] = ((from[0] + from[R * CML_PAGE]) + (from[2 * R * CML_PAGE] + from[3 * R * CML_PAGE])) * a.scale;
+                if (lane + 32 * h > sees) x[h] = -CUDART_INF_F;
+                if (ALL) kept[(size_t)m * a.kept_stride + p * CML_PAGE + lane + 32 * h] = x[h];
+            }
+            const float a0 = x[0], a1 = x[1];
             const float old = m_s[m], now = fmaxf(old, warp_max(fmaxf(a0, a1)));
             const float e0 = a0 == -CUDART_INF_F ? 0.f : exp2f(a0 - now), e1 = a1 == -CUDART_INF_F ? 0.f : exp2f(a1 - now);
             const float corr = old == -CUDART_INF_F ? 0.f : exp2f(old - now);
@@ -226,53 +262,55 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
             if (lane == 0) m_s[m] = now, l_s[m] = l_s[m] * corr + sum, c_s[m] = corr;
         }
         __syncthreads();
-        if (a.out && d < a.v_dim) {
-            const T* vs = reinterpret_cast<const T*>(ks + CML_PAGE * k_stride);
-            float t[R];
+        if (a.out && kk_first < groups) {
+            const T* vs = reinterpret_cast<const T*>(ks + CML_PAGE * k_stride) + d;
+            // where rows do not all see the same places, one that a row does not see adds nothing, whatever it holds
+            const bool careful = s.fresh > 1 && (p + 1) * CML_PAGE > s.start + 1;
 #pragma unroll
-            for (int m = 0; m < R; ++m) t[m] = 0.f;
-            if (s.fresh > 1 && (p + 1) * CML_PAGE > s.start + 1) {
-                // where rows do not all see the same places, one that a row does not see adds nothing, whatever it holds
-                for (int kk = kk_first; kk < kk_last; ++kk) {
-                    const float val = to_f32(vs[kk * a.v_dim + d]);
-#pragma unroll
-                    for (int m = 0; m < R; ++m) {
-                        const float w = p_s[kk * R + m];
-                        if (w != 0.f) t[m] = fmaf(w, val, t[m]);
-                    }
-                }
-            } else {
-#pragma unroll 8
-                for (int kk = kk_first; kk < kk_last; ++kk) {
-                    const float val = to_f32(vs[kk * a.v_dim + d]);
-#pragma unroll
-                    for (int m = 0; m < R; m += 4) {
-                        const float4 w = *reinterpret_cast<const float4*>(p_s + kk * R + m);
-                        t[m] = fmaf(w.x, val, t[m]);
-                        t[m + 1] = fmaf(w.y, val, t[m + 1]);
-                        t[m + 2] = fmaf(w.z, val, t[m + 2]);
-                        t[m + 3] = fmaf(w.w, val, t[m + 3]);
-                    }
-                }
+            for (int m = 0; m < R; ++m) {
+                const float f = m < rows ? c_s[m] : 1.f;
+                o[m][0] *= f, o[m][1] *= f, o[m][2] *= f, o[m][3] *= f;
             }
+            auto add = [&](int kk, bool zero) {
+                float v[4];
+                four_of<T>(vs + kk * a.v_dim, v);
 #pragma unroll
-            for (int m = 0; m < R; ++m)
-                if (m < rows) o[m] = o[m] * c_s[m] + t[m];
+                for (int m = 0; m < R; m += 4) {
+                    const float4 w4 = *reinterpret_cast<const float4*>(p_s + kk * R + m);
+                    const float w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[m + u][i] = fmaf(w[u], zero && w[u] == 0.f ? 0.f : v[i], o[m + u][i]);
+                }
+            };
+            if (careful)
+                for (int kk = kk_first; kk < CML_PAGE; kk += groups) add(kk, true);
+            else {
+#pragma unroll 4
+                for (int kk = kk_first; kk < CML_PAGE; kk += groups) add(kk, false);
+            }
         }
         __syncthreads();
     }
     cp_async_wait<0>();
     __syncthreads();
     pdl_launch_dependents();
-    if (a.out && d < a.v_dim && (!halves || kk_first > 0)) {
+    if (a.out) {                                                  // the groups' sums meet in the ring's room, in their order
+        float* const red = reinterpret_cast<float*>(raw);         // [groups][rows][v_dim]
+        if (kk_first < groups) {
 #pragma unroll
-        for (int m = 0; m < R; ++m) own[m * a.v_dim + d] = o[m];
+            for (int m = 0; m < R; ++m) *reinterpret_cast<float4*>(red + (kk_first * R + m) * a.v_dim + d) = make_float4(o[m][0], o[m][1], o[m][2], o[m][3]);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < R * a.v_dim; i += AW_THREADS) {
+            float x = 0.f;
+#pragma unroll 4
+            for (int g = 0; g < groups; ++g) x += red[g * R * a.v_dim + i];
+            own[i] = x;
+        }
     }
     __syncthreads();
-    if (a.out && halves && kk_first == 0 && d < a.v_dim) {        // the first half of the keys, then the second
-#pragma unroll
-        for (int m = 0; m < R; ++m) own[m * a.v_dim + d] = o[m] + own[m * a.v_dim + d];
-    }
     if (!ALL) {
         const size_t base = ((size_t)blockIdx.y * a.n_splits + split) * group_rows + m0;
         if ((int)threadIdx.x < rows) {
@@ -302,7 +340,6 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
     }
     __syncthreads();
     if (a.out) {                                                  // the output's elements in equal shares, the blocks in their order
-        const int group = a.heads / a.kv_heads;
         for (int i = split * AW_THREADS + threadIdx.x; i < rows * a.v_dim; i += team * AW_THREADS) {
             const int m = i / a.v_dim, d = i - m * a.v_dim;
             float x = 0.f;
@@ -1017,9 +1054,10 @@ static cudaError_t launch_plain(WeightArgs& a, cudaStream_t s) {
     const unsigned pairs = (unsigned)a.n_seqs * (unsigned)a.kv_heads;
     const int group_rows = a.max_new * (a.heads / a.kv_heads);
     const size_t k_page = (size_t)CML_PAGE * (a.k_dim * sizeof(T) + 16), v_page = a.out ? (size_t)CML_PAGE * a.v_dim * sizeof(T) : 0;
-    auto rest = [&](int rows) { return (size_t)rows * (a.k_dim + CML_PAGE + 3 + (a.out ? a.v_dim : 0)) * 4; };
+    auto rest = [&](int rows) { return (size_t)rows * (a.k_dim + 5 * CML_PAGE + 4 + (a.out ? a.v_dim : 0)) * 4; };
     a.stages = 2 * (k_page + v_page) + rest(AW_ROWS) <= 220 * 1024 ? 2 : 1;
-    const size_t ring = a.stages * (k_page + v_page);
+    const size_t groups = (size_t)AW_ROWS * AW_THREADS * 4 * 4;               // the output of all groups of threads, where the ring was
+    const size_t ring = a.stages * (k_page + v_page) > groups ? a.stages * (k_page + v_page) : groups;
     if (group_rows <= 4) return launch_plain_all<T, 4>(a, pairs, ring + rest(4), s);
     if (group_rows <= AW_ROWS) return launch_plain_all<T, AW_ROWS>(a, pairs, ring + rest(AW_ROWS), s);
     const size_t smem1 = ring + rest(AW_ROWS), smem3 = k_page + (size_t)AW_ROWS * a.k_dim * 4;
