@@ -110,43 +110,39 @@ template <> __device__ __forceinline__ float dot_chunk<bf16>(const unsigned char
     return s;
 }
 
-// q of R rows as float into shared memory (zeros where there is no row); a channel's rows are asked for at once.
+// A channel of R rows of q (zero where there is no row); all are asked for at once.
 template <typename T, int R>
-__device__ __forceinline__ void load_q(const WeightArgs& a, const Seq& s, int kvh, int m0, float* q_s) {
+__device__ __forceinline__ void ask_q(const WeightArgs& a, const Seq& s, int kvh, int m0, int d, float (&x)[R]) {
     const int group = a.heads / a.kv_heads;
-    for (int d = threadIdx.x; d < a.k_dim; d += AW_THREADS) {
-        float x[R];
 #pragma unroll
-        for (int m = 0; m < R; ++m) {
-            const bool in = m0 + m < s.rows;
-            const int j = in ? (m0 + m) / group : 0, h = in ? m0 + m - j * group : 0;
-            x[m] = to_f32(((const T*)a.q)[(long long)(s.row0 + j) * a.q_stride + (long long)(kvh * group + h) * a.k_dim + d]);
-            if (!in) x[m] = 0.f;
-        }
-#pragma unroll
-        for (int m = 0; m < R; ++m) q_s[m * a.k_dim + d] = x[m];
+    for (int m = 0; m < R; ++m) {
+        const bool in = m0 + m < s.rows;
+        const int j = in ? (m0 + m) / group : 0, h = in ? m0 + m - j * group : 0;
+        x[m] = to_f32(((const T*)a.q)[(long long)(s.row0 + j) * a.q_stride + (long long)(kvh * group + h) * a.k_dim + d]);
+        if (!in) x[m] = 0.f;
     }
 }
 
-// The scores of this thread's key (threadIdx.x & 63) for a quarter of the block's R rows (threadIdx.x >> 6), scaled and masked.
+// The products of this thread's key (threadIdx.x & 63) with R rows over its quarter (threadIdx.x >> 6) of the 16-byte pieces.
 template <typename T, int R>
-__device__ __forceinline__ void score_rows(const WeightArgs& a, const Seq& s, int m0, int place, bool there, const unsigned char* k_row,
-                                           const float* q_s, float (&out)[R / 4]) {
+__device__ __forceinline__ void quarter_products(const WeightArgs& a, const unsigned char* k_row, const float* q_s, float* part_s) {
     constexpr int N = 16 / sizeof(T);
-    const int group = a.heads / a.kv_heads, quarter = threadIdx.x >> 6;
-    float acc[R / 4];
+    const int key = threadIdx.x & 63, quarter = threadIdx.x >> 6, chunks = a.k_dim / N;
+    float acc[R];
 #pragma unroll
-    for (int m = 0; m < R / 4; ++m) acc[m] = 0.f;
-    const float* q = q_s + quarter * (R / 4) * a.k_dim;
-#pragma unroll 4
-    for (int d = 0; d < a.k_dim; d += N)
+    for (int m = 0; m < R; ++m) acc[m] = 0.f;
+#pragma unroll 2
+    for (int c = quarter; c < chunks; c += 4)
 #pragma unroll
-        for (int m = 0; m < R / 4; ++m) acc[m] += dot_chunk<T>(k_row + d * sizeof(T), q + m * a.k_dim + d);
+        for (int m = 0; m < R; ++m) acc[m] += dot_chunk<T>(k_row + c * 16, q_s + m * a.k_dim + c * N);
 #pragma unroll
-    for (int m = 0; m < R / 4; ++m) {
-        const int r = m0 + quarter * (R / 4) + m;
-        out[m] = there && r < s.rows && place <= s.start + r / group ? acc[m] * a.scale : -CUDART_INF_F;
-    }
+    for (int m = 0; m < R; ++m) part_s[(quarter * R + m) * CML_PAGE + key] = acc[m];
+}
+// The four quarters' sum for a row and key.
+template <int R>
+__device__ __forceinline__ float product_of(const float* part_s, int m, int key) {
+    const float* const from = part_s + m * CML_PAGE + key;
+    return (from[0] + from[R * CML_PAGE]) + (from[2 * R * CML_PAGE] + from[3 * R * CML_PAGE]);
 }
 
 template <typename T> __device__ __forceinline__ void four_of(const T* p, float (&v)[4]);
@@ -209,7 +205,12 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
         cp_async_commit();
     };
     fetch(p_first);
-    load_q<T, R>(a, s, kvh, m0, q_s);
+    for (int d = threadIdx.x; d < a.k_dim; d += AW_THREADS) {
+        float x[R];
+        ask_q<T, R>(a, s, kvh, m0, d, x);
+#pragma unroll
+        for (int m = 0; m < R; ++m) q_s[m * a.k_dim + d] = x[m];
+    }
     if (threadIdx.x < R) m_s[threadIdx.x] = -CUDART_INF_F, l_s[threadIdx.x] = 0.f;
     float o[R][4];
 #pragma unroll
@@ -225,20 +226,7 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
         else cp_async_wait<0>();
         __syncthreads();
         const unsigned char* ks = raw + (size_t)((p - p_first) & (a.stages - 1)) * page_bytes;
-        const int key = threadIdx.x & 63, quarter = threadIdx.x >> 6;
-        {
-            constexpr int N = 16 / sizeof(T);
-            const int chunks = a.k_dim / N;
-            float acc[R];
-#pragma unroll
-            for (int m = 0; m < R; ++m) acc[m] = 0.f;
-#pragma unroll 4
-            for (int c = quarter; c < chunks; c += 4)
-#pragma unroll
-                for (int m = 0; m < R; ++m) acc[m] += dot_chunk<T>(ks + key * k_stride + c * 16, q_s + m * a.k_dim + c * N);
-#pragma unroll
-            for (int m = 0; m < R; ++m) part_s[(quarter * R + m) * CML_PAGE + key] = acc[m];
-        }
+        quarter_products<T, R>(a, ks + (threadIdx.x & 63) * k_stride, q_s, part_s);
         __syncthreads();
         const int valid = valid_of(p);
         for (int m = warp; m < rows; m += AW_THREADS / 32) {
@@ -246,8 +234,7 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
             float x[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float* const from = part_s + m * CML_PAGE + lane + 32 * h;
-                x[h] = ((from[0] + from[R * CML_PAGE]) + (from[2 * R * CML_PAGE] + from[3 * R * CML_PAGE])) * a.scale;
+                x[h] = product_of<R>(part_s, m, lane + 32 * h) * a.scale;
                 if (lane + 32 * h > sees) x[h] = -CUDART_INF_F;
                 if (ALL) kept[(size_t)m * a.kept_stride + p * CML_PAGE + lane + 32 * h] = x[h];
             }
@@ -416,28 +403,34 @@ __global__ void __launch_bounds__(AW_THREADS) weights_sum_kernel(WeightArgs a) {
     const size_t at = ((size_t)page * a.kv_heads + kvh) * CML_PAGE;
     fetch_page<T>(raw, k_stride, (const T*)a.k + at * a.k_dim, a.k_dim, valid);
     cp_async_commit();
-    const int key = threadIdx.x & 63, quarter = threadIdx.x >> 6;
-    const int group_rows = a.max_new * (a.heads / a.kv_heads);
+    const int key = threadIdx.x & 63, quarter = threadIdx.x >> 6, place = p * CML_PAGE + key;
+    const int group = a.heads / a.kv_heads, group_rows = a.max_new * group;
+    float* const part_s = q_s + AW_ROWS * a.k_dim;                // [quarters][rows][page]
+    const bool has = (int)threadIdx.x < a.k_dim;                  // (256 channels at most, as many as threads)
+    float next[AW_ROWS];
+    if (has) ask_q<T, AW_ROWS>(a, s, kvh, 0, threadIdx.x, next);
+    cp_async_wait<0>();
     float gained = 0.f;
     for (int m0 = 0; m0 < s.rows; m0 += AW_ROWS) {
-        __syncthreads();
-        load_q<T, AW_ROWS>(a, s, kvh, m0, q_s);
-        cp_async_wait<0>();
-        __syncthreads();
-        float sc[AW_ROWS / 4];
-        score_rows<T, AW_ROWS>(a, s, m0, p * CML_PAGE + key, key < valid, raw + key * k_stride, q_s, sc);
+        if (has) {
 #pragma unroll
-        for (int m = 0; m < AW_ROWS / 4; ++m) {
-            const int r = m0 + quarter * (AW_ROWS / 4) + m;
-            if (r >= s.rows || sc[m] == -CUDART_INF_F) continue;
-            const float* j = a.joined + ((size_t)blockIdx.y * group_rows + r) * 2;
-            gained += exp2f(sc[m] - j[0]) * j[1];
+            for (int m = 0; m < AW_ROWS; ++m) q_s[m * a.k_dim + threadIdx.x] = next[m];
+        }
+        __syncthreads();
+        if (has && m0 + AW_ROWS < s.rows) ask_q<T, AW_ROWS>(a, s, kvh, m0 + AW_ROWS, threadIdx.x, next);      // beside the products of these
+        quarter_products<T, AW_ROWS>(a, raw + key * k_stride, q_s, part_s);
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < AW_ROWS / 4; ++u) {                   // a quarter of the rows each
+            const int m = quarter * (AW_ROWS / 4) + u, r = m0 + m;
+            if (r >= s.rows || place > s.start + r / group) continue;
+            const float2 j = *reinterpret_cast<const float2*>(a.joined + ((size_t)blockIdx.y * group_rows + r) * 2);
+            gained += exp2f(product_of<AW_ROWS>(part_s, m, key) * a.scale - j.x) * j.y;
         }
     }
     if (quarter > 0) other[quarter - 1][key] = gained;
     __syncthreads();
     if (quarter == 0 && key < valid) {
-        const int place = p * CML_PAGE + key;
         a.scores_out[at + key] = (place < s.old ? a.scores[at + key] : 0.f) + (((gained + other[0][key]) + other[1][key]) + other[2][key]);
     }
 }
@@ -1060,7 +1053,7 @@ static cudaError_t launch_plain(WeightArgs& a, cudaStream_t s) {
     const size_t ring = a.stages * (k_page + v_page) > groups ? a.stages * (k_page + v_page) : groups;
     if (group_rows <= 4) return launch_plain_all<T, 4>(a, pairs, ring + rest(4), s);
     if (group_rows <= AW_ROWS) return launch_plain_all<T, AW_ROWS>(a, pairs, ring + rest(AW_ROWS), s);
-    const size_t smem1 = ring + rest(AW_ROWS), smem3 = k_page + (size_t)AW_ROWS * a.k_dim * 4;
+    const size_t smem1 = ring + rest(AW_ROWS), smem3 = k_page + (size_t)AW_ROWS * (a.k_dim + 4 * CML_PAGE) * 4;
     cudaError_t e = cml_allow_smem<weights_part_kernel<T, AW_ROWS, false>>(smem1);
     if (e == cudaSuccess) e = cml_allow_smem<weights_sum_kernel<T>>(smem3);
     if (e != cudaSuccess) return e;
