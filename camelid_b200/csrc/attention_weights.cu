@@ -469,6 +469,9 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src
 
 #define AM_WARPS 4
 #define AM_STAGES 3
+// Keys of a tile: with heads of 64, 32 where 17 to 32 rows share them (8 sequences of 1,500 to 4,100 keys 28.4 us for 29.7 with 16), 16
+// where fewer do (8 sequences of 300 to 8,191 keys 22.1 us for 24.7 with 32: four blocks fit a multiprocessor, not two).
+template <int HD, int MT> constexpr int few_tile = HD == 128 || MT == 1 ? 16 : 32;
 
 // Up to 16 * MT rows of a (sequence, kv head). A warp takes every eighth tile of TILE keys of the block's stretch with a ring of
 // its own in shared memory, and the warps' ranges are joined at the end in their order. OUT: with values and output.
@@ -477,7 +480,7 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src
 // launch does it all. Otherwise (grid: stretches, pairs, row chunks) this is step (1).
 template <int HD, int MT, bool OUT, bool ALL>
 __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightArgs a) {
-    constexpr int TILE = HD == 128 ? 16 : 32;
+    constexpr int TILE = few_tile<HD, MT>;
     constexpr int LDS = HD + 8, KS = HD / 16, DT = HD / 8, NT = TILE / 8, KK = TILE / 16, CH = HD / 8;
     constexpr int HALF = TILE * LDS * 2, STAGE = HALF * (OUT ? 2 : 1);        // bytes
     constexpr int TEAM = MT == 1 ? 16 : 8;                                    // blocks of a cluster at most
@@ -738,6 +741,8 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
     pdl_launch_dependents();
     // the warps' ranges: [warp][16 * MT rows][maximum, sum, output]
     constexpr int RW = OUT ? HD + 4 : 4;
+    static_assert(AM_WARPS * 16 * MT * RW * 4 + (OUT ? 16 * MT * HD * 4 : 0) <= AM_WARPS * AM_STAGES * STAGE, "the results take the ring's room");
+    static_assert(!OUT || 16 * MT * TILE * 4 <= HALF, "the probabilities take the room of a tile's keys");
     float* red = reinterpret_cast<float*>(raw);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -1078,10 +1083,9 @@ static cudaError_t launch_all(const WeightArgs& a, unsigned pairs, int team, siz
 
 template <int HD>
 static cudaError_t launch_mma(const WeightArgs& a, int* err, cudaStream_t s) {
-    constexpr int TILE = HD == 128 ? 16 : 32;
     const unsigned pairs = (unsigned)a.n_seqs * (unsigned)a.kv_heads;
     const int rows = a.max_new * (a.heads / a.kv_heads);
-    constexpr size_t ring = (size_t)AM_WARPS * AM_STAGES * TILE * (HD + 8) * 2;
+    constexpr size_t ring1 = (size_t)AM_WARPS * AM_STAGES * few_tile<HD, 1> * (HD + 8) * 2, ring2 = ring1 / few_tile<HD, 1> * few_tile<HD, 2>;
     cudaError_t e;
     if (rows <= 32) {
         // Where the blocks of all sequences run at the same time, more of them; beyond that up to twice as many, for sequences of
@@ -1092,17 +1096,17 @@ static cudaError_t launch_mma(const WeightArgs& a, int* err, cudaStream_t s) {
         int team = 1;
         while (team < 8 && (pairs * team * 2 <= slots || (pairs * team * 2 <= 2 * slots && a.max_len >= team * 2 * 768)) && team * 128 < a.max_len) team *= 2;
         if (rows <= 16 && team == 8 && pairs * 16 <= (unsigned)cml_sm_count() && a.max_len >= 4096) team = 16;
-        if (rows <= 16) return a.out ? launch_all<HD, 1, true>(a, pairs, team, 2 * ring, s) : launch_all<HD, 1, false>(a, pairs, team, ring, s);
-        return a.out ? launch_all<HD, 2, true>(a, pairs, team, 2 * ring, s) : launch_all<HD, 2, false>(a, pairs, team, ring, s);
+        if (rows <= 16) return a.out ? launch_all<HD, 1, true>(a, pairs, team, 2 * ring1, s) : launch_all<HD, 1, false>(a, pairs, team, ring1, s);
+        return a.out ? launch_all<HD, 2, true>(a, pairs, team, 2 * ring2, s) : launch_all<HD, 2, false>(a, pairs, team, ring2, s);
     }
     // Without output and beyond the rows whose products are kept: tcgen05, in two launches (four sequences of 4,000 keys, 8 kv heads of
     // 128: 27.9 us whatever the rows up to 128; the one launch above takes 26.2 with 32 rows, 14.3 with 8, and its split form, which
     // stood here, 56 with 36 and 94 with 128).
     if (a.out == nullptr) return launch_tc<HD>(a, err, s);
-    e = cml_allow_smem<weights_part_mma_kernel<HD, 2, true, false>>(2 * ring);
+    e = cml_allow_smem<weights_part_mma_kernel<HD, 2, true, false>>(2 * ring2);
     if (e == cudaSuccess)
         e = launch_pdl(weights_part_mma_kernel<HD, 2, true, false>, dim3((unsigned)a.n_splits, pairs, (unsigned)((rows + 31) / 32)), dim3(AM_WARPS * 32),
-                       2 * ring, s, a);
+                       2 * ring2, s, a);
     if (e != cudaSuccess) return e;
     e = launch_pdl(weights_join_kernel<bf16>, dim3((unsigned)rows, pairs), dim3(AW_THREADS), 0, s, a);
     if (e != cudaSuccess) return e;
