@@ -102,6 +102,7 @@ template <int HD, int RT> struct WtPlan {
     static constexpr int STAGES = ROOM < 6 ? ROOM : 6;                        // what the rows of q leave room for
     static constexpr size_t SMEM = 1024 + (size_t)TILE * (RT + STAGES) + 256 + RT * 128 * 8 * 3;
     static constexpr int BUFS = 2;                                            // products of a side in tensor memory
+    static_assert(STAGES >= 2 && SMEM + 64 <= 227 * 1024, "a tile for each side, within a block's shared memory");
 };
 
 // Which stretch a block has. All sequences' key tiles are cut into stretches of the same number of tiles, the smallest for which they
@@ -113,6 +114,11 @@ struct WtShare {
 };
 __device__ __forceinline__ WtShare wt_share(const WeightArgs& a, int m0, int block, int blocks) {        // by a whole warp, the same in every lane
     const int lane = threadIdx.x & 31;
+    if (a.n_seqs == 1) {                       // (a microsecond less)
+        const Seq s = seq_of(a, 0);
+        const int total = m0 < s.rows ? (s.length + WT_KEYS - 1) / WT_KEYS : 0, tiles = max(1, (total + blocks - 1) / blocks);
+        return {block * tiles < total ? 0 : -1, block, tiles, (total + tiles - 1) / tiles};
+    }
     auto look_up = [&](int i) {
         if (i >= a.n_seqs) return 0;
         const Seq s = seq_of(a, i);
@@ -126,15 +132,18 @@ __device__ __forceinline__ WtShare wt_share(const WeightArgs& a, int m0, int blo
         total += k, longest = max(longest, k);
     }
     total = __reduce_add_sync(0xffffffffu, total);
-    int tiles = max(1, (total + blocks - 1) / blocks), most_tiles = max(tiles, __reduce_max_sync(0xffffffffu, longest));
-    while (tiles < most_tiles) {               // halved: stretches as long as the longest sequence, one of each, always fit
-        const int half = (tiles + most_tiles) / 2;
+    // Between what would fill all blocks and what always fits: every sequence has at most one stretch that is not full, and one of the
+    // longest's length each fits too.
+    int tiles = max(1, (total + blocks - 1) / blocks), fits = max(tiles, __reduce_max_sync(0xffffffffu, longest));
+    if (a.n_splits > 1) fits = max(tiles, min(fits, (total + a.n_splits - 2) / (a.n_splits - 1)));
+    while (tiles < fits) {
+        const int half = (tiles + fits) / 2;
         int n = 0, most = 0;
         for (int i = lane; i < a.n_seqs; i += 32) {
             const int k = (tiles_of(i) + half - 1) / half;
             n += k, most = max(most, k);
         }
-        if (__reduce_add_sync(0xffffffffu, n) <= blocks && __reduce_max_sync(0xffffffffu, most) <= a.n_splits) most_tiles = half;
+        if (__reduce_add_sync(0xffffffffu, n) <= blocks && __reduce_max_sync(0xffffffffu, most) <= a.n_splits) fits = half;
         else tiles = half + 1;
     }
     WtShare w = {-1, 0, tiles, 0};
@@ -184,20 +193,12 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     pdl_launch_dependents();
-    const WtShare share = wt_share(a, m0, blockIdx.x, gridDim.x);                 // every warp for itself
-    if (share.seq < 0) return;                                                // more blocks than stretches: the same for the whole block
-    const int split = share.split, seq = share.seq, kvh = blockIdx.y, pair = seq * a.kv_heads + kvh;
-    const Seq s = seq_of(a, seq);
-    const int first = split * share.tiles * WT_KEYS, last = min(s.length, first + share.tiles * WT_KEYS);
-    const int group = a.heads / a.kv_heads, group_rows = a.max_new * group;
-    const int n_tiles = (last - first + WT_KEYS - 1) / WT_KEYS;
-    const int rows = min(s.rows - m0, RT * 128), row_tiles = (rows + 127) / 128;
-    const int* const pages = a.table + (size_t)seq * a.width;
-    auto page_at = [&](int key) {                                             // the page of a key of this stretch, -1: none
-        const int page = key < last ? pages[key / CML_PAGE] : -1;
-        return page < a.n_pages ? page : -1;
-    };
-    if (threadIdx.x == 0) {
+    __shared__ WtShare share;
+    if (warp == 0) {                                                          // the other warps prepare what does not depend on it
+        const WtShare mine = wt_share(a, m0, blockIdx.x, gridDim.x);
+        if (lane == 0) share = mine;
+    }
+    if (threadIdx.x == 32) {
         for (int i = 0; i < STAGES; ++i) wt_init(k_full(i), 1), wt_init(k_empty(i), 1);
         for (int i = 0; i < 2 * BUFS; ++i) wt_init(s_full(i), 1), wt_init(s_empty(i), WT_WORKERS / 64);
         wt_init(q_ready, WT_WORKERS);
@@ -213,7 +214,21 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
     __syncthreads();
     wt_fence_after();
     const uint32_t tmem = *slot;
-
+    if (share.seq < 0) {                                                      // more blocks than stretches: the same for the whole block
+        if (warp == WT_WORKERS / 32 + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u * BUFS) : "memory");
+        return;
+    }
+    const int split = share.split, seq = share.seq, kvh = blockIdx.y, pair = seq * a.kv_heads + kvh;
+    const Seq s = seq_of(a, seq);
+    const int first = split * share.tiles * WT_KEYS, last = min(s.length, first + share.tiles * WT_KEYS);
+    const int group = a.heads / a.kv_heads, group_rows = a.max_new * group;
+    const int n_tiles = (last - first + WT_KEYS - 1) / WT_KEYS;
+    const int rows = min(s.rows - m0, RT * 128), row_tiles = (rows + 127) / 128;
+    const int* const pages = a.table + (size_t)seq * a.width;
+    auto page_at = [&](int key) {                                             // the page of a key of this stretch, -1: none
+        const int page = key < last ? pages[key / CML_PAGE] : -1;
+        return page < a.n_pages ? page : -1;
+    };
     if (warp == WT_WORKERS / 32) {
         if (lane == 0) {
             int issued = 0;
@@ -264,14 +279,18 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
         }
     } else {
         // q into its tiles, zeros where there is no row
-        constexpr int ROW = KB * 8;                                           // 16-byte pieces of a row
-        const int piece = threadIdx.x % ROW, x0 = threadIdx.x / ROW;
-        for (int m = x0; m < row_tiles * 128; m += WT_WORKERS / ROW) {
+        constexpr int ROW = KB * 8, STEP = WT_WORKERS / ROW;                  // 16-byte pieces of a row; rows between this thread's
+        const int piece = threadIdx.x % ROW, x0 = threadIdx.x / ROW, j_step = STEP / group, h_step = STEP - j_step * group;
+        int j = (m0 + x0) / group, h = m0 + x0 - j * group;                   // token and head of row x0, walked without further divisions
+        const bf16* const q0 = (const bf16*)a.q + (long long)s.row0 * a.q_stride + (long long)kvh * group * HD + piece * 8;
+#pragma unroll 4
+        for (int m = x0; m < row_tiles * 128; m += STEP) {
             const bool in = m < rows;
-            const int j = in ? (m0 + m) / group : 0;
-            const bf16* src = (const bf16*)a.q + (long long)(s.row0 + j) * a.q_stride + (long long)(kvh * group + (in ? m0 + m - j * group : 0)) * HD + piece * 8;
             const int r = m % 128;
-            cp_async16_or_zero(sQ + (m / 128) * TILE + (piece / 8) * BLOCK + (r >> 3) * 1024 + (r & 7) * 128 + (((piece & 7) ^ (r & 7)) << 4), src, in);
+            cp_async16_or_zero(sQ + (m / 128) * TILE + (piece / 8) * BLOCK + (r >> 3) * 1024 + (r & 7) * 128 + (((piece & 7) ^ (r & 7)) << 4),
+                               in ? q0 + (long long)j * a.q_stride + h * HD : q0, in);
+            j += j_step, h += h_step;
+            if (h >= group) h -= group, ++j;
         }
         cp_async_commit();
         if (SUM) {                                                            // the stretches of every row joined, in their order
