@@ -186,6 +186,26 @@ def test_window_at_the_limits_of_its_kernels(cuda, dim):
     _attention(cuda, [300, 40], [16, 9], 8, 2, dim, torch.bfloat16, with_out=False, loose=True, q_pad=8)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_window_of_many_unequal_sequences(cuda, dim):
+    """More sequences than lanes, than blocks of a kv head, some without new tokens, and rows in several passes."""
+    rng = random.Random(dim)
+    starts = [rng.choice((0, 3, 64, 127, 128, 300, 900)) for _ in range(40)]
+    news = [rng.choice((0, 1, 9, 17, 20)) for _ in range(40)]
+    _attention(cuda, starts, news, 8, 1, dim, torch.bfloat16, with_out=False, seed=dim)
+    _attention(cuda, starts[:21], news[:20] + [20], 32, 8, dim, torch.bfloat16, with_out=False, seed=dim + 1, in_place=False)
+    _attention(cuda, [500, 70, 0, 33], [70, 10, 33, 0], 16, 1, dim, torch.bfloat16, with_out=False, seed=3, spoil=float("nan"), in_place=False)
+    _attention(cuda, [4000, 0, 130], [9, 9, 9], 4, 1, dim, torch.bfloat16, with_out=False, seed=4)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim,v_dim", [(256, 16), (16, 256), (240, 112), (48, 240)])
+def test_float_path_with_keys_and_values_of_many_sizes(cuda, dtype, dim, v_dim):
+    for heads, kv_heads, starts, news in ((2, 1, [150, 64], [1, 2]), (8, 1, [500, 0, 63], [1, 1, 1]), (6, 2, [130, 7], [5, 3])):
+        _attention(cuda, starts, news, heads, kv_heads, dim, dtype, v_dim=v_dim, seed=heads)
+    _attention(cuda, [100, 5], [11, 4], 4, 2, dim, dtype, with_out=False, seed=9, spoil=float("inf"), in_place=False)
+
+
 def test_window_with_missing_pages(cuda):
     from camelid_b200.csrc import ops
     for dim in (64, 128):
@@ -425,6 +445,16 @@ def test_verify_matches_plain(cuda, vocab, temperature, with_probs):
 def test_verify_with_the_samplers_filters(cuda, vocab, filters):
     for with_probs in (True, False):
         assert _verify(cuda, vocab, [3, 0, 5], 0.8, with_probs, seed=vocab, **filters)[2] == 0
+
+
+@pytest.mark.parametrize("n", [1, 4, 5, 15, 16, 40])
+def test_verify_large_vocabularies(cuda, n):
+    """Every way a sequence's row is shared: sixteen, eight and four blocks, alone on a multiprocessor or not, groups of one tile and of several."""
+    lens = [(3 * i) % 5 for i in range(n)]
+    for vocab in (16400, 65536, 70001, 140003):
+        if n * vocab <= 1_200_000:
+            assert _verify(cuda, vocab, lens, 0.9, n * vocab <= 300_000, seed=n)[2] == 0
+            assert _verify(cuda, vocab, lens[::-1], 1.3, False, seed=n + 1, top_p=0.97)[2] == 0
 
 
 def test_verify_without_room_for_drafts(cuda):
