@@ -11,10 +11,10 @@
 // Sixteen warps of exponentials, in two sides that take the tiles in turn, one warp that brings keys, one that issues products.
 // With eight warps on halves of one tile, all were in the same phase and the exponentials' unit idled half of the time. Measured
 // over 64 rows (256 with their heads) of four prompts of 9,001 to 16,384 keys and 8 kv heads: 300 us on mma.sync, 145 with eight
-// warps here, 119 with stretches of equal work, 94 with sixteen warps and a ring as deep as shared memory allows. What bounds it:
-// the exponentials of both passes take 48 us (16 a cycle and multiprocessor), the products, whose two operands pass through
-// shared memory, 57 without them, the start of both kernels 21 (the passes alone, without exponentials and maxima, take 78 us,
-// with exponentials and one product in eight 84).
+// warps here, 119 with stretches of equal work, 94 with sixteen warps and a ring as deep as shared memory allows, 90 with a shorter
+// start. What bounds it: the exponentials of both passes take 48 us (16 a cycle and multiprocessor; their unit is busy 69% and 62% of
+// the time), the products, whose two operands pass through shared memory, about as long beside them, the start of both kernels 14.
+// One in four to eight of the exponentials as a polynomial on the other pipes made it slower (93 to 100 us).
 #pragma once
 #include <cuda.h>
 
