@@ -188,6 +188,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
     __shared__ SelectShared sh;
     __shared__ TeamSlots ts;
     __shared__ float fred[33];
+    __shared__ unsigned int counts_s[32];
     __shared__ double table[32];
     fill_table(table);
     if (threadIdx.x == 0) fs.n_list = 0u;
@@ -259,9 +260,63 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
         cum = fs0->cum;
         tm.sync();
     };
-    if (a.top_k > 0 && a.top_k < vocab) {
+    float edge = CUDART_INF_F;                                    // nothing at or beyond this place is among the first top_k
+    const bool first_k = a.top_k > 0 && a.top_k < vocab;
+    // The first top_k by counting: the bin of 1/64 in which they end; where no more than the list holds lies up to there, the list takes
+    // it all and the first k of it stay (8 rows-sharing sequences of 128,256 tokens, top_k 40: TODO).
+    if (first_k && a.top_k <= FS_CAP) {
+        for (int b = threadIdx.x; b < FS_BINS; b += SAMPLE_THREADS) fs.cnt[b] = 0u;
+        tm.sync();                                                // block 0's bins are clear before anyone adds to them
+        for_each_in_slice<8>(row, tm, [&](float v, int) {
+            const float x = xof(v);
+            if (x < (float)(FS_BINS / 64)) atomicAdd(&fs.cnt[(int)(x * 64.f)], 1u);
+        });
+        __syncthreads();
+        if (tm.rank != 0) {
+            for (int b = threadIdx.x; b < FS_BINS; b += SAMPLE_THREADS)
+                if (fs.cnt[b] != 0u) atomicAdd(&fs0->cnt[b], fs.cnt[b]);
+        }
+        tm.sync();
+        if (tm.rank == 0) {
+            const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+            for (int w = warp; w < 32; w += SAMPLE_THREADS / 32) {            // 64 bins a warp's turn
+                const unsigned int t = __reduce_add_sync(0xffffffffu, fs.cnt[w * 64 + lane] + fs.cnt[w * 64 + 32 + lane]);
+                if (lane == 0) counts_s[w] = t;
+            }
+            __syncthreads();
+            if (warp == 0) {
+                auto scan = [&](unsigned int c) {
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const unsigned int t = __shfl_up_sync(0xffffffffu, c, o);
+                        if (lane >= o) c += t;
+                    }
+                    return c;
+                };
+                const unsigned int k = (unsigned int)a.top_k, incl = scan(counts_s[lane]);
+                const unsigned int reach = __ballot_sync(0xffffffffu, incl >= k);
+                int bin = FS_BINS;
+                unsigned int upto = 0u;
+                if (reach) {
+                    const int w = __ffs(reach) - 1;
+                    const unsigned int before = __shfl_sync(0xffffffffu, incl - counts_s[lane], w);
+                    const unsigned int c0 = fs.cnt[w * 64 + 2 * lane], c1 = fs.cnt[w * 64 + 2 * lane + 1], pair = before + scan(c0 + c1);
+                    const int l = __ffs(__ballot_sync(0xffffffffu, pair >= k)) - 1;
+                    const bool second = pair - c1 < k;            // in this lane's pair: the first of the two that reaches k
+                    bin = __shfl_sync(0xffffffffu, w * 64 + 2 * lane + (second ? 1 : 0), l);
+                    upto = __shfl_sync(0xffffffffu, second ? pair : pair - c1, l);
+                }
+                if (lane == 0) fs.bin = bin, fs.status = (int)upto;
+            }
+        }
+        tm.sync();
+        if (fs0->bin < FS_BINS && fs0->status <= FS_CAP) edge = (float)(fs0->bin + 1) / 64.f;
+    }
+    const bool counted = edge < CUDART_INF_F;
+    if (first_k && !counted) {
         auto one = [](float, int) { return 1.0; };
         auto one_at = [](float) { return 1.0f; };
+        tm.sync();                                                // (every block has read block 0's verdict)
         if (!select_fast(row, tm, 0ull, (double)a.top_k, 0, xof, x_max, one, one_at, &fs, &ts, &key, &cum))
             select_slow(0ull, (double)a.top_k, 0, one);
         floor_key = key;
@@ -272,8 +327,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
     const float near = least > 0.0 ? -logf(a.min_p) * 1.001f + 0.01f : CUDART_INF_F;
     // Few candidates, the usual case where there is a min_p or a top_k: their keys are collected in one pass, sorted by block 0, and
     // the rest of the way goes along that list.
-    if (floor_key != 0ull || least > 0.0) {
-        if (a.top_k > 0 && a.top_k < vocab) {                     // the selection left its own list there
+    if (floor_key != 0ull || counted || least > 0.0) {
+        if (first_k && !counted) {                                // the selection left its own list there
             if (writer) fs.n_list = 0u;
             tm.sync();
         }
@@ -285,6 +340,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
             const unsigned int slot = atomicAdd(&fs0->n_list, 1u);
             if (slot < FS_CAP) fs0->list[slot] = ck;
         };
+        auto close = [&](float v) {
+            const float x = xof(v);
+            return x <= near && x < edge;
+        };
         const bool vec = (((uintptr_t)row) & 15) == 0;
         const int whole = vec ? tm.end & ~3 : tm.end;             // up to here in whole groups of four
         for (int g0 = tm.begin + (vec ? 4 : 1) * (int)threadIdx.x; g0 < whole; g0 += 16 * SAMPLE_THREADS) {
@@ -295,14 +354,14 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
                 for (int u = 0; u < 4; ++u) t[u] = *reinterpret_cast<const float4*>(row + min(g0 + u * 4 * SAMPLE_THREADS, whole - 4));
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    some |= (xof(t[u].x) <= near ? 1u : 0u) << (4 * u);
-                    some |= (xof(t[u].y) <= near ? 2u : 0u) << (4 * u);
-                    some |= (xof(t[u].z) <= near ? 4u : 0u) << (4 * u);
-                    some |= (xof(t[u].w) <= near ? 8u : 0u) << (4 * u);
+                    some |= (close(t[u].x) ? 1u : 0u) << (4 * u);
+                    some |= (close(t[u].y) ? 2u : 0u) << (4 * u);
+                    some |= (close(t[u].z) ? 4u : 0u) << (4 * u);
+                    some |= (close(t[u].w) ? 8u : 0u) << (4 * u);
                 }
             } else {
 #pragma unroll
-                for (int u = 0; u < 16; ++u) some |= (xof(row[min(g0 + u * SAMPLE_THREADS, whole - 1)]) <= near ? 1u : 0u) << u;
+                for (int u = 0; u < 16; ++u) some |= (close(row[min(g0 + u * SAMPLE_THREADS, whole - 1)]) ? 1u : 0u) << u;
             }
             while (some) {
                 const int u = __ffs(some) - 1;
@@ -311,7 +370,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
                 if (i < whole) consider(i);
             }
         }
-        if ((int)threadIdx.x < tm.end - whole && xof(row[whole + threadIdx.x]) <= near) consider(whole + threadIdx.x);
+        if ((int)threadIdx.x < tm.end - whole && close(row[whole + threadIdx.x])) consider(whole + threadIdx.x);
         tm.sync();
         const unsigned int n = fs0->n_list;
         if (n <= FS_CAP) {                                        // the same in every block
@@ -334,9 +393,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
                 }
                 if (threadIdx.x < 32) {                           // one warp adds up, 32 candidates at a time, in their order
                     const int lane = threadIdx.x;
+                    const unsigned int n_k = counted ? min(n, (unsigned int)a.top_k) : n;
                     double sum = 0.0;
-                    for (unsigned int i0 = 0; i0 < n; i0 += 32) {
-                        double w = i0 + lane < n ? raw_weight(value_of_key(fs.list[i0 + lane]), 0) : 0.0;
+                    for (unsigned int i0 = 0; i0 < n_k; i0 += 32) {
+                        double w = i0 + lane < n_k ? raw_weight(value_of_key(fs.list[i0 + lane]), 0) : 0.0;
 #pragma unroll
                         for (int o = 1; o < 32; o <<= 1) {
                             const double t = __shfl_up_sync(0xffffffffu, w, o);
@@ -345,11 +405,11 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
                         fs.lp[i0 + lane] = sum + w;               // cumulative; the list has room for whole warps
                         sum = __shfl_sync(0xffffffffu, sum + w, 31);
                     }
-                    unsigned int stay = n;                        // candidates that stay: up to the first that reaches top_p
+                    unsigned int stay = n_k;                      // candidates that stay: up to the first that reaches top_p
                     if (a.top_p < 1.f) {
                         const double target = (double)a.top_p * sum;
-                        for (unsigned int i0 = 0; i0 < n; i0 += 32) {
-                            const unsigned int hit = __ballot_sync(0xffffffffu, i0 + lane < n && fs.lp[i0 + lane] >= target);
+                        for (unsigned int i0 = 0; i0 < n_k; i0 += 32) {
+                            const unsigned int hit = __ballot_sync(0xffffffffu, i0 + lane < n_k && fs.lp[i0 + lane] >= target);
                             if (hit) { stay = i0 + __ffs(hit); break; }
                         }
                     }
