@@ -23,8 +23,8 @@
 // 64 sequences of 7 drafts over 128,256 tokens (263 MB of logits, 33 MB of the drafter's probabilities): 96 us, of which the sums take 70
 // (3.8 TB/s: the double operations of the exponentials, half of that unit's rate, and their chain) and the decisions 32 (two
 // steps of loads, the same exponentials over one row, three exchanges). One sequence of 4 drafts: 13.2 us, the two launches' time on the
-// host; 4 and 9 us on the device. With filters, 8 sequences of 4 drafts: 32.6 us, 20 of them the candidates (three passes over a row by
-// three blocks: maximum, listing, and their exchanges).
+// host; 4 and 9 us on the device. With a min_p and a top_p, 8 sequences of 4 drafts: 31 us, 18 of them the candidates (two passes over
+// a row by three blocks, maximum and listing, the sort and their exchanges); a top_k of 40 33 us, one of 1,000 44.
 #include "row_select.cuh"
 
 #define VF_PART 1024            // columns of a row that one warp adds up
@@ -263,7 +263,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
     float edge = CUDART_INF_F;                                    // nothing at or beyond this place is among the first top_k
     const bool first_k = a.top_k > 0 && a.top_k < vocab;
     // The first top_k by counting: the bin of 1/64 in which they end; where no more than the list holds lies up to there, the list takes
-    // it all and the first k of it stay (8 rows-sharing sequences of 128,256 tokens, top_k 40: TODO).
+    // it all and the first k of it stay (one sequence of 4 drafts over 128,256 tokens, top_k 40: 29 us, for 51 by a selection before
+    // the list).
     if (first_k && a.top_k <= FS_CAP) {
         for (int b = threadIdx.x; b < FS_BINS; b += SAMPLE_THREADS) fs.cnt[b] = 0u;
         tm.sync();                                                // block 0's bins are clear before anyone adds to them
@@ -391,30 +392,42 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 1) verify_floor_kernel(VerifyA
                         __syncthreads();
                     }
                 }
-                if (threadIdx.x < 32) {                           // one warp adds up, 32 candidates at a time, in their order
+                const unsigned int n_k = counted ? min(n, (unsigned int)a.top_k) : n;
+                for (unsigned int i = threadIdx.x; i < n_k; i += blockDim.x) fs.lp[i] = raw_weight(value_of_key(fs.list[i]), 0);
+                __syncthreads();
+                if (threadIdx.x < 32) {                           // one warp adds up, a run of candidates a lane, in their order
                     const int lane = threadIdx.x;
-                    const unsigned int n_k = counted ? min(n, (unsigned int)a.top_k) : n;
-                    double sum = 0.0;
-                    for (unsigned int i0 = 0; i0 < n_k; i0 += 32) {
-                        double w = i0 + lane < n_k ? raw_weight(value_of_key(fs.list[i0 + lane]), 0) : 0.0;
+                    const unsigned int run = ((n_k + 31) / 32) | 1u;          // (odd: no two lanes' runs meet a bank together)
+                    const unsigned int from = min(n_k, lane * run), to = min(n_k, from + run);
+                    double own = 0.0;
+                    for (unsigned int i = from; i < to; ++i) own += fs.lp[i];
+                    double incl = own;
 #pragma unroll
-                        for (int o = 1; o < 32; o <<= 1) {
-                            const double t = __shfl_up_sync(0xffffffffu, w, o);
-                            if (lane >= o) w += t;
-                        }
-                        fs.lp[i0 + lane] = sum + w;               // cumulative; the list has room for whole warps
-                        sum = __shfl_sync(0xffffffffu, sum + w, 31);
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const double t = __shfl_up_sync(0xffffffffu, incl, o);
+                        if (lane >= o) incl += t;
                     }
+                    const double sum = __shfl_sync(0xffffffffu, incl, 31);
                     unsigned int stay = n_k;                      // candidates that stay: up to the first that reaches top_p
+                    double total = sum;
                     if (a.top_p < 1.f) {
                         const double target = (double)a.top_p * sum;
-                        for (unsigned int i0 = 0; i0 < n_k; i0 += 32) {
-                            const unsigned int hit = __ballot_sync(0xffffffffu, i0 + lane < n_k && fs.lp[i0 + lane] >= target);
-                            if (hit) { stay = i0 + __ffs(hit); break; }
+                        const unsigned int hit = __ballot_sync(0xffffffffu, to > from && incl >= target);
+                        if (hit) {
+                            const int who = __ffs(hit) - 1;
+                            double c = incl - own;
+                            unsigned int i = from;
+                            if (lane == who)
+                                for (; i < to; ++i) {
+                                    c += fs.lp[i];
+                                    if (c >= target || i + 1 == to) { ++i; break; }       // (the last where rounding leaves it short)
+                                }
+                            stay = __shfl_sync(0xffffffffu, i, who);
+                            total = __shfl_sync(0xffffffffu, c, who);
                         }
                     }
                     if (lane == 0) {
-                        st.sum = fs.lp[stay - 1];
+                        st.sum = total;
                         st.max = mx;
                         a.stats[row_index] = st;
                         a.floors[row_index] = fs.list[stay - 1];
