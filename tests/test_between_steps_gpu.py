@@ -532,6 +532,23 @@ def test_verify_equal_logits(cuda):
     _verify(cuda, 40000, [0, 0], 1.0, False, logits=logits, room=1, top_k=12345)
 
 
+@pytest.mark.parametrize("vocab", [1531, 9001, 40000])
+def test_verify_equal_logits_at_the_border_of_top_k(cuda, vocab):
+    """Of equal logits the lower ids stay, whether they fit the candidates' list or not."""
+    gen = torch.Generator().manual_seed(vocab)
+    logits = torch.randn(5, vocab, generator=gen) - 8.0
+    for row in range(5):
+        places = torch.randperm(vocab, generator=gen)
+        logits[row, places[:1100]] = 1.0
+        logits[row, places[:100]] = 3.0 + torch.rand(100, generator=gen)
+    for top_k in (1, 99, 100, 101, 300, 1099, 1100, 1400):
+        for more in ({}, {"top_p": 0.7}, {"min_p": 0.1}):
+            assert _verify(cuda, vocab, [2, 1], 0.8, False, seed=top_k, logits=logits, top_k=top_k, **more)[2] == 0
+    flat = torch.zeros(5, vocab)
+    for top_k in (1, 40, 2048, 2049):
+        assert _verify(cuda, vocab, [2, 1], 1.0, False, seed=top_k, logits=flat, top_k=top_k)[2] == 0
+
+
 def test_verify_drafters_own_distribution_is_the_targets(cuda):
     """q = p: every draft stays, and where the draw of a rejection would be from nothing, p is drawn from."""
     gen = torch.Generator().manual_seed(4)
