@@ -192,7 +192,6 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
     const uint32_t q_ready = bars + 8u * (2 * STAGES + 4 * BUFS);             // 21 barriers at most
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
-    pdl_launch_dependents();
     __shared__ WtShare share;
     if (warp == 0) {                                                          // the other warps prepare what does not depend on it
         const WtShare mine = wt_share(a, m0, blockIdx.x, gridDim.x);
@@ -213,6 +212,8 @@ __global__ void __launch_bounds__(WT_THREADS, 1) weights_tc_kernel(const __grid_
     wt_fence_before();
     __syncthreads();
     wt_fence_after();
+    // Only now may the next kernel begin: one that takes tensor memory before it waits for this one must not find it before this block.
+    pdl_launch_dependents();
     const uint32_t tmem = *slot;
     if (share.seq < 0) {                                                      // more blocks than stretches: the same for the whole block
         if (warp == WT_WORKERS / 32 + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u * BUFS) : "memory");
