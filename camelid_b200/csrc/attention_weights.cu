@@ -1141,8 +1141,8 @@ extern "C" int cml_attn_paged_weights(const void* q, int dtype, long long q_stri
     a.joined = scratch;
     a.stats = a.joined + room(pairs * rows * 2);
     a.acc = a.stats + room(pairs * rows * 2 * a.n_splits);
+    a.kept = scratch;                                                         // (one launch keeps products, several keep the parts above)
     a.kept_stride = ((long long)max_len + CML_PAGE - 1) / CML_PAGE * CML_PAGE;
-    a.kept = a.acc + room(out ? pairs * rows * a.n_splits * v_dim : 0);
     if ((((uintptr_t)scratch) & 15) || (((uintptr_t)scores | (uintptr_t)scores_out) & 15)) return CML_ERR_BAD_ALIGN;
     // the tensor cores take rows of q that begin on 16 bytes
     const bool mma = dtype == CML_DTYPE_BF16 && (k_dim == 64 || k_dim == 128) && (out == nullptr || v_dim == k_dim) &&

@@ -2026,7 +2026,7 @@ def draws_at(positions: torch.Tensor, seed: torch.Tensor, draws: torch.Tensor):
 # ---------------------------------------------------------------------------------------
 # between two steps: which positions the cache keeps, which drafted tokens stay
 
-ATTN_WEIGHTS_KEPT_ROWS = 32     # rows of a kv head up to which the products q . k are kept for the weights
+ATTN_WEIGHTS_KEPT_ROWS = 32     # rows of a kv head up to which the products q . k are kept for the weights (8 in float)
 
 
 @functools.lru_cache(maxsize=512)
@@ -2047,9 +2047,11 @@ def attn_weights_plan(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int,
         splits = max(1, min((4 * SMS + blocks - 1) // blocks, (max_len + 4 * PAGE - 1) // (4 * PAGE)))
         split_keys = (((max_len + splits - 1) // splits + PAGE - 1) // PAGE) * PAGE
     splits = (max_len + split_keys - 1) // split_keys
-    parts = [pairs * rows * 2, pairs * rows * 2 * splits, pairs * rows * splits * value_dim if with_output else 0,
-             pairs * rows * ((max_len + PAGE - 1) // PAGE * PAGE) if rows <= ATTN_WEIGHTS_KEPT_ROWS else 0]
-    return split_keys, sum((n + 31) // 32 * 32 for n in parts)
+    # One launch keeps products, several keep the stretches' maxima, sums and outputs: a call takes one of the two, in the same room.
+    # (rows of q that do not begin on 16 bytes take the float kernels, where one launch serves eight rows)
+    kept = pairs * rows * ((max_len + PAGE - 1) // PAGE * PAGE) if rows <= (ATTN_WEIGHTS_KEPT_ROWS if fast else 8) else 0
+    parts = [pairs * rows * 2, pairs * rows * 2 * splits, pairs * rows * splits * value_dim if with_output else 0] if rows > 8 else []
+    return split_keys, max(kept, sum((n + 31) // 32 * 32 for n in parts))
 
 
 def attn_weights_floats(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype, max_new: int, max_len: int,

@@ -34,6 +34,20 @@ def test_scratch_sizes_grow_with_what_they_hold():
     assert ops.verify_bytes(0, 0, 100) >= 16 and ops.verify_bytes(4, 2, 5000) >= 4 * (16 * 5 + 8)
 
 
+def test_scratch_holds_what_one_form_of_the_kernels_keeps():
+    """One launch keeps the products, 4 bytes a row and place; several keep the stretches' statistics and outputs and no products."""
+    for dtype, rows in ((torch.bfloat16, 4), (torch.bfloat16, 8), (torch.float32, 4), (torch.float32, 8)):
+        assert ops.attn_weights_floats(16, 8 * rows, 8, 128, dtype, 1, 32768, True) == 16 * 8 * rows * 32768
+        assert ops.attn_weights_floats(3, 8 * rows, 8, 128, dtype, 1, 1000, False) == 3 * 8 * rows * 1024
+    for dtype, new in ((torch.float32, 4), (torch.bfloat16, 9)):                # 16 rows in float, 36 on the tensor cores
+        few, many = (ops.attn_weights_floats(16, 32, 8, 128, dtype, new, n, False) for n in (2048, 32768))
+        assert few <= many < 16 * 32 * new * 2048
+    # of 9 to 32 rows on the tensor cores: room for either form (rows of q off 16 bytes take the float kernels)
+    split_keys, floats = ops.attn_weights_plan(2, 32, 8, 64, 64, torch.bfloat16, 4, 8192, True)
+    splits = -(-8192 // split_keys)
+    assert floats == max(2 * 32 * 4 * 8192, 2 * 32 * 4 * (2 + splits * (2 + 64)))
+
+
 def test_kernel_entries_refuse_sizes_before_they_launch():
     """The C entries return the error of a size or type without touching a device."""
     att = ops._fn("attention_weights", "cml_attn_paged_weights")

@@ -129,6 +129,28 @@ def test_weights_with_strided_rows_and_loose_bounds(cuda, dtype, dim):
     _attention(cuda, [10, 333], [2, 1], 8, 4, dim, dtype, q_pad=3, loose=True)
 
 
+@pytest.mark.parametrize("with_out", [True, False])
+def test_weights_keep_within_their_scratch(cuda, monkeypatch, with_out):
+    """Every form of the kernels, also of rows that begin off 16 bytes, leaves alone what lies behind the scratch it asks for."""
+    from camelid_b200.csrc import ops
+    given = ops.attn_paged_weights
+    checked = []
+
+    def guarded(*args):
+        args = list(args)
+        room = torch.full((args[13].numel() + 4096,), 7.0, device=cuda)
+        args[13] = room[:args[13].numel()].fill_(float("nan"))
+        given(*args)
+        checked.append(bool((room[-4096:] == 7.0).all()))
+    monkeypatch.setattr(ops, "attn_paged_weights", guarded)
+    for dtype, dim, v_dim in ((torch.bfloat16, 64, 64), (torch.bfloat16, 128, 128), (torch.float32, 64, 64), (torch.bfloat16, 48, 80)):
+        for heads, kv_heads, news in ((4, 2, [1, 1, 1]), (8, 2, [5, 1, 2]), (4, 1, [8, 3, 0]), (8, 2, [3, 9, 1])):
+            for q_pad in (0, 3):
+                _attention(cuda, [700, 0, 129], news, heads, kv_heads, dim, dtype, with_out=with_out, v_dim=v_dim if with_out else None, q_pad=q_pad,
+                           seed=dim + heads, loose=news[1] == 9)
+    assert len(checked) == 32 and all(checked)
+
+
 def test_weights_with_values_of_another_size(cuda):
     _attention(cuda, [100, 3], [1, 2], 4, 2, 64, torch.bfloat16, v_dim=32)
     _attention(cuda, [100, 3], [1, 2], 4, 2, 32, torch.float32, v_dim=128)
