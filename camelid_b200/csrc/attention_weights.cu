@@ -1027,20 +1027,9 @@ static cudaError_t launch_team(K kernel, const WeightArgs& a, unsigned pairs, in
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-// Clusters of sixteen blocks have to be asked for, once a kernel.
-template <auto Kernel>
-static cudaError_t allow_wide_clusters() {
-    static bool allowed = false;
-    if (allowed) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    allowed = e == cudaSuccess;
-    return e;
-}
-
 template <typename T, int R>
 static cudaError_t launch_plain_all(const WeightArgs& a, unsigned pairs, size_t smem, cudaStream_t s) {
-    cudaError_t e = cml_allow_smem<weights_part_kernel<T, R, true>>(smem);
-    if (e == cudaSuccess) e = allow_wide_clusters<weights_part_kernel<T, R, true>>();
+    const cudaError_t e = cml_allow_smem<weights_part_kernel<T, R, true>>(smem);
     if (e != cudaSuccess) return e;
     int team = 1;                                                 // two blocks for every multiprocessor, none without a page of keys
     while (team < AW_TEAM && (long long)pairs * team < 2ll * cml_sm_count() && team * CML_PAGE < a.max_len) team *= 2;
@@ -1074,7 +1063,7 @@ template <int HD, int MT, bool OUT>
 static cudaError_t launch_all(const WeightArgs& a, unsigned pairs, int team, size_t smem, cudaStream_t s) {
     const auto kernel = weights_part_mma_kernel<HD, MT, OUT, true>;
     cudaError_t e = cml_allow_smem<weights_part_mma_kernel<HD, MT, OUT, true>>(smem);
-    if (e == cudaSuccess) e = allow_wide_clusters<weights_part_mma_kernel<HD, MT, OUT, true>>();
+    if (e == cudaSuccess && team > 8) e = cml_allow_wide_clusters<weights_part_mma_kernel<HD, MT, OUT, true>>();
     if (e != cudaSuccess) return e;
     return launch_team(kernel, a, pairs, team, AM_WARPS * 32, smem, s);
 }

@@ -122,25 +122,46 @@ static inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 b
     return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
 }
 
-// Raises a kernel's limit of dynamic shared memory, once per kernel and size: the call costs
+// What a module sets on or reads from a device once belongs to the device that was current then: it is remembered by the device's
+// number (beyond CML_DEVICES not at all).
+#define CML_DEVICES 32
+static inline int cml_device() {
+    int dev = -1;
+    return cudaGetDevice(&dev) == cudaSuccess && dev < CML_DEVICES ? dev : -1;
+}
+
+// Raises a kernel's limit of dynamic shared memory, once per kernel, device and size: the call costs
 // about as much as a launch's own bookkeeping and a step launches each kernel many times.
 template <auto Kernel>
 static inline cudaError_t cml_allow_smem(size_t smem) {
-    static size_t allowed = 0;
-    if (smem <= allowed) return cudaSuccess;
+    static size_t allowed[CML_DEVICES] = {};
+    const int dev = cml_device();
+    if (dev >= 0 && smem <= allowed[dev]) return cudaSuccess;
     const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) allowed = smem;
+    if (e == cudaSuccess && dev >= 0) allowed[dev] = smem;
+    return e;
+}
+
+// Clusters of sixteen blocks have to be asked for, once per kernel and device.
+template <auto Kernel>
+static inline cudaError_t cml_allow_wide_clusters() {
+    static bool allowed[CML_DEVICES] = {};
+    const int dev = cml_device();
+    if (dev >= 0 && allowed[dev]) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && dev >= 0) allowed[dev] = true;
     return e;
 }
 
 static inline int cml_sm_count() {
-    static int sms = 0;
-    if (sms <= 0) {
-        int dev = 0;
-        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
-            sms = 148;
+    static int counts[CML_DEVICES] = {};
+    const int dev = cml_device();
+    if (dev < 0) return 148;
+    if (counts[dev] <= 0 && (cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || counts[dev] <= 0)) {
+        counts[dev] = 0;
+        return 148;
     }
-    return sms;
+    return counts[dev];
 }
 
 static inline int cml_launch_status() {

@@ -879,11 +879,9 @@ extern "C" int cml_verify_drafts(const float* logits, long long ld, int n_rows, 
     const bool alone = n_seqs * team <= (team < 8 ? cml_sm_count() : cml_sm_count() * 5 / 6);
     cudaError_t e;
     if (vocab >= 65536 && n_seqs <= 4) {
-        // few sequences: sixteen blocks each (one of 128,256 tokens 9.4 us for 11.8), which have to be asked for once
-        static bool allowed = false;
-        e = allowed ? cudaSuccess : cudaFuncSetAttribute(verify_decide_kernel<1, 4>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        allowed = e == cudaSuccess;
-        if (allowed) e = launch_cluster(verify_decide_kernel<1, 4>, n_seqs * VF_TEAM, VF_THREADS, 0, VF_TEAM, s, a);
+        // few sequences: sixteen blocks each (one of 128,256 tokens 9.4 us for 11.8)
+        e = cml_allow_wide_clusters<verify_decide_kernel<1, 4>>();
+        if (e == cudaSuccess) e = launch_cluster(verify_decide_kernel<1, 4>, n_seqs * VF_TEAM, VF_THREADS, 0, VF_TEAM, s, a);
     } else if (alone && vocab <= team * VF_WARPS * 512) {         // four groups are enough (50,257 tokens: 9.5 us for 12.2 with eight)
         e = launch_cluster(verify_decide_kernel<1, 4>, n_seqs * team, VF_THREADS, 0, team, s, a);
     } else if (alone) {
