@@ -53,9 +53,26 @@ struct WeightArgs {
     float* stats;                // [seqs * kv heads][splits][rows][2]: maximum and sum of a stretch
     float* joined;               // [seqs * kv heads][rows][2]: maximum and 1 / sum of all
     float* acc;                  // [seqs * kv heads][splits][rows][v_dim]
-    float* kept;                 // [seqs * kv heads][rows][kept_stride]: q . k of steps of few rows
-    long long kept_stride;       // max_len rounded up to a page
+    float* kept;                 // q . k of steps of few rows: [blocks][rows][64], see kept_of
+    int kept_blocks;             // pages of the longest sequence, or 0: the blocks are the cache's own pages
 };
+
+// Where the products of a page of keys lie. A sequence's pages in its order need a rectangle, as long as the longest sequence for all;
+// where the cache has fewer pages than that, its own pages name the blocks (no page belongs to two sequences), so that the products
+// never take more than 4 bytes a row and cached key. A page that is none has no block then: nothing is kept of it or asked.
+struct Kept {
+    float* base;                 // of place 0 of block 0 of a sequence and kv head
+    int stride;                  // floats between blocks: the pages of a kv head, or of all
+    bool by_page;
+    __device__ __forceinline__ float* at(int p, int page) const { return base + (size_t)(by_page ? page : p) * stride; }
+};
+__device__ __forceinline__ Kept kept_of(const WeightArgs& a, int pair, int kvh, int rows) {
+    Kept k;
+    k.by_page = a.kept_blocks == 0;
+    k.stride = rows * CML_PAGE * (k.by_page ? a.kv_heads : 1);
+    k.base = a.kept + (k.by_page ? (size_t)kvh : (size_t)pair * a.kept_blocks) * (rows * CML_PAGE);
+    return k;
+}
 
 struct Seq {
     int start, fresh, length, row0, rows;      // rows: (token, head) pairs that share a kv head
@@ -189,7 +206,7 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
     const int* pages = a.table + (size_t)seq * a.width;
     const int p_first = first / CML_PAGE, p_last = (last + CML_PAGE - 1) / CML_PAGE;
     const int group_rows = a.max_new * (a.heads / a.kv_heads);
-    float* const kept = ALL ? a.kept + (size_t)blockIdx.y * group_rows * a.kept_stride : nullptr;
+    const Kept products = kept_of(a, blockIdx.y, kvh, group_rows);
     auto valid_of = [&](int p) {
         const int page = p < p_last ? pages[p] : -1;
         return page < 0 || page >= a.n_pages ? 0 : min(CML_PAGE, last - p * CML_PAGE);
@@ -229,6 +246,7 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
         quarter_products<T, R>(a, ks + (threadIdx.x & 63) * k_stride, q_s, part_s);
         __syncthreads();
         const int valid = valid_of(p);
+        float* const kept = ALL && valid > 0 ? products.at(p, pages[p]) : nullptr;
         for (int m = warp; m < rows; m += AW_THREADS / 32) {
             const int sees = min(valid - 1, s.start + (m0 + m) / group - p * CML_PAGE);       // the last key of the page that the row sees
             float x[2];
@@ -236,7 +254,7 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
             for (int h = 0; h < 2; ++h) {
                 x[h] = product_of<R>(part_s, m, lane + 32 * h) * a.scale;
                 if (lane + 32 * h > sees) x[h] = -CUDART_INF_F;
-                if (ALL) kept[(size_t)m * a.kept_stride + p * CML_PAGE + lane + 32 * h] = x[h];
+                if (ALL && valid > 0) kept[m * CML_PAGE + lane + 32 * h] = x[h];
             }
             const float a0 = x[0], a1 = x[1];
             const float old = m_s[m], now = fmaxf(old, warp_max(fmaxf(a0, a1)));
@@ -340,11 +358,12 @@ __global__ void __launch_bounds__(AW_THREADS) weights_part_kernel(WeightArgs a) 
         const int page = pages[place / CML_PAGE];
         if (page < 0 || page >= a.n_pages) continue;
         const size_t at = ((size_t)page * a.kv_heads + kvh) * CML_PAGE + place % CML_PAGE;
+        const float* const kept = products.at(place / CML_PAGE, page) + place % CML_PAGE;
         float gained = 0.f;
         const float old = a.scores[at];
 #pragma unroll
         for (int m = 0; m < R; ++m)
-            if (m < rows) gained += exp2f(kept[(size_t)m * a.kept_stride + place] - join_s[m].x) * join_s[m].y;
+            if (m < rows) gained += exp2f(kept[m * CML_PAGE] - join_s[m].x) * join_s[m].y;
         a.scores_out[at] = (place < s.old ? old : 0.f) + gained;
     }
     if (a.out) cg::this_cluster().sync();                         // a block's output stays until every block has read it
@@ -505,7 +524,7 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
     const int n_mine = max(0, t_last - t_first - warp + AM_WARPS - 1) / AM_WARPS;
     auto there = [&](int page) { return page >= 0 && page < a.n_pages; };
     int page_next = 0 < n_mine ? pages[(t_first + warp) * TILE / CML_PAGE] : -1;         // a tile's page is looked up a tile ahead
-    unsigned int missing = 0u;                                                // a bit for each stage: its page is none
+    int ahead[AM_STAGES - 1];                                                 // the pages of the tiles in flight, -1: none
     // this lane's 16 bytes of a tile's first rows, in the page and in the stage; the others lie at constant distances
     const int lane_row = lane / CH, lane_in = lane_row * HD + lane % CH * 8;
     const uint32_t lane_out = mine32 + (uint32_t)(lane_row * LDS + lane % CH * 8) * 2;
@@ -514,6 +533,7 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
     const size_t page_elems = (size_t)a.kv_heads * CML_PAGE * HD;
     int next_tile = t_first + warp, next_stage = 0, to_issue = n_mine;
     auto issue = [&]() {
+        int follow = -1;
         if (to_issue > 0) {
             const int t = next_tile, page = page_next;
             next_tile += AM_WARPS;
@@ -522,7 +542,7 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
             const size_t at = (size_t)(ok ? page : 0) * page_elems + (size_t)(t * TILE % CML_PAGE) * HD;
             const uint32_t dst = lane_out + (uint32_t)next_stage * STAGE;
             const int valid = ok ? last - t * TILE : 0;
-            missing = ok ? missing & ~(1u << next_stage) : missing | (1u << next_stage);
+            follow = ok ? page : -1;
             if (valid >= TILE) {
 #pragma unroll
                 for (int c = 0; c < TILE * CH / 32; ++c) {
@@ -539,6 +559,9 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
             }
             next_stage = next_stage + 1 == AM_STAGES ? 0 : next_stage + 1;
         }
+#pragma unroll
+        for (int i = 0; i < AM_STAGES - 2; ++i) ahead[i] = ahead[i + 1];
+        ahead[AM_STAGES - 2] = follow;
         cp_async_commit();
     };
 #pragma unroll
@@ -572,14 +595,15 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
     }
     const int mat = lane >> 3, rr = lane & 7;
     const int group_rows = a.max_new * group;
-    float* const kept = ALL ? a.kept + (size_t)blockIdx.y * group_rows * a.kept_stride : nullptr;
+    const Kept products = kept_of(a, blockIdx.y, kvh, group_rows);
     int stage = 0;
     const uint32_t k_frag = mine32 + (uint32_t)(((mat >> 1) * 8 + rr) * LDS + (mat & 1) * 8) * 2;
     const uint32_t v_frag = mine32 + HALF + (uint32_t)(((mat & 1) * 8 + rr) * LDS + (mat >> 1) * 8) * 2;
     for (int place0 = (t_first + warp) * TILE; place0 < last; place0 += AM_WARPS * TILE) {
         cp_async_wait<AM_STAGES - 2>();
         __syncwarp();
-        const bool ok = (missing >> stage & 1u) == 0u;
+        const int page = ahead[0];
+        const bool ok = page >= 0;
         issue();
         const uint32_t k32 = k_frag + (uint32_t)stage * STAGE, v32 = v_frag + (uint32_t)stage * STAGE;
         unsigned char* const here = mine + (size_t)stage * STAGE;
@@ -615,11 +639,12 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
                         if (!(ok && key < last && key <= pos[mt][i >> 1])) x[mt][n][i] = -CUDART_INF_F;
                     }
             }
-            if (ALL) {
+            if (ALL && ok) {
+                float* const kept = products.at(place0 / CML_PAGE, page) + key0 % CML_PAGE;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
                     if (pos[mt][h] >= 0) {
-                        float* row = kept + (size_t)(mt * 16 + (lane >> 2) + 8 * h) * a.kept_stride + key0;
+                        float* row = kept + (mt * 16 + (lane >> 2) + 8 * h) * CML_PAGE;
 #pragma unroll
                         for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(row + n * 8) = make_float2(x[mt][n][2 * h], x[mt][n][2 * h + 1]);
                     }
@@ -842,7 +867,8 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
             at[u] = ((size_t)(has[u] ? page : 0) * a.kv_heads + kvh) * CML_PAGE + place % CML_PAGE;
             const float4 t = *reinterpret_cast<const float4*>(a.scores + at[u]);
             old[u][0] = t.x, old[u][1] = t.y, old[u][2] = t.z, old[u][3] = t.w;
-            x[u] = kept + (has[u] ? place : first);
+            // (no place: any products that are there; what comes of them goes nowhere)
+            x[u] = has[u] ? products.at(place / CML_PAGE, page) + place % CML_PAGE : a.kept;
             g[u][0] = g[u][1] = g[u][2] = g[u][3] = 0.f;
         }
 #pragma unroll 4
@@ -850,7 +876,7 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
             const float2 j = join_s[m];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const float4 t = *reinterpret_cast<const float4*>(x[u] + (size_t)m * a.kept_stride);
+                const float4 t = *reinterpret_cast<const float4*>(x[u] + m * CML_PAGE);
                 g[u][0] = fmaf(fast_exp2(fmaf(t.x, a.scale, -j.x)), j.y, g[u][0]);
                 g[u][1] = fmaf(fast_exp2(fmaf(t.y, a.scale, -j.x)), j.y, g[u][1]);
                 g[u][2] = fmaf(fast_exp2(fmaf(t.z, a.scale, -j.x)), j.y, g[u][2]);
@@ -1131,7 +1157,8 @@ extern "C" int cml_attn_paged_weights(const void* q, int dtype, long long q_stri
     a.stats = a.joined + room(pairs * rows * 2);
     a.acc = a.stats + room(pairs * rows * 2 * a.n_splits);
     a.kept = scratch;                                                         // (one launch keeps products, several keep the parts above)
-    a.kept_stride = ((long long)max_len + CML_PAGE - 1) / CML_PAGE * CML_PAGE;
+    const int blocks = (max_len + CML_PAGE - 1) / CML_PAGE;                   // ops.attn_weights_plan has the same rule
+    a.kept_blocks = (long long)n_seqs * blocks <= n_pages ? blocks : 0;
     if ((((uintptr_t)scratch) & 15) || (((uintptr_t)scores | (uintptr_t)scores_out) & 15)) return CML_ERR_BAD_ALIGN;
     // the tensor cores take rows of q that begin on 16 bytes
     const bool mma = dtype == CML_DTYPE_BF16 && (k_dim == 64 || k_dim == 128) && (out == nullptr || v_dim == k_dim) &&

@@ -48,6 +48,15 @@ def test_scratch_holds_what_one_form_of_the_kernels_keeps():
     assert floats == max(2 * 32 * 4 * 8192, 2 * 32 * 4 * (2 + splits * (2 + 64)))
 
 
+def test_products_are_kept_for_no_more_pages_than_the_cache_has():
+    """One long sequence among many short ones does not size the scratch for all."""
+    sizes = (64, 32, 8, 128, torch.bfloat16, 8, 131_072, True)
+    assert ops.attn_weights_floats(*sizes) == 64 * 8 * 32 * 131_072
+    assert ops.attn_weights_floats(*sizes, n_pages=3000) == 8 * 32 * 3000 * 64
+    assert ops.attn_weights_floats(*sizes, n_pages=1 << 20) == ops.attn_weights_floats(*sizes)
+    assert ops.attn_weights_floats(2, 8, 8, 96, torch.float32, 5, 1000, False, n_pages=20) == 8 * 5 * 20 * 64
+
+
 def test_kernel_entries_refuse_sizes_before_they_launch():
     """The C entries return the error of a size or type without touching a device."""
     att = ops._fn("attention_weights", "cml_attn_paged_weights")

@@ -151,6 +151,30 @@ def test_weights_keep_within_their_scratch(cuda, monkeypatch, with_out):
     assert len(checked) == 32 and all(checked)
 
 
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64), (torch.bfloat16, 48)])
+def test_products_of_unequal_sequences_take_the_caches_pages(cuda, monkeypatch, dtype, dim):
+    """One long sequence among short ones: the scratch of the cache's pages is smaller than a rectangle, and enough. Cached places,
+    single tokens, drafted steps, rows that see nothing of a page, a sequence without new tokens."""
+    from camelid_b200.csrc import ops
+    given = ops.attn_paged_weights
+    used = []
+
+    def exact(q, out, k, v, scores, table, row0, start, new, heads, max_new, max_len, scale, scratch, *more):
+        small = ops.attn_weights_floats(table.shape[0], heads, k.shape[1], k.shape[3], q.dtype, max_new, max_len, out is not None,
+                                        n_pages=k.shape[0])
+        room = torch.full((small + 4096,), 7.0, device=cuda)
+        given(q, out, k, v, scores, table, row0, start, new, heads, max_new, max_len, scale, room[:small].fill_(float("nan")), *more)
+        assert bool((room[small:] == 7.0).all())
+        used.append((small, scratch.numel()))
+    monkeypatch.setattr(ops, "attn_paged_weights", exact)
+    group = 2 if dtype == torch.float32 or dim == 48 else 4
+    for news in ([1] * 6, [4, 1, 0, 2, 3, 1]):
+        for with_out in (True, False):
+            _attention(cuda, [3000, 5, 64, 0, 130, 63], news, 2 * group, 2, dim, dtype, with_out=with_out, seed=dim + news[0], in_place=news[0] == 1)
+    # (of 9 rows and more the room holds the other form's parts as well: 12 pairs * 16 rows * (2 + splits * (2 + dim)))
+    assert all(small < rectangle for small, rectangle in used) and len(used) == 4
+
+
 def test_weights_with_values_of_another_size(cuda):
     _attention(cuda, [100, 3], [1, 2], 4, 2, 64, torch.bfloat16, v_dim=32)
     _attention(cuda, [100, 3], [1, 2], 4, 2, 32, torch.float32, v_dim=128)
