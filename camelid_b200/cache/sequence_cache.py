@@ -25,7 +25,7 @@ _STATE_DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "int32": 
 
 class SequenceCache:
     def __init__(self, entry_specs: list, entry_sources: list, *, max_tokens: int, max_position: int,
-                 dtype: torch.dtype, device, max_slots: Optional[int] = None, track_weights: bool = False):
+                 dtype: torch.dtype, device, max_slots: Optional[int] = None, track_weights: bool = False, weights_scratch: int = 0):
         n_pages = max(1, (int(max_tokens) + PAGE - 1) // PAGE)
         n_slots = int(max_slots) if max_slots else n_pages
         self.dtype = dtype
@@ -74,7 +74,7 @@ class SequenceCache:
         self.book = CacheBook(kv_specs, n_pages, n_slots, max_position)
         need = self.bytes_needed(kv_specs, counts_kv, state_specs, counts_state, n_pages, n_slots, dtype)
         if track_weights:
-            need += sum(self.score_bytes(s, c, n_pages) for s, c in zip(kv_specs, counts_kv))
+            need += sum(self.score_bytes(s, c, n_pages) for s, c in zip(kv_specs, counts_kv)) + 4 * int(weights_scratch)
         if self.device.type == "cuda":
             free, _total = torch.cuda.mem_get_info(self.device)
             if need > free:
@@ -93,6 +93,9 @@ class SequenceCache:
         self.scores = None
         if track_weights:
             self.scores = [torch.zeros(t.shape[:-1], dtype=torch.float32, device=self.device) for t in self.k]
+        # ``weights_scratch`` float32 numbers for the attention that keeps weights: one piece for all layers, steps and captured
+        # graphs of this cache, which never run at the same time
+        self.weights_scratch = torch.empty(int(weights_scratch), dtype=torch.float32, device=self.device) if track_weights else None
         self.bytes = need
 
     @staticmethod

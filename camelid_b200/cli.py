@@ -6,7 +6,7 @@
     camelid replay --model DIR --dtype T --out DIR --max-tokens N     (bin/trace_run)
     camelid bench [--batch 8] [--prompt-tokens 2048] [--decode-steps 256] ...
     camelid random-model CONFIG.json OUT --seed S
-    camelid memory MODEL_OR_CONFIG --dtype T --max-tokens N [--max-slots S]     bytes of weights, cache, workspace
+    camelid memory MODEL_OR_CONFIG --dtype T --max-tokens N [--max-slots S] [--track-weights]     bytes of weights, cache, workspace
 
 Option names and meanings are the reference's where it has them: ``bench-generate MODEL
 --prompt-file --prompt --max-tokens (128) --temperature (0.0) --iterations (1) --warmup
@@ -128,7 +128,7 @@ def cmd_memory(args) -> int:
     if config.endswith(".json"):
         with open(config) as f:
             config = json.load(f)
-    plan = memory_plan(config, args.dtype, args.max_tokens, args.max_slots)
+    plan = memory_plan(config, args.dtype, args.max_tokens, args.max_slots, track_weights=args.track_weights)
     print(json.dumps({**plan.as_dict(), "max_tokens": plan.max_tokens, "max_slots": plan.max_slots,
                       "step_tokens": plan.step_tokens, "dtype": args.dtype}), flush=True)
     return 0
@@ -171,6 +171,7 @@ def main(argv=None) -> int:
     me.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     me.add_argument("--max-tokens", type=int, default=4096)
     me.add_argument("--max-slots", type=int, default=None)
+    me.add_argument("--track-weights", action="store_true", help="of a cache that keeps attention weights")
     be = sub.add_parser("bench", help="decode and prefill throughput with random weights")
     be.add_argument("--batch", type=int, default=8)
     be.add_argument("--prompt-tokens", type=int, default=2048)

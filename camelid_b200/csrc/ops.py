@@ -2031,10 +2031,11 @@ ATTN_WEIGHTS_KEPT_ROWS = 32     # rows of a kv head up to which the products q .
 
 @functools.lru_cache(maxsize=512)
 def attn_weights_plan(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int, value_dim: int, dtype: torch.dtype, max_new: int,
-                      max_len: int, with_output: bool, n_pages: int | None = None) -> tuple:
+                      max_len: int, with_output: bool, n_pages: int | None = None, aligned: bool | None = None) -> tuple:
     """(keys of a stretch, float32 numbers of scratch) of ``attn_paged_weights``: a sequence's keys are cut into stretches so that
     the blocks fill the device, none shorter than four pages. Made from sizes alone, without a device. ``n_pages``: of the cache;
-    products are kept for no more pages than it has."""
+    products are kept for no more pages than it has. ``aligned``: whether the rows of q begin on 16 bytes, which the tensor cores
+    ask for (None: room for both)."""
     pairs, rows = max(1, n_seqs) * n_kv_heads, max_new * (n_heads // n_kv_heads)
     fast = dtype == torch.bfloat16 and head_dim in (64, 128) and value_dim == head_dim
     if fast and not with_output and rows > ATTN_WEIGHTS_KEPT_ROWS:
@@ -2049,11 +2050,12 @@ def attn_weights_plan(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: int,
         split_keys = (((max_len + splits - 1) // splits + PAGE - 1) // PAGE) * PAGE
     splits = (max_len + split_keys - 1) // split_keys
     # One launch keeps products, several keep the stretches' maxima, sums and outputs: a call takes one of the two, in the same room.
-    # (rows of q that do not begin on 16 bytes take the float kernels, where one launch serves eight rows)
+    # (the float kernels, which also take rows of q that do not begin on 16 bytes, serve eight rows in one launch)
     kept_pages = max(1, n_seqs) * ((max_len + PAGE - 1) // PAGE)
     kept_pages = kept_pages if n_pages is None else min(kept_pages, n_pages)
-    kept = n_kv_heads * rows * kept_pages * PAGE if rows <= (ATTN_WEIGHTS_KEPT_ROWS if fast else 8) else 0
-    parts = [pairs * rows * 2, pairs * rows * 2 * splits, pairs * rows * splits * value_dim if with_output else 0] if rows > 8 else []
+    kept = n_kv_heads * rows * kept_pages * PAGE if rows <= (ATTN_WEIGHTS_KEPT_ROWS if fast and aligned is not False else 8) else 0
+    parts = [pairs * rows * 2, pairs * rows * 2 * splits, pairs * rows * splits * value_dim if with_output else 0]
+    parts = parts if rows > (ATTN_WEIGHTS_KEPT_ROWS if fast and aligned else 8) else []
     return split_keys, max(kept, sum((n + 31) // 32 * 32 for n in parts))
 
 
@@ -2063,6 +2065,29 @@ def attn_weights_floats(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: in
     them the answer serves a cache of any size, and sequences of unequal lengths ask for as much each as the longest."""
     return attn_weights_plan(n_seqs, n_heads, n_kv_heads, head_dim, head_dim if value_dim is None else value_dim, dtype, max_new, max_len,
                              bool(with_output), n_pages)[1]
+
+
+def attn_weights_room(slots: int, n_pages: int, n_heads: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype, max_new: int,
+                      with_output: bool) -> int:
+    """float32 numbers of scratch that serve ``attn_paged_weights`` for any step of up to ``slots`` sequences with up to ``max_new`` new
+    tokens each over a cache of ``n_pages`` pages (values as wide as keys, rows of q on 16 bytes): what the largest needs,
+    by bounds on the stretches."""
+    group = n_heads // n_kv_heads
+    rows, fast = max_new * group, dtype == torch.bfloat16 and head_dim in (64, 128)
+    together, limit = (32, ATTN_WEIGHTS_KEPT_ROWS) if fast else (8, 8)
+    room = n_kv_heads * min(rows, limit) * n_pages * PAGE
+    if rows > limit:
+        joined = slots * n_kv_heads * rows * 2
+        if fast and not with_output:
+            # n sequences have at most c - n + 1 stretches each, c blocks of a kv head
+            c = SMS // n_kv_heads
+            split_rows, width = n_kv_heads * rows * max(slots, ((c + 1) // 2) * ((c + 2) // 2)), 2
+        else:
+            # blocks * stretches <= what fills the device and one more each, and a block has at most ``together`` rows
+            blocks = slots * n_kv_heads * ((rows + together - 1) // together)
+            split_rows, width = together * (4 * SMS + blocks), 2 + (head_dim if with_output else 0)
+        room = max(room, joined + split_rows * width + 3 * 32)
+    return room
 
 
 def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, seq_start, seq_new, n_heads: int, max_new: int,
@@ -2105,7 +2130,8 @@ def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, 
         raise KernelError(f"attn_paged_weights: max_new {max_new} and max_len {max_len} must be at least one")
     if not 0.0 < scale < float("inf"):
         raise KernelError(f"attn_paged_weights: the scale must be a positive number, got {scale}")
-    split_keys, floats = attn_weights_plan(n_seqs, n_heads, kv_heads, head_dim, value_dim, dtype, max_new, max_len, out is not None, n_pages)
+    split_keys, floats = attn_weights_plan(n_seqs, n_heads, kv_heads, head_dim, value_dim, dtype, max_new, max_len, out is not None, n_pages,
+                                           q_stride % 8 == 0 and q.data_ptr() % 16 == 0)
     if err is None and out is None:             # only the kernels without output wait on barriers
         if q.device not in _simt_err and torch.cuda.is_current_stream_capturing():
             raise KernelError("attn_paged_weights: the default error word is made by a first call outside of a graph's capture (or pass err)")

@@ -237,6 +237,12 @@ class StepContext:
         """Where the running entry keeps the attention weights of its positions (None: it keeps none, or borrows its keys)."""
         return None if self.cache_source is not None else self.cache.scores_of(self.entry)
 
+    def weights_scratch(self, floats: int) -> torch.Tensor:
+        """float32 scratch for the attention that keeps weights: the cache's own, which serves every step it can hold (a buffer of the
+        step's workspace where it was made without)."""
+        own = self.cache.weights_scratch
+        return own if own is not None and own.numel() >= floats else self.buffer("attn_weights", (floats,), torch.float32)
+
     def observed_rows(self, tokens: int):
         """(row0, start, new) of every sequence's last rows of the step, ``tokens`` at most: made once a step on the device."""
         if self.observed is None or self.observed[0] != tokens:

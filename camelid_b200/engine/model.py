@@ -20,6 +20,7 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
+from ..cache.book import PAGE
 from ..cache.sequence_cache import SequenceCache
 from ..config.plan import ModelPlan
 from ..config.registry import load_config
@@ -120,9 +121,14 @@ class DecoderModel:
         specs.update(self.head.tensor_specs())
         return specs
 
-    def memory_plan(self, max_tokens: int = 0, max_slots: int | None = None, step_tokens: int | None = None):
+    def memory_plan(self, max_tokens: int = 0, max_slots: int | None = None, step_tokens: int | None = None, track_weights: bool = False):
         from ..memory import plan_for_model
-        return plan_for_model(self, max_tokens, max_slots, step_tokens)
+        return plan_for_model(self, max_tokens, max_slots, step_tokens, track_weights)
+
+    def weights_scratch(self, n_pages: int, n_slots: int) -> int:
+        """float32 numbers of scratch of a cache that keeps attention weights: what the mixers that keep any ask for, the most of them."""
+        mixers = [getattr(self.blocks[e.layer], "mixer", None) for e in self.schedule if e.cache_source is None]
+        return max((m.weights_scratch(n_slots, n_pages, self.dtype) for m in mixers if getattr(m, "keeps_weights", False)), default=0)
 
     def load_tensors(self, source, available_bytes: int | None = None) -> None:
         """``source``: ``ModelFiles`` or a dict name -> tensor. Checks names and shapes first, then
@@ -183,11 +189,15 @@ class DecoderModel:
                                       f"{self.blocks[e.layer].mixer.position.rotary_dim} is no multiple of 16")
         free = device_free_bytes(self.device)
         if free is not None:
-            self.memory_plan(max_tokens, max_slots).check(free, f"a cache for {max_tokens} tokens on {self.device}",
-                                                          parts=("cache", "workspace"))
+            self.memory_plan(max_tokens, max_slots, track_weights=track_weights).check(
+                free, f"a cache for {max_tokens} tokens on {self.device}", parts=("cache", "workspace"))
+        scratch = 0
+        if track_weights:
+            n_pages = max(1, (int(max_tokens) + PAGE - 1) // PAGE)
+            scratch = self.weights_scratch(n_pages, int(max_slots) if max_slots else n_pages)
         return SequenceCache(self.entry_cache_specs(), self.entry_cache_sources(),
                              max_tokens=max_tokens, max_position=self.plan.max_position, dtype=self.dtype,
-                             device=self.device, max_slots=max_slots, track_weights=track_weights)
+                             device=self.device, max_slots=max_slots, track_weights=track_weights, weights_scratch=scratch)
 
     def evict(self, cache: SequenceCache, slots: list, keep: int, *, first: int = 4, recent: int | None = None) -> list:
         """Cut the sequences in ``slots`` that are longer than ``keep`` to that many positions, in place: of every layer and kv head the

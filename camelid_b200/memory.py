@@ -64,14 +64,15 @@ def _numel(shape) -> int:
     return n
 
 
-def plan_for_model(model, max_tokens: int = 0, max_slots: int | None = None, step_tokens: int | None = None) -> MemoryPlan:
+def plan_for_model(model, max_tokens: int = 0, max_slots: int | None = None, step_tokens: int | None = None,
+                   track_weights: bool = False) -> MemoryPlan:
     """The plan of a built (not necessarily loaded) ``DecoderModel``; no device is touched."""
     e = _elem(model.dtype)
     specs = model.tensor_specs()
     weights = sum(_numel(s.shape) * e for s in specs.values())
     n_pages = max(1, (int(max_tokens) + PAGE - 1) // PAGE) if max_tokens else 0
     n_slots = int(max_slots) if max_slots else n_pages
-    cache = 0
+    cache = scores = 0
     seen_sources = model.entry_cache_sources()
     widest_kv = 0
     for entry_needs, src in zip(model.entry_cache_specs(), seen_sources):
@@ -80,6 +81,7 @@ def plan_for_model(model, max_tokens: int = 0, max_slots: int | None = None, ste
         for spec in flatten_specs(entry_needs):
             if isinstance(spec, KVSpec):
                 cache += n_pages * spec.n_kv_heads * PAGE * (spec.head_dim + spec.stored_value_dim) * e
+                scores += 4 * n_pages * spec.n_kv_heads * PAGE
                 widest_kv = max(widest_kv, spec.n_kv_heads * max(spec.head_dim, spec.value_dim))
             elif isinstance(spec, StateSpec):
                 from .cache.sequence_cache import _STATE_DTYPES
@@ -98,18 +100,23 @@ def plan_for_model(model, max_tokens: int = 0, max_slots: int | None = None, ste
     # scratch of a part's own kernels (buffers go by their names, which the layers share: the largest counts)
     workspace += max((p.workspace(rows, min(rows, max(n_slots, 1))) for b in model.blocks if hasattr(b, "parts") for p in b.parts()), default=0)
     workspace += 4 * max(n_slots, 1) * model.vocab_size
+    if track_weights:
+        # the scores, once more while a step is captured, and one scratch for all steps
+        cache += scores
+        workspace += scores + 4 * model.weights_scratch(n_pages, max(n_slots, 1))
     return MemoryPlan(int(weights), int(cache), int(workspace), int(max_tokens), int(n_slots), int(rows))
 
 
 def memory_plan(config, dtype="bfloat16", max_tokens: int = 0, max_slots: int | None = None,
-                step_tokens: int | None = None) -> MemoryPlan:
+                step_tokens: int | None = None, track_weights: bool = False) -> MemoryPlan:
     """``config``: a config.json dict or a model folder. Bytes of weights, cache (for
     ``max_tokens`` live tokens, each sequence's count rounded up to 64, and ``max_slots``
     sequences) and workspace (a step of ``step_tokens`` rows; default the smaller of
-    ``max_tokens`` and 2,048). Runs without a device."""
+    ``max_tokens`` and 2,048). ``track_weights``: of a cache that keeps attention weights, with its scores and its
+    scratch. Runs without a device."""
     from .engine.model import DecoderModel, parse_dtype
     model = DecoderModel.from_config(config, dtype=parse_dtype(dtype), device="cpu")
-    return plan_for_model(model, max_tokens, max_slots, step_tokens)
+    return plan_for_model(model, max_tokens, max_slots, step_tokens, track_weights)
 
 
 def device_free_bytes(device) -> int | None:

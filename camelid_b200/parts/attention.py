@@ -144,13 +144,19 @@ class GroupedQueryAttention(Part):
             self._attend(ctx, q, out, k_pages, v_pages, table, tensor_cores=False)
         linear.add_into_residual(ctx, out, self.w_o, residual, "o_partial")
 
+    def weights_scratch(self, slots: int, n_pages: int, dtype: torch.dtype) -> int:
+        rooms = [ops.attn_weights_room(slots, n_pages, self.num_heads, self.num_kv_heads, self.head_dim, dtype, new, with_output)
+                 for new, with_output in ((self.weighed_tokens, True), (self.observed_tokens, False))]
+        return max(rooms)
+
     def _weigh(self, ctx, q, out, k_pages, v_pages, scores, table, tokens: int):
         """The step's rows (``out``: with their attention output), or the last ``tokens`` of each sequence, add their weights to the
         kept scores. Lengths are bounded by the block table, so a captured step serves any of them."""
         max_new, max_len = min(ctx.max_new, tokens), table.shape[1] * PAGE
         row0, start, new = (ctx.seq_row0, ctx.seq_start, ctx.seq_new) if ctx.max_new <= tokens else ctx.observed_rows(tokens)
-        scratch = ctx.buffer("attn_weights", (ops.attn_weights_floats(ctx.n_seqs, self.num_heads, self.num_kv_heads, self.head_dim, q.dtype,
-                                                                      max_new, max_len, out is not None),), torch.float32)
+        plan = ops.attn_weights_plan(ctx.n_seqs, self.num_heads, self.num_kv_heads, self.head_dim, self.head_dim, q.dtype, max_new, max_len,
+                                     out is not None, k_pages.shape[0], True)
+        scratch = ctx.weights_scratch(plan[1])
         ops.attn_paged_weights(q, out, k_pages, v_pages if out is not None else None, scores, table, row0, start, new, self.num_heads, max_new,
                                max_len, self.scale, scratch, seq_cached=ctx.seq_start, err=linear._err_word(q.device))
 

@@ -115,6 +115,11 @@ class Part:
         """The same for a step of ``rows`` rows of up to ``sequences`` sequences, for parts whose scratch depends on both."""
         return rows * self.workspace_per_row()
 
+    def weights_scratch(self, slots: int, n_pages: int, dtype: torch.dtype) -> int:
+        """Mixers that keep weights: float32 numbers of scratch that serve any step of up to ``slots`` sequences over a cache of
+        ``n_pages`` pages. The cache holds them (``ctx.weights_scratch``) and the memory plan counts them."""
+        return 0
+
     def query_tile_sizes(self) -> list:
         """Mixers: the sizes of query tiles (rows per tile) their prefill kernels ask the
         step context for; a pair (rows per tile, least) for tiles of portions of at least so many rows."""

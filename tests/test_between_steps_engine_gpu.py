@@ -249,3 +249,26 @@ def test_drafts_verification_and_eviction_together(cuda):
             held = [h if len(h) <= 60 else h[:2] + h[len(h) - 58:] for h in held]
         cache.book.audit()
         assert [cache.length(s) for s in slots] == [len(h) for h in held]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_all_steps_of_a_tracked_cache_share_one_scratch(cuda, dtype):
+    """Prompts, drafted steps and single tokens, eager and captured, of several layouts: the scratch is the one the cache was made with."""
+    import camelid_b200
+    lm = _model(ONE_WIDE, dtype)
+    vocab = ONE_WIDE["vocab_size"]
+    cache = lm.new_cache(2048, max_slots=4, track_weights=True)
+    at = cache.weights_scratch.data_ptr()
+    slots = [cache.alloc_slot() for _ in range(3)]
+    for news in ([400, 30, 9], [1, 1, 1], [5, 1, 3], [5, 1, 3], [5, 1, 3], [8, 8, 8], [8, 8, 8], [20, 1, 40], [20, 1, 40], [1, 1, 1], [2, 1, 1]):
+        lm.step(cache, [camelid_b200.StepEntry(s, tokens(n + s, n, vocab), [n - 1]) for s, n in zip(slots, news)])
+    lm.model.decode_fed(cache, slots, [1, 2, 3], 5)
+    lm.model.check_device_errors()
+    spaces = [lm.model.workspace] + [g.ctx.ws for kept in (lm.model._graphs, lm.model._step_graphs) for g in kept[cache].values()]
+    assert len(spaces) >= 4 and not any(name == "attn_weights" for ws in spaces for name, _ in ws._bufs)
+    assert cache.weights_scratch.data_ptr() == at
+    group = ONE_WIDE["num_attention_heads"] // ONE_WIDE["num_key_value_heads"]
+    seen = [sum(min(n, 32) for n in each) + 5 for each in ((400, 1, 5, 5, 5, 8, 8, 20, 20, 1, 2), (30, 1, 1, 1, 1, 8, 8, 1, 1, 1, 1), (9, 1, 3, 3, 3, 8, 8, 40, 40, 1, 1))]
+    for s, n in zip(slots, seen):
+        line = torch.cat([cache.scores[0][0, p] for p in cache.book.pages[0][s]], dim=1)[:, :cache.length(s)].double()
+        assert torch.allclose(line.sum(1), torch.full_like(line.sum(1), float(group * n)), rtol=1e-5)

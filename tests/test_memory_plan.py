@@ -117,3 +117,52 @@ def test_shares_of_single_tokens_over_a_latent():
             assert pages < 4 or rows * part.row_blocks * 2 > ops.SMS
     assert pages_a_block(32, 1, 148) == 1 and pages_a_block(128, 1, 148) == 2 and pages_a_block(8, 128, 148) == 0
     assert [pages_a_block(p, 2, 148, True) for p in (4, 9, 17)] == [2, 3, 3] and pages_a_block(9, 128, 148, True) == 6
+
+
+def test_plan_counts_scores_and_scratch_of_a_cache_that_keeps_weights():
+    from camelid_b200 import DecoderModel
+    cfg = benchmark.config_for(2)                              # 16 layers, 8 kv heads of 64, 4 heads each
+    sizes = dict(max_tokens=8 * 4096, max_slots=8)
+    plain, tracked = memory_plan(cfg, "bfloat16", **sizes), memory_plan(cfg, "bfloat16", **sizes, track_weights=True)
+    scores = 4 * 16 * 8 * 8 * 4096
+    assert tracked.cache == plain.cache + scores and tracked.weights == plain.weights
+    # the products of 8 new tokens of 4 heads for every cached position, and the scores once more beside a capture
+    assert tracked.workspace >= plain.workspace + scores + 4 * 8 * 32 * 8 * 4096
+    assert tracked.workspace < plain.workspace + scores + 4 * 8 * 32 * 8 * 4096 + (32 << 20)
+    model = DecoderModel.from_config(TINY_B, dtype=torch.float32, device="cpu")
+    plan, bare = (model.memory_plan(1024, 4, track_weights=t) for t in (True, False))
+    cache, without = (model.new_cache(1024, 4, track_weights=t) for t in (True, False))
+    assert cache.bytes - without.bytes == 4 * sum(t.numel() for t in cache.scores) + 4 * cache.weights_scratch.numel()
+    assert plan.total - bare.total == cache.bytes - without.bytes + 4 * sum(t.numel() for t in cache.scores)
+    assert without.weights_scratch is None and cache.weights_scratch.numel() == model.weights_scratch(16, 4)
+
+
+def test_new_cache_refuses_scores_and_scratch_that_do_not_fit(monkeypatch):
+    from camelid_b200 import DecoderModel, memory
+    model = DecoderModel.from_config(TINY_B, dtype=torch.float32, device="cpu")
+    need = {t: (lambda p: p.cache + p.workspace)(model.memory_plan(4096, 8, track_weights=t)) for t in (True, False)}
+    monkeypatch.setattr(memory, "device_free_bytes", lambda device: need[True] - 1)
+    model.new_cache(4096, 8)
+    with pytest.raises(MemoryBudgetError) as e:
+        model.new_cache(4096, 8, track_weights=True)
+    assert e.value.needed == need[True] > need[False]
+    monkeypatch.setattr(memory, "device_free_bytes", lambda device: need[True])
+    model.new_cache(4096, 8, track_weights=True)
+
+
+def test_one_scratch_serves_every_step_of_a_cache():
+    """The bound holds for any number of sequences, new tokens, heads and table widths; it follows the cache's pages."""
+    import random
+    from camelid_b200.csrc import ops
+    rng = random.Random(3)
+    for _ in range(4000):
+        kv, group = rng.choice((1, 2, 3, 5, 8, 16, 40)), rng.choice((1, 2, 3, 4, 6, 8, 16))
+        dim, dtype = rng.choice((16, 64, 96, 128, 256)), rng.choice((torch.bfloat16, torch.float32))
+        slots, n_pages = int(2 ** rng.uniform(0, 9)), int(2 ** rng.uniform(0, 13))
+        most, with_output = rng.choice(((8, True), (32, False)))
+        room = ops.attn_weights_room(slots, n_pages, kv * group, kv, dim, dtype, most, with_output)
+        for _ in range(10):
+            n, new, width = rng.randint(1, slots), rng.randint(1, most), int(2 ** rng.uniform(0, 14))
+            floats = ops.attn_weights_plan(n, kv * group, kv, dim, dim, dtype, new, width * 64, with_output, n_pages, True)[1]
+            assert floats <= room, (kv, group, dim, dtype, slots, n_pages, n, new, width, with_output)
+    assert ops.attn_weights_room(64, 4096, 32, 8, 128, torch.bfloat16, 8, True) == 8 * 32 * 4096 * 64
