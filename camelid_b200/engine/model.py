@@ -88,7 +88,7 @@ class DecoderModel:
                               and all(p.graph_safe_any_step for p in self._single_parts()))
         self._seen_layouts = weakref.WeakKeyDictionary()   # cache -> {key: times seen}
         self._step_graphs = weakref.WeakKeyDictionary()    # cache -> {key: StepGraph}, oldest first
-        self._turnings: dict = {}                           # position encoding -> what evict has to know of it
+        self._turnings: dict = {}                           # position encoding -> its frequencies, for evict
 
     # ---- construction ----
     @classmethod
@@ -221,31 +221,32 @@ class DecoderModel:
             ints = torch.tensor([lengths[s] for s in cut] + [keep] * n, dtype=torch.int32).to(self.device)
             for g, spec in enumerate(book.kv_specs):
                 table = torch.tensor(book.block_table(g, cut), dtype=torch.int32).to(self.device)
-                entries = [(i, cache.entry_kv[i][1], self.blocks[e.layer].mixer.position) for i, e in enumerate(self.schedule)
+                entries = [(cache.entry_kv[i][1], self.blocks[e.layer].mixer) for i, e in enumerate(self.schedule)
                            if e.cache_source is None and cache.entry_kv[i][0] == g]
                 # entries whose positions turn alike move together
                 alike: dict = {}
-                for _, at, pos in sorted(entries, key=lambda x: x[1]):
-                    alike.setdefault(self._turning(pos), []).append((at, pos))
-                for group in alike.values():
+                for at, mixer in sorted(entries, key=lambda x: x[0]):
+                    alike.setdefault(self._turning(mixer), []).append((at, mixer.position))
+                for (interleaved, _), group in alike.items():
                     ats, pos = [at for at, _ in group], group[0][1]
                     whole = ats == list(range(cache.k[g].shape[0]))
                     for at in [slice(None)] if whole else [slice(a, a + 1) for a in ats]:
                         k, scores = cache.k[g][at], cache.scores[g][at]
                         kept = torch.empty((k.shape[0], n, spec.n_kv_heads, keep), dtype=torch.int32, device=self.device)
                         ops.evict_positions(k, cache.v[g][at], scores, table, table, ints[:n], ints[n:], kept, first, recent,
-                                            inv_freq=pos.inv_freq if pos.rotary_dim else None, interleaved=self._turning(pos)[0])
+                                            inv_freq=pos.inv_freq if pos.rotary_dim else None, interleaved=interleaved)
             for s in cut:
                 book.truncate(s, keep)
         return [min(lengths[s], keep) for s in slots]
 
-    def _turning(self, position) -> tuple:
-        """(pairs are neighbours, frequencies) of a position encoding, as numbers: read from the device once."""
+    def _turning(self, mixer) -> tuple:
+        """(pairs are neighbours, frequencies) of the keys that a mixer caches; the frequencies are read from the device once."""
+        position = mixer.position
         known = self._turnings.get(position)
         if known is None:
-            known = (getattr(position, "pairing", "split") == "interleaved", tuple(position.inv_freq.tolist()))
-            self._turnings[position] = known
-        return known
+            known = self._turnings[position] = tuple(position.inv_freq.tolist())
+        pairing = getattr(mixer, "key_pairing", "") or getattr(position, "pairing", "split")
+        return pairing == "interleaved", known
 
     # ---- the step ----
     def _validate(self, cache: SequenceCache, entries: list) -> list:

@@ -32,6 +32,7 @@ class GroupedQueryAttention(Part):
     accepts_row_scale = True
     keeps_weights = True
     keeps_weights_in = ("forward",)
+    key_pairing = "split"           # what the rotary kernels of this mixer write, whatever its position encoding calls its pairs
 
     # In a cache that keeps attention weights: steps of up to ``weighed_tokens`` new tokens a sequence run the attention that keeps
     # them; of longer ones (prompts) the last ``observed_tokens`` rows of every sequence are asked what they look at.

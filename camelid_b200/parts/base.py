@@ -73,6 +73,9 @@ class Part:
     # methods in which it does. A class that overrides one of them says ``keeps_weights`` again if it does so too.
     keeps_weights: bool = False
     keeps_weights_in: tuple = ()
+    # Mixers that keep weights: which channels of their cached keys turn together, "split" (i and i + half of the rotary size) or
+    # "interleaved" (neighbours); eviction turns them back that way. Empty: as the position encoding's ``pairing`` says.
+    key_pairing: str = ""
     # The methods in which the rows and their scale are taken. A class that overrides one of them says ``accepts_row_scale``
     # again if it takes the scale too; otherwise its rows come complete.
     takes_rows: tuple = ()

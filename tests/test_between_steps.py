@@ -149,6 +149,31 @@ def test_evict_refuses_before_anything_changes():
     cache.book.audit()
 
 
+def test_evict_turns_keys_as_the_mixer_wrote_them(monkeypatch):
+    """The dense mixer's kernels pair a channel with the one half the rotary size on, whatever the position encoding calls its pairs; a
+    mixer that does not say how it pairs goes by the encoding."""
+    model = DecoderModel.from_config(TINY_A, device="cpu")
+    for b in model.blocks:
+        b.mixer.position.pairing = "interleaved"
+        b.mixer.position.load({}, "cpu", torch.float32)
+    cache = model.new_cache(256, track_weights=True)
+    turned = []
+    monkeypatch.setattr(ops, "evict_positions", lambda *args, interleaved, **kw: turned.append(interleaved))
+
+    def once():
+        slot = cache.alloc_slot()
+        cache.book.extend(slot, 100)
+        cache.book.commit(slot, 100)
+        assert model.evict(cache, [slot], 8) == [8]
+        cache.free_slot(slot)
+        now = list(turned)
+        turned.clear()
+        return now
+    assert once() == [False]                                                # all layers turn alike: one call
+    model.blocks[0].mixer.key_pairing = ""
+    assert sorted(once()) == [False] * (len(model.blocks) - 1) + [True]
+
+
 # ---- drafted tokens -----------------------------------------------------------------------------------------------------
 class Rolling:
     """A cache of the bookkeeping alone."""

@@ -272,3 +272,20 @@ def test_all_steps_of_a_tracked_cache_share_one_scratch(cuda, dtype):
     for s, n in zip(slots, seen):
         line = torch.cat([cache.scores[0][0, p] for p in cache.book.pages[0][s]], dim=1)[:, :cache.length(s)].double()
         assert torch.allclose(line.sum(1), torch.full_like(line.sum(1), float(group * n)), rtol=1e-5)
+
+
+def test_evicted_keys_whose_encoding_names_other_pairs(cuda):
+    """A position encoding that calls its pairs neighbours in the mixer that always pairs split halves: evicted keys are a fresh sequence's."""
+    import camelid_b200
+    lm = _model(ONE_LAYER, "float32")
+    lm.model.blocks[0].mixer.position.pairing = "interleaved"
+    cache, fresh = lm.new_cache(512, track_weights=True), lm.new_cache(512)
+    text = tokens(4, 200, ONE_LAYER["vocab_size"])
+    slot, other = cache.alloc_slot(), fresh.alloc_slot()
+    lm.step(cache, [camelid_b200.StepEntry(slot, text, [])])
+    assert lm.evict(cache, [slot], 70, first=3, recent=67) == [70]
+    lm.step(fresh, [camelid_b200.StepEntry(other, text[:3] + text[-67:], [])])
+    m, t = (torch.cat([c.k[0][0, p] for p in c.book.pages[0][s]], dim=1)[:, :70] for c, s in ((cache, slot), (fresh, other)))
+    # the rotary kernel rounds position * frequency: half a step of 2^-16 up to position 199, of 2^-17 up to 69; a pair is at most
+    # sqrt(2) of its larger number long; sixteen roundings of sines, products and sums
+    assert float((m - t).abs().max()) <= (2 ** 0.5 * (2.0 ** -17 + 2.0 ** -18) + 16 * 2.0 ** -24) * float(t.abs().max())
