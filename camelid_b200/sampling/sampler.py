@@ -84,7 +84,7 @@ class Sampler:
     def verify(self, logits: torch.Tensor, drafts: list, histories: list, draft_probs: list | None = None, row0: list | None = None) -> tuple:
         """Which drafted tokens stay, and the token behind them. ``logits``: float32 on the device, for every sequence a row for each
         of its ``drafts`` (a list of tokens) and one more, packed or from the rows ``row0`` on (adjusted in place when penalties or
-        biases are set); ``histories``: per sequence the tokens before its drafts; ``draft_probs``: per sequence the drafter's probabilities
+        biases are set: then no row belongs to two); ``histories``: per sequence the tokens before its drafts; ``draft_probs``: per sequence the drafter's probabilities
         (float32 [drafts, vocabulary] on the device), or None where it was certain of its tokens. Returns (accepted drafts,
         next tokens), two lists. The draws come from the sampler's seed and the history's length: the next token's
         from the stream of ``sample``, the acceptances' from one of their own."""
@@ -104,6 +104,8 @@ class Sampler:
         if o.adjusts:
             # a row's history ends with the drafts before it; rows that no sequence names are left alone
             named = {r + j: list(h) + list(d[:j]) for r, h, d in zip(row0, histories, drafts) for j in range(len(d) + 1)}
+            if len(named) < n + sum(len(d) for d in drafts):
+                raise SamplingError("two sequences share rows of logits, which penalties and biases would adjust for one of them alone")
             entries, biases = self._adjust_entries(list(named.values()))
             if entries:
                 at = list(named)

@@ -306,6 +306,17 @@ def test_drafted_loop_refusals():
     assert cache.book.slots.n_held == 0
 
 
+def test_verification_refuses_rows_that_two_sequences_adjust():
+    """A row is adjusted in place by one history: two sequences that name it would get one answer for both."""
+    from camelid_b200.sampling import Sampler, SamplingOptions
+    sampler = Sampler(SamplingOptions(temperature=0.5, repeat_penalty=1.2, seed=1), 10, "cpu")
+    logits = torch.zeros(3, 10)
+    for drafts, row0 in (([[1], [2]], [0, 1]), ([[1], []], [0, 0]), ([[], []], [2, 2])):
+        with pytest.raises(SamplingError):
+            sampler.verify(logits, drafts, [[3], [4]], row0=row0)
+    assert bool((logits == 0).all())
+
+
 def test_lookup_drafts():
     look = PromptLookup(3, 2)
     assert look([]) == [] and look([5]) == [] and look([1, 2, 3]) == []
