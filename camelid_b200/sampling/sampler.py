@@ -129,7 +129,8 @@ class Sampler:
                     probs[i, :len(d)] = p
                 else:                                                # certain drafts among others with probabilities
                     for j, t in enumerate(d):
-                        probs[i, j, int(t)] = 1.0
+                        if 0 <= int(t) < self.vocab_size:            # (a token that is none is rejected and reported by the kernel)
+                            probs[i, j, int(t)] = 1.0
         out = torch.empty((n, room + 2), dtype=torch.int32, device=self.device)
         counts, chosen = torch.empty(n, dtype=torch.int32, device=self.device), torch.empty((n, room + 1), dtype=torch.int32, device=self.device)
         scratch = torch.empty(ops.verify_bytes(rows, n, self.vocab_size), dtype=torch.uint8, device=self.device)

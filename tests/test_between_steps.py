@@ -317,6 +317,26 @@ def test_verification_refuses_rows_that_two_sequences_adjust():
     assert bool((logits == 0).all())
 
 
+def test_certain_drafts_outside_the_vocabulary_beside_probabilities(monkeypatch):
+    """A draft that is no token reaches the kernel, which rejects and reports it, whatever the other sequences bring."""
+    from camelid_b200.sampling import Sampler, SamplingOptions
+    sampler = Sampler(SamplingOptions(temperature=0.5, seed=1), 10, "cpu")
+    given = []
+
+    def verify(logits, row0, lens, drafts, probs, accept, draws, *rest):
+        given.append((drafts.tolist(), probs))
+        counts, tokens = rest[4], rest[5]
+        counts.zero_(), tokens.zero_()
+    monkeypatch.setattr(ops, "verify_drafts", verify)
+    certain = [[10, 3], [-1, 2]]
+    for d in certain:
+        sampler.verify(torch.zeros(5, 10), [[4], d], [[1], [2]], [torch.full((1, 10), 0.1), None])
+        drafts, probs = given.pop()
+        want = torch.zeros(2, 10)
+        want[1, d[1]] = 1.0
+        assert drafts == [[4, 0], d] and torch.equal(probs[1], want) and bool((probs[0, 0] == 0.1).all())
+
+
 def test_lookup_drafts():
     look = PromptLookup(3, 2)
     assert look([]) == [] and look([5]) == [] and look([1, 2, 3]) == []
