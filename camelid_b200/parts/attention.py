@@ -31,7 +31,7 @@ class GroupedQueryAttention(Part):
     handles_pending = True
     accepts_row_scale = True
     keeps_weights = True
-    keeps_weights_in = ("forward",)
+    keeps_weights_in = ("forward", "_attend")      # (few tokens are attended to by the kernel that keeps weights, not by _attend)
     key_pairing = "split"           # what the rotary kernels of this mixer write, whatever its position encoding calls its pairs
 
     # In a cache that keeps attention weights: steps of up to ``weighed_tokens`` new tokens a sequence run the attention that keeps

@@ -130,6 +130,24 @@ def test_only_mixers_that_keep_weights_are_tracked():
         DecoderModel.from_config(FOMATAR["mixed"], device="cpu").new_cache(128, track_weights=True)
 
 
+def test_a_mixer_with_attention_of_its_own_is_not_tracked():
+    """In a tracked cache steps of few tokens run the weighing kernel in place of ``_attend``: a class that changes what that does has to
+    say that it keeps weights."""
+    from camelid_b200.parts.attention import GroupedQueryAttention
+
+    class Own(GroupedQueryAttention):
+        def _attend(self, ctx, q, out, *rest, **kw):
+            super()._attend(ctx, q, out, *rest, **kw)
+
+    class Said(Own):
+        keeps_weights = True
+    assert not Own.keeps_weights and Said.keeps_weights
+    model = DecoderModel.from_config(TINY_A, device="cpu")
+    model.blocks[0].mixer.__class__ = Own
+    with pytest.raises(ConfigError):
+        model.new_cache(128, track_weights=True)
+
+
 def test_evict_refuses_before_anything_changes():
     model = DecoderModel.from_config(TINY_A, device="cpu")
     cache = model.new_cache(128)
