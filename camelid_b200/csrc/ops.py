@@ -2105,7 +2105,7 @@ def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, 
     (int32 [1]; by default ``simt_error_word``) is set if one of the kernels' bounded waits runs out. No page stands in two rows of
     the table."""
     scores_out = scores if scores_out is None else scores_out
-    _here(q, out, k_pages, v_pages, scores, scores_out, block_table, seq_row0, seq_start, seq_new, scratch, seq_cached)
+    _here(q, out, k_pages, v_pages, scores, scores_out, block_table, seq_row0, seq_start, seq_new, scratch, seq_cached, err)
     n_pages, kv_heads, page, head_dim = shape = k_pages.shape
     n_seqs, width = block_table.shape
     rows, q_width = q.shape
@@ -2119,6 +2119,7 @@ def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, 
     assert block_table.is_contiguous() and seq_row0.is_contiguous() and seq_start.is_contiguous() and seq_new.is_contiguous()
     assert seq_row0.numel() == seq_start.numel() == seq_new.numel() == n_seqs
     assert seq_cached is None or (seq_cached.dtype == torch.int32 and seq_cached.numel() == n_seqs and seq_cached.is_contiguous())
+    assert err is None or err.dtype == torch.int32
     assert (out is None) == (v_pages is None), "an output needs values, and values an output"
     value_dim, out_stride = head_dim, 0
     if out is not None:

@@ -223,6 +223,22 @@ def test_weights_with_missing_pages(cuda):
         assert bool(((s_dev.cpu().double() - ref_scores).abs() <= tol_scores + 1e-30).all())
 
 
+def test_weights_refuse_an_error_word_elsewhere(cuda):
+    """The kernels would write it: on the host, or as another type."""
+    from camelid_b200 import KernelError
+    from camelid_b200.csrc import ops
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)        # noqa: E731
+    k, s = torch.zeros(1, 1, PAGE, 64, dtype=torch.bfloat16, device=cuda), torch.zeros(1, 1, PAGE, device=cuda)
+    q = torch.zeros(2, 64, dtype=torch.bfloat16, device=cuda)
+    scratch = torch.empty(ops.attn_weights_floats(1, 1, 1, 64, torch.bfloat16, 2, 64, False), device=cuda)
+    args = (q, None, k, None, s, ints([[0]]), ints([0]), ints([0]), ints([2]), 1, 2, 64, 0.125, scratch)
+    with pytest.raises(KernelError):
+        ops.attn_paged_weights(*args, err=torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(AssertionError):
+        ops.attn_paged_weights(*args, err=torch.zeros(1, device=cuda))
+    ops.attn_paged_weights(*args, err=ints([0]))
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 def test_window_at_the_limits_of_its_kernels(cuda, dim):
     """Rows just below, at and beyond what the tensor-memory kernels take, and stretches that end inside a tile."""
