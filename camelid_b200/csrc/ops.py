@@ -2067,6 +2067,16 @@ def attn_weights_floats(n_seqs: int, n_heads: int, n_kv_heads: int, head_dim: in
                              bool(with_output), n_pages)[1]
 
 
+@functools.lru_cache(maxsize=512)
+def _attn_weights_call(n_seqs, n_heads, n_kv_heads, head_dim, value_dim, dtype, max_new, max_len, with_output, n_pages, aligned) -> tuple:
+    """(keys of a stretch, float32 numbers of scratch, kernels launched) of a call: one for few rows, two for every 512 rows on tcgen05,
+    else three."""
+    plan = attn_weights_plan(n_seqs, n_heads, n_kv_heads, head_dim, value_dim, dtype, max_new, max_len, with_output, n_pages, aligned)
+    rows, fast = max_new * (n_heads // n_kv_heads), aligned and dtype == torch.bfloat16 and head_dim in (64, 128) and value_dim == head_dim
+    one = rows <= (ATTN_WEIGHTS_KEPT_ROWS if fast else 8)
+    return *plan, 1 if one else 2 * ((rows + 511) // 512) if fast and not with_output else 3
+
+
 def attn_weights_room(slots: int, n_pages: int, n_heads: int, n_kv_heads: int, head_dim: int, dtype: torch.dtype, max_new: int,
                       with_output: bool) -> int:
     """float32 numbers of scratch that serve ``attn_paged_weights`` for any step of up to ``slots`` sequences with up to ``max_new`` new
@@ -2119,7 +2129,6 @@ def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, 
     assert block_table.is_contiguous() and seq_row0.is_contiguous() and seq_start.is_contiguous() and seq_new.is_contiguous()
     assert seq_row0.numel() == seq_start.numel() == seq_new.numel() == n_seqs
     assert seq_cached is None or (seq_cached.dtype == torch.int32 and seq_cached.numel() == n_seqs and seq_cached.is_contiguous())
-    assert err is None or err.dtype == torch.int32
     assert (out is None) == (v_pages is None), "an output needs values, and values an output"
     value_dim, out_stride = head_dim, 0
     if out is not None:
@@ -2131,19 +2140,22 @@ def attn_paged_weights(q, out, k_pages, v_pages, scores, block_table, seq_row0, 
         raise KernelError(f"attn_paged_weights: max_new {max_new} and max_len {max_len} must be at least one")
     if not 0.0 < scale < float("inf"):
         raise KernelError(f"attn_paged_weights: the scale must be a positive number, got {scale}")
-    split_keys, floats = attn_weights_plan(n_seqs, n_heads, kv_heads, head_dim, value_dim, dtype, max_new, max_len, out is not None, n_pages,
-                                           q_stride % 8 == 0 and q.data_ptr() % 16 == 0)
-    if err is None and out is None:             # only the kernels without output wait on barriers
+    q_at = q.data_ptr()
+    split_keys, floats, launches = _attn_weights_call(n_seqs, n_heads, kv_heads, head_dim, value_dim, dtype, max_new, max_len, out is not None, n_pages,
+                                                      not (q_stride & 7 or q_at & 15))
+    if err is not None:
+        assert err.dtype == torch.int32
+    elif out is None:                           # only the kernels without output wait on barriers
         if q.device not in _simt_err and torch.cuda.is_current_stream_capturing():
             raise KernelError("attn_paged_weights: the default error word is made by a first call outside of a graph's capture (or pass err)")
         err = simt_error_word(q.device)
     if scratch.dtype != torch.float32 or scratch.numel() < floats or not scratch.is_contiguous():
         raise KernelError(f"attn_paged_weights: the scratch must be {floats} contiguous float32 numbers (attn_weights_floats)")
     _check(_fn("attention_weights", "cml_attn_paged_weights")(
-        q.data_ptr(), dtype_code(dtype), q_stride, _p(out), out_stride, k_pages.data_ptr(), _p(v_pages), scores.data_ptr(),
+        q_at, dtype_code(dtype), q_stride, _p(out), out_stride, k_pages.data_ptr(), _p(v_pages), scores.data_ptr(),
         scores_out.data_ptr(), block_table.data_ptr(), width, n_pages, seq_row0.data_ptr(), seq_start.data_ptr(), seq_new.data_ptr(),
         _p(seq_cached), n_seqs, rows, n_heads, kv_heads, head_dim, value_dim, max_new, max_len, scale, split_keys, scratch.data_ptr(),
-        _p(err), _stream()), "attn_paged_weights", 3)
+        _p(err), _stream()), "attn_paged_weights", launches)
 
 
 def evict_positions(k_pages, v_pages, scores, block_table, out_table, lengths, keeps, kept, first: int, recent: int, inv_freq=None,

@@ -15,7 +15,7 @@
 // Everything that a decision rests on is computed in double, because a rounding of 2^-24 in a sum over 128,256 tokens
 // would move one draw in a hundred to a neighbouring token: exp((l - max) / T), its sums, the thresholds.
 //
-// Two launches, three with filters: (1) the maximum and the sum of every row, in parts of 1,024 columns, or, with
+// Two launches: (1) the maximum and the sum of every row, in parts of 1,024 columns, or, with
 // filters, the same of the candidates, by a cluster per row (row_select.cuh); (2) a cluster per sequence decides how
 // many tokens stay, adds up the one row that the next token is drawn from, warp by warp, and walks the warp's stretch
 // in which the crossing lies.

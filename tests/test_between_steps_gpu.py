@@ -749,3 +749,44 @@ def test_the_same_call_twice_gives_the_same_bits(cuda):
             call()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(changed, first)), i
+
+
+def test_launches_are_counted_as_they_are_captured(cuda):
+    """What the count of launches gains is the number of kernels in a captured call's graph, for every form."""
+    import ctypes
+    from camelid_b200.csrc import ops
+    nodes_of = ctypes.CDLL("libcudart.so.12").cudaGraphGetNodes
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)        # noqa: E731
+    err = ints([0])
+    calls = []
+    for dtype, dim, heads, new, with_out, pad, want in (
+            (torch.bfloat16, 64, 4, 1, True, 0, 1), (torch.bfloat16, 128, 4, 8, True, 0, 1), (torch.bfloat16, 64, 4, 9, True, 0, 3),
+            (torch.bfloat16, 64, 4, 8, False, 0, 1), (torch.bfloat16, 64, 4, 9, False, 0, 2), (torch.bfloat16, 64, 4, 200, False, 0, 4),
+            (torch.bfloat16, 64, 4, 3, True, 3, 3), (torch.float32, 64, 4, 2, True, 0, 1), (torch.float32, 64, 4, 3, False, 0, 3)):
+        k = torch.zeros(4, 1, PAGE, dim, dtype=dtype, device=cuda)
+        q = torch.zeros(new, heads * dim + pad, dtype=dtype, device=cuda)[:, :heads * dim]
+        out = torch.zeros(new, heads * dim, dtype=dtype, device=cuda) if with_out else None
+        scratch = torch.empty(ops.attn_weights_floats(1, heads, 1, dim, dtype, new, 256, with_out), device=cuda)
+        args = (q, out, k, k if with_out else None, torch.zeros(4, 1, PAGE, device=cuda), ints([[0, 1, 2, 3]]), ints([0]), ints([0]), ints([new]), heads,
+                new, 256, 0.1, scratch)
+        calls.append((lambda args=args: ops.attn_paged_weights(*args, err=err), want))
+    table = ints([[0, 1, 2, 3]])
+    evict = (k, k.clone(), torch.zeros(4, 1, PAGE, device=cuda), table, table, ints([200]), ints([100]), ints([[[0] * 100]]), 1, 2)
+    calls.append((lambda: ops.evict_positions(*evict), 2))
+    for temperature, top_p in ((0.0, 1.0), (0.7, 1.0), (0.7, 0.9)):
+        args = (torch.zeros(2, 90, device=cuda), ints([0]), ints([1]), ints([[3]]), None, torch.zeros(1, 1, device=cuda), torch.zeros(1, device=cuda),
+                temperature, 0, top_p, 0.0, ints([0]), ints([[0, 0]]), err, torch.empty(ops.verify_bytes(2, 1, 90), dtype=torch.uint8, device=cuda))
+        calls.append((lambda args=args: ops.verify_drafts(*args), 2))
+    side = torch.cuda.Stream()
+    for i, (call, want) in enumerate(calls):
+        with torch.cuda.stream(side):
+            call()                                          # kernels are loaded and their limits set before a capture
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph(keep_graph=True)
+        before = ops.launch_count()
+        with torch.cuda.graph(graph):
+            call()
+        assert ops.launch_count() - before == want, i
+        n = ctypes.c_size_t(0)
+        assert nodes_of(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(n)) == 0
+        assert n.value == want, i
