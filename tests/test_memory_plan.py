@@ -166,3 +166,16 @@ def test_one_scratch_serves_every_step_of_a_cache():
             floats = ops.attn_weights_plan(n, kv * group, kv, dim, dim, dtype, new, width * 64, with_output, n_pages, True)[1]
             assert floats <= room, (kv, group, dim, dtype, slots, n_pages, n, new, width, with_output)
     assert ops.attn_weights_room(64, 4096, 32, 8, 128, torch.bfloat16, 8, True) == 8 * 32 * 4096 * 64
+
+
+def test_memory_command_of_a_tracked_cache(tmp_path, capsys):
+    import json
+    from camelid_b200 import cli
+    path = tmp_path / "config.json"
+    path.write_text(json.dumps(TINY_B))
+    plans = []
+    for more in ([], ["--track-weights"]):
+        assert cli.main(["memory", str(path), "--dtype", "float32", "--max-tokens", "1024", "--max-slots", "4", *more]) == 0
+        plans.append(json.loads(capsys.readouterr().out))
+    want = memory_plan(TINY_B, "float32", max_tokens=1024, max_slots=4, track_weights=True).as_dict()
+    assert {k: plans[1][k] for k in want} == want and plans[1]["cache"] > plans[0]["cache"]
