@@ -65,7 +65,8 @@ class LanguageModel:
         """Generate for a list of prompts (lists of token ids). Returns the generated ids per
         prompt (the stop token included), or ``GenerationResult`` objects with ``details``. ``drafter``: a callable
         that gives the tokens it expects after a history (``PromptLookup``, a smaller model): a step then brings them along
-        and keeps those that the model would have drawn; greedy tokens are the same with it."""
+        and keeps those that the model would have drawn. Greedy tokens are the same with it up to rounding: a step of several
+        tokens adds its products in another order than one of single tokens, so near-equal logits may go the other way."""
         single = bool(prompts) and isinstance(prompts[0], int)
         if single:
             prompts = [prompts]

@@ -289,3 +289,77 @@ def test_evicted_keys_whose_encoding_names_other_pairs(cuda):
     # the rotary kernel rounds position * frequency: half a step of 2^-16 up to position 199, of 2^-17 up to 69; a pair is at most
     # sqrt(2) of its larger number long; sixteen roundings of sines, products and sums
     assert float((m - t).abs().max()) <= (2 ** 0.5 * (2.0 ** -17 + 2.0 ** -18) + 16 * 2.0 ** -24) * float(t.abs().max())
+
+
+def _observe(lm, cache, seen):
+    """Wraps the model's step: counts how many rows of each slot a tracked cache observes."""
+    step = lm.model.step
+
+    def counted(c, entries):
+        if c is cache:
+            most = max(len(e.tokens) for e in entries)
+            for e in entries:
+                seen[e.slot] = seen.get(e.slot, 0) + (len(e.tokens) if most <= 8 else min(len(e.tokens), 32))
+        return step(c, entries)
+    lm.model.step = counted
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_drafted_rows_weigh_once_each(cuda, model_folders, dtype):
+    """Drafts that stay: after every step a sequence's scores sum to the rows observed of it, whatever steps brought them."""
+    import camelid_b200
+    lm = camelid_b200.load(model_folders["tiny_d"], dtype=dtype)
+    prompts = [tokens(60 + i, n, 331) for i, n in enumerate([30, 7, 12])]
+    cache, seen, looked = lm.new_cache(1024, track_weights=True), {}, []
+    _observe(lm, cache, seen)
+
+    def drafter(history):                       # (certain of one token: in float32 it is the model's own, so all drafts stay)
+        return known[tuple(history[:1])][len(history):len(history) + 1 + len(history) % 4]
+    known = {}
+    for p, w in zip(prompts, lm.generate(prompts, max_tokens=24, stop_token_ids=())):
+        known[(p[0],)] = list(p) + w
+    assert len(known) == 3
+    rejected = [0]
+    truncate = cache.truncate
+
+    def dropped(slot, length):
+        rejected[0] += 1
+        return truncate(slot, length)
+    cache.truncate = dropped
+
+    def check(live):
+        for slot, n in seen.items():
+            if not cache.book.slots.is_held(slot):
+                continue
+            line = torch.cat([cache.scores[0][:, p] for p in cache.book.pages[0][slot]], dim=2)[:, :, :cache.length(slot)].double()
+            total = line.sum(2)
+            if rejected[0] == 0:
+                assert torch.allclose(total, torch.full_like(total, 3.0 * n), rtol=1e-5)
+            else:                               # what looked at rejected places went with them, nothing came twice
+                assert bool((total <= 3.0 * n * (1 + 1e-5)).all())
+            looked.append(slot)
+    lm.generate(prompts, max_tokens=24, stop_token_ids=(), drafter=drafter, cache=cache, on_step=check)
+    assert len(looked) >= 9 and (dtype == "bfloat16" or rejected[0] == 0)
+
+
+def test_bfloat16_drafted_tokens_differ_at_near_ties_alone(cuda, model_folders):
+    """Where drafted generation first leaves the plain one, the plain run's logits of the two tokens are as near as rounding makes them."""
+    import camelid_b200
+    lm = camelid_b200.load(model_folders["tiny_d"], dtype="bfloat16")
+    prompts = [tokens(80 + i, n, 331) for i, n in enumerate([30, 7, 64, 1])]
+    want = lm.generate(prompts, max_tokens=40, stop_token_ids=())
+    known = [list(p) + w for p, w in zip(prompts, want)]
+
+    def right(history):
+        full = next((k for k in known if k[:len(history)] == history), None)
+        return full[len(history):len(history) + 5] if full else []
+    got = lm.generate(prompts, max_tokens=40, stop_token_ids=(), drafter=right)
+    for p, g, w in zip(prompts, got, want):
+        at = next((j for j in range(40) if g[j] != w[j]), None)
+        if at is None:
+            continue
+        cache = lm.new_cache(1024)
+        slot = cache.alloc_slot()
+        row = lm.step(cache, [camelid_b200.StepEntry(slot, p + w[:at], [len(p) + at - 1])])[0]
+        # the caches of one step and of many agree to 4e-2 of the largest logit (as the tracked and the plain cache's do)
+        assert float(row[w[at]] - row[g[at]]) <= 2 * 4e-2 * float(row.abs().max())
