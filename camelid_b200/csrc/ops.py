@@ -2162,7 +2162,8 @@ def evict_positions(k_pages, v_pages, scores, block_table, out_table, lengths, k
                     interleaved: bool = False):
     """Keep min(keeps[i], lengths[i]) places of every sequence i, chosen for each cache entry and kv head: its ``first`` places, its
     ``recent`` last ones (cut to what is kept in all) and those of the largest ``scores``, the lower place among equals (a
-    score that is not a number counts as the lowest). No page stands in two rows of the table. They move, in order, to the places 0.. of the pages in
+    score that is not a number, or of a page that the table does not name, counts as the lowest; a place of such a page that stays all the
+    same leaves its new place as it was). No page stands in two rows of the table. They move, in order, to the places 0.. of the pages in
     ``out_table``, which is ``block_table`` itself (the cache closes its gaps in place) or names pages that ``block_table``
     does not. Keys, values and scores: [pages, kv heads, 64(, size)] or, for several entries with one table, [entries, pages, ...];
     ``v_pages`` None: values live in the key rows. ``kept`` int32 [(entries,) sequences, kv heads, room] gets the old places in order

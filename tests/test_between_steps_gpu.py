@@ -790,3 +790,36 @@ def test_launches_are_counted_as_they_are_captured(cuda):
         n = ctypes.c_size_t(0)
         assert nodes_of(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(n)) == 0
         assert n.value == want, i
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_from_tables_wider_than_the_kept_scores(cuda, in_place):
+    """Scores beyond place 49,152 are read again for every digit; the border lies in either part."""
+    _evict(cuda, [50_300, 49_153], [900, 49_100], 4, 64, entries=1, heads=1, dim=16, v_dim=0, in_place=in_place, rotary=0, seed=11)
+    _evict(cuda, [50_300], [700], 0, 0, entries=1, heads=1, dim=16, v_dim=0, in_place=in_place, rotary=16, seed=12,
+           scores=lambda e, p, h: torch.randint(0, 30000, (e, p, h, PAGE), generator=torch.Generator().manual_seed(5)).float() - 15000.0)
+
+
+def test_evict_with_missing_pages(cuda):
+    """Places of a page that the table does not name stay last of all, even behind infinitely low scores; where they have to stay, what
+    stands at their new places is left alone."""
+    from camelid_b200.csrc import ops
+    gen = torch.Generator().manual_seed(2)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)        # noqa: E731
+    for missing in (-1, 6, 2 ** 31 - 1):
+        k, s = torch.randn(6, 1, PAGE, 32, generator=gen), torch.full((6, 1, PAGE), -float("inf"))
+        table = [[5, missing, 2, 4]]
+        for out_table, keep, first in ((table, 128, 0), (table, 256, 0), ([[0, 1, 3]], 130, 70)):
+            k_dev, s_dev, kept = k.to(cuda), s.to(cuda), torch.full((1, 1, 256), -7, dtype=torch.int32, device=cuda)
+            t = ints(table)
+            ops.evict_positions(k_dev, None, s_dev, t, t if out_table is table else ints(out_table), ints([256]), ints([keep]), kept, first, 0)
+            there = [p for p in range(256) if p // PAGE != 1]
+            want = [p for p in range(256) if p < first or p in there[max(0, min(first, 64)):]][:keep] if first else sorted(
+                there[:keep] + [p for p in range(64, 128)][:max(0, keep - 192)])
+            assert kept[0, 0].tolist() == want + [-7] * (256 - len(want)), (missing, keep, first)
+            ref = k.clone()
+            for j, p in enumerate(want):
+                dst = out_table[0][j // PAGE]
+                if p in there and 0 <= dst < 6:
+                    ref[dst, 0, j % PAGE] = k[table[0][p // PAGE], 0, p % PAGE]
+            assert torch.equal(k_dev.cpu(), ref), (missing, keep, first)
