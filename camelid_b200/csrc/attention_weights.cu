@@ -488,11 +488,11 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src
 
 #define AM_WARPS 4
 #define AM_STAGES 3
-// Keys of a tile: with heads of 64, 32 where 17 to 32 rows share them (8 sequences of 1,500 to 4,100 keys 28.4 us for 29.7 with 16), 16
+// Keys of a tile: with heads of 64, 32 where 17 to 32 rows share them (8 sequences of 1,500 to 4,100 keys 27.7 us for 28.7 with 16), 16
 // where fewer do (8 sequences of 300 to 8,191 keys 22.1 us for 24.7 with 32: four blocks fit a multiprocessor, not two).
 template <int HD, int MT> constexpr int few_tile = HD == 128 || MT == 1 ? 16 : 32;
 
-// Up to 16 * MT rows of a (sequence, kv head). A warp takes every eighth tile of TILE keys of the block's stretch with a ring of
+// Up to 16 * MT rows of a (sequence, kv head). A warp takes every fourth tile of TILE keys of the block's stretch with a ring of
 // its own in shared memory, and the warps' ranges are joined at the end in their order. OUT: with values and output.
 // ALL (grid: cluster, pairs): the blocks of a cluster share all keys of a sequence, exchange their rows' maxima and sums over
 // distributed shared memory, join the output and sum the weights of their own keys, whose products they kept: one
@@ -901,7 +901,7 @@ __global__ void __launch_bounds__(AM_WARPS * 32) weights_part_mma_kernel(WeightA
 }
 
 #define AR_WARPS 4
-// (3) for more than 16 rows: a warp keeps 64 keys in registers as the operand of 16 rows and lets the rows of q pass, so that a
+// (3) for more than 32 rows with output: a warp keeps 64 keys in registers as the operand of 16 rows and lets the rows of q pass, so that a
 // key's sum over the rows stays in one quad of lanes, in the order of the rows. Grid (256 keys, pairs).
 #define AC_ROWS 32              // rows of q in a stage
 #define AC_STAGES 4

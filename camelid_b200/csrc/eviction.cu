@@ -5,9 +5,9 @@
 // and a score that is not a number counts as the lowest. The places that stay move up, in order, to the places
 // 0 .. M - 1 of the out table's pages with their values and scores. With rotary frequencies the keys are turned by the
 // angle of the distance they move, so that a key's place is again its position: (a, b) at place p, moved to j, becomes
-// (a cos t - b sin t, b cos t + a sin t) with t = (j - p) f. The angle is formed in double and reduced to one turn
-// before it is rounded (positions reach 2^20, where a float product would be off by 0.06 of a radian); the turn itself is
-// float, and a bfloat16 key is rounded once per move.
+// (a cos t - b sin t, b cos t + a sin t) with t = (j - p) f. The frequency, formed in double once, is a
+// fraction of a turn in 64 bits; its product with the whole places moved wraps to one turn by itself, and only that is rounded (positions
+// reach 2^20, where a float product would be off by 0.06 of a radian). The turn itself is float, and a bfloat16 key is rounded once per move.
 //
 // Two launches. (1) A block per unit finds the score at the border by its digits and lists the places that stay in order.
 // (2) The rows move through registers. The out table may be the table itself: place kept[j] >= j, so the rows of the j-th
@@ -238,7 +238,7 @@ template <typename T> __device__ __forceinline__ void sine_cosine(unsigned int p
 template <> __device__ __forceinline__ void sine_cosine<float>(unsigned int places, uint2 turns, float* sn, float* cs) {
     sincospif(phase_of(places, turns) * 4.656612873077393e-10f, sn, cs);      // 2^-31: half turns
 }
-// bfloat16 keys take the fast functions: off by 2^-20.9, an eighth of a percent of their rounding
+// bfloat16 keys take the fast functions: off by 2^-20.9, a 7,600th of the keys' own rounding (2^-8)
 template <> __device__ __forceinline__ void sine_cosine<bf16>(unsigned int places, uint2 turns, float* sn, float* cs) {
     const float x = phase_of(places, turns) * 1.4629180792671596e-09f;        // 2 pi 2^-32
     asm("sin.approx.ftz.f32 %0, %1;" : "=f"(*sn) : "f"(x));
